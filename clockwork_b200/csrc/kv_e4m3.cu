@@ -1,0 +1,288 @@
+// Writing the paged cache behind the norms of the heads and the position rotation, and reading an 8-bit cache back.
+//
+// norm_rotate_store, per token t and head: x = the head's entries of the [q | k | v] row, float32;
+//     q, k:  x <- x * rsqrt(mean(x^2) + eps) * w        (where the layer norms its heads)
+//            (x_j, x_{j + rot/2}) turned by position * inv_freq[j], j < rot/2
+// q is rounded once to the run's type and handed on; k (float32, not rounded before) and v become rows of the cache: 8-bit rows
+// (kv_e4m3.cuh) or rows of the run's type.  The angle is position * inv_freq as a product of two floats with its rounding error
+// made good: sin(p + e) = sin p (1 - e^2/2) + e cos p with p + e the exact product, |e| <= 2^-24 p, so that a position of a million is
+// still turned to a few 2^-24.
+//
+// read_pages: code * 2^(E - 127) in bfloat16 (exact) or float32 for the positions of every request's context, at the same page
+// and slot of a plain cache; the rest of a request's last page becomes zero.  Both are streams over memory.
+#include "kv_e4m3.cuh"
+
+struct StoreParams {
+    const void* qkv; void* q_out;
+    const int* positions; const int* slots;
+    const float* inv_freq; const float* q_weight; const float* k_weight;
+    void* k_cache; void* v_cache; uint8_t* k_exp; uint8_t* v_exp;  // k_exp null: a plain cache
+    int nh, nkv, hd, rot, page_size, num_slots;
+    float eps;
+    int* status;
+};
+
+__device__ __forceinline__ void turn_of(float position, float freq, float& sn, float& cs) {
+    const float p = position * freq, e = fmaf(position, freq, -p);
+    float s, c;
+    sincosf(p, &s, &c);
+    const float less = 1.f - 0.5f * e * e;
+    sn = s * less + c * e;
+    cs = c * less - s * e;
+}
+
+// A token per block.  LG neighbouring lanes share a head; a lane holds two quads of it: the two halves of four pairs that turn
+// together (the lanes below rot / 8), or eight entries behind them.  So pairs never leave a thread, the mean of squares and the
+// largest magnitude are shuffles among LG lanes, and all accesses are of 8 or 16 bytes.
+template <typename T, int LG>
+__global__ void norm_rotate_store_kernel(const StoreParams p) {
+    extern __shared__ float turn[];  // cos[rot / 2], sin[rot / 2]
+    pdl_enter();
+    const int t = blockIdx.x, half = p.rot >> 1;
+    {
+        const float pos = (float)p.positions[t];
+        for (int j = threadIdx.x; j < half; j += blockDim.x) turn_of(pos, p.inv_freq[j], turn[half + j], turn[j]);
+    }
+    int slot = p.slots[t];
+    if (slot >= p.num_slots) {
+        if (threadIdx.x == 0) cw_report(p.status, CW_ST_SLOT_RANGE, t, slot);
+        slot = -1;
+    }
+    const int page = slot >= 0 ? slot / p.page_size : 0, off = slot >= 0 ? slot - page * p.page_size : 0;
+    __syncthreads();
+    const int heads = p.nh + 2 * p.nkv, l = threadIdx.x % LG, turning = p.rot >> 3;
+    const bool there = l < (p.hd >> 3), turns = l < turning;
+    const int a_at = turns ? 4 * l : p.rot + 8 * (l - turning), b_at = turns ? half + 4 * l : a_at + 4;
+    const T* row = (const T*)p.qkv + (size_t)t * heads * p.hd;
+    for (int head0 = 0; head0 < heads; head0 += blockDim.x / LG) {  // (whole warps go round together: the shuffles below)
+        const int head = head0 + threadIdx.x / LG;
+        const bool live = head < heads && there, is_q = head < p.nh, is_v = head >= p.nh + p.nkv;
+        float4 a = make_float4(0.f, 0.f, 0.f, 0.f), b = a;
+        if (live) {
+            a = Vec4<T>::load(row + (size_t)head * p.hd + a_at);
+            b = Vec4<T>::load(row + (size_t)head * p.hd + b_at);
+        }
+        const float* weight = is_q ? p.q_weight : p.k_weight;
+        if (p.q_weight != nullptr || p.k_weight != nullptr) {
+            float sum = a.x * a.x + a.y * a.y + a.z * a.z + a.w * a.w + b.x * b.x + b.y * b.y + b.z * b.z + b.w * b.w;
+#pragma unroll
+            for (int o = LG / 2; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+            if (live && !is_v && weight != nullptr) {
+                const float r = rsqrtf(sum / (float)p.hd + p.eps);
+                const float4 wa = *reinterpret_cast<const float4*>(weight + a_at), wb = *reinterpret_cast<const float4*>(weight + b_at);
+                a.x *= r * wa.x; a.y *= r * wa.y; a.z *= r * wa.z; a.w *= r * wa.w;
+                b.x *= r * wb.x; b.y *= r * wb.y; b.z *= r * wb.z; b.w *= r * wb.w;
+            }
+        }
+        if (live && !is_v && turns) {
+            const float4 cs = *reinterpret_cast<const float4*>(turn + 4 * l), sn = *reinterpret_cast<const float4*>(turn + half + 4 * l);
+            const float4 x = a, y = b;
+            a.x = x.x * cs.x - y.x * sn.x; a.y = x.y * cs.y - y.y * sn.y; a.z = x.z * cs.z - y.z * sn.z; a.w = x.w * cs.w - y.w * sn.w;
+            b.x = y.x * cs.x + x.x * sn.x; b.y = y.y * cs.y + x.y * sn.y; b.z = y.z * cs.z + x.z * sn.z; b.w = y.w * cs.w + x.w * sn.w;
+        }
+        if (live && is_q) {
+            T* out = (T*)p.q_out + ((size_t)t * p.nh + head) * p.hd;
+            Vec4<T>::store(out + a_at, a);
+            Vec4<T>::store(out + b_at, b);
+        }
+        const int kvh = is_v ? head - p.nh - p.nkv : head - p.nh;
+        const size_t at = ((size_t)(slot < 0 ? 0 : slot) * p.nkv + kvh) * p.hd;
+        if (p.k_exp == nullptr) {
+            if (live && !is_q && slot >= 0) {
+                T* out = (T*)(is_v ? p.v_cache : p.k_cache) + at;
+                Vec4<T>::store(out + a_at, a);
+                Vec4<T>::store(out + b_at, b);
+            }
+            continue;
+        }
+        a.x = kv_clamped(a.x); a.y = kv_clamped(a.y); a.z = kv_clamped(a.z); a.w = kv_clamped(a.w);
+        b.x = kv_clamped(b.x); b.y = kv_clamped(b.y); b.z = kv_clamped(b.z); b.w = kv_clamped(b.w);
+        float big = fmaxf(fmaxf(fmaxf(fabsf(a.x), fabsf(a.y)), fmaxf(fabsf(a.z), fabsf(a.w))),
+                          fmaxf(fmaxf(fabsf(b.x), fabsf(b.y)), fmaxf(fabsf(b.z), fabsf(b.w))));
+        big = fmaxf(big, 0.f);  // (a row of NaN alone)
+#pragma unroll
+        for (int o = LG / 2; o > 0; o >>= 1) big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, o));
+        if (live && !is_q && slot >= 0) {
+            const int power = kv_power(big);
+            const float d = kv_down(power);
+            uint8_t* out = (uint8_t*)(is_v ? p.v_cache : p.k_cache) + at;
+            *reinterpret_cast<uint32_t*>(out + a_at) = kv_codes(a.x * d, a.y * d, a.z * d, a.w * d);
+            *reinterpret_cast<uint32_t*>(out + b_at) = kv_codes(b.x * d, b.y * d, b.z * d, b.w * d);
+            if (l == 0) (is_v ? p.v_exp : p.k_exp)[((size_t)page * p.nkv + kvh) * p.page_size + off] = (uint8_t)power;
+        }
+    }
+}
+
+// Any even rotary span and any alignment: a warp per head, an entry per lane and round.
+template <typename T>
+__global__ void norm_rotate_store_any_kernel(const StoreParams p) {
+    extern __shared__ float turn[];
+    pdl_enter();
+    const int t = blockIdx.x, half = p.rot >> 1, lane = threadIdx.x & 31;
+    const float pos = (float)p.positions[t];
+    for (int j = threadIdx.x; j < half; j += blockDim.x) turn_of(pos, p.inv_freq[j], turn[half + j], turn[j]);
+    int slot = p.slots[t];
+    if (slot >= p.num_slots) {
+        if (threadIdx.x == 0) cw_report(p.status, CW_ST_SLOT_RANGE, t, slot);
+        slot = -1;
+    }
+    const int page = slot >= 0 ? slot / p.page_size : 0, off = slot >= 0 ? slot - page * p.page_size : 0;
+    __syncthreads();
+    const int heads = p.nh + 2 * p.nkv;
+    for (int head = threadIdx.x >> 5; head < heads; head += blockDim.x >> 5) {
+        const bool is_q = head < p.nh, is_v = head >= p.nh + p.nkv;
+        const T* x = (const T*)p.qkv + ((size_t)t * heads + head) * p.hd;
+        const float* weight = is_v ? nullptr : is_q ? p.q_weight : p.k_weight;
+        float r = 1.f;
+        if (weight != nullptr) {
+            float sum = 0.f;
+            for (int j = lane; j < p.hd; j += 32) sum += to_f(x[j]) * to_f(x[j]);
+            r = rsqrtf(warp_sum(sum) / (float)p.hd + p.eps);
+        }
+        auto normed = [&](int j) { return weight != nullptr ? to_f(x[j]) * (r * weight[j]) : to_f(x[j]); };
+        auto entry = [&](int j) {
+            if (is_v || j >= p.rot) return normed(j);
+            return j < half ? normed(j) * turn[j] - normed(j + half) * turn[half + j]
+                            : normed(j) * turn[j - half] + normed(j - half) * turn[j];
+        };
+        const int kvh = is_v ? head - p.nh - p.nkv : head - p.nh;
+        const size_t at = ((size_t)(slot < 0 ? 0 : slot) * p.nkv + kvh) * p.hd;
+        if (is_q) {
+            for (int j = lane; j < p.hd; j += 32) ((T*)p.q_out)[((size_t)t * p.nh + head) * p.hd + j] = from_f<T>(entry(j));
+        } else if (slot >= 0 && p.k_exp == nullptr) {
+            for (int j = lane; j < p.hd; j += 32) ((T*)(is_v ? p.v_cache : p.k_cache))[at + j] = from_f<T>(entry(j));
+        } else if (slot >= 0) {
+            float big = 0.f;
+            for (int j = lane; j < p.hd; j += 32) big = fmaxf(big, fabsf(kv_clamped(entry(j))));
+            const int power = kv_power(warp_max(big));
+            uint8_t* out = (uint8_t*)(is_v ? p.v_cache : p.k_cache) + at;
+            for (int j = lane; j < p.hd; j += 32)
+                out[j] = __nv_cvt_float_to_fp8(kv_clamped(entry(j)) * kv_down(power), __NV_SATFINITE, __NV_E4M3);
+            if (lane == 0) (is_v ? p.v_exp : p.k_exp)[((size_t)page * p.nkv + kvh) * p.page_size + off] = (uint8_t)power;
+        }
+    }
+}
+
+static inline bool aligned(const void* p, int bytes) { return ((uintptr_t)p & (bytes - 1)) == 0; }
+
+template <typename T>
+static int store_launch(const StoreParams& p, int N, cudaStream_t stream) {
+    const int heads = p.nh + 2 * p.nkv, smem = p.rot * (int)sizeof(float);
+    const int w = 4 * (int)sizeof(T);
+    const bool quads = p.rot % 8 == 0 && p.hd % 8 == 0 && aligned(p.qkv, w) && aligned(p.q_out, w) &&
+                       aligned(p.k_cache, p.k_exp ? 4 : w) && aligned(p.v_cache, p.k_exp ? 4 : w) && aligned(p.q_weight, 16) &&
+                       aligned(p.k_weight, 16);
+    if (!quads) {
+        const int threads = heads < 8 ? heads * 32 : 256;
+        return cw_launch(norm_rotate_store_any_kernel<T>, dim3(N), dim3(threads), smem, stream, 1u, p);
+    }
+    int lg = 2;
+    while (lg * 8 < p.hd) lg *= 2;
+    const int threads = min(512, (heads * lg + 31) / 32 * 32);
+    switch (lg) {
+        case 2: return cw_launch(norm_rotate_store_kernel<T, 2>, dim3(N), dim3(threads), smem, stream, 1u, p);
+        case 4: return cw_launch(norm_rotate_store_kernel<T, 4>, dim3(N), dim3(threads), smem, stream, 1u, p);
+        case 8: return cw_launch(norm_rotate_store_kernel<T, 8>, dim3(N), dim3(threads), smem, stream, 1u, p);
+        case 16: return cw_launch(norm_rotate_store_kernel<T, 16>, dim3(N), dim3(threads), smem, stream, 1u, p);
+        default: return cw_launch(norm_rotate_store_kernel<T, 32>, dim3(N), dim3(threads), smem, stream, 1u, p);
+    }
+}
+
+// q_out [N, nh * hd]; slots[t] < 0: the token is not stored.  k_exp and v_exp null: the cache is of the run's type.
+// rot 0: nothing turns (inv_freq may be null).  The norms' weights are float32 [hd] or null.
+extern "C" int cw_norm_rotate_store(const void* qkv, void* q_out, const int* positions, const int* slots, const float* inv_freq,
+                                    const float* q_weight, const float* k_weight, void* k_cache, void* v_cache, uint8_t* k_exp,
+                                    uint8_t* v_exp, int N, int nh, int nkv, int hd, int rot, int page_size, int num_pages, float eps,
+                                    int dtype, int* status, cudaStream_t stream) {
+    if (N == 0) return CW_OK;
+    if (N < 0 || nh <= 0 || nkv <= 0 || hd <= 0 || hd > 256 || rot < 0 || rot > hd || rot % 2 || page_size <= 0 || num_pages <= 0 ||
+        (long long)num_pages * page_size > 0x7FFFFFFF || (rot > 0 && inv_freq == nullptr) || (k_exp == nullptr) != (v_exp == nullptr))
+        return CW_ERR_BAD_SIZE;
+    const StoreParams p = {qkv, q_out, positions, slots, inv_freq, q_weight, k_weight, k_cache, v_cache, k_exp, v_exp,
+                           nh, nkv, hd, rot, page_size, num_pages * page_size, eps, status};
+    if (dtype == 0) return store_launch<float>(p, N, stream);
+    if (dtype == 1) return store_launch<bf16>(p, N, stream);
+    return CW_ERR_BAD_DTYPE;
+}
+
+struct ReadParams {
+    const uint8_t* k; const uint8_t* v; const uint8_t* k_exp; const uint8_t* v_exp;
+    void* k_out; void* v_out;
+    const int* block_tables; const int* ctx_lens; const int* q_start;
+    int requests, nkv, hd, page_size, max_blocks, num_pages, window, least_rows;
+    int* status;
+};
+
+// Units are pages of a request, keys and values apart.  A page's codes are one run of memory, and so is where they go; a thread
+// takes 16 codes at a time, whose row has one power.
+template <typename T>
+__global__ void __launch_bounds__(256) read_pages_kernel(const ReadParams p) {
+    __shared__ int sh[36];
+    pdl_enter();
+    auto first_block = [&](int s, int ctx) { return p.window > 0 ? max(0, ctx - p.window) / p.page_size : 0; };
+    // (a portion's first row sees `window` keys before it: the window reaches back from there)
+    auto span = [&](int s, int& from) {
+        int ctx = p.ctx_lens[s], first = ctx;
+        if (p.q_start != nullptr) {
+            const int rows = p.q_start[s + 1] - p.q_start[s];
+            if (rows < p.least_rows) return 0;
+            first = ctx - rows + 1;
+        }
+        from = first_block(s, first);
+        return max(0, min((ctx + p.page_size - 1) / p.page_size, p.max_blocks) - from);
+    };
+    const UnitRange r = units_of_block([&](int s) { int from; return 2 * span(s, from); }, p.requests, 1, gridDim.x, blockIdx.x, sh);
+    int s = r.request, at = r.offset;
+    const int chunks = p.hd >> 4, items = p.page_size * p.nkv * chunks;
+    for (int u = r.first; u < r.last; ++s, at = 0) {
+        int from = 0;
+        const int n = 2 * span(s, from), ctx = p.ctx_lens[s];
+        for (; at < n && u < r.last; ++at, ++u) {
+            const bool is_v = at & 1;
+            const int block = from + (at >> 1), page = p.block_tables[(size_t)s * p.max_blocks + block];
+            if (page < 0 || page >= p.num_pages) {
+                if (threadIdx.x == 0) cw_report(p.status, CW_ST_PAGE_RANGE, s, page);
+                continue;
+            }
+            const uint4* src = reinterpret_cast<const uint4*>(is_v ? p.v : p.k) + (size_t)page * items;
+            const uint8_t* powers = (is_v ? p.v_exp : p.k_exp) + (size_t)page * p.nkv * p.page_size;
+            T* dst = (T*)(is_v ? p.v_out : p.k_out) + (size_t)page * items * 16;
+            const int live = min(p.page_size, ctx - block * p.page_size);
+            for (int i = threadIdx.x; i < items; i += blockDim.x) {
+                const int row = i / chunks, token = row / p.nkv, head = row - token * p.nkv;
+                uint4 codes = make_uint4(0, 0, 0, 0);
+                float up = 0.f;
+                if (token < live) {
+                    codes = src[i];
+                    up = kv_up(powers[head * p.page_size + token]);
+                }
+                const uint32_t w[4] = {codes.x, codes.y, codes.z, codes.w};
+#pragma unroll
+                for (int q = 0; q < 4; ++q) {
+                    const float2 lo = kv_float2(w[q]), hi = kv_float2(w[q] >> 16);
+                    Vec4<T>::store(dst + (size_t)i * 16 + q * 4, make_float4(lo.x * up, lo.y * up, hi.x * up, hi.y * up));
+                }
+            }
+        }
+    }
+}
+
+// q_start (or null): only requests with at least `least_rows` rows (1 or more) are read.  window > 0: from the page on that the first of a request's
+// rows (its last position without q_start) still sees.
+extern "C" int cw_read_pages(const uint8_t* k, const uint8_t* v, const uint8_t* k_exp, const uint8_t* v_exp, void* k_out, void* v_out,
+                             const int* block_tables, const int* ctx_lens, const int* q_start, int requests, int nkv, int hd,
+                             int page_size, int max_blocks, int num_pages, int window, int least_rows, int blocks, int dtype,
+                             int* status, cudaStream_t stream) {
+    if (requests == 0) return CW_OK;
+    if (requests < 0 || nkv <= 0 || hd <= 0 || hd % 16 || page_size <= 0 || max_blocks <= 0 || num_pages <= 0 || window < 0 || blocks <= 0 || least_rows < 1 ||
+        !aligned(k, 16) || !aligned(v, 16) || !aligned(k_out, 16) || !aligned(v_out, 16) ||
+        (long long)page_size * nkv * (hd >> 4) > 0x7FFFFFFF)
+        return CW_ERR_BAD_SIZE;
+    const ReadParams p = {k, v, k_exp, v_exp, k_out, v_out, block_tables, ctx_lens, q_start, requests, nkv, hd, page_size,
+                          max_blocks, num_pages, window, least_rows, status};
+    if (dtype == 0) return cw_launch(read_pages_kernel<float>, dim3(blocks), dim3(256), 0, stream, 1u, p);
+    if (dtype == 1) return cw_launch(read_pages_kernel<bf16>, dim3(blocks), dim3(256), 0, stream, 1u, p);
+    return CW_ERR_BAD_DTYPE;
+}
+
+CW_TRACE_TU(kv_e4m3)

@@ -1,0 +1,106 @@
+// The 8-bit form of cached keys and values.  A row (one token's key or value in one KV head) is `hd` e4m3 codes and one byte E;
+// entry = code * 2^(E - 127).  E is the smallest, from 3 on, that keeps the row's largest magnitude within 448, e4m3's largest
+// number: a power of two, so that scaling is exact in both directions (the code's 4 bits are the only rounding, at most half a
+// step, 2^-4 of an entry that is no subnormal code), every held entry is a bfloat16 number, and the tensor cores can multiply
+// codes and leave the powers to float32.  Magnitudes beyond 1.875 * 2^127 are held as that (infinities too: the largest number
+// whose code times its power is finite); a NaN entry is held as NaN and has no say in E; a row of zeros has E = 127.
+//
+// Codes lie like the plain cache, [pages, page_size, nkv, hd]; the powers [pages, nkv, page_size], so that those of a head's
+// tokens in a page are neighbours.
+#pragma once
+#include <cuda_fp16.h>
+#include <cuda_fp8.h>
+#include "common.cuh"
+
+#define KV_BIGGEST __int_as_float(0x7F700000)  // 1.875 * 2^127
+
+// NaN passes through (fminf and fmaxf would drop it)
+__device__ __forceinline__ float kv_clamped(float x) { return fabsf(x) > KV_BIGGEST ? copysignf(KV_BIGGEST, x) : x; }
+
+// E for the largest magnitude of a row (0 <= big <= KV_BIGGEST)
+__device__ __forceinline__ int kv_power(float big) {
+    const uint32_t bits = __float_as_uint(big);
+    if (bits == 0) return 127;
+    return max(3, (int)(bits >> 23) - 8 + ((bits & 0x7FFFFF) > 0x600000 ? 1 : 0));  // 448 = 1.75 * 2^8
+}
+__device__ __forceinline__ float kv_down(int power) { return __int_as_float((254 - power) << 23); }  // 2^(127 - E): to codes
+__device__ __forceinline__ float kv_up(int power) { return __int_as_float(power << 23); }            // 2^(E - 127) (E = 0: 0)
+
+// four numbers, already divided by the row's power, as four codes
+__device__ __forceinline__ uint32_t kv_codes(float a, float b, float c, float d) {
+    const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(a, b), __NV_SATFINITE, __NV_E4M3);
+    const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(c, d), __NV_SATFINITE, __NV_E4M3);
+    return lo | hi << 16;
+}
+// two codes as two half-precision numbers (exact: the format's 4 exponent and 3 fraction bits fit)
+__device__ __forceinline__ uint32_t kv_half2(uint32_t codes) {
+    const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)codes, __NV_E4M3);
+    return (uint32_t)h.x | (uint32_t)h.y << 16;
+}
+__device__ __forceinline__ float2 kv_float2(uint32_t codes) {
+    const uint32_t h = kv_half2(codes & 0xFFFF);
+    return __half22float2(*reinterpret_cast<const __half2*>(&h));
+}
+
+// The requests' work, cut evenly over the blocks of a grid: request s brings units(s) units, numbered through all requests;
+// block b owns units [b * quota, (b + 1) * quota), quota = ceil(total / blocks), at least `least`.  Every block works this out
+// from the lengths on the device (so that a captured launch follows them).  All threads of the block call it; `sh`: 36 words
+// of shared memory, free again after a barrier of the caller's.
+struct UnitRange {
+    int total, quota;
+    int first, last;     // this block's units [first, last)
+    int request, offset; // where unit `first` lies: request and unit within it
+};
+template <class F>
+__device__ __forceinline__ UnitRange units_of_block(F units, int requests, int least, int blocks, int block, int* sh) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = (blockDim.x + 31) >> 5;
+    UnitRange r;
+    int sum = 0;
+    const int mine = threadIdx.x < requests ? units(threadIdx.x) : 0;  // (looked up once where a thread per request suffices)
+    sum = mine;
+    for (int s = threadIdx.x + blockDim.x; s < requests; s += blockDim.x) sum += units(s);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    if (lane == 0) sh[warp] = sum;
+    __syncthreads();
+    r.total = 0;
+    for (int w = 0; w < warps; ++w) r.total += sh[w];
+    r.quota = max(least, (r.total + blocks - 1) / blocks);
+    r.first = (int)min((long long)block * r.quota, (long long)r.total);
+    r.last = min(r.total, r.first + r.quota);
+    r.request = r.offset = 0;
+    if (r.first >= r.last) return r;
+    int base = 0;
+    for (int s0 = 0; s0 < requests; s0 += blockDim.x) {
+        const int s = s0 + threadIdx.x;
+        const int n = s0 == 0 ? mine : s < requests ? units(s) : 0;
+        int upto = n;  // units of this chunk's requests up to and with s
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int v = __shfl_up_sync(0xffffffffu, upto, o);
+            if (lane >= o) upto += v;
+        }
+        __syncthreads();  // (the words of the round before are read)
+        if (lane == 31) sh[warp] = upto;
+        if (threadIdx.x == 0) sh[32] = -1;
+        __syncthreads();
+        int before = base, chunk = 0;
+        for (int w = 0; w < warps; ++w) {
+            if (w < warp) before += sh[w];
+            chunk += sh[w];
+        }
+        const int from = before + upto - n;
+        if (from <= r.first && r.first < from + n) {
+            sh[32] = s;
+            sh[33] = r.first - from;
+        }
+        __syncthreads();
+        if (sh[32] >= 0) {
+            r.request = sh[32];
+            r.offset = sh[33];
+            break;
+        }
+        base += chunk;
+    }
+    return r;
+}

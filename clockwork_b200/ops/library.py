@@ -77,6 +77,10 @@ _SIGNATURES: dict[str, list] = {
     "cw_latent_prepare": [P, I, P, I, I, P, P, P, P, P, I, F, P, P, I, I, I, I, I, I, F, I, I, P, P],
     "cw_latent_attention": [P, P, P, P, P, P, P, I, P, I, I, I, I, I, I, I, F, I, I, P, I, P, P],
     "cw_latent_attention_on_tensor_cores": [I, I],
+    # a cache in 8 bits (csrc/kv_e4m3.cu, csrc/attention_decode_e4m3.cu)
+    "cw_norm_rotate_store": [P, P, P, P, P, P, P, P, P, P, P, I, I, I, I, I, I, I, F, I, P, P],
+    "cw_read_pages": [P, P, P, P, P, P, P, P, P, I, I, I, I, I, I, I, I, I, I, P, P],
+    "cw_attention_decode_e4m3": [P, I, P, P, P, P, P, P, P, P, I, I, I, I, I, I, I, I, F, I, P, P],
 }
 _OPTIONAL: dict[str, list] = {}
 

@@ -1,0 +1,299 @@
+"""Python faces of the kernels of a cache that holds keys and values in 8 bits (``csrc/kv_e4m3.cu``,
+``csrc/attention_decode_e4m3.cu``), and of the write into a cache behind norms of the query and key heads.
+
+A cached row (one token's key or value in one KV head) is e4m3 codes and one power of two: entry = code * 2^(E - 127), E the
+smallest that keeps the row's largest magnitude within 448.  Held entries are bfloat16 numbers, so reading them back in
+bfloat16 rounds nothing.  Magnitudes beyond 1.875 * 2^127, infinities among them, are held as that; NaN is held as NaN.
+
+Like the package's other ops, the calls run on the current stream of the current device, which must be the tensors' own, report
+page and slot numbers outside the pool into ``status`` (``ops.raise_on_status``) and may be captured in CUDA graphs.
+"""
+
+from __future__ import annotations
+
+from typing import NamedTuple
+
+import torch
+
+from . import _ptr, _stream, dtype_code
+from .library import check, library
+
+CODES = torch.float8_e4m3fn
+MAX_HEAD_DIM = 256
+
+
+class PlainPages(NamedTuple):
+    """One layer's cache in the run's own type: [pages, page_size, nkv, hd] each."""
+
+    k: torch.Tensor
+    v: torch.Tensor
+
+
+class E4M3Pages(NamedTuple):
+    """One layer's cache in 8 bits: codes ``torch.float8_e4m3fn`` [pages, page_size, nkv, hd], powers uint8 [pages, nkv, page_size]."""
+
+    k: torch.Tensor
+    v: torch.Tensor
+    k_exp: torch.Tensor
+    v_exp: torch.Tensor
+
+
+def allocate_pages(num_pages: int, page_size: int, num_kv_heads: int, head_dim: int, device) -> E4M3Pages:
+    """An empty cache of one layer (every entry 0)."""
+    codes = torch.zeros(2, num_pages, page_size, num_kv_heads, head_dim, dtype=torch.uint8, device=device).view(CODES)
+    exps = torch.zeros(2, num_pages, num_kv_heads, page_size, dtype=torch.uint8, device=device)
+    return E4M3Pages(codes[0], codes[1], exps[0], exps[1])
+
+
+def _check_device(t: torch.Tensor) -> None:
+    if not t.is_cuda:
+        raise ValueError("the tensors must be CUDA tensors (no CPU path exists)")
+    if t.get_device() != torch.cuda.current_device():
+        raise ValueError(f"the tensors are on {t.device}, the current device is cuda:{torch.cuda.current_device()}")
+
+
+def _same_place(device: torch.device, **tensors) -> None:
+    for name, t in tensors.items():
+        if t is not None and t.device != device:
+            raise ValueError(f"{name} is on {t.device}, expected {device}")
+
+
+def _ints(t: torch.Tensor, name: str, ndim: int, entries: int | None = None) -> None:
+    if t.dtype != torch.int32 or t.dim() != ndim or not t.is_contiguous():
+        raise ValueError(f"{name} must be a contiguous int32 tensor of {ndim} dimension(s)")
+    if entries is not None and t.shape[0] != entries:
+        raise ValueError(f"{name} must have {entries} entries, got {t.shape[0]}")
+
+
+def _check_status(status: torch.Tensor) -> None:
+    if status.dtype != torch.int32 or status.numel() < 4:
+        raise ValueError("status must be 4 int32 words (ops.new_status)")
+
+
+def check_pages(cache: E4M3Pages) -> None:
+    """Refuses codes and powers whose types, shapes or layouts do not belong together."""
+    if not isinstance(cache, E4M3Pages):
+        raise ValueError(f"an 8-bit cache (E4M3Pages) is needed, got {type(cache).__name__}")
+    k, v, ke, ve = cache
+    if k.dtype != CODES or v.dtype != CODES or ke.dtype != torch.uint8 or ve.dtype != torch.uint8:
+        raise ValueError("codes must be float8_e4m3fn and powers uint8")
+    if k.dim() != 4 or k.shape != v.shape or ke.shape != ve.shape or tuple(ke.shape) != (k.shape[0], k.shape[2], k.shape[1]):
+        raise ValueError(f"codes {tuple(k.shape)}, {tuple(v.shape)} and powers {tuple(ke.shape)}, {tuple(ve.shape)} do not belong together: "
+                         "[pages, page_size, nkv, hd] and [pages, nkv, page_size]")
+    if not (k.is_contiguous() and v.is_contiguous() and ke.is_contiguous() and ve.is_contiguous()):
+        raise ValueError("codes and powers must be contiguous")
+    if k.shape[0] * k.shape[1] >= 1 << 31:
+        raise ValueError("a cache holds fewer than 2^31 slots")
+    if (k.data_ptr() | v.data_ptr()) % 16:
+        raise ValueError("codes must start at a multiple of 16 bytes")
+    if not k.device == v.device == ke.device == ve.device:
+        raise ValueError("codes and powers must be on one device")
+
+
+def _check_heads(cache, num_kv_heads: int, head_dim: int) -> None:
+    if tuple(cache.k.shape[2:]) != (num_kv_heads, head_dim):
+        raise ValueError(f"the cache holds {tuple(cache.k.shape[2:])} KV heads and entries, expected {(num_kv_heads, head_dim)}")
+
+
+def norm_rotate_store(qkv: torch.Tensor, positions: torch.Tensor, slots: torch.Tensor, inv_freq: torch.Tensor | None, cache,
+                      num_heads: int, num_kv_heads: int, head_dim: int, status: torch.Tensor, *,
+                      q_weight: torch.Tensor | None = None, k_weight: torch.Tensor | None = None, eps: float = 0.0) -> torch.Tensor:
+    """What lies between the [q | k | v] product and attention, in one pass: ``qkv`` [N, (nh + 2 nkv) hd] (float32 or bfloat16;
+    left as it is), RMS norms of every query and key head with float32 ``q_weight``, ``k_weight`` [hd] (None: not normed), the
+    rotation of each head's leading ``2 * len(inv_freq)`` entries by ``positions`` (None: none turn; entry j pairs with
+    j + len(inv_freq)), and the write of k and v at ``slots`` (< 0: not stored) of ``cache`` (``E4M3Pages``, or ``PlainPages``
+    of qkv's type).  Returns q [N, nh * hd].  Everything up to the one rounding of each output is float32."""
+    code = dtype_code(qkv.dtype)
+    if qkv.dim() != 2 or not qkv.is_contiguous() or qkv.shape[1] != (num_heads + 2 * num_kv_heads) * head_dim:
+        raise ValueError(f"qkv must be contiguous [N, (nh + 2 nkv) * hd], got {tuple(qkv.shape)}")
+    if not 0 < head_dim <= MAX_HEAD_DIM:
+        raise ValueError(f"head_dim {head_dim} must be positive and at most {MAX_HEAD_DIM}")
+    n = qkv.shape[0]
+    _ints(positions, "positions", 1, n)
+    _ints(slots, "slots", 1, n)
+    _check_status(status)
+    quantised = isinstance(cache, E4M3Pages)
+    if quantised:
+        check_pages(cache)
+    elif cache.k.dtype != qkv.dtype or cache.v.dtype != qkv.dtype or cache.k.dim() != 4 or cache.k.shape != cache.v.shape or \
+            not (cache.k.is_contiguous() and cache.v.is_contiguous()):
+        raise ValueError("a plain cache is two contiguous [pages, page_size, nkv, hd] tensors of qkv's type")
+    _check_heads(cache, num_kv_heads, head_dim)
+    rot = 0
+    if inv_freq is not None:
+        if inv_freq.dtype != torch.float32 or inv_freq.dim() != 1 or not inv_freq.is_contiguous():
+            raise ValueError("inv_freq must be a contiguous float32 vector")
+        rot = 2 * inv_freq.shape[0]
+        if rot > head_dim:
+            raise ValueError(f"inv_freq turns {rot} entries of heads of {head_dim}")
+    for name, w in (("q_weight", q_weight), ("k_weight", k_weight)):
+        if w is not None and (w.dtype != torch.float32 or tuple(w.shape) != (head_dim,) or not w.is_contiguous()):
+            raise ValueError(f"{name} must be contiguous float32 [{head_dim}]")
+    _same_place(qkv.device, positions=positions, slots=slots, inv_freq=inv_freq, q_weight=q_weight, k_weight=k_weight,
+                cache=cache.k, values=cache.v, status=status)
+    _check_device(qkv)
+    q = torch.empty((n, num_heads * head_dim), dtype=qkv.dtype, device=qkv.device)
+    check(library().cw_norm_rotate_store(
+        _ptr(qkv), _ptr(q), _ptr(positions), _ptr(slots), _ptr(inv_freq) if rot else None, _ptr(q_weight), _ptr(k_weight), _ptr(cache.k),
+        _ptr(cache.v), _ptr(cache.k_exp) if quantised else None, _ptr(cache.v_exp) if quantised else None, n, num_heads, num_kv_heads,
+        head_dim, rot, cache.k.shape[1], cache.k.shape[0], float(eps), code, _ptr(status), _stream()), "norm_rotate_store")
+    return q
+
+
+READ_BLOCKS = 148 * 4
+
+
+def read_pages(cache: E4M3Pages, block_tables: torch.Tensor, ctx_lens: torch.Tensor, out_k: torch.Tensor, out_v: torch.Tensor,
+               status: torch.Tensor, *, window: int | None = None, q_start: torch.Tensor | None = None, skip_single: bool = False) -> None:
+    """The keys and values of positions [0, ctx_lens[s]) of every request, through ``block_tables`` [S, max_blocks], into plain
+    pages ``out_k``, ``out_v`` [pages, page_size, nkv, hd] (float32 or bfloat16) at the same pages and slots.  What is left of a
+    request's last page becomes zero; no other page is touched.  ``window``: from the page on that a query at the request's last
+    position sees with that window.  ``q_start`` [S + 1] (the rows that the requests bring to a step): only requests that bring
+    rows are read (``skip_single``: more than one row), and the window is that of their first row."""
+    check_pages(cache)
+    for name, t in (("out_k", out_k), ("out_v", out_v)):
+        if t.shape != cache.k.shape or not t.is_contiguous() or t.dtype != out_k.dtype or t.data_ptr() % 16:
+            raise ValueError(f"{name} must be contiguous, like the codes in shape, 16-byte aligned and of one type with the other")
+    _ints(block_tables, "block_tables", 2)
+    s = block_tables.shape[0]
+    _ints(ctx_lens, "ctx_lens", 1, s)
+    if q_start is not None:
+        _ints(q_start, "q_start", 1, s + 1)
+    if cache.k.shape[3] % 16:
+        raise ValueError(f"head_dim {cache.k.shape[3]} must be a multiple of 16")
+    if window is not None and window <= 0:
+        raise ValueError("window must be positive or None")
+    _check_status(status)
+    _same_place(cache.k.device, out_k=out_k, out_v=out_v, block_tables=block_tables, ctx_lens=ctx_lens, q_start=q_start, status=status)
+    _check_device(cache.k)
+    pages, page_size, nkv, hd = cache.k.shape
+    check(library().cw_read_pages(_ptr(cache.k), _ptr(cache.v), _ptr(cache.k_exp), _ptr(cache.v_exp), _ptr(out_k), _ptr(out_v),
+                                  _ptr(block_tables), _ptr(ctx_lens), _ptr(q_start), s, nkv, hd, page_size, block_tables.shape[1], pages,
+                                  int(window or 0), 2 if skip_single else 1, READ_BLOCKS, dtype_code(out_k.dtype), _ptr(status), _stream()), "read_pages")
+
+
+def attention_decode(q: torch.Tensor, cache: E4M3Pages, block_tables: torch.Tensor, ctx_lens: torch.Tensor, num_heads: int,
+                     scale: float, status: torch.Tensor, *, window: int | None = None, q_start: torch.Tensor | None = None,
+                     out: torch.Tensor | None = None) -> torch.Tensor:
+    """One query token per request over an 8-bit cache: ``q`` [S, >= nh * hd] (float32 or bfloat16, unit column stride; row s
+    belongs to request s), ``ctx_lens`` [S] the tokens of each request in the cache, its own included.  ``window``: a request sees
+    its last ``window`` tokens only.  Returns [S, nh * hd]; a request of no tokens gets zeros.
+
+    ``q_start`` (int32 [S + 1]) with ``out`` ([N, nh * hd]): the requests are those of a flat batch of N rows that also holds
+    prompt portions; only requests with exactly one row are served, the others' rows are left alone."""
+    code = dtype_code(q.dtype)
+    check_pages(cache)
+    pages, page_size, nkv, hd = cache.k.shape
+    if q.dim() != 2 or q.shape[1] < num_heads * hd or q.stride(1) != 1:
+        raise ValueError("q must be [rows, >= nh * hd] with unit column stride")
+    if num_heads <= 0 or num_heads % nkv:
+        raise ValueError(f"num_heads {num_heads} is not a multiple of the cache's {nkv} KV heads")
+    if hd % 16 or hd > MAX_HEAD_DIM:
+        raise ValueError(f"head_dim {hd} must be a multiple of 16, at most {MAX_HEAD_DIM}")
+    _ints(block_tables, "block_tables", 2)
+    s = block_tables.shape[0]
+    _ints(ctx_lens, "ctx_lens", 1, s)
+    if window is not None and window <= 0:
+        raise ValueError("window must be positive or None")
+    _check_status(status)
+    if q_start is not None:
+        _ints(q_start, "q_start", 1, s + 1)
+        if out is None:
+            raise ValueError("a flat batch needs the output tensor")
+    elif q.shape[0] != s:
+        raise ValueError(f"q has {q.shape[0]} rows for {s} requests")
+    if out is None:
+        out = torch.empty((s, num_heads * hd), dtype=q.dtype, device=q.device)
+    elif out.dtype != q.dtype or tuple(out.shape) != (q.shape[0], num_heads * hd) or not out.is_contiguous():
+        raise ValueError("out must be contiguous [rows, nh * hd] of q's type")
+    _same_place(q.device, cache=cache.k, block_tables=block_tables, ctx_lens=ctx_lens, q_start=q_start, out=out, status=status)
+    _check_device(q)
+    stride = q.stride(0) if q.shape[0] > 1 else max(q.stride(0), num_heads * hd)
+    check(library().cw_attention_decode_e4m3(
+        _ptr(q), stride, _ptr(out), _ptr(cache.k), _ptr(cache.v), _ptr(cache.k_exp), _ptr(cache.v_exp), _ptr(block_tables),
+        _ptr(ctx_lens), _ptr(q_start), s, num_heads, nkv, hd, page_size, block_tables.shape[1], pages, int(window or 0), float(scale), code,
+        _ptr(status), _stream()), "attention_decode_e4m3")
+    return out
+
+
+def decode_step(qkv: torch.Tensor, positions: torch.Tensor, slots: torch.Tensor, inv_freq: torch.Tensor | None, cache: E4M3Pages,
+                block_tables: torch.Tensor, ctx_lens: torch.Tensor, num_heads: int, num_kv_heads: int, head_dim: int, scale: float,
+                status: torch.Tensor, *, q_weight: torch.Tensor | None = None, k_weight: torch.Tensor | None = None,
+                eps: float = 0.0, window: int | None = None) -> torch.Tensor:
+    """``norm_rotate_store`` of one new token per request, then ``attention_decode`` of it: what an attention layer does between
+    its two products while every request decodes.  ``ctx_lens`` count the new tokens."""
+    q = norm_rotate_store(qkv, positions, slots, inv_freq, cache, num_heads, num_kv_heads, head_dim, status, q_weight=q_weight,
+                          k_weight=k_weight, eps=eps)
+    return attention_decode(q, cache, block_tables, ctx_lens, num_heads, scale, status, window=window)
+
+
+# ---- prompt portions --------------------------------------------------------------------------------------------------------
+class PortionPlan(NamedTuple):
+    """How the portions of a step are cut into work for ``attention_portions``; made once per step, shared by layers of the same
+    heads."""
+
+    q_lens: tuple
+    ctx_lens: tuple
+    item_seq: torch.Tensor
+    item_q0: torch.Tensor
+    item_split: torch.Tensor | None
+    items: int
+    tok_seq: torch.Tensor
+    positions: torch.Tensor
+
+
+def plan_portions(q_lens, ctx_lens, num_heads: int, num_kv_heads: int, head_dim: int, page_size: int, device) -> PortionPlan:
+    """``q_lens``: the rows that each request brings; ``ctx_lens``: its tokens in the cache with them (both on the host)."""
+    from . import attention_fast as fast
+
+    q_lens, ctx_lens = tuple(int(n) for n in q_lens), tuple(int(c) for c in ctx_lens)
+    if len(q_lens) != len(ctx_lens) or any(n < 0 or c < n for n, c in zip(q_lens, ctx_lens)):
+        raise ValueError("every request has a length and a context that holds its rows")
+    cuts = fast._cuts_for(num_heads, head_dim, page_size)
+    seqs, q0s, words = fast.prefill_work_items(q_lens, ctx_lens, cuts, fast._sm_count(torch.device(device)) if cuts else 0)
+    rows = [(s, c - n + r) for s, (n, c) in enumerate(zip(q_lens, ctx_lens)) for r in range(n)]
+    n = len(seqs)
+    host = torch.tensor(seqs + q0s + words + [r[0] for r in rows] + [r[1] for r in rows], dtype=torch.int32)
+    dev = host.to(device)
+    cut = any(w & 0xFF != 1 for w in words)
+    return PortionPlan(q_lens, ctx_lens, dev[:n], dev[n : 2 * n], dev[2 * n : 3 * n] if cut else None, n, dev[3 * n : 3 * n + len(rows)],
+                       dev[3 * n + len(rows) :])
+
+
+_read_scratch: dict = {}
+_retired_scratch: list = []  # outgrown sets stay: captured graphs may point at them
+
+
+def portion_scratch(cache: E4M3Pages, dtype: torch.dtype) -> PlainPages:
+    """One layer's pages in the run's type, where portions' contexts are read back to; one set per device, type and shape of a
+    row, zero at first, replaced by a larger one when a cache has more pages."""
+    pages, page_size, nkv, hd = cache.k.shape
+    key = (cache.k.get_device(), dtype, page_size, nkv, hd)
+    held = _read_scratch.get(key)
+    if held is None or held.shape[1] < pages:
+        if torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("the scratch pages of attention_portions must exist before a graph is captured: run the step once first")
+        if held is not None:
+            _retired_scratch.append(held)
+        held = _read_scratch[key] = torch.zeros(2, pages, page_size, nkv, hd, dtype=dtype, device=cache.k.device)
+    return PlainPages(held[0, :pages], held[1, :pages])
+
+
+def attention_portions(q: torch.Tensor, cache: E4M3Pages, block_tables: torch.Tensor, q_start: torch.Tensor, ctx_lens: torch.Tensor,
+                       plan: PortionPlan, num_heads: int, scale: float, status: torch.Tensor, *, window: int | None = None) -> torch.Tensor:
+    """Causal attention of prompt portions over an 8-bit cache: ``q`` [N, >= nh * hd]; request s owns rows
+    q_start[s]:q_start[s + 1] and has ctx_lens[s] tokens in the cache, its rows' among them, at the end.  Returns [N, nh * hd]
+    (rows behind the last request's: undefined).  The contexts are read back into scratch pages that calls on a device share:
+    calls that may overlap on the GPU (different streams) must be serialised."""
+    from . import attention_ref
+    from . import attention_fast as fast
+
+    check_pages(cache)
+    _, page_size, nkv, hd = cache.k.shape
+    held = portion_scratch(cache, q.dtype)
+    read_pages(cache, block_tables, ctx_lens, held.k, held.v, status, window=window, q_start=q_start)
+    if q.dtype == torch.bfloat16 and hd in fast.PREFILL_HEAD_DIMS:
+        return fast.attention_prefill(q, held.k, held.v, block_tables, q_start, ctx_lens, plan.item_seq, plan.item_q0, plan.items, num_heads,
+                                      nkv, hd, scale, window, status, item_split=plan.item_split)
+    return attention_ref(q, held.k, held.v, block_tables, plan.tok_seq, plan.positions, num_heads, nkv, hd, scale, window, status, q_start,
+                         list(zip(plan.q_lens, plan.ctx_lens)))

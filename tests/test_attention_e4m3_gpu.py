@@ -1,0 +1,183 @@
+"""Attention over an 8-bit cache, of single tokens and of prompt portions, against float64.  Slots that no request owns hold NaN."""
+
+import pytest
+import torch
+
+from clockwork_b200 import ops
+from clockwork_b200.ops import quantised
+from tests.e4m3_tools import attention, attention_bound, context, filled_pages
+from tests.gpu_tools import DEV
+
+pytestmark = pytest.mark.gpu
+WEIGHT_BITS = 11  # the least that a kernel here holds a weight in: half precision (half a step, 2^-11 of it)
+
+
+def _on(*tensors):
+    return [None if t is None else t.to(DEV) for t in tensors]
+
+
+def _check(out, q, cache, tables, ctx, rows, page, window, scale, dtype, bits=WEIGHT_BITS):
+    """``rows``: (request, first row, rows, position of the first) of what is looked at."""
+    nh, hd = q.shape[1] // cache[0].shape[3], cache[0].shape[3]
+    for s, at, n, first in rows:
+        k, v = (context(cache[i], cache[2 + i], tables[s], ctx[s], page) for i in (0, 1))
+        want, size, score = attention(q[at : at + n].double().view(n, nh, hd), k, v, first, window, scale)
+        got = out[at : at + n].double().cpu().view(n, nh, hd)
+        bound = attention_bound(want, size, score, hd, dtype, bits)
+        finite, worst = bool(got.isfinite().all()), float(((got - want).abs() / bound).max())
+        assert finite and worst <= 1.0, f"request {s}"
+
+
+DECODE = [  # heads, contexts, page size, window
+    ((12, 2, 128), [1], 16, None), ((12, 2, 128), [1024] * 8, 16, None), ((28, 4, 128), [1, 2, 31, 32, 33, 63, 64, 65, 500, 4000], 16, None),
+    ((16, 16, 64), [5, 700, 128], 8, 100), ((9, 3, 32), [77, 3], 32, None), ((16, 1, 64), [900], 64, None), ((24, 2, 128), [300, 4], 16, 33),
+    ((8, 4, 256), [129, 1000], 16, None), ((6, 2, 96), [200, 41], 8, None), ((4, 1, 16), [50, 51], 16, None), ((10, 2, 80), [333], 16, 7),
+    ((3, 1, 160), [90], 5, None), ((48, 2, 64), [257, 12], 16, None), ((40, 1, 192), [260], 16, None), ((32, 2, 256), [70, 513], 16, None),
+    ((2, 2, 112), [19], 3, 1), ((5, 5, 48), [64, 65], 1, None), ((12, 2, 128), [20000, 3, 9000], 16, None)]
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("heads, ctx, page, window", DECODE)
+def test_decode(heads, ctx, page, window, dtype):
+    nh, nkv, hd = heads
+    g = torch.Generator().manual_seed(sum(ctx) + nh * hd)
+    cache, tables = filled_pages(ctx, page, nkv, hd, g)
+    q = (torch.randn(len(ctx), nh * hd, generator=g) * torch.exp(0.5 * torch.randn(len(ctx), 1, generator=g))).to(dtype)
+    status = ops.new_status(DEV)
+    out = quantised.attention_decode(q.to(DEV), quantised.E4M3Pages(*_on(*cache)), *_on(tables, torch.tensor(ctx, dtype=torch.int32)), nh,
+                                     hd**-0.5, status, window=window)
+    ops.raise_on_status(status)
+    assert out.dtype == dtype
+    _check(out, q, cache, tables, ctx, [(s, s, 1, c - 1) for s, c in enumerate(ctx)], page, window, hd**-0.5, dtype)
+
+
+def test_decode_of_empty_contexts_and_many_requests():
+    """Padding rows (contexts of 0) give zeros, also between others and when they are all there is."""
+    nh, nkv, hd, page = 6, 2, 64, 16
+    g = torch.Generator().manual_seed(1)
+    for ctx in ([0], [0, 70, 0, 0, 3, 0], [(i * 7) % 40 for i in range(700)]):
+        cache, tables = filled_pages(ctx, page, nkv, hd, g)
+        q = torch.randn(len(ctx), nh * hd, generator=g).bfloat16()
+        status = ops.new_status(DEV)
+        out = quantised.attention_decode(q.to(DEV), quantised.E4M3Pages(*_on(*cache)), *_on(tables, torch.tensor(ctx, dtype=torch.int32)),
+                                         nh, 0.2, status)
+        ops.raise_on_status(status)
+        assert all((out[s] == 0).all() for s, c in enumerate(ctx) if c == 0)
+        _check(out, q, cache, tables, ctx, [(s, s, 1, c - 1) for s, c in list(enumerate(ctx))[:60] if c], page, None, 0.2, torch.bfloat16)
+
+
+def test_decode_beside_portions():
+    """A flat batch: only requests of one row are served, other rows and rows behind the last request stay as they were; q is a
+    column slice of a wider matrix."""
+    nh, nkv, hd, page = 12, 2, 128, 16
+    ctx, new = [50, 300, 20, 0, 41], [1, 17, 1, 0, 1]
+    g = torch.Generator().manual_seed(2)
+    cache, tables = filled_pages(ctx, page, nkv, hd, g)
+    starts = [sum(new[:i]) for i in range(6)]
+    wide = torch.randn(starts[-1] + 3, nh * hd + 64, generator=g).bfloat16()
+    out = torch.full((wide.shape[0], nh * hd), 5.0, dtype=torch.bfloat16, device=DEV)
+    status = ops.new_status(DEV)
+    got = quantised.attention_decode(wide.to(DEV)[:, : nh * hd], quantised.E4M3Pages(*_on(*cache)),
+                                     *_on(tables, torch.tensor(ctx, dtype=torch.int32)), nh, 0.1, status,
+                                     q_start=torch.tensor(starts, dtype=torch.int32, device=DEV), out=out)
+    ops.raise_on_status(status)
+    assert got is out
+    mine = [starts[s] for s in range(5) if new[s] == 1]
+    rest = [r for r in range(out.shape[0]) if r not in mine]
+    assert (out[rest] == 5.0).all()
+    _check(out, wide[:, : nh * hd].contiguous(), cache, tables, ctx, [(s, starts[s], 1, ctx[s] - 1) for s in (0, 2, 4)], page, None, 0.1, torch.bfloat16)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_decode_of_extreme_rows(dtype):
+    """A sink (a large score on a value of zeros), values of very different sizes, scores that differ by hundreds, keys and values
+    of all zeros, queries near the ends of the type."""
+    nh, nkv, hd, page, c = 4, 1, 64, 16, 200
+    g = torch.Generator().manual_seed(5)
+    (k, v, ke, ve), tables = filled_pages([c] * 3, page, nkv, hd, g, spread=0.2)
+    ids = tables[0].long()
+    v.view(torch.uint8)[ids[0], 3] = 0
+    ve[ids[0], 0, 3] = 127
+    k.view(torch.uint8)[ids[0], 3] = torch.full((hd,), 448.0).to(k.dtype).view(torch.uint8)
+    ke[ids[0], 0, 3] = 127 - 6                      # the sink's key: 7 in every entry
+    ve[ids[2], 0, :] = 127 - 30                     # tiny values
+    ve[ids[3], 0, 0] = 127 + 15                     # a huge one
+    k.view(torch.uint8)[tables[1].long()] = 0       # request 1: all scores 0
+    v.view(torch.uint8)[tables[2, 1].long()] = 0    # request 2: values of zeros among others
+    q = torch.randn(3, nh * hd, generator=g)
+    q[0, :hd] = 3.0
+    q[0, hd : 2 * hd] = -3.0
+    q[2] *= 2.0**-100
+    q[1] *= 2.0**60
+    q = q.to(dtype)
+    cache, status = (k, v, ke, ve), ops.new_status(DEV)
+    out = quantised.attention_decode(q.to(DEV), quantised.E4M3Pages(*_on(*cache)), *_on(tables, torch.full((3,), c, dtype=torch.int32)), nh,
+                                     0.125, status)
+    ops.raise_on_status(status)
+    _check(out, q, cache, tables, [c] * 3, [(s, s, 1, c - 1) for s in range(3)], page, None, 0.125, dtype)
+
+
+def test_decode_reports_pages_outside_the_pool():
+    g = torch.Generator().manual_seed(6)
+    cache, tables = filled_pages([100, 60], 16, 1, 64, g)
+    tables[0, 2], tables[1, 1] = 1000, -1
+    status = ops.new_status(DEV)
+    out = quantised.attention_decode(torch.ones(2, 64, dtype=torch.bfloat16, device=DEV), quantised.E4M3Pages(*_on(*cache)),
+                                     *_on(tables, torch.tensor([100, 60], dtype=torch.int32)), 1, 0.1, status)
+    assert out.isfinite().all()  # (the tokens of such pages count for nothing)
+    with pytest.raises(RuntimeError, match="page id"):
+        ops.raise_on_status(status)
+
+
+PORTIONS = [  # heads, rows of each request, tokens behind them, page size, window
+    ((12, 2, 128), [130], [0], 16, None), ((12, 2, 128), [64, 1, 200], [300, 40, 0], 16, None), ((4, 4, 64), [150, 0, 7], [0, 9, 1000], 8, 60),
+    ((4, 2, 16), [33], [12], 4, None), ((6, 2, 96), [20, 50], [5, 0], 16, None), ((2, 1, 256), [40], [77], 16, None)]
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("heads, new, behind, page, window", PORTIONS)
+def test_portions(heads, new, behind, page, window, dtype):
+    nh, nkv, hd = heads
+    ctx = [a + b for a, b in zip(new, behind)]
+    g = torch.Generator().manual_seed(sum(ctx) + hd)
+    cache, tables = filled_pages(ctx, page, nkv, hd, g)
+    starts = [sum(new[:i]) for i in range(len(new) + 1)]
+    q = torch.randn(starts[-1], nh * hd, generator=g).to(dtype)
+    status = ops.new_status(DEV)
+    plan = quantised.plan_portions(new, ctx, nh, nkv, hd, page, torch.device(DEV))
+    out = quantised.attention_portions(q.to(DEV), quantised.E4M3Pages(*_on(*cache)), *_on(tables, torch.tensor(starts, dtype=torch.int32),
+                                       torch.tensor(ctx, dtype=torch.int32)), plan, nh, hd**-0.5, status, window=window)
+    ops.raise_on_status(status)
+    # (the bfloat16 kernels hold a weight in that type: half a step, 2^-8 of it)
+    _check(out, q, cache, tables, ctx, [(s, starts[s], n, ctx[s] - n) for s, n in enumerate(new) if n], page, window, hd**-0.5, dtype,
+           8 if dtype == torch.bfloat16 else 24)
+
+
+@pytest.mark.parametrize("norm", [False, True])
+def test_a_request_from_its_prompt_on(norm):
+    """The operators as a layer uses them: a prompt's portions stored and attended, then single tokens; every row against float64
+    attention over what the cache holds by then."""
+    nh, nkv, hd, page, dtype = 12, 2, 128, 16, torch.bfloat16
+    g = torch.Generator().manual_seed(7)
+    cache = quantised.allocate_pages(12, page, nkv, hd, DEV)
+    status = ops.new_status(DEV)
+    tables = torch.randperm(12, generator=g)[:8].to(torch.int32)[None]
+    freq = (10000.0 ** -(torch.arange(0, hd, 2).double() / hd)).float().to(DEV)
+    w = [1.0 + 0.2 * torch.randn(hd, generator=g).to(DEV) if norm else None for _ in range(2)]
+    done = 0
+    for n in (40, 37, 1, 1, 1, 1):
+        qkv = torch.randn(n, (nh + 2 * nkv) * hd, generator=g).to(dtype).to(DEV)
+        at = torch.arange(done, done + n, dtype=torch.int32)
+        slots = tables[0, (at // page).long()] * page + at % page
+        done += n
+        ctx = torch.tensor([done], dtype=torch.int32, device=DEV)
+        args = dict(q_weight=w[0], k_weight=w[1], eps=1e-6)
+        q = quantised.norm_rotate_store(qkv, at.to(DEV), slots.to(DEV), freq, cache, nh, nkv, hd, status, **args)
+        if n > 1:
+            plan = quantised.plan_portions([n], [done], nh, nkv, hd, page, torch.device(DEV))
+            out = quantised.attention_portions(q, cache, tables.to(DEV), torch.tensor([0, n], dtype=torch.int32, device=DEV), ctx, plan, nh,
+                                               0.09, status)
+        else:
+            out = quantised.decode_step(qkv, at.to(DEV), slots.to(DEV), freq, cache, tables.to(DEV), ctx, nh, nkv, hd, 0.09, status, **args)
+        ops.raise_on_status(status)
+        _check(out, q.cpu(), tuple(t.cpu() for t in cache), tables, [done], [(0, 0, n, done - n)], page, None, 0.09, dtype, 8 if n > 1 else WEIGHT_BITS)

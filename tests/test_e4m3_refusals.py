@@ -1,0 +1,98 @@
+"""What the operators of the 8-bit cache refuse, on the CPU: everything is looked at before the device is."""
+
+import pytest
+import torch
+
+from clockwork_b200.ops import quantised
+from tests.e4m3_tools import CODES, filled_pages, nearest_codes, quantise
+
+
+def _args(n=3, nh=4, nkv=2, hd=32, page=8, pages=4, dtype=torch.bfloat16):
+    cache = quantised.E4M3Pages(torch.zeros(pages, page, nkv, hd).to(CODES), torch.zeros(pages, page, nkv, hd).to(CODES),
+                                torch.zeros(pages, nkv, page, dtype=torch.uint8), torch.zeros(pages, nkv, page, dtype=torch.uint8))
+    ints = torch.zeros(n, dtype=torch.int32)
+    return dict(qkv=torch.zeros(n, (nh + 2 * nkv) * hd, dtype=dtype), positions=ints, slots=ints.clone(), inv_freq=torch.ones(hd // 2), cache=cache,
+                num_heads=nh, num_kv_heads=nkv, head_dim=hd, status=torch.zeros(4, dtype=torch.int32))
+
+
+STORE = [
+    (dict(qkv=torch.zeros(3, 256, dtype=torch.float16)), "dtype"), (dict(qkv=torch.zeros(3, 250, dtype=torch.bfloat16)), "qkv"),
+    (dict(qkv=torch.zeros(256, 3, dtype=torch.bfloat16).T), "qkv"), (dict(positions=torch.zeros(3)), "positions"),
+    (dict(positions=torch.zeros(2, dtype=torch.int32)), "positions"), (dict(slots=torch.zeros(3, dtype=torch.int64)), "slots"),
+    (dict(inv_freq=torch.ones(17)), "turns"), (dict(inv_freq=torch.ones(16, dtype=torch.float64)), "inv_freq"),
+    (dict(q_weight=torch.ones(31)), "q_weight"), (dict(k_weight=torch.ones(32, dtype=torch.bfloat16)), "k_weight"),
+    (dict(num_kv_heads=1, num_heads=6), "KV heads"), (dict(status=torch.zeros(3, dtype=torch.int32)), "status"),
+    (dict(cache=quantised.PlainPages(torch.zeros(4, 8, 2, 32), torch.zeros(4, 8, 2, 32))), "plain cache"),
+    (dict(head_dim=512, num_kv_heads=0, num_heads=0, qkv=torch.zeros(3, 0, dtype=torch.bfloat16)), "head_dim"), ({}, "CUDA")]
+
+
+@pytest.mark.parametrize("change, words", STORE)
+def test_store_refuses(change, words):
+    with pytest.raises(ValueError, match=words):
+        quantised.norm_rotate_store(**{**_args(), **change})
+
+
+def _bad_caches():
+    c = _args()["cache"]
+    yield c._replace(k=c.k.float()), "float8"
+    yield c._replace(v_exp=c.v_exp.to(torch.int8)), "uint8"
+    yield c._replace(k_exp=torch.zeros(4, 8, 2, dtype=torch.uint8)), "belong"
+    yield c._replace(v=torch.zeros(4, 8, 2, 16).to(CODES)), "belong"
+    yield c._replace(k=torch.zeros(4, 2, 8, 32).to(CODES).transpose(1, 2)), "contiguous"
+    yield quantised.PlainPages(c.k, c.v), "8-bit cache"
+
+
+@pytest.mark.parametrize("cache, words", list(_bad_caches()))
+def test_caches_that_do_not_fit_together_are_refused(cache, words):
+    with pytest.raises(ValueError, match=words):
+        quantised.attention_decode(torch.zeros(3, 128, dtype=torch.bfloat16), cache, torch.zeros(3, 2, dtype=torch.int32),
+                                   torch.zeros(3, dtype=torch.int32), 4, 1.0, torch.zeros(4, dtype=torch.int32))
+
+
+DECODE = [(dict(q=torch.zeros(3, 100, dtype=torch.bfloat16)), "q must"), (dict(q=torch.zeros(4, 128, dtype=torch.bfloat16)), "rows"),
+          (dict(num_heads=3), "multiple"), (dict(num_heads=0), "multiple"), (dict(window=0), "window"), (dict(ctx_lens=torch.zeros(2, dtype=torch.int32)), "ctx_lens"),
+          (dict(block_tables=torch.zeros(3, 2, dtype=torch.int64)), "block_tables"), (dict(q_start=torch.zeros(4, dtype=torch.int32)), "output"),
+          (dict(out=torch.zeros(3, 128)), "out"), (dict(q=torch.zeros(3, 256, dtype=torch.bfloat16)[:, ::2]), "stride"), ({}, "CUDA")]
+
+
+@pytest.mark.parametrize("change, words", DECODE)
+def test_decode_refuses(change, words):
+    args = dict(q=torch.zeros(3, 128, dtype=torch.bfloat16), cache=_args()["cache"], block_tables=torch.zeros(3, 2, dtype=torch.int32),
+                ctx_lens=torch.zeros(3, dtype=torch.int32), num_heads=4, scale=1.0, status=torch.zeros(4, dtype=torch.int32))
+    with pytest.raises(ValueError, match=words):
+        quantised.attention_decode(**{**args, **change})
+
+
+READ = [(dict(out_k=torch.zeros(4, 8, 2, 16)), "out_k"), (dict(out_v=torch.zeros(4, 8, 2, 32, dtype=torch.bfloat16)), "out_v"), (dict(window=-1), "window"),
+        (dict(q_start=torch.zeros(3, dtype=torch.int32)), "q_start"), (dict(status=torch.zeros(4)), "status"), ({}, "CUDA")]
+
+
+@pytest.mark.parametrize("change, words", READ)
+def test_read_refuses(change, words):
+    args = dict(cache=_args()["cache"], block_tables=torch.zeros(3, 2, dtype=torch.int32), ctx_lens=torch.zeros(3, dtype=torch.int32),
+                out_k=torch.zeros(4, 8, 2, 32), out_v=torch.zeros(4, 8, 2, 32), status=torch.zeros(4, dtype=torch.int32))
+    with pytest.raises(ValueError, match=words):
+        quantised.read_pages(**{**args, **change})
+
+
+def test_plans_of_impossible_portions_are_refused():
+    with pytest.raises(ValueError, match="context"):
+        quantised.plan_portions([3, 2], [5, 1], 4, 2, 32, 8, "cpu")
+    with pytest.raises(ValueError, match="context"):
+        quantised.plan_portions([3], [5, 1], 4, 2, 32, 8, "cpu")
+
+
+def test_the_oracle_rounds_as_the_type_does():
+    x = torch.cat([torch.linspace(-448, 448, 4097).double(), torch.ldexp(torch.linspace(1, 2, 65).double(), torch.tensor(-9))])
+    assert torch.equal(nearest_codes(x), x.float().to(CODES).double())
+
+
+def test_the_oracle_holds_rows_within_half_a_step():
+    g = torch.Generator().manual_seed(1)
+    x = torch.randn(200, 64, generator=g) * torch.exp(3 * torch.randn(200, 1, generator=g))
+    codes, e = quantise(x)
+    unit = torch.exp2(e.double() - 127)[:, None]
+    assert ((codes.double() * unit - x.double()).abs() <= torch.maximum(2.0**-4 * x.double().abs(), 2.0**-10 * unit)).all()
+    assert (codes.double().abs().amax(1) > 216).all()  # no power is larger than it has to be (224, rounded)
+    cache, tables = filled_pages([9, 0, 3], 4, 2, 16, g)
+    assert tables.shape == (3, 3) and (tables[1] == -1).all() and cache[0].dtype == CODES

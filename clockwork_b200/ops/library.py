@@ -80,7 +80,8 @@ _SIGNATURES: dict[str, list] = {
     # a cache in 8 bits (csrc/kv_e4m3.cu, csrc/attention_decode_e4m3.cu)
     "cw_norm_rotate_store": [P, P, P, P, P, P, P, P, P, P, P, I, I, I, I, I, I, I, F, I, P, P],
     "cw_read_pages": [P, P, P, P, P, P, P, P, P, I, I, I, I, I, I, I, I, I, I, P, P],
-    "cw_attention_decode_e4m3": [P, I, P, P, P, P, P, P, P, P, I, I, I, I, I, I, I, I, F, I, P, P],
+    "cw_attention_decode_e4m3": [P, I, P, P, P, P, P, P, P, P, I, I, I, I, I, I, I, I, F, I, I, P, P, P, P],
+    "cw_attention_decode_e4m3_scratch": [I, I, I, I, I, I, P, P],
 }
 _OPTIONAL: dict[str, list] = {}
 

@@ -11,6 +11,8 @@ page and slot numbers outside the pool into ``status`` (``ops.raise_on_status``)
 
 from __future__ import annotations
 
+import ctypes
+import functools
 from typing import NamedTuple
 
 import torch
@@ -172,15 +174,63 @@ def read_pages(cache: E4M3Pages, block_tables: torch.Tensor, ctx_lens: torch.Ten
                                   int(window or 0), 2 if skip_single else 1, READ_BLOCKS, dtype_code(out_k.dtype), _ptr(status), _stream()), "read_pages")
 
 
+class DecodeWorkspace:
+    """Scratch of ``attention_decode`` for up to ``requests`` requests of these heads: partial results (of a size that goes by the
+    GPU alone) and counters that are zero between calls.  Calls that may overlap on the GPU must not share one."""
+
+    def __init__(self, requests: int, num_heads: int, num_kv_heads: int, head_dim: int, device) -> None:
+        floats, words = _scratch_sizes(requests, num_heads, num_kv_heads, head_dim, _sms(device))
+        self.floats = torch.empty(floats, dtype=torch.float32, device=device)
+        self.words = torch.zeros(words, dtype=torch.int32, device=device)
+
+
+def _sms(device) -> int:
+    from . import attention_fast
+
+    return attention_fast._sm_count(torch.device(device))
+
+
+@functools.lru_cache(maxsize=256)
+def _scratch_sizes(requests: int, num_heads: int, num_kv_heads: int, head_dim: int, sms: int) -> tuple[int, int]:
+    floats, words = ctypes.c_longlong(0), ctypes.c_int(0)
+    check(library().cw_attention_decode_e4m3_scratch(requests, num_heads, num_kv_heads, head_dim, 1, sms, ctypes.addressof(floats),
+                                                     ctypes.addressof(words)), "attention_decode_e4m3_scratch")
+    return floats.value, words.value
+
+
+_workspaces: dict = {}  # (device, stream) -> the scratch of calls that bring none
+
+
+def _workspace(workspace: DecodeWorkspace | None, requests: int, num_heads: int, num_kv_heads: int, head_dim: int, device: torch.device,
+               stream: int, sms: int) -> DecodeWorkspace:
+    """The caller's workspace, or the one of the current stream, replaced by a larger one when a call needs more.  A call that is being
+    captured and brings none gets one of its own in the graph's memory, cleared at every replay: graphs may be replayed on any
+    stream."""
+    floats, words = _scratch_sizes(requests, num_heads, num_kv_heads, head_dim, sms)
+    if workspace is not None:
+        if workspace.floats.numel() < floats or workspace.words.numel() < words or workspace.floats.device != device:
+            raise ValueError("the workspace was made for fewer requests, other heads or another device")
+        return workspace
+    if torch.cuda.is_current_stream_capturing():
+        return DecodeWorkspace(requests, num_heads, num_kv_heads, head_dim, device)
+    held = _workspaces.get((device.index, stream))
+    if held is None or held.floats.numel() < floats or held.words.numel() < words:
+        held = _workspaces[device.index, stream] = DecodeWorkspace(max(requests, 256), num_heads, num_kv_heads, max(head_dim, 128), device)
+        if held.words.numel() < words or held.floats.numel() < floats:  # (heads of 128 come in other groups than larger ones)
+            held = _workspaces[device.index, stream] = DecodeWorkspace(requests, num_heads, num_kv_heads, head_dim, device)
+    return held
+
+
 def attention_decode(q: torch.Tensor, cache: E4M3Pages, block_tables: torch.Tensor, ctx_lens: torch.Tensor, num_heads: int,
                      scale: float, status: torch.Tensor, *, window: int | None = None, q_start: torch.Tensor | None = None,
-                     out: torch.Tensor | None = None) -> torch.Tensor:
+                     out: torch.Tensor | None = None, workspace: DecodeWorkspace | None = None) -> torch.Tensor:
     """One query token per request over an 8-bit cache: ``q`` [S, >= nh * hd] (float32 or bfloat16, unit column stride; row s
     belongs to request s), ``ctx_lens`` [S] the tokens of each request in the cache, its own included.  ``window``: a request sees
     its last ``window`` tokens only.  Returns [S, nh * hd]; a request of no tokens gets zeros.
 
     ``q_start`` (int32 [S + 1]) with ``out`` ([N, nh * hd]): the requests are those of a flat batch of N rows that also holds
-    prompt portions; only requests with exactly one row are served, the others' rows are left alone."""
+    prompt portions; only requests with exactly one row are served, the others' rows are left alone.  ``workspace``: the call's scratch (default:
+    one per stream)."""
     code = dtype_code(q.dtype)
     check_pages(cache)
     pages, page_size, nkv, hd = cache.k.shape
@@ -209,22 +259,24 @@ def attention_decode(q: torch.Tensor, cache: E4M3Pages, block_tables: torch.Tens
     _same_place(q.device, cache=cache.k, block_tables=block_tables, ctx_lens=ctx_lens, q_start=q_start, out=out, status=status)
     _check_device(q)
     stride = q.stride(0) if q.shape[0] > 1 else max(q.stride(0), num_heads * hd)
+    stream, sms = _stream(), _sms(q.device)
+    scratch = _workspace(workspace, s, num_heads, nkv, hd, q.device, stream, sms) if code == 1 and hd % 32 == 0 else None
     check(library().cw_attention_decode_e4m3(
         _ptr(q), stride, _ptr(out), _ptr(cache.k), _ptr(cache.v), _ptr(cache.k_exp), _ptr(cache.v_exp), _ptr(block_tables),
-        _ptr(ctx_lens), _ptr(q_start), s, num_heads, nkv, hd, page_size, block_tables.shape[1], pages, int(window or 0), float(scale), code,
-        _ptr(status), _stream()), "attention_decode_e4m3")
+        _ptr(ctx_lens), _ptr(q_start), s, num_heads, nkv, hd, page_size, block_tables.shape[1], pages, int(window or 0), float(scale), code, sms,
+        scratch and scratch.floats.data_ptr(), scratch and scratch.words.data_ptr(), _ptr(status), stream), "attention_decode_e4m3")
     return out
 
 
 def decode_step(qkv: torch.Tensor, positions: torch.Tensor, slots: torch.Tensor, inv_freq: torch.Tensor | None, cache: E4M3Pages,
                 block_tables: torch.Tensor, ctx_lens: torch.Tensor, num_heads: int, num_kv_heads: int, head_dim: int, scale: float,
                 status: torch.Tensor, *, q_weight: torch.Tensor | None = None, k_weight: torch.Tensor | None = None,
-                eps: float = 0.0, window: int | None = None) -> torch.Tensor:
+                eps: float = 0.0, window: int | None = None, workspace: DecodeWorkspace | None = None) -> torch.Tensor:
     """``norm_rotate_store`` of one new token per request, then ``attention_decode`` of it: what an attention layer does between
     its two products while every request decodes.  ``ctx_lens`` count the new tokens."""
     q = norm_rotate_store(qkv, positions, slots, inv_freq, cache, num_heads, num_kv_heads, head_dim, status, q_weight=q_weight,
                           k_weight=k_weight, eps=eps)
-    return attention_decode(q, cache, block_tables, ctx_lens, num_heads, scale, status, window=window)
+    return attention_decode(q, cache, block_tables, ctx_lens, num_heads, scale, status, window=window, workspace=workspace)
 
 
 # ---- prompt portions --------------------------------------------------------------------------------------------------------

@@ -6,10 +6,10 @@
 //
 // The step is a stream of codes from memory, 2 (hd + 1) bytes per token and KV head, so all query heads of a KV head (16 at
 // most, or 8) share what a block fetches.  Work is cut by the contexts themselves: requests, KV heads and tiles of 32 tokens
-// are numbered through, and every block of a grid that fills the SMs once takes an equal run of tiles, wherever requests begin
-// and end in it (units_of_block); so contexts of any lengths fill the GPU, and no scratch grows with them.  A run's tiles go to
-// four warps in turn.  Each warp has a ring of tiles in shared memory of its own, filled by 16-byte asynchronous copies two or
-// more tiles ahead, so that warps never wait for one another while they stream.
+// are numbered through, and every warp of a grid that fills the SMs once takes an equal run of tiles, wherever requests begin
+// and end in it (units_of_block); so contexts of any lengths fill the GPU, and no scratch grows with them.  Each warp has a ring
+// of tiles in shared memory of its own, filled by 16-byte asynchronous copies two or more tiles ahead and on into the next
+// request, so that warps never wait for one another while they stream.
 //
 // Codes become half-precision numbers exactly (cvt) on their way into mma.sync.m16n8k16, which costs less here than it could
 // save elsewhere: at the rate of memory the tensor cores are a fifth busy.  Tokens are the M side of S^T = K Q^T and the codes'
@@ -23,9 +23,10 @@
 // (11 bits, off by at most 2^-12 of themselves, or by 2^-39 of the largest contribution), and the denominator, float32, sums
 // p_j 2^(127 - Ev_j).  (It overflows, and the result is 0, where a context's values are all below 2^-88.)
 //
-// A segment (request, KV head) that lies in one block's run is finished there; the pieces of one that several blocks share go
-// to scratch of two pieces per block, and the block that comes last merges them in the blocks' order (more than 24: twelve at a time
-// first, each by the last of the twelve).  The result does not depend on who comes last.
+// A segment (request, KV head and group) that lies in one warp's run is finished by it.  At the end of its run a block adds up
+// its warps' pieces of shared segments in order; the pieces of one that several blocks share go to scratch of two per block, and
+// the block that comes last merges them in the blocks' order (more than 24: twelve at a time first, each by the last of the
+// twelve).  The result does not depend on who comes last.
 #include "attention_mma.cuh"
 #include "kv_e4m3.cuh"
 
@@ -39,8 +40,9 @@ struct DecodeE4m3Params {
     // the streaming kernel
     int page_shift;          // log2 of the page size, or -1
     int groups, heads_each;  // groups of query heads per KV head, heads in a group (the last may have fewer)
-    float* part_o;           // [2 * blocks][heads of a group][hd]
-    float* part_ml;          // [2 * blocks][heads of a group][2]
+    float* heads_o;          // [4 * blocks][8 or 16][hd]: ends of segments that an earlier warp began
+    float* part_o;           // [2 * blocks][8 or 16][hd]
+    float* part_ml;          // [2 * blocks][8 or 16][2]
     int* counters;           // [requests * nkv * groups] and [2 * blocks], zero between launches
 };
 
@@ -67,14 +69,15 @@ __device__ __forceinline__ uint32_t half2_of(float a, float b) {
     return *reinterpret_cast<const uint32_t*>(&h);
 }
 
-template <int HD>
+template <int HD, int NT>
 struct Stream {
     static constexpr int CH = HD / 16;                 // 16-byte chunks of a row
     static constexpr int TILE_BYTES = TILE_TOKENS * HD;  // K or V of a tile
-    static constexpr int PER_SM = HD <= 128 ? 2 : 1;   // blocks on an SM
-    static constexpr int FIT = (PER_SM == 2 ? 98304 : 196608) / (WARPS * 2 * TILE_BYTES);
+    static constexpr int PER_SM = HD > 128 ? 1 : NT == 1 ? 3 : 2;  // blocks on an SM (registers: 168, 255)
+    static constexpr int FIT = 196608 / PER_SM / (WARPS * 2 * TILE_BYTES);
     static constexpr int ST = FIT > 8 ? 8 : FIT;       // tiles in a warp's ring
     static constexpr int RING = WARPS * ST * 2 * TILE_BYTES;
+    static constexpr bool SWIZZLED = HD % 128 == 0 || HD == 64;
     // Where chunk c of row r lies.  Rows of 128 bytes and multiples are swizzled so that the reads below (K: two rows' four chunks
     // at a time; V: a chunk of four rows two apart) meet no bank twice; of 64 bytes: the same over lines of two rows.
     static __device__ __forceinline__ int at(int r, int c) {
@@ -82,19 +85,38 @@ struct Stream {
         if (HD == 64) return (r >> 1) * 128 + (((((r & 1) << 2) | c) ^ (((r >> 1) & 3) << 1)) << 4);
         return r * HD + (c << 4);
     }
+    // A lane copies chunks lane, lane + 32, ..  Where the j-th lies, from where the first does: rows of a power of two of chunks.
+    static __device__ __forceinline__ int copied(int first, int j, int lane) {
+        if (HD == 128) return (first ^ ((j & 1) << 6)) + j * 512;
+        if (HD == 256) return (first ^ ((j & 3) << 5)) + j * 512;
+        if (32 % CH == 0) return first + j * 512;
+        const int i = j * 32 + lane;
+        return at(i / CH, i % CH);
+    }
+};
+
+// e4m3 pairs of a word's halves as half-precision pairs
+__device__ __forceinline__ void halves_of(uint32_t word, uint32_t& lo, uint32_t& hi) {
+    asm("{\n\t.reg .b16 a, b;\n\tmov.b32 {a, b}, %2;\n\tcvt.rn.f16x2.e4m3x2 %0, a;\n\tcvt.rn.f16x2.e4m3x2 %1, b;\n\t}" : "=r"(lo), "=r"(hi) : "r"(word));
+}
+
+// A run of tiles through requests and segments: which tile it stands at.
+struct Walk {
+    int s, ctx, begin, tiles;  // the request, its context, the first position it sees, its tiles
+    int seg, tile;             // KV head and group; tile of it
 };
 
 template <int HD, int NT>
-__global__ void __launch_bounds__(WARPS * 32, Stream<HD>::PER_SM) decode_e4m3_kernel(const DecodeE4m3Params p) {
-    using C = Stream<HD>;
-    constexpr int ROWS = 8 * NT, ST = C::ST;
+__global__ void __launch_bounds__(WARPS * 32, Stream<HD, NT>::PER_SM) decode_e4m3_kernel(const DecodeE4m3Params p) {
+    using C = Stream<HD, NT>;
+    constexpr int ROWS = 8 * NT, ST = C::ST, CH = C::CH;
     constexpr int WORDS = HD / 32;  // a thread's 4-byte words of a V row
     extern __shared__ __align__(128) uint8_t ring_s[];
-    __shared__ __align__(16) __half q_s[ROWS][HD + 8];
-    __shared__ float qf_s[ROWS];
-    __shared__ int slot_s[WARPS][ST][TILE_TOKENS];
-    __shared__ uint32_t power_at_s[WARPS][ST][TILE_TOKENS];
-    __shared__ float m_s[WARPS][ROWS], l_s[WARPS][ROWS], w_s[ROWS][WARPS + 2];
+    __shared__ uint32_t row_s[WARPS][ST][TILE_TOKENS];       // 16-byte chunk where a token's row begins; ~0: it does not count
+    __shared__ uint32_t power_at_s[WARPS][ST][TILE_TOKENS];  // where its powers are
+    __shared__ float m_s[2 * WARPS][ROWS], l_s[2 * WARPS][ROWS];
+    __shared__ int piece_s[2 * WARPS][3];  // segment (-1: no such piece), its first unit, its tiles
+    __shared__ float ml_s[ROWS][2];
     __shared__ int sh[36];
     __shared__ int last_s;
     pdl_enter();
@@ -108,389 +130,448 @@ __global__ void __launch_bounds__(WARPS * 32, Stream<HD>::PER_SM) decode_e4m3_ke
     auto tiles_of = [&](int ctx) {
         return ctx <= 0 ? 0 : (ctx + TILE_TOKENS - 1) / TILE_TOKENS - begin_of(ctx) / TILE_TOKENS;
     };
-    const UnitRange range =
-        units_of_block([&](int s) { return per_request * tiles_of(context_of(s)); }, p.requests, WARPS, gridDim.x, blockIdx.x, sh);
+    // (a block's run is a whole number of equal runs for its warps)
+    UnitRange range = units_of_block([&](int s) { return per_request * tiles_of(context_of(s)); }, p.requests, 1, gridDim.x * WARPS,
+                                     blockIdx.x * WARPS, sh);
+    const int block_units = range.quota * WARPS;
     for (int s = blockIdx.x; s < p.requests; s += gridDim.x) {  // rows without a context: zeros
         if (context_of(s) != 0) continue;
         const int row = p.q_start != nullptr ? p.q_start[s] : s;
         for (int i = tid; i < p.nh * HD; i += blockDim.x) ((bf16*)p.out)[(size_t)row * p.nh * HD + i] = __float2bfloat16_rn(0.f);
     }
+    if (range.first >= range.last) return;
+    // ---- where this warp's run begins ----
+    const int first = range.first + warp * range.quota, last = min(range.total, first + range.quota);
+    Walk at = {};
+    auto enter = [&](Walk& w, int s) {  // the next request from s on that has tiles
+        for (; s < p.requests; ++s) {
+            const int ctx = context_of(s), n = tiles_of(ctx);
+            if (n > 0) {
+                w = {s, ctx, begin_of(ctx), n, 0, 0};
+                return;
+            }
+        }
+        w = {p.requests - 1, 0, 0, 0x7FFFFFFF / per_request, 0, 0};  // (lengths that change under the call: tokens that do not count)
+    };
+    auto step = [&](Walk& w, int units, bool more) {  // `units` tiles on within its segment, then on to where the next one is
+        w.tile += units;
+        if (w.tile == w.tiles) {
+            w.tile = 0;
+            if (++w.seg == per_request && more) enter(w, w.s + 1);
+        }
+    };
+    if (first < last) {
+        int skip = range.offset + warp * range.quota;
+        enter(at, range.request);
+        while (skip >= at.tiles * per_request) {
+            skip -= at.tiles * per_request;
+            enter(at, at.s + 1);
+        }
+        at.seg = skip / at.tiles;
+        at.tile = skip - at.seg * at.tiles;
+    }
     uint8_t* my_ring = ring_s + warp * ST * 2 * C::TILE_BYTES;
     const uint32_t my_ring_addr = smem_addr(my_ring);
-    int s = range.request, offset = range.offset;
-    for (int unit = range.first; unit < range.last; ++s, offset = 0) {
-        const int ctx = context_of(s), tiles = tiles_of(ctx);
-        if (tiles <= 0) continue;
-        const int begin = begin_of(ctx), tile_base = begin / TILE_TOKENS;
-        const int row = p.q_start != nullptr ? p.q_start[s] : s;
-        const int* table = p.block_tables + (size_t)s * p.max_blocks;
-        for (int seg = offset / tiles; seg < per_request && unit < range.last; ++seg) {
-            const int seg_first = unit - (offset - seg * tiles);  // the segment's first unit
-            const int ta = offset - seg * tiles, tb = min(tiles, ta + range.last - unit);
-            const int kvh = seg / p.groups, h0 = kvh * (p.nh / p.nkv) + (seg % p.groups) * p.heads_each;
-            const int rows = min(p.heads_each, p.nh / p.nkv - (seg % p.groups) * p.heads_each);
-            unit += tb - ta;
-            offset = (seg + 1) * tiles;
-            // ---- the group's queries in half precision, a power of two out of each ----
-            for (int r = warp; r < ROWS; r += WARPS) {
-                constexpr int E = HD / 32;
-                float x[E], big = 0.f;
-#pragma unroll
-                for (int e = 0; e < E; ++e) {
-                    x[e] = r < rows ? __bfloat162float(((const bf16*)p.q)[(size_t)row * p.q_stride + (size_t)(h0 + r) * HD + e * 32 + lane]) : 0.f;
-                    big = fmaxf(big, fabsf(x[e]));
-                }
-                big = warp_max(big);
-                const int sh_q = big > 0.f ? min(126, 14 - (int)((__float_as_uint(big) >> 23) & 255) + 127) : 0;
-#pragma unroll
-                for (int e = 0; e < E; ++e) q_s[r][e * 32 + lane] = __float2half_rn(ldexpf(x[e], sh_q));
-                if (lane == 0) qf_s[r] = ldexpf(p.scale * 1.4426950408889634f, -sh_q);
+    // ---- fetching: ST - 1 tiles ahead of the products, through the segments' ends ----
+    Walk ahead = at;
+    int to_fetch = max(0, last - first), fetch_stage = 0, ahead_page = -1, ahead_pos = 0;
+    const int copy_lane = C::at(lane / CH, lane % CH);
+    auto look_up = [&]() {  // the page of this lane's token of the tile that is fetched next
+        ahead_page = -1;
+        if (to_fetch <= 0) return;
+        ahead_pos = (ahead.begin / TILE_TOKENS + ahead.tile) * TILE_TOKENS + lane;
+        if (ahead_pos >= ahead.begin && ahead_pos < ahead.ctx)
+            ahead_page = p.block_tables[(size_t)ahead.s * p.max_blocks + (p.page_shift >= 0 ? ahead_pos >> p.page_shift : ahead_pos / p.page_size)];
+    };
+    auto fetch = [&]() {
+        if (to_fetch > 0) {
+            const int kvh = p.groups == 1 ? ahead.seg : ahead.seg / p.groups;
+            uint32_t row = ~0u, power_at = 0;
+            if (ahead_page >= 0 && ahead_page < p.num_pages) {
+                const int off = p.page_shift >= 0 ? ahead_pos & (p.page_size - 1) : ahead_pos % p.page_size;
+                row = ((uint32_t)(ahead_page * p.page_size + off) * p.nkv + kvh) * CH;
+                power_at = ((uint32_t)ahead_page * p.nkv + kvh) * p.page_size + off;
+            } else if (ahead_pos >= ahead.begin && ahead_pos < ahead.ctx) {
+                cw_report(p.status, CW_ST_PAGE_RANGE, ahead.s, ahead_page);
             }
-            __syncthreads();
-            // k-steps of K's 16-byte (or, in rows that are no multiple of 64, 8-byte) pieces: B fragments of the same entries
-            constexpr int PIECE = HD % 64 == 0 ? 16 : 8, STEPS = PIECE / 4, PIECES = HD / (4 * PIECE);
-            uint32_t qb[NT][PIECES][STEPS][2];
+            row_s[warp][fetch_stage][lane] = row;
+            power_at_s[warp][fetch_stage][lane] = power_at;
+            __syncwarp();
+            const uint32_t base = my_ring_addr + fetch_stage * 2 * C::TILE_BYTES;
+#pragma unroll
+            for (int j = 0; j < CH; ++j) {
+                const int i = j * 32 + lane;
+                const uint32_t from = row_s[warp][fetch_stage][32 % CH == 0 ? j * (32 / CH) + lane / CH : i / CH];
+                const bool there = from != ~0u;
+                const size_t src = (size_t)(there ? from + (32 % CH == 0 ? lane % CH : i % CH) : 0u) * 16;
+                const uint32_t dst = base + C::copied(copy_lane, j, lane);
+                copy16(dst, p.k + src, there);
+                copy16(dst + C::TILE_BYTES, p.v + src, there);
+            }
+            if (++fetch_stage == ST) fetch_stage = 0;
+            --to_fetch;
+            step(ahead, 1, to_fetch > 0);
+            look_up();
+        }
+        cp_async_commit();
+    };
+    // a lane looks up the powers of token 8 t + g a tile ahead of their use: K's, V's, and whether the token counts
+    uint32_t k_power = 0, v_power = 0, counts = 0;
+    auto look_at_powers = [&](int stage) {
+        const uint32_t i = power_at_s[warp][stage][8 * t + g];
+        counts = row_s[warp][stage][8 * t + g];
+        k_power = p.k_exp[i];
+        v_power = p.v_exp[i];
+    };
+    look_up();
+    for (int i = 0; i < ST - 1; ++i) fetch();
+    __syncwarp();
+    int unit = first, stage = 0;
+    if (first < last) look_at_powers(0);
+    if (lane < 2) piece_s[2 * warp + lane][0] = -1;
+    // where this lane's K pieces and V words lie in a tile (rows 16 and 8 further: the same swizzle)
+    const int k_at = C::at(g, HD % 64 == 0 ? t : t >> 1) + (HD % 64 == 0 ? 0 : 8 * (t & 1));
+    constexpr int PIECE = HD % 64 == 0 ? 16 : 8, STEPS = PIECE / 4, PIECES = HD / (4 * PIECE);
+    while (unit < last) {
+        const int row = p.q_start != nullptr ? p.q_start[at.s] : at.s;
+        const int part = p.groups == 1 ? 0 : at.seg % p.groups, kvh = p.groups == 1 ? at.seg : at.seg / p.groups;
+        const int h0 = kvh * (p.nh / p.nkv) + part * p.heads_each, rows = min(p.heads_each, p.nh / p.nkv - part * p.heads_each);
+        const int n_tiles = min(at.tiles - at.tile, last - unit);
+        // ---- the group's queries, as B fragments over the entries that a lane's pieces of K hold: half precision, a power of two out ----
+        uint32_t qb[NT][PIECES][STEPS][2];
+        float qf[NT][2], m[NT][2], l[NT][2], o[NT][HD / 16][4];
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+            const bf16* q = (const bf16*)p.q + (size_t)row * p.q_stride + (size_t)(h0 + 8 * n + g) * HD;
+            float big = 0.f;
+#pragma unroll
+            for (int b = 0; b < PIECES; ++b)
+#pragma unroll
+                for (int i = 0; i < STEPS; ++i)
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) {
+                        uint32_t w = 0;
+                        if (8 * n + g < rows) w = *reinterpret_cast<const uint32_t*>(q + b * 4 * PIECE + t * PIECE + 4 * i + 2 * e);
+                        qb[n][b][i][e] = w;
+                        big = fmaxf(big, fmaxf(fabsf(__uint_as_float(w << 16)), fabsf(__uint_as_float(w & 0xFFFF0000u))));
+                    }
+            big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 1));
+            big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 2));
+            const int up = big > 0.f ? min(126, 141 - (int)((__float_as_uint(big) >> 23) & 255)) : 0;  // big becomes 2^14 to 2^15
+            const float by = __int_as_float((127 + up) << 23);  // (-114 <= up <= 126)
+#pragma unroll
+            for (int b = 0; b < PIECES; ++b)
+#pragma unroll
+                for (int i = 0; i < STEPS; ++i)
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) {
+                        const uint32_t w = qb[n][b][i][e];
+                        qb[n][b][i][e] = half2_of(__uint_as_float(w << 16) * by, __uint_as_float(w & 0xFFFF0000u) * by);
+                    }
+            const float back = p.scale * 1.4426950408889634f * __int_as_float((127 - up) << 23);  // of head 8 n + g, lanes 4 g ..
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                qf[n][e] = __shfl_sync(0xffffffffu, back, 4 * (2 * t + e));
+                m[n][e] = -INFINITY;
+                l[n][e] = 0.f;
+            }
+#pragma unroll
+            for (int j = 0; j < HD / 16; ++j) o[n][j][0] = o[n][j][1] = o[n][j][2] = o[n][j][3] = 0.f;
+        }
+        for (int i = 0; i < n_tiles; ++i) {
+            fetch();
+            cp_async_wait<ST - 1>();
+            __syncwarp();
+            const int next = stage + 1 == ST ? 0 : stage + 1;
+            const uint32_t powers = counts == ~0u ? 0u : k_power | v_power << 8 | 1u << 16;
+            if (unit + i + 1 < last) look_at_powers(next);
+            const uint8_t* kt = my_ring + stage * 2 * C::TILE_BYTES;
+            const uint8_t* vt = kt + C::TILE_BYTES;
+            float sc[NT][2][4];
 #pragma unroll
             for (int n = 0; n < NT; ++n)
 #pragma unroll
-                for (int b = 0; b < PIECES; ++b)
+                for (int u = 0; u < 2; ++u) sc[n][u][0] = sc[n][u][1] = sc[n][u][2] = sc[n][u][3] = 0.f;
 #pragma unroll
-                    for (int i = 0; i < STEPS; ++i) {
-                        const uint2 w = *reinterpret_cast<const uint2*>(&q_s[8 * n + g][b * 4 * PIECE + t * PIECE + 4 * i]);
-                        qb[n][b][i][0] = w.x;
-                        qb[n][b][i][1] = w.y;
+            for (int b = 0; b < PIECES; ++b) {
+                const uint8_t* kb = kt + (HD % 128 == 0 ? (k_at ^ ((b & 1) << 6)) + (b >> 1) * 128 : k_at + b * 4 * PIECE);
+#pragma unroll
+                for (int u = 0; u < 2; ++u) {
+                    uint32_t lo[STEPS], hi[STEPS];  // rows g and g + 8
+                    if (PIECE == 16) {
+                        const uint4 x = *reinterpret_cast<const uint4*>(kb + 16 * u * HD), y = *reinterpret_cast<const uint4*>(kb + (16 * u + 8) * HD);
+                        lo[0] = x.x; lo[1] = x.y; lo[STEPS - 2] = x.z; lo[STEPS - 1] = x.w;
+                        hi[0] = y.x; hi[1] = y.y; hi[STEPS - 2] = y.z; hi[STEPS - 1] = y.w;
+                    } else {
+                        const uint2 x = *reinterpret_cast<const uint2*>(kb + 16 * u * HD), y = *reinterpret_cast<const uint2*>(kb + (16 * u + 8) * HD);
+                        lo[0] = x.x; lo[1] = x.y;
+                        hi[0] = y.x; hi[1] = y.y;
                     }
-            float qf[NT][2], m[NT][2], l[NT][2], o[NT][HD / 16][4];
 #pragma unroll
-            for (int n = 0; n < NT; ++n) {
+                    for (int k = 0; k < STEPS; ++k) {
+                        uint32_t a[4];
+                        halves_of(lo[k], a[0], a[2]);
+                        halves_of(hi[k], a[1], a[3]);
 #pragma unroll
-                for (int e = 0; e < 2; ++e) {
-                    qf[n][e] = qf_s[8 * n + 2 * t + e];
-                    m[n][e] = -INFINITY;
-                    l[n][e] = 0.f;
+                        for (int n = 0; n < NT; ++n) mma_half(sc[n][u], a, qb[n][b][k][0], qb[n][b][k][1]);
+                    }
                 }
-#pragma unroll
-                for (int j = 0; j < HD / 16; ++j) o[n][j][0] = o[n][j][1] = o[n][j][2] = o[n][j][3] = 0.f;
             }
-            // ---- this warp's tiles ----
-            const int mine = tb - ta > warp ? (tb - ta - warp + WARPS - 1) / WARPS : 0;
-            auto position = [&](int i) { return (tile_base + ta + warp + i * WARPS) * TILE_TOKENS + lane; };
-            auto page_of = [&](int i) -> int {  // of this lane's token of tile i
-                const int pos = position(i);
-                if (i >= mine || pos < begin || pos >= ctx) return -1;
-                return table[p.page_shift >= 0 ? pos >> p.page_shift : pos / p.page_size];
-            };
-            auto fetch = [&](int i, int page) {
-                if (i < mine) {
-                    const int stage = i % ST, pos = position(i);
-                    int slot = -1;
-                    uint32_t power_at = 0;
-                    if (page >= 0 && page < p.num_pages) {
-                        const int off = p.page_shift >= 0 ? pos & (p.page_size - 1) : pos % p.page_size;
-                        slot = page * p.page_size + off;
-                        power_at = ((uint32_t)page * p.nkv + kvh) * p.page_size + off;
-                    } else if (pos >= begin && pos < ctx) {
-                        cw_report(p.status, CW_ST_PAGE_RANGE, s, page);
-                    }
-                    slot_s[warp][stage][lane] = slot;
-                    power_at_s[warp][stage][lane] = power_at;
-                    __syncwarp();
-                    const uint32_t base = my_ring_addr + stage * 2 * C::TILE_BYTES;
+            // scores of tokens 8 x + g (x = 2 u, 2 u + 1) for heads 2 t, 2 t + 1
+            float vs[4];  // 2^(127 - Ev)
 #pragma unroll
-                    for (int j = 0; j < C::CH; ++j) {
-                        const int idx = j * 32 + lane, r = idx / C::CH, c = idx % C::CH;
-                        const int sl = slot_s[warp][stage][r];
-                        const size_t src = ((size_t)max(sl, 0) * p.nkv + kvh) * HD + c * 16;
-                        copy16(base + C::at(r, c), p.k + src, sl >= 0);
-                        copy16(base + C::TILE_BYTES + C::at(r, c), p.v + src, sl >= 0);
-                    }
-                }
-                cp_async_commit();
-            };
-            // a lane holds the powers of token 8 t + g: K's, V's, and whether the token counts
-            auto powers_of = [&](int i) -> uint32_t {
-                if (i >= mine) return 0;
-                const int token = 8 * t + g, stage = i % ST;
-                if (slot_s[warp][stage][token] < 0) return 0;
-                const uint32_t at = power_at_s[warp][stage][token];
-                return (uint32_t)p.k_exp[at] | (uint32_t)p.v_exp[at] << 8 | 1u << 16;
-            };
-            for (int i = 0; i < ST - 1; ++i) fetch(i, page_of(i));
-            int page_ahead = page_of(ST - 1);
-            __syncwarp();
-            uint32_t powers = powers_of(0);
-            for (int i = 0; i < mine; ++i) {
-                fetch(i + ST - 1, page_ahead);
-                page_ahead = page_of(i + ST);
-                cp_async_wait<ST - 1>();
-                __syncwarp();
-                const uint32_t powers_next = powers_of(i + 1);
-                const uint8_t* kt = my_ring + (i % ST) * 2 * C::TILE_BYTES;
-                const uint8_t* vt = kt + C::TILE_BYTES;
-                float sc[NT][2][4];
+            for (int x = 0; x < 4; ++x) {
+                const uint32_t w = __shfl_sync(0xffffffffu, powers, (lane & ~3) | x);
+                const float kf = kv_up(w & 255), ev = (w >> 16) != 0 ? (float)((int)((w >> 8) & 255) - 127) : -INFINITY;
+                vs[x] = kv_down((w >> 8) & 255);
 #pragma unroll
                 for (int n = 0; n < NT; ++n)
 #pragma unroll
-                    for (int u = 0; u < 2; ++u) sc[n][u][0] = sc[n][u][1] = sc[n][u][2] = sc[n][u][3] = 0.f;
+                    for (int e = 0; e < 2; ++e) sc[n][x >> 1][2 * (x & 1) + e] = fmaf(sc[n][x >> 1][2 * (x & 1) + e] * qf[n][e], kf, ev);
+            }
+            uint32_t pb[NT][2][2];
 #pragma unroll
-                for (int b = 0; b < PIECES; ++b)
+            for (int n = 0; n < NT; ++n) {
+                float keep[2];
 #pragma unroll
-                    for (int u = 0; u < 2; ++u) {
-                        uint32_t lo[STEPS], hi[STEPS];  // rows g and g + 8
-                        if (PIECE == 16) {
-                            const uint4 x = *reinterpret_cast<const uint4*>(kt + C::at(16 * u + g, 4 * b + t));
-                            const uint4 y = *reinterpret_cast<const uint4*>(kt + C::at(16 * u + 8 + g, 4 * b + t));
-                            lo[0] = x.x; lo[1] = x.y; lo[STEPS - 2] = x.z; lo[STEPS - 1] = x.w;
-                            hi[0] = y.x; hi[1] = y.y; hi[STEPS - 2] = y.z; hi[STEPS - 1] = y.w;
-                        } else {
-                            const uint2 x = *reinterpret_cast<const uint2*>(kt + C::at(16 * u + g, 2 * b + (t >> 1)) + 8 * (t & 1));
-                            const uint2 y = *reinterpret_cast<const uint2*>(kt + C::at(16 * u + 8 + g, 2 * b + (t >> 1)) + 8 * (t & 1));
-                            lo[0] = x.x; lo[1] = x.y;
-                            hi[0] = y.x; hi[1] = y.y;
-                        }
+                for (int e = 0; e < 2; ++e) {
+                    float top = fmaxf(fmaxf(sc[n][0][e], sc[n][0][2 + e]), fmaxf(sc[n][1][e], sc[n][1][2 + e]));
 #pragma unroll
-                        for (int k = 0; k < STEPS; ++k) {
-                            const uint32_t a[4] = {kv_half2(lo[k] & 0xFFFF), kv_half2(hi[k] & 0xFFFF), kv_half2(lo[k] >> 16), kv_half2(hi[k] >> 16)};
-#pragma unroll
-                            for (int n = 0; n < NT; ++n) mma_half(sc[n][u], a, qb[n][b][k][0], qb[n][b][k][1]);
-                        }
-                    }
-                // scores of tokens 8 x + g (x = 2 u, 2 u + 1) for heads 2 t, 2 t + 1
-                float vs[4];  // 2^(127 - Ev)
-                {
-                    float ev[4], kf[4];
-                    bool there[4];
-#pragma unroll
-                    for (int x = 0; x < 4; ++x) {
-                        const uint32_t w = __shfl_sync(0xffffffffu, powers, (lane & ~3) | x);
-                        kf[x] = kv_up(w & 255);
-                        ev[x] = (float)((int)((w >> 8) & 255) - 127);
-                        vs[x] = kv_down((w >> 8) & 255);
-                        there[x] = (w >> 16) != 0;
-                    }
-#pragma unroll
-                    for (int n = 0; n < NT; ++n)
-#pragma unroll
-                        for (int u = 0; u < 2; ++u)
-#pragma unroll
-                            for (int e = 0; e < 4; ++e) {
-                                const int x = 2 * u + (e >> 1);
-                                sc[n][u][e] = there[x] ? fmaf(sc[n][u][e] * qf[n][e & 1], kf[x], ev[x]) : -INFINITY;
-                            }
-                }
-                uint32_t pb[NT][2][2];
-#pragma unroll
-                for (int n = 0; n < NT; ++n) {
-                    float keep[2];
-#pragma unroll
-                    for (int e = 0; e < 2; ++e) {
-                        float top = fmaxf(fmaxf(sc[n][0][e], sc[n][0][2 + e]), fmaxf(sc[n][1][e], sc[n][1][2 + e]));
-#pragma unroll
-                        for (int d = 4; d < 32; d <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
-                        const float m_new = fmaxf(m[n][e], top), ref = m_new == -INFINITY ? 0.f : m_new - 14.f;
-                        keep[e] = fast_exp2(m[n][e] - 14.f - ref);
-                        m[n][e] = m_new;
-                        float sum = 0.f;
-#pragma unroll
-                        for (int u = 0; u < 2; ++u)
-#pragma unroll
-                            for (int r = 0; r < 2; ++r) {
-                                const float w = fast_exp2(sc[n][u][2 * r + e] - ref);
-                                sc[n][u][2 * r + e] = w;
-                                sum = fmaf(w, vs[2 * u + r], sum);
-                            }
-                        l[n][e] = fmaf(l[n][e], keep[e], sum);
-                    }
-                    if (__any_sync(0xffffffffu, keep[0] != 1.f || keep[1] != 1.f)) {
-#pragma unroll
-                        for (int j = 0; j < HD / 16; ++j) {
-                            o[n][j][0] *= keep[0]; o[n][j][1] *= keep[1]; o[n][j][2] *= keep[0]; o[n][j][3] *= keep[1];
-                        }
-                    }
+                    for (int d = 4; d < 32; d <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
+                    const float m_new = fmaxf(m[n][e], top), ref = m_new == -INFINITY ? 0.f : m_new - 14.f;
+                    keep[e] = fast_exp2(m[n][e] - 14.f - ref);
+                    m[n][e] = m_new;
+                    float sum = 0.f;
 #pragma unroll
                     for (int u = 0; u < 2; ++u)
 #pragma unroll
-                        for (int r = 0; r < 2; ++r) pb[n][u][r] = transposed(half2_of(sc[n][u][2 * r], sc[n][u][2 * r + 1]));
+                        for (int r = 0; r < 2; ++r) {
+                            const float w = fast_exp2(sc[n][u][2 * r + e] - ref);
+                            sc[n][u][2 * r + e] = w;
+                            sum = fmaf(w, vs[2 * u + r], sum);
+                        }
+                    l[n][e] = fmaf(l[n][e], keep[e], sum);
                 }
-                // O^T += V^T P^T: a thread pairs tokens (2 t, 2 t + 1) and (2 t + 8, 2 t + 9); its words of a row: 16 bytes of every
-                // 128, then 8 of 64 and 4 of 32
+                if (__any_sync(0xffffffffu, keep[0] != 1.f || keep[1] != 1.f)) {
 #pragma unroll
-                for (int u = 0; u < 2; ++u) {
-                    uint32_t w[4][WORDS];
-#pragma unroll
-                    for (int x = 0; x < 4; ++x) {
-                        const int r = 16 * u + 2 * t + (x & 1) + 8 * (x >> 1);
-                        constexpr int W16 = HD / 128;
-#pragma unroll
-                        for (int j = 0; j < W16; ++j) {
-                            const uint4 v = *reinterpret_cast<const uint4*>(vt + C::at(r, 8 * j + g));
-                            w[x][4 * j] = v.x; w[x][4 * j + 1] = v.y; w[x][4 * j + 2] = v.z; w[x][4 * j + 3] = v.w;
-                        }
-                        if (HD % 128 >= 64) {
-                            const uint2 v = *reinterpret_cast<const uint2*>(vt + C::at(r, 8 * W16 + (g >> 1)) + 8 * (g & 1));
-                            w[x][4 * W16] = v.x;
-                            w[x][4 * W16 + 1] = v.y;
-                        }
-                        if (HD % 64 == 32) w[x][WORDS - 1] = *reinterpret_cast<const uint32_t*>(vt + C::at(r, HD / 16 - 2 + (g >> 2)) + 4 * (g & 3));
-                    }
-#pragma unroll
-                    for (int j = 0; j < WORDS; ++j) {
-                        const uint32_t a01 = __byte_perm(w[0][j], w[1][j], 0x5140), a23 = __byte_perm(w[0][j], w[1][j], 0x7362);
-                        const uint32_t b01 = __byte_perm(w[2][j], w[3][j], 0x5140), b23 = __byte_perm(w[2][j], w[3][j], 0x7362);
-                        const uint32_t even[4] = {kv_half2(a01 & 0xFFFF), kv_half2(a01 >> 16), kv_half2(b01 & 0xFFFF), kv_half2(b01 >> 16)};
-                        const uint32_t odd[4] = {kv_half2(a23 & 0xFFFF), kv_half2(a23 >> 16), kv_half2(b23 & 0xFFFF), kv_half2(b23 >> 16)};
-#pragma unroll
-                        for (int n = 0; n < NT; ++n) {
-                            mma_half(o[n][2 * j], even, pb[n][u][0], pb[n][u][1]);
-                            mma_half(o[n][2 * j + 1], odd, pb[n][u][0], pb[n][u][1]);
-                        }
+                    for (int j = 0; j < HD / 16; ++j) {
+                        o[n][j][0] *= keep[0]; o[n][j][1] *= keep[1]; o[n][j][2] *= keep[0]; o[n][j][3] *= keep[1];
                     }
                 }
-                powers = powers_next;
-                __syncwarp();  // the stage is free
+#pragma unroll
+                for (int u = 0; u < 2; ++u)
+#pragma unroll
+                    for (int r = 0; r < 2; ++r) pb[n][u][r] = transposed(half2_of(sc[n][u][2 * r], sc[n][u][2 * r + 1]));
             }
-            cp_async_wait<0>();
-            // ---- the four warps' shares ----
+            // O^T += V^T P^T: a thread pairs tokens (2 t, 2 t + 1) and (2 t + 8, 2 t + 9); its words of a row: 16 bytes of every
+            // 128, then 8 of 64 and 4 of 32
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+                uint32_t w[4][WORDS];
+#pragma unroll
+                for (int x = 0; x < 4; ++x) {
+                    constexpr int W16 = HD / 128;
+                    // (of row 2 t + (x & 1); 8 and 16 rows further: the same swizzle)
+                    const uint8_t* vr = vt + (16 * u + 8 * (x >> 1)) * HD;
+                    const int r = 2 * t + (x & 1);
+#pragma unroll
+                    for (int j = 0; j < W16; ++j) {
+                        const uint4 v = *reinterpret_cast<const uint4*>(vr + C::at(r, g) + 128 * j);
+                        w[x][4 * j] = v.x; w[x][4 * j + 1] = v.y; w[x][4 * j + 2] = v.z; w[x][4 * j + 3] = v.w;
+                    }
+                    if (HD % 128 >= 64) {
+                        const uint2 v = *reinterpret_cast<const uint2*>(vr + C::at(r, 8 * W16 + (g >> 1)) + 8 * (g & 1));
+                        w[x][4 * W16] = v.x;
+                        w[x][4 * W16 + 1] = v.y;
+                    }
+                    if (HD % 64 == 32) w[x][WORDS - 1] = *reinterpret_cast<const uint32_t*>(vr + C::at(r, HD / 16 - 2 + (g >> 2)) + 4 * (g & 3));
+                }
+#pragma unroll
+                for (int j = 0; j < WORDS; ++j) {
+                    uint32_t even[4], odd[4];
+                    halves_of(__byte_perm(w[0][j], w[1][j], 0x5140), even[0], even[1]);
+                    halves_of(__byte_perm(w[0][j], w[1][j], 0x7362), odd[0], odd[1]);
+                    halves_of(__byte_perm(w[2][j], w[3][j], 0x5140), even[2], even[3]);
+                    halves_of(__byte_perm(w[2][j], w[3][j], 0x7362), odd[2], odd[3]);
+#pragma unroll
+                    for (int n = 0; n < NT; ++n) {
+                        mma_half(o[n][2 * j], even, pb[n][u][0], pb[n][u][1]);
+                        mma_half(o[n][2 * j + 1], odd, pb[n][u][0], pb[n][u][1]);
+                    }
+                }
+            }
+            stage = next;
+            __syncwarp();  // the stage is free
+        }
+        // ---- the run has left the segment, or ends in it ----
+        const bool begins = at.tile == 0, ends = at.tile + n_tiles == at.tiles;
+        const int piece = 2 * warp + (ends ? 0 : 1);
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int e = 0; e < 2; ++e)
+#pragma unroll
+                for (int d = 4; d < 32; d <<= 1) l[n][e] += __shfl_xor_sync(0xffffffffu, l[n][e], d);
+        if (!(begins && ends) && g == 0) {
 #pragma unroll
             for (int n = 0; n < NT; ++n)
 #pragma unroll
                 for (int e = 0; e < 2; ++e) {
+                    m_s[piece][8 * n + 2 * t + e] = m[n][e];
+                    l_s[piece][8 * n + 2 * t + e] = l[n][e];
+                }
+            if (lane == 0) {
+                piece_s[piece][0] = at.s * per_request + at.seg;
+                piece_s[piece][1] = unit - at.tile;
+                piece_s[piece][2] = at.tiles;
+            }
+        }
+        if (!ends) cp_async_wait<0>();  // (nothing is in flight any more: the run is over)
+        __syncwarp();
+        float* sums = ends ? p.heads_o + (size_t)(blockIdx.x * WARPS + warp) * ROWS * HD : reinterpret_cast<float*>(my_ring);
+        static_assert(ROWS * HD * 4 <= C::RING / WARPS, "a piece must fit over a warp's ring");
 #pragma unroll
-                    for (int d = 4; d < 32; d <<= 1) l[n][e] += __shfl_xor_sync(0xffffffffu, l[n][e], d);
-                    if (g == 0) {
-                        m_s[warp][8 * n + 2 * t + e] = m[n][e];
-                        l_s[warp][8 * n + 2 * t + e] = l[n][e];
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int j = 0; j < WORDS; ++j) {
+                const int d = j < HD / 128 * 4 ? (j / 4) * 128 + 16 * g + 4 * (j % 4)
+                              : (HD % 128 >= 64 && j < HD / 128 * 4 + 2) ? HD / 128 * 128 + 8 * g + 4 * (j - HD / 128 * 4) : HD - 32 + 4 * g;
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    const int r = 8 * n + 2 * t + e;
+                    const float4 x = make_float4(o[n][2 * j][e], o[n][2 * j][2 + e], o[n][2 * j + 1][e], o[n][2 * j + 1][2 + e]);
+                    if (begins && ends) {
+                        const float inv = l[n][e] == 0.f ? 0.f : 1.f / l[n][e];
+                        if (r < rows)
+                            Vec4<bf16>::store((bf16*)p.out + ((size_t)row * p.nh + h0 + r) * HD + d, make_float4(x.x * inv, x.y * inv, x.z * inv, x.w * inv));
+                    } else {
+                        *reinterpret_cast<float4*>(sums + r * HD + d) = x;
                     }
                 }
-            __syncthreads();  // the rings are read: the partial sums lie over them
-            float* sums = reinterpret_cast<float*>(ring_s);  // [WARPS][ROWS][HD]
-            static_assert(WARPS * ROWS * HD * 4 <= C::RING, "the partial sums must fit over the rings");
-#pragma unroll
-            for (int n = 0; n < NT; ++n)
-#pragma unroll
-                for (int j = 0; j < WORDS; ++j) {
-                    const int d = j < HD / 128 * 4 ? (j / 4) * 128 + 16 * g + 4 * (j % 4)
-                                  : (HD % 128 >= 64 && j < HD / 128 * 4 + 2) ? HD / 128 * 128 + 8 * g + 4 * (j - HD / 128 * 4) : HD - 32 + 4 * g;
-#pragma unroll
-                    for (int e = 0; e < 2; ++e)
-                        *reinterpret_cast<float4*>(sums + (warp * ROWS + 8 * n + 2 * t + e) * HD + d) =
-                            make_float4(o[n][2 * j][e], o[n][2 * j][2 + e], o[n][2 * j + 1][e], o[n][2 * j + 1][2 + e]);
-                }
-            if (tid < ROWS) {
-                float top = -INFINITY, total = 0.f;
-#pragma unroll
-                for (int w = 0; w < WARPS; ++w) top = fmaxf(top, m_s[w][tid]);
-#pragma unroll
-                for (int w = 0; w < WARPS; ++w) {
-                    const float f = m_s[w][tid] == -INFINITY ? 0.f : fast_exp2(m_s[w][tid] - top);
-                    w_s[tid][w] = f;
-                    total += f * l_s[w][tid];
-                }
-                w_s[tid][WARPS] = top;
-                w_s[tid][WARPS + 1] = total;
+            }
+        unit += n_tiles;
+        step(at, n_tiles, unit < last);
+    }
+    cp_async_wait<0>();
+    __syncthreads();
+    // ---- the warps' pieces, in order: neighbours of one segment are added up ----
+    for (int x = 0; x < 2 * WARPS;) {
+        const int segment = piece_s[x][0];
+        if (segment < 0) {
+            ++x;
+            continue;
+        }
+        const int seg_first = piece_s[x][1], tiles = piece_s[x][2];
+        int end = x + 1;
+        while (end < 2 * WARPS && (piece_s[end][0] < 0 || piece_s[end][0] == segment)) ++end;
+        const int s = segment / per_request, seg = segment % per_request;
+        const int row = p.q_start != nullptr ? p.q_start[s] : s, part = seg % p.groups;
+        const int h0 = seg / p.groups * (p.nh / p.nkv) + part * p.heads_each, rows = min(p.heads_each, p.nh / p.nkv - part * p.heads_each);
+        const int first_block = seg_first / block_units, last_block = (seg_first + tiles - 1) / block_units;
+        const int pieces = last_block - first_block + 1;
+        const int my_piece = 2 * blockIdx.x + (seg_first < range.first ? 0 : 1);
+        for (int i = tid; i < rows * (HD / 4); i += blockDim.x) {
+            const int r = i / (HD / 4), d = i % (HD / 4) * 4;
+            float top = -INFINITY, total = 0.f;
+            for (int y = x; y < end; ++y)
+                if (piece_s[y][0] >= 0) top = fmaxf(top, m_s[y][r]);
+            float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+            for (int y = x; y < end; ++y) {
+                if (piece_s[y][0] < 0) continue;
+                const float* from = (y & 1) ? reinterpret_cast<const float*>(ring_s + (y >> 1) * ST * 2 * C::TILE_BYTES)
+                                            : p.heads_o + (size_t)(blockIdx.x * WARPS + (y >> 1)) * ROWS * HD;
+                const float4 v = *reinterpret_cast<const float4*>(from + r * HD + d);
+                const float f = m_s[y][r] == -INFINITY ? 0.f : fast_exp2(m_s[y][r] - top);
+                total = fmaf(f, l_s[y][r], total);
+                sum.x = fmaf(f, v.x, sum.x); sum.y = fmaf(f, v.y, sum.y); sum.z = fmaf(f, v.z, sum.z); sum.w = fmaf(f, v.w, sum.w);
+            }
+            if (pieces == 1) {
+                const float inv = total == 0.f ? 0.f : 1.f / total;
+                Vec4<bf16>::store((bf16*)p.out + ((size_t)row * p.nh + h0 + r) * HD + d, make_float4(sum.x * inv, sum.y * inv, sum.z * inv, sum.w * inv));
+            } else {
+                *reinterpret_cast<float4*>(p.part_o + ((size_t)my_piece * ROWS + r) * HD + d) = sum;
+                if (d == 0) *reinterpret_cast<float2*>(p.part_ml + ((size_t)my_piece * ROWS + r) * 2) = make_float2(top, total);
+            }
+        }
+        x = end;
+        if (pieces == 1) continue;
+        // piece number y of the segment: of block first_block + y, its second one where the segment begins in it
+        auto place = [&](int y) { return (size_t)2 * (first_block + y) + (y == 0 ? 1 : 0); };
+        int from = 0, count = pieces, stride = 1;
+        int* counter = p.counters + segment;
+        bool final = true;
+        if (pieces > 2 * MERGE_AT_ONCE) {
+            const int y = blockIdx.x - first_block;
+            from = y - y % MERGE_AT_ONCE;
+            count = min(MERGE_AT_ONCE, pieces - from);
+            counter = p.counters + p.requests * per_request + place(from);
+            final = false;
+        }
+        for (;;) {
+            // the barrier orders all threads' stores before thread 0's release; the last block's acquire, followed by the
+            // next barrier, its threads' loads behind everybody's stores
+            __syncthreads();
+            if (tid == 0) {
+                int before;
+                asm volatile("atom.add.acq_rel.gpu.global.s32 %0, [%1], 1;" : "=r"(before) : "l"(counter) : "memory");
+                last_s = before == count - 1;
+                if (last_s) *counter = 0;
             }
             __syncthreads();
-            const int first_block = seg_first / range.quota, last_block = (seg_first + tiles - 1) / range.quota;
-            const int pieces = last_block - first_block + 1;
-            const int my_piece = 2 * blockIdx.x + (seg_first < range.first ? 0 : 1);
+            if (!last_s) break;
             for (int i = tid; i < rows * (HD / 4); i += blockDim.x) {
                 const int r = i / (HD / 4), d = i % (HD / 4) * 4;
+                float top = -INFINITY, total = 0.f;
                 float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll
-                for (int w = 0; w < WARPS; ++w) {
-                    const float4 x = *reinterpret_cast<const float4*>(sums + (w * ROWS + r) * HD + d);
-                    const float f = w_s[r][w];
-                    sum.x = fmaf(f, x.x, sum.x); sum.y = fmaf(f, x.y, sum.y); sum.z = fmaf(f, x.z, sum.z); sum.w = fmaf(f, x.w, sum.w);
-                }
-                if (pieces == 1) {
-                    const float total = w_s[r][WARPS + 1], inv = total == 0.f ? 0.f : 1.f / total;
-                    Vec4<bf16>::store((bf16*)p.out + ((size_t)row * p.nh + h0 + r) * HD + d, make_float4(sum.x * inv, sum.y * inv, sum.z * inv, sum.w * inv));
-                } else {
-                    *reinterpret_cast<float4*>(p.part_o + ((size_t)my_piece * ROWS + r) * HD + d) = sum;
-                    if (d == 0) *reinterpret_cast<float2*>(p.part_ml + ((size_t)my_piece * ROWS + r) * 2) = make_float2(w_s[r][WARPS], w_s[r][WARPS + 1]);
-                }
-            }
-            if (pieces > 1) {
-                // piece number x of the segment: of block first_block + x, its second one where the segment begins in it
-                auto place = [&](int x) { return (size_t)2 * (first_block + x) + (x == 0 ? 1 : 0); };
-                int from = 0, count = pieces, step = 1;
-                int* counter = p.counters + s * per_request + seg;
-                bool final = true;
-                if (pieces > 2 * MERGE_AT_ONCE) {
-                    const int x = blockIdx.x - first_block;
-                    from = x - x % MERGE_AT_ONCE;
-                    count = min(MERGE_AT_ONCE, pieces - from);
-                    counter = p.counters + p.requests * per_request + place(from);
-                    final = false;
-                }
-                for (;;) {
-                    // the barrier orders all threads' stores before thread 0's release; the last block's acquire, followed by the
-                    // next barrier, its threads' loads behind everybody's stores
-                    __syncthreads();
-                    if (tid == 0) {
-                        int before;
-                        asm volatile("atom.add.acq_rel.gpu.global.s32 %0, [%1], 1;" : "=r"(before) : "l"(counter) : "memory");
-                        last_s = before == count - 1;
-                        if (last_s) *counter = 0;
-                    }
-                    __syncthreads();
-                    if (!last_s) break;
-                    for (int i = tid; i < rows * (HD / 4); i += blockDim.x) {
-                        const int r = i / (HD / 4), d = i % (HD / 4) * 4;
-                        float top = -INFINITY, total = 0.f;
-                        float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll 1
-                        for (int x0 = 0; x0 < count; x0 += MERGE_AT_ONCE) {
-                            float2 ml[MERGE_AT_ONCE];
-                            float4 v[MERGE_AT_ONCE];
+                for (int y0 = 0; y0 < count; y0 += MERGE_AT_ONCE) {
+                    float2 ml[MERGE_AT_ONCE];
+                    float4 v[MERGE_AT_ONCE];
 #pragma unroll
-                            for (int x = 0; x < MERGE_AT_ONCE; ++x) {
-                                ml[x] = make_float2(-INFINITY, 0.f);
-                                v[x] = make_float4(0.f, 0.f, 0.f, 0.f);
-                                if (x0 + x < count) {
-                                    const size_t at = place(from + (x0 + x) * step) * ROWS + r;
-                                    ml[x] = __ldcg(reinterpret_cast<const float2*>(p.part_ml) + at);
-                                    v[x] = __ldcg(reinterpret_cast<const float4*>(p.part_o + at * HD + d));
-                                }
-                            }
-                            float next = top;
-#pragma unroll
-                            for (int x = 0; x < MERGE_AT_ONCE; ++x) next = fmaxf(next, ml[x].x);
-                            const float keep = top == -INFINITY ? 0.f : fast_exp2(top - next);
-                            total *= keep; sum.x *= keep; sum.y *= keep; sum.z *= keep; sum.w *= keep;
-                            top = next;
-#pragma unroll
-                            for (int x = 0; x < MERGE_AT_ONCE; ++x) {
-                                const float f = ml[x].x == -INFINITY ? 0.f : fast_exp2(ml[x].x - top);
-                                total = fmaf(f, ml[x].y, total);
-                                sum.x = fmaf(f, v[x].x, sum.x); sum.y = fmaf(f, v[x].y, sum.y);
-                                sum.z = fmaf(f, v[x].z, sum.z); sum.w = fmaf(f, v[x].w, sum.w);
-                            }
-                        }
-                        if (final) {
-                            const float inv = total == 0.f ? 0.f : 1.f / total;
-                            Vec4<bf16>::store((bf16*)p.out + ((size_t)row * p.nh + h0 + r) * HD + d,
-                                              make_float4(sum.x * inv, sum.y * inv, sum.z * inv, sum.w * inv));
-                        } else {  // over the first of the twelve, whose four sums this thread alone reads and writes
-                            *reinterpret_cast<float4*>(p.part_o + (place(from) * ROWS + r) * HD + d) = sum;
-                            if (d == 0) {
-                                w_s[r][0] = top;
-                                w_s[r][1] = total;
-                            }
+                    for (int y = 0; y < MERGE_AT_ONCE; ++y) {
+                        ml[y] = make_float2(-INFINITY, 0.f);
+                        v[y] = make_float4(0.f, 0.f, 0.f, 0.f);
+                        if (y0 + y < count) {
+                            const size_t i_at = place(from + (y0 + y) * stride) * ROWS + r;
+                            ml[y] = __ldcg(reinterpret_cast<const float2*>(p.part_ml) + i_at);
+                            v[y] = __ldcg(reinterpret_cast<const float4*>(p.part_o + i_at * HD + d));
                         }
                     }
-                    if (final) break;
-                    __syncthreads();  // (their maxima and sums are read by all)
-                    if (tid < rows) *reinterpret_cast<float2*>(p.part_ml + (place(from) * ROWS + tid) * 2) = make_float2(w_s[tid][0], w_s[tid][1]);
-                    from = 0;
-                    count = (pieces + MERGE_AT_ONCE - 1) / MERGE_AT_ONCE;
-                    step = MERGE_AT_ONCE;
-                    counter = p.counters + s * per_request + seg;
-                    final = true;
+                    float next = top;
+#pragma unroll
+                    for (int y = 0; y < MERGE_AT_ONCE; ++y) next = fmaxf(next, ml[y].x);
+                    const float keep = top == -INFINITY ? 0.f : fast_exp2(top - next);
+                    total *= keep; sum.x *= keep; sum.y *= keep; sum.z *= keep; sum.w *= keep;
+                    top = next;
+#pragma unroll
+                    for (int y = 0; y < MERGE_AT_ONCE; ++y) {
+                        const float f = ml[y].x == -INFINITY ? 0.f : fast_exp2(ml[y].x - top);
+                        total = fmaf(f, ml[y].y, total);
+                        sum.x = fmaf(f, v[y].x, sum.x); sum.y = fmaf(f, v[y].y, sum.y);
+                        sum.z = fmaf(f, v[y].z, sum.z); sum.w = fmaf(f, v[y].w, sum.w);
+                    }
+                }
+                if (final) {
+                    const float inv = total == 0.f ? 0.f : 1.f / total;
+                    Vec4<bf16>::store((bf16*)p.out + ((size_t)row * p.nh + h0 + r) * HD + d, make_float4(sum.x * inv, sum.y * inv, sum.z * inv, sum.w * inv));
+                } else {  // over the first of the twelve, whose four sums this thread alone reads and writes
+                    *reinterpret_cast<float4*>(p.part_o + (place(from) * ROWS + r) * HD + d) = sum;
+                    if (d == 0) {
+                        ml_s[r][0] = top;
+                        ml_s[r][1] = total;
+                    }
                 }
             }
-            __syncthreads();  // before the rings, the queries and the factors are written again
+            if (final) break;
+            __syncthreads();  // (their maxima and sums are read by all)
+            if (tid < rows) *reinterpret_cast<float2*>(p.part_ml + (place(from) * ROWS + tid) * 2) = make_float2(ml_s[tid][0], ml_s[tid][1]);
+            from = 0;
+            count = (pieces + MERGE_AT_ONCE - 1) / MERGE_AT_ONCE;
+            stride = MERGE_AT_ONCE;
+            counter = p.counters + segment;
+            final = true;
         }
+        __syncthreads();  // before last_s and ml_s are written again
     }
     cw_trace_end();
 }
@@ -572,7 +653,7 @@ __global__ void __launch_bounds__(ANY_TOKENS) decode_e4m3_any_kernel(const Decod
 
 template <int HD, int NT>
 static int stream_launch(const DecodeE4m3Params& p, int sms, cudaStream_t stream) {
-    using C = Stream<HD>;
+    using C = Stream<HD, NT>;
     static bool configured[64] = {};  // (per device)
     int device = 0;
     cudaGetDevice(&device);
@@ -601,8 +682,8 @@ static int groups_of(int nh, int nkv, int hd, int dtype) {
 extern "C" int cw_attention_decode_e4m3_scratch(int requests, int nh, int nkv, int hd, int dtype, int sms, long long* floats, int* words) {
     if (requests < 0 || nh <= 0 || nkv <= 0 || nh % nkv || hd <= 0 || hd > 256 || sms <= 0) return CW_ERR_BAD_SIZE;
     const int groups = groups_of(nh, nkv, hd, dtype);
-    const long long pieces = groups ? 4LL * sms : 0;  // two blocks an SM, two pieces a block
-    *floats = pieces * 16 * (hd + 2);
+    const long long pieces = groups ? 6LL * sms : 0;  // three blocks an SM at most, two pieces a block
+    *floats = pieces * 16 * (hd + 2) + 2 * pieces * 16 * hd;
     *words = groups ? (int)(requests * nkv * groups + pieces) : 0;
     return CW_OK;
 }
@@ -620,14 +701,15 @@ extern "C" int cw_attention_decode_e4m3(const void* q, int q_stride, void* out, 
         return CW_ERR_BAD_SIZE;
     DecodeE4m3Params p = {q, q_stride, out, k, v, k_exp, v_exp, block_tables, ctx_lens, q_start, requests, nh, nkv, hd, page_size,
                           max_blocks, num_pages, window, scale, status};
-    const int groups = groups_of(nh, nkv, hd, dtype);
-    if (groups && floats != nullptr && words != nullptr && (long long)num_pages * page_size * nkv < (1LL << 32) &&
+    const int groups = ((uintptr_t)q % 4 || q_stride % 2) ? 0 : groups_of(nh, nkv, hd, dtype);  // (queries are read in pairs)
+    if (groups && floats != nullptr && words != nullptr && (long long)num_pages * page_size * nkv * (hd / 16) < 0xFFFFFFFFLL &&
         (long long)requests * nkv * groups * ((long long)max_blocks * page_size / TILE_TOKENS + 2) < 0x7FFFFFFF) {
         p.page_shift = (page_size & (page_size - 1)) == 0 ? __builtin_ctz(page_size) : -1;
         p.groups = groups;
         p.heads_each = (nh / nkv + groups - 1) / groups;
         p.part_o = floats;
-        p.part_ml = floats + 4LL * sms * 16 * hd;
+        p.heads_o = floats + 6LL * sms * 16 * hd;
+        p.part_ml = p.heads_o + 12LL * sms * 16 * hd;
         p.counters = words;
         switch (hd) {
             case 32: return stream_launch_heads<32>(p, sms, stream);

@@ -104,6 +104,14 @@ __device__ __forceinline__ void halves_of(uint32_t word, uint32_t& lo, uint32_t&
 struct Walk {
     int s, ctx, begin, tiles;  // the request, its context, the first position it sees, its tiles
     int seg, tile;             // KV head and group; tile of it
+    int left;                  // units of the run that are left
+};
+
+// Part of a segment that several warps share.
+struct Piece {
+    int segment;           // -1: there is none
+    int row, head, heads;  // where its outputs go
+    int first_block, blocks;  // which blocks have pieces of it
 };
 
 template <int HD, int NT>
@@ -114,11 +122,11 @@ __global__ void __launch_bounds__(WARPS * 32, Stream<HD, NT>::PER_SM) decode_e4m
     extern __shared__ __align__(128) uint8_t ring_s[];
     __shared__ uint32_t row_s[WARPS][ST][TILE_TOKENS];       // 16-byte chunk where a token's row begins; ~0: it does not count
     __shared__ uint32_t power_at_s[WARPS][ST][TILE_TOKENS];  // where its powers are
-    __shared__ float m_s[2 * WARPS][ROWS], l_s[2 * WARPS][ROWS];
-    __shared__ int piece_s[2 * WARPS][3];  // segment (-1: no such piece), its first unit, its tiles
-    __shared__ float ml_s[ROWS][2];
+    __shared__ float m_s[2 * WARPS][ROWS], l_s[2 * WARPS][ROWS], f_s[2 * WARPS][ROWS];
+    __shared__ Piece piece_s[2 * WARPS];  // of every warp: the end of a segment that began before its run, and what its run ends in
+    __shared__ float top_s[2 * WARPS][ROWS], total_s[2 * WARPS][ROWS];  // of a group of pieces, at its first
     __shared__ int sh[36];
-    __shared__ int last_s;
+    __shared__ int last_s[2];
     pdl_enter();
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
     const int per_request = p.nkv * p.groups;
@@ -130,9 +138,11 @@ __global__ void __launch_bounds__(WARPS * 32, Stream<HD, NT>::PER_SM) decode_e4m
     auto tiles_of = [&](int ctx) {
         return ctx <= 0 ? 0 : (ctx + TILE_TOKENS - 1) / TILE_TOKENS - begin_of(ctx) / TILE_TOKENS;
     };
-    // (a block's run is a whole number of equal runs for its warps)
-    UnitRange range = units_of_block([&](int s) { return per_request * tiles_of(context_of(s)); }, p.requests, 1, gridDim.x * WARPS,
-                                     blockIdx.x * WARPS, sh);
+    // A segment is its tiles and, before them, a unit for what changing to it costs (about a tile's time).  A block's run is a
+    // whole number of equal runs for its warps.
+    auto units_of = [&](int tiles) { return tiles > 0 ? per_request * (tiles + 1) : 0; };
+    const UnitRange range = units_of_block([&](int s) { return units_of(tiles_of(context_of(s))); }, p.requests, 1, gridDim.x * WARPS,
+                                           blockIdx.x * WARPS, sh);
     const int block_units = range.quota * WARPS;
     for (int s = blockIdx.x; s < p.requests; s += gridDim.x) {  // rows without a context: zeros
         if (context_of(s) != 0) continue;
@@ -141,50 +151,59 @@ __global__ void __launch_bounds__(WARPS * 32, Stream<HD, NT>::PER_SM) decode_e4m
     }
     if (range.first >= range.last) return;
     // ---- where this warp's run begins ----
-    const int first = range.first + warp * range.quota, last = min(range.total, first + range.quota);
+    const int first = range.first + warp * range.quota;
     Walk at = {};
+    at.left = min(range.total, first + range.quota) - first;
     auto enter = [&](Walk& w, int s) {  // the next request from s on that has tiles
+        w.seg = w.tile = 0;
         for (; s < p.requests; ++s) {
-            const int ctx = context_of(s), n = tiles_of(ctx);
-            if (n > 0) {
-                w = {s, ctx, begin_of(ctx), n, 0, 0};
-                return;
-            }
+            w.s = s;
+            w.ctx = context_of(s);
+            w.tiles = tiles_of(w.ctx);
+            w.begin = begin_of(w.ctx);
+            if (w.tiles > 0) return;
         }
-        w = {p.requests - 1, 0, 0, 0x7FFFFFFF / per_request, 0, 0};  // (lengths that change under the call: tokens that do not count)
+        w.ctx = 0;  // (lengths that change under the call: tokens that do not count)
+        w.tiles = 0x7FFFFFFF / per_request - 1;
     };
-    auto step = [&](Walk& w, int units, bool more) {  // `units` tiles on within its segment, then on to where the next one is
-        w.tile += units;
+    auto step = [&](Walk& w, int tiles) {  // so many tiles on within its segment, and on to the next one's first
+        w.tile += tiles;
+        w.left -= tiles;
         if (w.tile == w.tiles) {
             w.tile = 0;
-            if (++w.seg == per_request && more) enter(w, w.s + 1);
+            --w.left;
+            if (++w.seg == per_request && w.left > 0) enter(w, w.s + 1);
         }
     };
-    if (first < last) {
+    int seg_unit = 0;  // of the segment that the run stands in: the unit before its tiles
+    if (at.left > 0) {
         int skip = range.offset + warp * range.quota;
         enter(at, range.request);
-        while (skip >= at.tiles * per_request) {
-            skip -= at.tiles * per_request;
+        while (skip >= units_of(at.tiles)) {
+            skip -= units_of(at.tiles);
             enter(at, at.s + 1);
         }
-        at.seg = skip / at.tiles;
-        at.tile = skip - at.seg * at.tiles;
+        at.seg = skip / (at.tiles + 1);
+        skip -= at.seg * (at.tiles + 1);
+        seg_unit = first - skip;
+        at.tile = max(0, skip - 1);
+        if (skip == 0) --at.left;
     }
     uint8_t* my_ring = ring_s + warp * ST * 2 * C::TILE_BYTES;
     const uint32_t my_ring_addr = smem_addr(my_ring);
     // ---- fetching: ST - 1 tiles ahead of the products, through the segments' ends ----
     Walk ahead = at;
-    int to_fetch = max(0, last - first), fetch_stage = 0, ahead_page = -1, ahead_pos = 0;
+    int fetch_stage = 0, ahead_page = -1, ahead_pos = 0;
     const int copy_lane = C::at(lane / CH, lane % CH);
     auto look_up = [&]() {  // the page of this lane's token of the tile that is fetched next
         ahead_page = -1;
-        if (to_fetch <= 0) return;
+        if (ahead.left <= 0) return;
         ahead_pos = (ahead.begin / TILE_TOKENS + ahead.tile) * TILE_TOKENS + lane;
         if (ahead_pos >= ahead.begin && ahead_pos < ahead.ctx)
             ahead_page = p.block_tables[(size_t)ahead.s * p.max_blocks + (p.page_shift >= 0 ? ahead_pos >> p.page_shift : ahead_pos / p.page_size)];
     };
     auto fetch = [&]() {
-        if (to_fetch > 0) {
+        if (ahead.left > 0) {
             const int kvh = p.groups == 1 ? ahead.seg : ahead.seg / p.groups;
             uint32_t row = ~0u, power_at = 0;
             if (ahead_page >= 0 && ahead_page < p.num_pages) {
@@ -209,8 +228,7 @@ __global__ void __launch_bounds__(WARPS * 32, Stream<HD, NT>::PER_SM) decode_e4m
                 copy16(dst + C::TILE_BYTES, p.v + src, there);
             }
             if (++fetch_stage == ST) fetch_stage = 0;
-            --to_fetch;
-            step(ahead, 1, to_fetch > 0);
+            step(ahead, 1);
             look_up();
         }
         cp_async_commit();
@@ -226,17 +244,17 @@ __global__ void __launch_bounds__(WARPS * 32, Stream<HD, NT>::PER_SM) decode_e4m
     look_up();
     for (int i = 0; i < ST - 1; ++i) fetch();
     __syncwarp();
-    int unit = first, stage = 0;
-    if (first < last) look_at_powers(0);
-    if (lane < 2) piece_s[2 * warp + lane][0] = -1;
+    int stage = 0;
+    if (at.left > 0) look_at_powers(0);
+    if (lane < 2) piece_s[2 * warp + lane].segment = -1;
     // where this lane's K pieces and V words lie in a tile (rows 16 and 8 further: the same swizzle)
     const int k_at = C::at(g, HD % 64 == 0 ? t : t >> 1) + (HD % 64 == 0 ? 0 : 8 * (t & 1));
     constexpr int PIECE = HD % 64 == 0 ? 16 : 8, STEPS = PIECE / 4, PIECES = HD / (4 * PIECE);
-    while (unit < last) {
+    while (at.left > 0) {
         const int row = p.q_start != nullptr ? p.q_start[at.s] : at.s;
         const int part = p.groups == 1 ? 0 : at.seg % p.groups, kvh = p.groups == 1 ? at.seg : at.seg / p.groups;
         const int h0 = kvh * (p.nh / p.nkv) + part * p.heads_each, rows = min(p.heads_each, p.nh / p.nkv - part * p.heads_each);
-        const int n_tiles = min(at.tiles - at.tile, last - unit);
+        const int n_tiles = min(at.tiles - at.tile, at.left);
         // ---- the group's queries, as B fragments over the entries that a lane's pieces of K hold: half precision, a power of two out ----
         uint32_t qb[NT][PIECES][STEPS][2];
         float qf[NT][2], m[NT][2], l[NT][2], o[NT][HD / 16][4];
@@ -284,7 +302,7 @@ __global__ void __launch_bounds__(WARPS * 32, Stream<HD, NT>::PER_SM) decode_e4m
             __syncwarp();
             const int next = stage + 1 == ST ? 0 : stage + 1;
             const uint32_t powers = counts == ~0u ? 0u : k_power | v_power << 8 | 1u << 16;
-            if (unit + i + 1 < last) look_at_powers(next);
+            if (i + 1 < n_tiles || ahead.left > 0 || fetch_stage != next) look_at_powers(next);
             const uint8_t* kt = my_ring + stage * 2 * C::TILE_BYTES;
             const uint8_t* vt = kt + C::TILE_BYTES;
             float sc[NT][2][4];
@@ -421,9 +439,8 @@ __global__ void __launch_bounds__(WARPS * 32, Stream<HD, NT>::PER_SM) decode_e4m
                     l_s[piece][8 * n + 2 * t + e] = l[n][e];
                 }
             if (lane == 0) {
-                piece_s[piece][0] = at.s * per_request + at.seg;
-                piece_s[piece][1] = unit - at.tile;
-                piece_s[piece][2] = at.tiles;
+                const int first_block = (seg_unit + 1) / block_units;
+                piece_s[piece] = {at.s * per_request + at.seg, row, h0, rows, first_block, (seg_unit + at.tiles) / block_units - first_block + 1};
             }
         }
         if (!ends) cp_async_wait<0>();  // (nothing is in flight any more: the run is over)
@@ -449,77 +466,110 @@ __global__ void __launch_bounds__(WARPS * 32, Stream<HD, NT>::PER_SM) decode_e4m
                     }
                 }
             }
-        unit += n_tiles;
-        step(at, n_tiles, unit < last);
+        if (ends) seg_unit += at.tiles + 1;
+        step(at, n_tiles);
     }
     cp_async_wait<0>();
     __syncthreads();
-    // ---- the warps' pieces, in order: neighbours of one segment are added up ----
-    for (int x = 0; x < 2 * WARPS;) {
-        const int segment = piece_s[x][0];
-        if (segment < 0) {
-            ++x;
-            continue;
-        }
-        const int seg_first = piece_s[x][1], tiles = piece_s[x][2];
-        int end = x + 1;
-        while (end < 2 * WARPS && (piece_s[end][0] < 0 || piece_s[end][0] == segment)) ++end;
-        const int s = segment / per_request, seg = segment % per_request;
-        const int row = p.q_start != nullptr ? p.q_start[s] : s, part = seg % p.groups;
-        const int h0 = seg / p.groups * (p.nh / p.nkv) + part * p.heads_each, rows = min(p.heads_each, p.nh / p.nkv - part * p.heads_each);
-        const int first_block = seg_first / block_units, last_block = (seg_first + tiles - 1) / block_units;
-        const int pieces = last_block - first_block + 1;
-        const int my_piece = 2 * blockIdx.x + (seg_first < range.first ? 0 : 1);
-        for (int i = tid; i < rows * (HD / 4); i += blockDim.x) {
-            const int r = i / (HD / 4), d = i % (HD / 4) * 4;
-            float top = -INFINITY, total = 0.f;
-            for (int y = x; y < end; ++y)
-                if (piece_s[y][0] >= 0) top = fmaxf(top, m_s[y][r]);
-            float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
-            for (int y = x; y < end; ++y) {
-                if (piece_s[y][0] < 0) continue;
-                const float* from = (y & 1) ? reinterpret_cast<const float*>(ring_s + (y >> 1) * ST * 2 * C::TILE_BYTES)
-                                            : p.heads_o + (size_t)(blockIdx.x * WARPS + (y >> 1)) * ROWS * HD;
-                const float4 v = *reinterpret_cast<const float4*>(from + r * HD + d);
-                const float f = m_s[y][r] == -INFINITY ? 0.f : fast_exp2(m_s[y][r] - top);
-                total = fmaf(f, l_s[y][r], total);
-                sum.x = fmaf(f, v.x, sum.x); sum.y = fmaf(f, v.y, sum.y); sum.z = fmaf(f, v.z, sum.z); sum.w = fmaf(f, v.w, sum.w);
+    // ---- the block's pieces, in order: neighbours of one segment are added up ----
+    auto same = [&](int x, int y) { return piece_s[y].segment == piece_s[x].segment; };  // (pieces of one segment are neighbours)
+    for (int i = tid; i < 2 * WARPS * ROWS; i += blockDim.x) {  // what each is multiplied by; the sum of weights at the group's first
+        const int x = i / ROWS, r = i % ROWS;
+        if (piece_s[x].segment < 0) continue;
+        float top = -INFINITY, total = 0.f;
+        bool leads = true;
+        for (int y = 0; y < 2 * WARPS; ++y)
+            if (same(x, y)) {
+                top = fmaxf(top, m_s[y][r]);
+                leads = leads && y >= x;
             }
-            if (pieces == 1) {
-                const float inv = total == 0.f ? 0.f : 1.f / total;
-                Vec4<bf16>::store((bf16*)p.out + ((size_t)row * p.nh + h0 + r) * HD + d, make_float4(sum.x * inv, sum.y * inv, sum.z * inv, sum.w * inv));
-            } else {
-                *reinterpret_cast<float4*>(p.part_o + ((size_t)my_piece * ROWS + r) * HD + d) = sum;
-                if (d == 0) *reinterpret_cast<float2*>(p.part_ml + ((size_t)my_piece * ROWS + r) * 2) = make_float2(top, total);
+        for (int y = 0; y < 2 * WARPS; ++y)
+            if (leads && same(x, y) && m_s[y][r] != -INFINITY) total = fmaf(fast_exp2(m_s[y][r] - top), l_s[y][r], total);
+        f_s[x][r] = m_s[x][r] == -INFINITY ? 0.f : fast_exp2(m_s[x][r] - top);
+        if (leads) {
+            top_s[x][r] = top;
+            total_s[x][r] = total;
+        }
+    }
+    __syncthreads();
+    int came = -1, goes = -1;  // first pieces of the two segments, at most, that blocks before and after this one have pieces of as well
+    for (int x = 0; x < 2 * WARPS;) {
+        int end = x + 1;
+        if (piece_s[x].segment >= 0) {
+            while (end < 2 * WARPS && (piece_s[end].segment < 0 || same(x, end))) ++end;
+            const Piece& s = piece_s[x];
+            const int my_piece = 2 * blockIdx.x + (blockIdx.x == s.first_block ? 1 : 0);
+            if (s.blocks > 1 && blockIdx.x == s.first_block) goes = x;
+            if (s.blocks > 1 && blockIdx.x != s.first_block) came = x;
+#pragma unroll 1
+            for (int i = tid; i < s.heads * (HD / 4); i += blockDim.x) {
+                const int r = i / (HD / 4), d = i % (HD / 4) * 4;
+                float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 1
+                for (int y = x; y < end; ++y) {
+                    if (piece_s[y].segment < 0) continue;
+                    float4 v;
+                    if (y & 1)
+                        v = *reinterpret_cast<const float4*>(ring_s + (y >> 1) * ST * 2 * C::TILE_BYTES + (r * HD + d) * 4);
+                    else
+                        v = *reinterpret_cast<const float4*>(p.heads_o + ((size_t)(blockIdx.x * WARPS + (y >> 1)) * ROWS + r) * HD + d);
+                    const float f = f_s[y][r];
+                    sum.x = fmaf(f, v.x, sum.x); sum.y = fmaf(f, v.y, sum.y); sum.z = fmaf(f, v.z, sum.z); sum.w = fmaf(f, v.w, sum.w);
+                }
+                const float total = total_s[x][r];
+                if (s.blocks == 1) {
+                    const float inv = total == 0.f ? 0.f : 1.f / total;
+                    Vec4<bf16>::store((bf16*)p.out + ((size_t)s.row * p.nh + s.head + r) * HD + d, make_float4(sum.x * inv, sum.y * inv, sum.z * inv, sum.w * inv));
+                } else {
+                    *reinterpret_cast<float4*>(p.part_o + ((size_t)my_piece * ROWS + r) * HD + d) = sum;
+                    if (d == 0) *reinterpret_cast<float2*>(p.part_ml + ((size_t)my_piece * ROWS + r) * 2) = make_float2(top_s[x][r], total);
+                }
             }
         }
         x = end;
-        if (pieces == 1) continue;
-        // piece number y of the segment: of block first_block + y, its second one where the segment begins in it
-        auto place = [&](int y) { return (size_t)2 * (first_block + y) + (y == 0 ? 1 : 0); };
-        int from = 0, count = pieces, stride = 1;
-        int* counter = p.counters + segment;
-        bool final = true;
-        if (pieces > 2 * MERGE_AT_ONCE) {
-            const int y = blockIdx.x - first_block;
-            from = y - y % MERGE_AT_ONCE;
-            count = min(MERGE_AT_ONCE, pieces - from);
-            counter = p.counters + p.requests * per_request + place(from);
-            final = false;
+    }
+    if (came < 0 && goes < 0) {
+        cw_trace_end();
+        return;
+    }
+    // ---- segments that other blocks have pieces of: thread e counts this block in at segment e's counter ----
+    // (pieces by number: y is of block first_block + y, its second one where the segment begins in it)
+    auto twelves = [&](const Piece& s) { return s.blocks > 2 * MERGE_AT_ONCE; };  // added up by twelves first
+    auto place = [&](const Piece& s, int y) { return (size_t)2 * (s.first_block + y) + (y == 0 ? 1 : 0); };
+    // the barrier orders all threads' stores before the release; the last block's acquire, followed by the next barrier, its
+    // threads' loads behind everybody's stores
+    auto count_in = [&](int* counter, int count) {
+        int before;
+        asm volatile("atom.add.acq_rel.gpu.global.s32 %0, [%1], 1;" : "=r"(before) : "l"(counter) : "memory");
+        if (before == count - 1) *counter = 0;
+        return before == count - 1;
+    };
+    __syncthreads();
+    if (tid < 2) {
+        const int x = tid == 0 ? came : goes;
+        bool is_last = false;
+        if (x >= 0) {
+            const Piece& s = piece_s[x];
+            const int y = blockIdx.x - s.first_block, from = y - y % MERGE_AT_ONCE;
+            if (twelves(s))
+                is_last = count_in(p.counters + p.requests * per_request + place(s, from), min(MERGE_AT_ONCE, s.blocks - from));
+            else
+                is_last = count_in(p.counters + s.segment, s.blocks);
         }
+        last_s[tid] = is_last;
+    }
+    __syncthreads();
+#pragma unroll 1
+    for (int e = 0; e < 2; ++e) {
+        if (!last_s[e]) continue;
+        const Piece s = piece_s[e == 0 ? came : goes];
+        const int y = blockIdx.x - s.first_block;
+        bool final = !twelves(s);
+        int from = final ? 0 : y - y % MERGE_AT_ONCE, count = final ? s.blocks : min(MERGE_AT_ONCE, s.blocks - from), stride = 1;
+#pragma unroll 1
         for (;;) {
-            // the barrier orders all threads' stores before thread 0's release; the last block's acquire, followed by the
-            // next barrier, its threads' loads behind everybody's stores
-            __syncthreads();
-            if (tid == 0) {
-                int before;
-                asm volatile("atom.add.acq_rel.gpu.global.s32 %0, [%1], 1;" : "=r"(before) : "l"(counter) : "memory");
-                last_s = before == count - 1;
-                if (last_s) *counter = 0;
-            }
-            __syncthreads();
-            if (!last_s) break;
-            for (int i = tid; i < rows * (HD / 4); i += blockDim.x) {
+#pragma unroll 1
+            for (int i = tid; i < s.heads * (HD / 4); i += blockDim.x) {
                 const int r = i / (HD / 4), d = i % (HD / 4) * 4;
                 float top = -INFINITY, total = 0.f;
                 float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
@@ -528,50 +578,52 @@ __global__ void __launch_bounds__(WARPS * 32, Stream<HD, NT>::PER_SM) decode_e4m
                     float2 ml[MERGE_AT_ONCE];
                     float4 v[MERGE_AT_ONCE];
 #pragma unroll
-                    for (int y = 0; y < MERGE_AT_ONCE; ++y) {
-                        ml[y] = make_float2(-INFINITY, 0.f);
-                        v[y] = make_float4(0.f, 0.f, 0.f, 0.f);
-                        if (y0 + y < count) {
-                            const size_t i_at = place(from + (y0 + y) * stride) * ROWS + r;
-                            ml[y] = __ldcg(reinterpret_cast<const float2*>(p.part_ml) + i_at);
-                            v[y] = __ldcg(reinterpret_cast<const float4*>(p.part_o + i_at * HD + d));
+                    for (int k = 0; k < MERGE_AT_ONCE; ++k) {
+                        ml[k] = make_float2(-INFINITY, 0.f);
+                        v[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+                        if (y0 + k < count) {
+                            const size_t i_at = place(s, from + (y0 + k) * stride) * ROWS + r;
+                            ml[k] = __ldcg(reinterpret_cast<const float2*>(p.part_ml) + i_at);
+                            v[k] = __ldcg(reinterpret_cast<const float4*>(p.part_o + i_at * HD + d));
                         }
                     }
                     float next = top;
 #pragma unroll
-                    for (int y = 0; y < MERGE_AT_ONCE; ++y) next = fmaxf(next, ml[y].x);
+                    for (int k = 0; k < MERGE_AT_ONCE; ++k) next = fmaxf(next, ml[k].x);
                     const float keep = top == -INFINITY ? 0.f : fast_exp2(top - next);
                     total *= keep; sum.x *= keep; sum.y *= keep; sum.z *= keep; sum.w *= keep;
                     top = next;
 #pragma unroll
-                    for (int y = 0; y < MERGE_AT_ONCE; ++y) {
-                        const float f = ml[y].x == -INFINITY ? 0.f : fast_exp2(ml[y].x - top);
-                        total = fmaf(f, ml[y].y, total);
-                        sum.x = fmaf(f, v[y].x, sum.x); sum.y = fmaf(f, v[y].y, sum.y);
-                        sum.z = fmaf(f, v[y].z, sum.z); sum.w = fmaf(f, v[y].w, sum.w);
+                    for (int k = 0; k < MERGE_AT_ONCE; ++k) {
+                        const float f = ml[k].x == -INFINITY ? 0.f : fast_exp2(ml[k].x - top);
+                        total = fmaf(f, ml[k].y, total);
+                        sum.x = fmaf(f, v[k].x, sum.x); sum.y = fmaf(f, v[k].y, sum.y);
+                        sum.z = fmaf(f, v[k].z, sum.z); sum.w = fmaf(f, v[k].w, sum.w);
                     }
                 }
                 if (final) {
                     const float inv = total == 0.f ? 0.f : 1.f / total;
-                    Vec4<bf16>::store((bf16*)p.out + ((size_t)row * p.nh + h0 + r) * HD + d, make_float4(sum.x * inv, sum.y * inv, sum.z * inv, sum.w * inv));
+                    Vec4<bf16>::store((bf16*)p.out + ((size_t)s.row * p.nh + s.head + r) * HD + d, make_float4(sum.x * inv, sum.y * inv, sum.z * inv, sum.w * inv));
                 } else {  // over the first of the twelve, whose four sums this thread alone reads and writes
-                    *reinterpret_cast<float4*>(p.part_o + (place(from) * ROWS + r) * HD + d) = sum;
+                    *reinterpret_cast<float4*>(p.part_o + (place(s, from) * ROWS + r) * HD + d) = sum;
                     if (d == 0) {
-                        ml_s[r][0] = top;
-                        ml_s[r][1] = total;
+                        top_s[0][r] = top;
+                        total_s[0][r] = total;
                     }
                 }
             }
+            __syncthreads();  // (maxima and sums of the pieces are read by all; top_s and total_s are free)
             if (final) break;
-            __syncthreads();  // (their maxima and sums are read by all)
-            if (tid < rows) *reinterpret_cast<float2*>(p.part_ml + (place(from) * ROWS + tid) * 2) = make_float2(ml_s[tid][0], ml_s[tid][1]);
+            if (tid < s.heads) *reinterpret_cast<float2*>(p.part_ml + (place(s, from) * ROWS + tid) * 2) = make_float2(top_s[0][tid], total_s[0][tid]);
             from = 0;
-            count = (pieces + MERGE_AT_ONCE - 1) / MERGE_AT_ONCE;
+            count = (s.blocks + MERGE_AT_ONCE - 1) / MERGE_AT_ONCE;
             stride = MERGE_AT_ONCE;
-            counter = p.counters + segment;
             final = true;
+            __syncthreads();
+            if (tid == 0) sh[0] = count_in(p.counters + s.segment, count);
+            __syncthreads();
+            if (sh[0] == 0) break;
         }
-        __syncthreads();  // before last_s and ml_s are written again
     }
     cw_trace_end();
 }

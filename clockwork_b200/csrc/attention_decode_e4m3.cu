@@ -25,8 +25,8 @@
 //
 // A segment (request, KV head and group) that lies in one warp's run is finished by it.  At the end of its run a block adds up
 // its warps' pieces of shared segments in order; the pieces of one that several blocks share go to scratch of two per block, and
-// the block that comes last merges them in the blocks' order (more than 24: twelve at a time first, each by the last of the
-// twelve).  The result does not depend on who comes last.
+// the block that comes last merges them in the blocks' order (more than 24: eight at a time first, each by the last of the
+// eight).  The result does not depend on who comes last.
 #include "attention_mma.cuh"
 #include "kv_e4m3.cuh"
 
@@ -48,7 +48,10 @@ struct DecodeE4m3Params {
 
 #define TILE_TOKENS 32
 #define WARPS 4
-#define MERGE_AT_ONCE 12
+#define MERGE_AT_ONCE 8
+#ifndef LEAST_UNITS
+#define LEAST_UNITS 2
+#endif
 
 __device__ __forceinline__ void mma_half(float* d, const uint32_t* a, uint32_t b0, uint32_t b1) {
     asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
@@ -125,8 +128,7 @@ __global__ void __launch_bounds__(WARPS * 32, Stream<HD, NT>::PER_SM) decode_e4m
     __shared__ float m_s[2 * WARPS][ROWS], l_s[2 * WARPS][ROWS], f_s[2 * WARPS][ROWS];
     __shared__ Piece piece_s[2 * WARPS];  // of every warp: the end of a segment that began before its run, and what its run ends in
     __shared__ float top_s[2 * WARPS][ROWS], total_s[2 * WARPS][ROWS];  // of a group of pieces, at its first
-    __shared__ int sh[36];
-    __shared__ int last_s[2];
+    __shared__ int last_s[2], final_s;
     pdl_enter();
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
     const int per_request = p.nkv * p.groups;
@@ -139,23 +141,79 @@ __global__ void __launch_bounds__(WARPS * 32, Stream<HD, NT>::PER_SM) decode_e4m
         return ctx <= 0 ? 0 : (ctx + TILE_TOKENS - 1) / TILE_TOKENS - begin_of(ctx) / TILE_TOKENS;
     };
     // A segment is its tiles and, before them, a unit for what changing to it costs (about a tile's time).  A block's run is a
-    // whole number of equal runs for its warps.
+    // whole number of equal runs for its warps.  Every warp finds its own: four neighbouring requests per lane, 128 at a time.
     auto units_of = [&](int tiles) { return tiles > 0 ? per_request * (tiles + 1) : 0; };
-    const UnitRange range = units_of_block([&](int s) { return units_of(tiles_of(context_of(s))); }, p.requests, 1, gridDim.x * WARPS,
-                                           blockIdx.x * WARPS, sh);
-    const int block_units = range.quota * WARPS;
-    for (int s = blockIdx.x; s < p.requests; s += gridDim.x) {  // rows without a context: zeros
-        if (context_of(s) != 0) continue;
-        const int row = p.q_start != nullptr ? p.q_start[s] : s;
-        for (int i = tid; i < p.nh * HD; i += blockDim.x) ((bf16*)p.out)[(size_t)row * p.nh * HD + i] = __float2bfloat16_rn(0.f);
+    const int warps = gridDim.x * WARPS, chunks = (p.requests + 127) / 128;
+    int context[4], total = 0;
+    for (int c = chunks - 1; c >= 0; --c) {  // (the last one looked at is the first: what it holds is used again below)
+        int units = 0;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) context[j] = c * 128 + 4 * lane + j < p.requests ? context_of(c * 128 + 4 * lane + j) : -1;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) units += units_of(tiles_of(context[j]));
+        total += units;
     }
-    if (range.first >= range.last) return;
-    // ---- where this warp's run begins ----
-    const int first = range.first + warp * range.quota;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
+    const int quota = max(LEAST_UNITS, (total + warps - 1) / warps), block_units = quota * WARPS;
+    const int first = (int)min((long long)(blockIdx.x * WARPS + warp) * quota, (long long)total);
+    auto zeros = [&]() {  // the rows of requests without a context
+        for (int s = blockIdx.x; s < p.requests; s += gridDim.x) {
+            if (context_of(s) != 0) continue;
+            const int row = p.q_start != nullptr ? p.q_start[s] : s;
+            for (int i = tid; i < p.nh * HD; i += blockDim.x) ((bf16*)p.out)[(size_t)row * p.nh * HD + i] = __float2bfloat16_rn(0.f);
+        }
+    };
+    if ((long long)blockIdx.x * block_units >= total) {
+        zeros();
+        return;
+    }
     Walk at = {};
-    at.left = min(range.total, first + range.quota) - first;
+    at.left = min(total, first + quota) - first;
+    int seg_unit = 0;  // of the segment that the run stands in: the unit before its tiles
+    if (at.left > 0) {
+        int before = 0, skip = 0;
+        for (int c = 0; c < chunks; ++c) {
+            int units[4], sum = 0;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                if (c > 0) context[j] = c * 128 + 4 * lane + j < p.requests ? context_of(c * 128 + 4 * lane + j) : -1;
+                units[j] = units_of(tiles_of(context[j]));
+                sum += units[j];
+            }
+            int upto = sum;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const int v = __shfl_up_sync(0xffffffffu, upto, o);
+                if (lane >= o) upto += v;
+            }
+            const int chunk = __shfl_sync(0xffffffffu, upto, 31);
+            if (first < before + chunk) {
+                int from = before + upto - sum, mine = 0, ctx = context[0];
+#pragma unroll
+                for (int j = 0; j < 3; ++j)
+                    if (mine == j && first >= from + units[j]) {
+                        from += units[j];
+                        mine = j + 1;
+                        ctx = context[j + 1];
+                    }
+                const int who = __ffs(__ballot_sync(0xffffffffu, first < before + upto)) - 1;
+                skip = first - __shfl_sync(0xffffffffu, from, who);
+                at.s = c * 128 + 4 * who + __shfl_sync(0xffffffffu, mine, who);
+                at.ctx = __shfl_sync(0xffffffffu, ctx, who);
+                break;
+            }
+            before += chunk;
+        }
+        at.tiles = max(1, tiles_of(at.ctx));
+        at.begin = begin_of(at.ctx);
+        at.seg = skip / (at.tiles + 1);
+        skip -= at.seg * (at.tiles + 1);
+        seg_unit = first - skip;
+        at.tile = max(0, skip - 1);
+        if (skip == 0) --at.left;
+    }
     auto enter = [&](Walk& w, int s) {  // the next request from s on that has tiles
-        w.seg = w.tile = 0;
         for (; s < p.requests; ++s) {
             w.s = s;
             w.ctx = context_of(s);
@@ -164,7 +222,20 @@ __global__ void __launch_bounds__(WARPS * 32, Stream<HD, NT>::PER_SM) decode_e4m
             if (w.tiles > 0) return;
         }
         w.ctx = 0;  // (lengths that change under the call: tokens that do not count)
-        w.tiles = 0x7FFFFFFF / per_request - 1;
+        w.tiles = 0x7FFFFFFF;
+    };
+    // where a segment's queries are, and how many heads it has
+    auto query_row = [&](const Walk& w) { return p.q_start != nullptr ? p.q_start[w.s] : w.s; };
+    auto first_head = [&](const Walk& w) {
+        return p.groups == 1 ? w.seg * p.heads_each : w.seg / p.groups * (p.nh / p.nkv) + w.seg % p.groups * p.heads_each;
+    };
+    auto heads_of = [&](const Walk& w) { return p.groups == 1 ? p.heads_each : min(p.heads_each, p.nh / p.nkv - w.seg % p.groups * p.heads_each); };
+    auto call_queries = [&](const Walk& w) {  // brings a segment's queries near, ahead of their use
+        const bf16* q = (const bf16*)p.q + (size_t)query_row(w) * p.q_stride + (size_t)first_head(w) * HD;
+        for (int i = lane * 16; i < heads_of(w) * HD; i += 512) {  // a sector each
+            uint32_t unused;
+            asm volatile("ld.global.u32 %0, [%1];" : "=r"(unused) : "l"(q + i));
+        }
     };
     auto step = [&](Walk& w, int tiles) {  // so many tiles on within its segment, and on to the next one's first
         w.tile += tiles;
@@ -172,23 +243,14 @@ __global__ void __launch_bounds__(WARPS * 32, Stream<HD, NT>::PER_SM) decode_e4m
         if (w.tile == w.tiles) {
             w.tile = 0;
             --w.left;
-            if (++w.seg == per_request && w.left > 0) enter(w, w.s + 1);
+            if (++w.seg == per_request) {
+                w.seg = 0;
+                if (w.left > 0) enter(w, w.s + 1);
+            }
+            return w.left > 0;
         }
+        return false;  // (whether it stands in a new segment)
     };
-    int seg_unit = 0;  // of the segment that the run stands in: the unit before its tiles
-    if (at.left > 0) {
-        int skip = range.offset + warp * range.quota;
-        enter(at, range.request);
-        while (skip >= units_of(at.tiles)) {
-            skip -= units_of(at.tiles);
-            enter(at, at.s + 1);
-        }
-        at.seg = skip / (at.tiles + 1);
-        skip -= at.seg * (at.tiles + 1);
-        seg_unit = first - skip;
-        at.tile = max(0, skip - 1);
-        if (skip == 0) --at.left;
-    }
     uint8_t* my_ring = ring_s + warp * ST * 2 * C::TILE_BYTES;
     const uint32_t my_ring_addr = smem_addr(my_ring);
     // ---- fetching: ST - 1 tiles ahead of the products, through the segments' ends ----
@@ -228,8 +290,9 @@ __global__ void __launch_bounds__(WARPS * 32, Stream<HD, NT>::PER_SM) decode_e4m
                 copy16(dst + C::TILE_BYTES, p.v + src, there);
             }
             if (++fetch_stage == ST) fetch_stage = 0;
-            step(ahead, 1);
+            const bool other = step(ahead, 1);
             look_up();
+            if (other) call_queries(ahead);
         }
         cp_async_commit();
     };
@@ -242,6 +305,8 @@ __global__ void __launch_bounds__(WARPS * 32, Stream<HD, NT>::PER_SM) decode_e4m
         v_power = p.v_exp[i];
     };
     look_up();
+    if (at.left > 0) call_queries(at);
+#pragma unroll 1
     for (int i = 0; i < ST - 1; ++i) fetch();
     __syncwarp();
     int stage = 0;
@@ -251,9 +316,7 @@ __global__ void __launch_bounds__(WARPS * 32, Stream<HD, NT>::PER_SM) decode_e4m
     const int k_at = C::at(g, HD % 64 == 0 ? t : t >> 1) + (HD % 64 == 0 ? 0 : 8 * (t & 1));
     constexpr int PIECE = HD % 64 == 0 ? 16 : 8, STEPS = PIECE / 4, PIECES = HD / (4 * PIECE);
     while (at.left > 0) {
-        const int row = p.q_start != nullptr ? p.q_start[at.s] : at.s;
-        const int part = p.groups == 1 ? 0 : at.seg % p.groups, kvh = p.groups == 1 ? at.seg : at.seg / p.groups;
-        const int h0 = kvh * (p.nh / p.nkv) + part * p.heads_each, rows = min(p.heads_each, p.nh / p.nkv - part * p.heads_each);
+        const int row = query_row(at), h0 = first_head(at), rows = heads_of(at);
         const int n_tiles = min(at.tiles - at.tile, at.left);
         // ---- the group's queries, as B fragments over the entries that a lane's pieces of K hold: half precision, a power of two out ----
         uint32_t qb[NT][PIECES][STEPS][2];
@@ -471,70 +534,81 @@ __global__ void __launch_bounds__(WARPS * 32, Stream<HD, NT>::PER_SM) decode_e4m
     }
     cp_async_wait<0>();
     __syncthreads();
-    // ---- the block's pieces, in order: neighbours of one segment are added up ----
-    auto same = [&](int x, int y) { return piece_s[y].segment == piece_s[x].segment; };  // (pieces of one segment are neighbours)
-    for (int i = tid; i < 2 * WARPS * ROWS; i += blockDim.x) {  // what each is multiplied by; the sum of weights at the group's first
+    // ---- the block's pieces, in order: those of one segment, which are neighbours, are added up ----
+    const int segment_of_lane = lane < 2 * WARPS ? piece_s[lane].segment : -2 - lane;
+    const uint32_t alike = __match_any_sync(0xffffffffu, segment_of_lane);
+    const uint32_t leads = __ballot_sync(0xffffffffu, segment_of_lane >= 0 && (alike & ((1u << lane) - 1)) == 0);
+    for (int i = tid; i < 2 * WARPS * ROWS; i += blockDim.x) {  // what each piece is multiplied by; the sum of weights at the group's first
         const int x = i / ROWS, r = i % ROWS;
-        if (piece_s[x].segment < 0) continue;
-        float top = -INFINITY, total = 0.f;
-        bool leads = true;
-        for (int y = 0; y < 2 * WARPS; ++y)
-            if (same(x, y)) {
-                top = fmaxf(top, m_s[y][r]);
-                leads = leads && y >= x;
-            }
-        for (int y = 0; y < 2 * WARPS; ++y)
-            if (leads && same(x, y) && m_s[y][r] != -INFINITY) total = fmaf(fast_exp2(m_s[y][r] - top), l_s[y][r], total);
-        f_s[x][r] = m_s[x][r] == -INFINITY ? 0.f : fast_exp2(m_s[x][r] - top);
-        if (leads) {
-            top_s[x][r] = top;
-            total_s[x][r] = total;
+        const uint32_t group = __shfl_sync(0xffffffffu, alike, x);
+        float m[2 * WARPS], top = -INFINITY, sum = 0.f;
+#pragma unroll
+        for (int y = 0; y < 2 * WARPS; ++y) {
+            m[y] = (group >> y) & 1 ? m_s[y][r] : -INFINITY;
+            top = fmaxf(top, m[y]);
         }
+#pragma unroll
+        for (int y = 0; y < 2 * WARPS; ++y)
+            if (m[y] != -INFINITY) sum = fmaf(fast_exp2(m[y] - top), l_s[y][r], sum);
+        const float own = m_s[x][r];
+        f_s[x][r] = own == -INFINITY ? 0.f : fast_exp2(own - top);
+        top_s[x][r] = top;
+        total_s[x][r] = sum;
     }
     __syncthreads();
     int came = -1, goes = -1;  // first pieces of the two segments, at most, that blocks before and after this one have pieces of as well
-    for (int x = 0; x < 2 * WARPS;) {
-        int end = x + 1;
-        if (piece_s[x].segment >= 0) {
-            while (end < 2 * WARPS && (piece_s[end].segment < 0 || same(x, end))) ++end;
-            const Piece& s = piece_s[x];
-            const int my_piece = 2 * blockIdx.x + (blockIdx.x == s.first_block ? 1 : 0);
-            if (s.blocks > 1 && blockIdx.x == s.first_block) goes = x;
-            if (s.blocks > 1 && blockIdx.x != s.first_block) came = x;
 #pragma unroll 1
-            for (int i = tid; i < s.heads * (HD / 4); i += blockDim.x) {
-                const int r = i / (HD / 4), d = i % (HD / 4) * 4;
+    for (uint32_t todo = leads; todo != 0; todo &= todo - 1) {
+        const int x = __ffs(todo) - 1;
+        const uint32_t group = __shfl_sync(0xffffffffu, alike, x);
+        const int head = __ffs(group & 0x55) - 1;  // the one piece, if any, that lies in global memory
+        const Piece& s = piece_s[x];
+        const bool whole = s.blocks == 1, begins_here = blockIdx.x == s.first_block;
+        if (!whole) (begins_here ? goes : came) = x;
+        float* part = p.part_o + (size_t)(2 * blockIdx.x + begins_here) * ROWS * HD;
+        const int items = s.heads * (HD / 4);
+#pragma unroll 1
+        for (int i0 = tid; i0 < items; i0 += 2 * WARPS * 32) {  // four outputs each, two such at a time: all loads before their use
+            float4 v[2][WARPS + 1];
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                const int i = i0 + e * WARPS * 32;
+                v[e][WARPS] = make_float4(0.f, 0.f, 0.f, 0.f);
+                if (head >= 0 && i < items) v[e][WARPS] = *reinterpret_cast<const float4*>(p.heads_o + (size_t)(blockIdx.x * WARPS + (head >> 1)) * ROWS * HD + i * 4);
+#pragma unroll
+                for (int w = 0; w < WARPS; ++w)
+                    v[e][w] = i < items && (group >> (2 * w + 1)) & 1 ? *reinterpret_cast<const float4*>(ring_s + w * ST * 2 * C::TILE_BYTES + i * 16)
+                                                                      : make_float4(0.f, 0.f, 0.f, 0.f);
+            }
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                const int i = i0 + e * WARPS * 32, r = i / (HD / 4);
+                if (i >= items) break;
                 float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 1
-                for (int y = x; y < end; ++y) {
-                    if (piece_s[y].segment < 0) continue;
-                    float4 v;
-                    if (y & 1)
-                        v = *reinterpret_cast<const float4*>(ring_s + (y >> 1) * ST * 2 * C::TILE_BYTES + (r * HD + d) * 4);
-                    else
-                        v = *reinterpret_cast<const float4*>(p.heads_o + ((size_t)(blockIdx.x * WARPS + (y >> 1)) * ROWS + r) * HD + d);
-                    const float f = f_s[y][r];
-                    sum.x = fmaf(f, v.x, sum.x); sum.y = fmaf(f, v.y, sum.y); sum.z = fmaf(f, v.z, sum.z); sum.w = fmaf(f, v.w, sum.w);
+#pragma unroll
+                for (int w = 0; w <= WARPS; ++w) {
+                    const float f = w < WARPS ? ((group >> (2 * w + 1)) & 1 ? f_s[2 * w + 1][r] : 0.f) : head >= 0 ? f_s[head][r] : 0.f;
+                    sum.x = fmaf(f, v[e][w].x, sum.x); sum.y = fmaf(f, v[e][w].y, sum.y); sum.z = fmaf(f, v[e][w].z, sum.z); sum.w = fmaf(f, v[e][w].w, sum.w);
                 }
                 const float total = total_s[x][r];
-                if (s.blocks == 1) {
+                if (whole) {
                     const float inv = total == 0.f ? 0.f : 1.f / total;
-                    Vec4<bf16>::store((bf16*)p.out + ((size_t)s.row * p.nh + s.head + r) * HD + d, make_float4(sum.x * inv, sum.y * inv, sum.z * inv, sum.w * inv));
+                    Vec4<bf16>::store((bf16*)p.out + ((size_t)s.row * p.nh + s.head) * HD + i * 4, make_float4(sum.x * inv, sum.y * inv, sum.z * inv, sum.w * inv));
                 } else {
-                    *reinterpret_cast<float4*>(p.part_o + ((size_t)my_piece * ROWS + r) * HD + d) = sum;
-                    if (d == 0) *reinterpret_cast<float2*>(p.part_ml + ((size_t)my_piece * ROWS + r) * 2) = make_float2(top_s[x][r], total);
+                    *reinterpret_cast<float4*>(part + i * 4) = sum;
+                    if (i % (HD / 4) == 0) *reinterpret_cast<float2*>(p.part_ml + ((size_t)(2 * blockIdx.x + begins_here) * ROWS + r) * 2) = make_float2(top_s[x][r], total);
                 }
             }
         }
-        x = end;
     }
+    zeros();
     if (came < 0 && goes < 0) {
         cw_trace_end();
         return;
     }
     // ---- segments that other blocks have pieces of: thread e counts this block in at segment e's counter ----
     // (pieces by number: y is of block first_block + y, its second one where the segment begins in it)
-    auto twelves = [&](const Piece& s) { return s.blocks > 2 * MERGE_AT_ONCE; };  // added up by twelves first
+    auto by_eights = [&](const Piece& s) { return s.blocks > 3 * MERGE_AT_ONCE; };  // added up by eights first
     auto place = [&](const Piece& s, int y) { return (size_t)2 * (s.first_block + y) + (y == 0 ? 1 : 0); };
     // the barrier orders all threads' stores before the release; the last block's acquire, followed by the next barrier, its
     // threads' loads behind everybody's stores
@@ -551,7 +625,7 @@ __global__ void __launch_bounds__(WARPS * 32, Stream<HD, NT>::PER_SM) decode_e4m
         if (x >= 0) {
             const Piece& s = piece_s[x];
             const int y = blockIdx.x - s.first_block, from = y - y % MERGE_AT_ONCE;
-            if (twelves(s))
+            if (by_eights(s))
                 is_last = count_in(p.counters + p.requests * per_request + place(s, from), min(MERGE_AT_ONCE, s.blocks - from));
             else
                 is_last = count_in(p.counters + s.segment, s.blocks);
@@ -564,51 +638,67 @@ __global__ void __launch_bounds__(WARPS * 32, Stream<HD, NT>::PER_SM) decode_e4m
         if (!last_s[e]) continue;
         const Piece s = piece_s[e == 0 ? came : goes];
         const int y = blockIdx.x - s.first_block;
-        bool final = !twelves(s);
+        bool final = !by_eights(s);
         int from = final ? 0 : y - y % MERGE_AT_ONCE, count = final ? s.blocks : min(MERGE_AT_ONCE, s.blocks - from), stride = 1;
 #pragma unroll 1
         for (;;) {
+            const int items = s.heads * (HD / 4);
 #pragma unroll 1
-            for (int i = tid; i < s.heads * (HD / 4); i += blockDim.x) {
-                const int r = i / (HD / 4), d = i % (HD / 4) * 4;
-                float top = -INFINITY, total = 0.f;
-                float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+            for (int i0 = tid; i0 < items; i0 += 2 * WARPS * 32) {  // two at a time, eight pieces of each: one trip to the L2
+                float top[2] = {-INFINITY, -INFINITY}, total[2] = {0.f, 0.f};
+                float4 sum[2] = {make_float4(0.f, 0.f, 0.f, 0.f), make_float4(0.f, 0.f, 0.f, 0.f)};
 #pragma unroll 1
                 for (int y0 = 0; y0 < count; y0 += MERGE_AT_ONCE) {
-                    float2 ml[MERGE_AT_ONCE];
-                    float4 v[MERGE_AT_ONCE];
+                    float2 ml[2][MERGE_AT_ONCE];
+                    float4 v[2][MERGE_AT_ONCE];
+                    // (in units of a piece's rows; the segment's very first piece lies one further)
+                    size_t at_piece = (size_t)2 * (s.first_block + from + y0 * stride);
 #pragma unroll
                     for (int k = 0; k < MERGE_AT_ONCE; ++k) {
-                        ml[k] = make_float2(-INFINITY, 0.f);
-                        v[k] = make_float4(0.f, 0.f, 0.f, 0.f);
-                        if (y0 + k < count) {
-                            const size_t i_at = place(s, from + (y0 + k) * stride) * ROWS + r;
-                            ml[k] = __ldcg(reinterpret_cast<const float2*>(p.part_ml) + i_at);
-                            v[k] = __ldcg(reinterpret_cast<const float4*>(p.part_o + i_at * HD + d));
+                        const size_t here = (at_piece + (k == 0 && from + y0 == 0 ? 1 : 0)) * ROWS;
+#pragma unroll
+                        for (int e = 0; e < 2; ++e) {
+                            const int i = i0 + e * WARPS * 32;
+                            ml[e][k] = make_float2(-INFINITY, 0.f);
+                            v[e][k] = make_float4(0.f, 0.f, 0.f, 0.f);
+                            if (y0 + k < count && i < items) {
+                                ml[e][k] = __ldcg(reinterpret_cast<const float2*>(p.part_ml) + here + i / (HD / 4));
+                                v[e][k] = __ldcg(reinterpret_cast<const float4*>(p.part_o + here * HD) + i);
+                            }
+                        }
+                        at_piece += 2 * stride;
+                    }
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) {
+                        float next = top[e];
+#pragma unroll
+                        for (int k = 0; k < MERGE_AT_ONCE; ++k) next = fmaxf(next, ml[e][k].x);
+                        const float keep = top[e] == -INFINITY ? 0.f : fast_exp2(top[e] - next);
+                        total[e] *= keep; sum[e].x *= keep; sum[e].y *= keep; sum[e].z *= keep; sum[e].w *= keep;
+                        top[e] = next;
+#pragma unroll
+                        for (int k = 0; k < MERGE_AT_ONCE; ++k) {
+                            const float f = ml[e][k].x == -INFINITY ? 0.f : fast_exp2(ml[e][k].x - next);
+                            total[e] = fmaf(f, ml[e][k].y, total[e]);
+                            sum[e].x = fmaf(f, v[e][k].x, sum[e].x); sum[e].y = fmaf(f, v[e][k].y, sum[e].y);
+                            sum[e].z = fmaf(f, v[e][k].z, sum[e].z); sum[e].w = fmaf(f, v[e][k].w, sum[e].w);
                         }
                     }
-                    float next = top;
-#pragma unroll
-                    for (int k = 0; k < MERGE_AT_ONCE; ++k) next = fmaxf(next, ml[k].x);
-                    const float keep = top == -INFINITY ? 0.f : fast_exp2(top - next);
-                    total *= keep; sum.x *= keep; sum.y *= keep; sum.z *= keep; sum.w *= keep;
-                    top = next;
-#pragma unroll
-                    for (int k = 0; k < MERGE_AT_ONCE; ++k) {
-                        const float f = ml[k].x == -INFINITY ? 0.f : fast_exp2(ml[k].x - top);
-                        total = fmaf(f, ml[k].y, total);
-                        sum.x = fmaf(f, v[k].x, sum.x); sum.y = fmaf(f, v[k].y, sum.y);
-                        sum.z = fmaf(f, v[k].z, sum.z); sum.w = fmaf(f, v[k].w, sum.w);
-                    }
                 }
-                if (final) {
-                    const float inv = total == 0.f ? 0.f : 1.f / total;
-                    Vec4<bf16>::store((bf16*)p.out + ((size_t)s.row * p.nh + s.head + r) * HD + d, make_float4(sum.x * inv, sum.y * inv, sum.z * inv, sum.w * inv));
-                } else {  // over the first of the twelve, whose four sums this thread alone reads and writes
-                    *reinterpret_cast<float4*>(p.part_o + (place(s, from) * ROWS + r) * HD + d) = sum;
-                    if (d == 0) {
-                        top_s[0][r] = top;
-                        total_s[0][r] = total;
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    const int i = i0 + e * WARPS * 32;
+                    if (i >= items) break;
+                    if (final) {
+                        const float inv = total[e] == 0.f ? 0.f : 1.f / total[e];
+                        Vec4<bf16>::store((bf16*)p.out + ((size_t)s.row * p.nh + s.head) * HD + i * 4,
+                                          make_float4(sum[e].x * inv, sum[e].y * inv, sum[e].z * inv, sum[e].w * inv));
+                    } else {  // over the first of the eight, whose four sums this thread alone reads and writes
+                        *reinterpret_cast<float4*>(p.part_o + place(s, from) * ROWS * HD + i * 4) = sum[e];
+                        if (i % (HD / 4) == 0) {
+                            top_s[0][i / (HD / 4)] = top[e];
+                            total_s[0][i / (HD / 4)] = total[e];
+                        }
                     }
                 }
             }
@@ -620,9 +710,9 @@ __global__ void __launch_bounds__(WARPS * 32, Stream<HD, NT>::PER_SM) decode_e4m
             stride = MERGE_AT_ONCE;
             final = true;
             __syncthreads();
-            if (tid == 0) sh[0] = count_in(p.counters + s.segment, count);
+            if (tid == 0) final_s = count_in(p.counters + s.segment, count);
             __syncthreads();
-            if (sh[0] == 0) break;
+            if (final_s == 0) break;
         }
     }
     cw_trace_end();

@@ -832,10 +832,17 @@ extern "C" int cw_attention_decode_e4m3_scratch(int requests, int nh, int nkv, i
 
 // q [rows, q_stride >= nh * hd], out [rows, nh * hd]; request s owns row s, or with q_start rows q_start[s] .. q_start[s + 1], and
 // then only requests with one row are served.  A context of length 0 gives zeros.  `floats`, `words`: the scratch.
-extern "C" int cw_attention_decode_e4m3(const void* q, int q_stride, void* out, const uint8_t* k, const uint8_t* v, const uint8_t* k_exp,
-                                        const uint8_t* v_exp, const int* block_tables, const int* ctx_lens, const int* q_start,
-                                        int requests, int nh, int nkv, int hd, int page_size, int max_blocks, int num_pages, int window,
-                                        float scale, int dtype, int sms, float* floats, int* words, int* status, cudaStream_t stream) {
+extern "C" int cw_attention_decode_e4m3(const char* block) {
+    ArgumentWords w(block);
+    const void* q = w.pointer(); void* out = w.pointer();
+    const uint8_t *k = (const uint8_t*)w.pointer(), *v = (const uint8_t*)w.pointer(), *k_exp = (const uint8_t*)w.pointer(), *v_exp = (const uint8_t*)w.pointer();
+    const int *block_tables = (const int*)w.pointer(), *ctx_lens = (const int*)w.pointer(), *q_start = (const int*)w.pointer();
+    float* floats = (float*)w.pointer();
+    int *words = (int*)w.pointer(), *status = (int*)w.pointer();
+    const cudaStream_t stream = (cudaStream_t)w.pointer();
+    const int q_stride = w.number(), requests = w.number(), nh = w.number(), nkv = w.number(), hd = w.number(), page_size = w.number(),
+              max_blocks = w.number(), num_pages = w.number(), window = w.number(), dtype = w.number(), sms = w.number();
+    const float scale = (float)w.real();
     if (requests == 0) return CW_OK;
     if (requests < 0 || nh <= 0 || nkv <= 0 || nh % nkv || hd <= 0 || hd % 16 || hd > 256 || page_size <= 0 || max_blocks <= 0 ||
         num_pages <= 0 || window < 0 || q_stride < nh * hd || ((uintptr_t)k | (uintptr_t)v) % 16 || requests > 65535 || sms <= 0 ||

@@ -190,10 +190,19 @@ static int store_launch(const StoreParams& p, int N, cudaStream_t stream) {
 
 // q_out [N, nh * hd]; slots[t] < 0: the token is not stored.  k_exp and v_exp null: the cache is of the run's type.
 // rot 0: nothing turns (inv_freq may be null).  The norms' weights are float32 [hd] or null.
-extern "C" int cw_norm_rotate_store(const void* qkv, void* q_out, const int* positions, const int* slots, const float* inv_freq,
-                                    const float* q_weight, const float* k_weight, void* k_cache, void* v_cache, uint8_t* k_exp,
-                                    uint8_t* v_exp, int N, int nh, int nkv, int hd, int rot, int page_size, int num_pages, float eps,
-                                    int dtype, int* status, cudaStream_t stream) {
+// The arguments come as one block of words (kv_e4m3.cuh), in the order of the names below.
+extern "C" int cw_norm_rotate_store(const char* block) {
+    ArgumentWords w(block);
+    const void* qkv = w.pointer(); void* q_out = w.pointer();
+    const int *positions = (const int*)w.pointer(), *slots = (const int*)w.pointer();
+    const float *inv_freq = (const float*)w.pointer(), *q_weight = (const float*)w.pointer(), *k_weight = (const float*)w.pointer();
+    void *k_cache = w.pointer(), *v_cache = w.pointer();
+    uint8_t *k_exp = (uint8_t*)w.pointer(), *v_exp = (uint8_t*)w.pointer();
+    int* status = (int*)w.pointer();
+    const cudaStream_t stream = (cudaStream_t)w.pointer();
+    const int N = w.number(), nh = w.number(), nkv = w.number(), hd = w.number(), rot = w.number(), page_size = w.number(), num_pages = w.number(),
+              dtype = w.number();
+    const float eps = (float)w.real();
     if (N == 0) return CW_OK;
     if (N < 0 || nh <= 0 || nkv <= 0 || hd <= 0 || hd > 256 || rot < 0 || rot > hd || rot % 2 || page_size <= 0 || num_pages <= 0 ||
         (long long)num_pages * page_size > 0x7FFFFFFF || (rot > 0 && inv_freq == nullptr) || (k_exp == nullptr) != (v_exp == nullptr))
@@ -269,10 +278,15 @@ __global__ void __launch_bounds__(256) read_pages_kernel(const ReadParams p) {
 
 // q_start (or null): only requests with at least `least_rows` rows (1 or more) are read.  window > 0: from the page on that the first of a request's
 // rows (its last position without q_start) still sees.
-extern "C" int cw_read_pages(const uint8_t* k, const uint8_t* v, const uint8_t* k_exp, const uint8_t* v_exp, void* k_out, void* v_out,
-                             const int* block_tables, const int* ctx_lens, const int* q_start, int requests, int nkv, int hd,
-                             int page_size, int max_blocks, int num_pages, int window, int least_rows, int blocks, int dtype,
-                             int* status, cudaStream_t stream) {
+extern "C" int cw_read_pages(const char* block) {
+    ArgumentWords w(block);
+    const uint8_t *k = (const uint8_t*)w.pointer(), *v = (const uint8_t*)w.pointer(), *k_exp = (const uint8_t*)w.pointer(), *v_exp = (const uint8_t*)w.pointer();
+    void *k_out = w.pointer(), *v_out = w.pointer();
+    const int *block_tables = (const int*)w.pointer(), *ctx_lens = (const int*)w.pointer(), *q_start = (const int*)w.pointer();
+    int* status = (int*)w.pointer();
+    const cudaStream_t stream = (cudaStream_t)w.pointer();
+    const int requests = w.number(), nkv = w.number(), hd = w.number(), page_size = w.number(), max_blocks = w.number(), num_pages = w.number(),
+              window = w.number(), least_rows = w.number(), blocks = w.number(), dtype = w.number();
     if (requests == 0) return CW_OK;
     if (requests < 0 || nkv <= 0 || hd <= 0 || hd % 16 || page_size <= 0 || max_blocks <= 0 || num_pages <= 0 || window < 0 || blocks <= 0 || least_rows < 1 ||
         !aligned(k, 16) || !aligned(v, 16) || !aligned(k_out, 16) || !aligned(v_out, 16) ||

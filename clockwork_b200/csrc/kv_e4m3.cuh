@@ -10,7 +10,28 @@
 #pragma once
 #include <cuda_fp16.h>
 #include <cuda_fp8.h>
+#include <string.h>
 #include "common.cuh"
+
+// Arguments of an entry point as one block of 8-byte words, read in order.  Whole numbers that no int holds become -1, which every
+// entry point refuses as a size.
+struct ArgumentWords {
+    const char* at;
+    explicit ArgumentWords(const char* block) : at(block) {}
+    template <typename T>
+    T next() {
+        T x;
+        memcpy(&x, at, sizeof(T));
+        at += sizeof(T);
+        return x;
+    }
+    void* pointer() { return (void*)next<uint64_t>(); }
+    int number() {
+        const long long x = next<long long>();
+        return x < -1 || x > 0x7FFFFFFF ? -1 : (int)x;
+    }
+    double real() { return next<double>(); }
+};
 
 #define KV_BIGGEST __int_as_float(0x7F700000)  // 1.875 * 2^127
 

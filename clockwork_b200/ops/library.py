@@ -4,7 +4,7 @@ from __future__ import annotations
 
 import ctypes
 import threading
-from ctypes import c_float, c_int, c_longlong, c_void_p
+from ctypes import c_char_p, c_float, c_int, c_longlong, c_void_p
 
 _lock = threading.Lock()
 _lib: ctypes.CDLL | None = None
@@ -78,9 +78,7 @@ _SIGNATURES: dict[str, list] = {
     "cw_latent_attention": [P, P, P, P, P, P, P, I, P, I, I, I, I, I, I, I, F, I, I, P, I, P, P],
     "cw_latent_attention_on_tensor_cores": [I, I],
     # a cache in 8 bits (csrc/kv_e4m3.cu, csrc/attention_decode_e4m3.cu)
-    "cw_norm_rotate_store": [P, P, P, P, P, P, P, P, P, P, P, I, I, I, I, I, I, I, F, I, P, P],
-    "cw_read_pages": [P, P, P, P, P, P, P, P, P, I, I, I, I, I, I, I, I, I, I, P, P],
-    "cw_attention_decode_e4m3": [P, I, P, P, P, P, P, P, P, P, I, I, I, I, I, I, I, I, F, I, I, P, P, P, P],
+    "cw_norm_rotate_store": [c_char_p], "cw_read_pages": [c_char_p], "cw_attention_decode_e4m3": [c_char_p],
     "cw_attention_decode_e4m3_scratch": [I, I, I, I, I, I, P, P],
 }
 _OPTIONAL: dict[str, list] = {}

@@ -13,12 +13,19 @@ from __future__ import annotations
 
 import ctypes
 import functools
+import struct
 from typing import NamedTuple
 
 import torch
 
-from . import _ptr, _stream, dtype_code
+from . import _stream, dtype_code
 from .library import check, library
+
+# The entry points of this module take one block of words (pointers and whole numbers, then the floats), which costs a third of what
+# as many ctypes arguments do: 2 of 5 us of a call whose kernel may take 4.
+_STORE_ARGS = struct.Struct("21qd").pack
+_READ_ARGS = struct.Struct("21q").pack
+_DECODE_ARGS = struct.Struct("24qd").pack
 
 CODES = torch.float8_e4m3fn
 MAX_HEAD_DIM = 256
@@ -47,54 +54,56 @@ def allocate_pages(num_pages: int, page_size: int, num_kv_heads: int, head_dim: 
     return E4M3Pages(codes[0], codes[1], exps[0], exps[1])
 
 
-def _check_device(t: torch.Tensor) -> None:
-    if not t.is_cuda:
+def _check_device(index: int) -> None:
+    """``index``: the tensors' ``get_device()``."""
+    if index < 0:
         raise ValueError("the tensors must be CUDA tensors (no CPU path exists)")
-    if t.get_device() != torch.cuda.current_device():
-        raise ValueError(f"the tensors are on {t.device}, the current device is cuda:{torch.cuda.current_device()}")
+    if index != torch.cuda.current_device():
+        raise ValueError(f"the tensors are on cuda:{index}, the current device is cuda:{torch.cuda.current_device()}")
 
 
-def _same_place(device: torch.device, **tensors) -> None:
+def _elsewhere(index: int, **tensors) -> None:
     for name, t in tensors.items():
-        if t is not None and t.device != device:
-            raise ValueError(f"{name} is on {t.device}, expected {device}")
+        if t is not None and t.get_device() != index:
+            raise ValueError(f"{name} is on {t.device}, the others are not")
 
 
 def _ints(t: torch.Tensor, name: str, ndim: int, entries: int | None = None) -> None:
-    if t.dtype != torch.int32 or t.dim() != ndim or not t.is_contiguous():
+    if t.dtype is not torch.int32 or t.dim() != ndim or not t.is_contiguous():
         raise ValueError(f"{name} must be a contiguous int32 tensor of {ndim} dimension(s)")
     if entries is not None and t.shape[0] != entries:
         raise ValueError(f"{name} must have {entries} entries, got {t.shape[0]}")
 
 
 def _check_status(status: torch.Tensor) -> None:
-    if status.dtype != torch.int32 or status.numel() < 4:
+    if status.dtype is not torch.int32 or status.numel() < 4:
         raise ValueError("status must be 4 int32 words (ops.new_status)")
 
 
-def check_pages(cache: E4M3Pages) -> None:
-    """Refuses codes and powers whose types, shapes or layouts do not belong together."""
+_PAGE_TYPES = (CODES, CODES, torch.uint8, torch.uint8)
+
+
+def check_pages(cache: E4M3Pages) -> tuple[int, int, int, int]:
+    """(pages, page_size, nkv, hd) of a cache; refuses codes and powers whose types, shapes or layouts do not belong together."""
     if not isinstance(cache, E4M3Pages):
         raise ValueError(f"an 8-bit cache (E4M3Pages) is needed, got {type(cache).__name__}")
     k, v, ke, ve = cache
-    if k.dtype != CODES or v.dtype != CODES or ke.dtype != torch.uint8 or ve.dtype != torch.uint8:
+    if (k.dtype, v.dtype, ke.dtype, ve.dtype) != _PAGE_TYPES:
         raise ValueError("codes must be float8_e4m3fn and powers uint8")
-    if k.dim() != 4 or k.shape != v.shape or ke.shape != ve.shape or tuple(ke.shape) != (k.shape[0], k.shape[2], k.shape[1]):
+    shape = k.shape
+    if len(shape) != 4 or v.shape != shape or ke.shape != (shape[0], shape[2], shape[1]) or ve.shape != ke.shape:
         raise ValueError(f"codes {tuple(k.shape)}, {tuple(v.shape)} and powers {tuple(ke.shape)}, {tuple(ve.shape)} do not belong together: "
                          "[pages, page_size, nkv, hd] and [pages, nkv, page_size]")
     if not (k.is_contiguous() and v.is_contiguous() and ke.is_contiguous() and ve.is_contiguous()):
         raise ValueError("codes and powers must be contiguous")
-    if k.shape[0] * k.shape[1] >= 1 << 31:
+    if shape[0] * shape[1] >= 1 << 31:
         raise ValueError("a cache holds fewer than 2^31 slots")
     if (k.data_ptr() | v.data_ptr()) % 16:
         raise ValueError("codes must start at a multiple of 16 bytes")
-    if not k.device == v.device == ke.device == ve.device:
+    index = k.get_device()
+    if v.get_device() != index or ke.get_device() != index or ve.get_device() != index:
         raise ValueError("codes and powers must be on one device")
-
-
-def _check_heads(cache, num_kv_heads: int, head_dim: int) -> None:
-    if tuple(cache.k.shape[2:]) != (num_kv_heads, head_dim):
-        raise ValueError(f"the cache holds {tuple(cache.k.shape[2:])} KV heads and entries, expected {(num_kv_heads, head_dim)}")
+    return shape
 
 
 def norm_rotate_store(qkv: torch.Tensor, positions: torch.Tensor, slots: torch.Tensor, inv_freq: torch.Tensor | None, cache,
@@ -116,11 +125,14 @@ def norm_rotate_store(qkv: torch.Tensor, positions: torch.Tensor, slots: torch.T
     _check_status(status)
     quantised = isinstance(cache, E4M3Pages)
     if quantised:
-        check_pages(cache)
+        shape = check_pages(cache)
     elif cache.k.dtype != qkv.dtype or cache.v.dtype != qkv.dtype or cache.k.dim() != 4 or cache.k.shape != cache.v.shape or \
             not (cache.k.is_contiguous() and cache.v.is_contiguous()):
         raise ValueError("a plain cache is two contiguous [pages, page_size, nkv, hd] tensors of qkv's type")
-    _check_heads(cache, num_kv_heads, head_dim)
+    else:
+        shape = cache.k.shape
+    if shape[2] != num_kv_heads or shape[3] != head_dim:
+        raise ValueError(f"the cache holds {tuple(shape[2:])} KV heads and entries, expected {(num_kv_heads, head_dim)}")
     rot = 0
     if inv_freq is not None:
         if inv_freq.dtype != torch.float32 or inv_freq.dim() != 1 or not inv_freq.is_contiguous():
@@ -131,14 +143,16 @@ def norm_rotate_store(qkv: torch.Tensor, positions: torch.Tensor, slots: torch.T
     for name, w in (("q_weight", q_weight), ("k_weight", k_weight)):
         if w is not None and (w.dtype != torch.float32 or tuple(w.shape) != (head_dim,) or not w.is_contiguous()):
             raise ValueError(f"{name} must be contiguous float32 [{head_dim}]")
-    _same_place(qkv.device, positions=positions, slots=slots, inv_freq=inv_freq, q_weight=q_weight, k_weight=k_weight,
-                cache=cache.k, values=cache.v, status=status)
-    _check_device(qkv)
-    q = torch.empty((n, num_heads * head_dim), dtype=qkv.dtype, device=qkv.device)
-    check(library().cw_norm_rotate_store(
-        _ptr(qkv), _ptr(q), _ptr(positions), _ptr(slots), _ptr(inv_freq) if rot else None, _ptr(q_weight), _ptr(k_weight), _ptr(cache.k),
-        _ptr(cache.v), _ptr(cache.k_exp) if quantised else None, _ptr(cache.v_exp) if quantised else None, n, num_heads, num_kv_heads,
-        head_dim, rot, cache.k.shape[1], cache.k.shape[0], float(eps), code, _ptr(status), _stream()), "norm_rotate_store")
+    index = qkv.get_device()
+    _elsewhere(index, positions=positions, slots=slots, inv_freq=inv_freq, q_weight=q_weight, k_weight=k_weight, cache=cache.k, values=cache.v,
+               status=status)
+    _check_device(index)
+    q = qkv.new_empty((n, num_heads * head_dim))
+    check(library().cw_norm_rotate_store(_STORE_ARGS(
+        qkv.data_ptr(), q.data_ptr(), positions.data_ptr(), slots.data_ptr(), inv_freq.data_ptr() if rot else 0,
+        0 if q_weight is None else q_weight.data_ptr(), 0 if k_weight is None else k_weight.data_ptr(), cache.k.data_ptr(), cache.v.data_ptr(),
+        cache.k_exp.data_ptr() if quantised else 0, cache.v_exp.data_ptr() if quantised else 0, status.data_ptr(), _stream(), n, num_heads,
+        num_kv_heads, head_dim, rot, shape[1], shape[0], code, eps)), "norm_rotate_store")
     return q
 
 
@@ -152,7 +166,7 @@ def read_pages(cache: E4M3Pages, block_tables: torch.Tensor, ctx_lens: torch.Ten
     request's last page becomes zero; no other page is touched.  ``window``: from the page on that a query at the request's last
     position sees with that window.  ``q_start`` [S + 1] (the rows that the requests bring to a step): only requests that bring
     rows are read (``skip_single``: more than one row), and the window is that of their first row."""
-    check_pages(cache)
+    pages, page_size, nkv, hd = check_pages(cache)
     for name, t in (("out_k", out_k), ("out_v", out_v)):
         if t.shape != cache.k.shape or not t.is_contiguous() or t.dtype != out_k.dtype or t.data_ptr() % 16:
             raise ValueError(f"{name} must be contiguous, like the codes in shape, 16-byte aligned and of one type with the other")
@@ -161,17 +175,18 @@ def read_pages(cache: E4M3Pages, block_tables: torch.Tensor, ctx_lens: torch.Ten
     _ints(ctx_lens, "ctx_lens", 1, s)
     if q_start is not None:
         _ints(q_start, "q_start", 1, s + 1)
-    if cache.k.shape[3] % 16:
-        raise ValueError(f"head_dim {cache.k.shape[3]} must be a multiple of 16")
+    if hd % 16:
+        raise ValueError(f"head_dim {hd} must be a multiple of 16")
     if window is not None and window <= 0:
         raise ValueError("window must be positive or None")
     _check_status(status)
-    _same_place(cache.k.device, out_k=out_k, out_v=out_v, block_tables=block_tables, ctx_lens=ctx_lens, q_start=q_start, status=status)
-    _check_device(cache.k)
-    pages, page_size, nkv, hd = cache.k.shape
-    check(library().cw_read_pages(_ptr(cache.k), _ptr(cache.v), _ptr(cache.k_exp), _ptr(cache.v_exp), _ptr(out_k), _ptr(out_v),
-                                  _ptr(block_tables), _ptr(ctx_lens), _ptr(q_start), s, nkv, hd, page_size, block_tables.shape[1], pages,
-                                  int(window or 0), 2 if skip_single else 1, READ_BLOCKS, dtype_code(out_k.dtype), _ptr(status), _stream()), "read_pages")
+    index = cache.k.get_device()
+    _elsewhere(index, out_k=out_k, out_v=out_v, block_tables=block_tables, ctx_lens=ctx_lens, q_start=q_start, status=status)
+    _check_device(index)
+    check(library().cw_read_pages(_READ_ARGS(
+        cache.k.data_ptr(), cache.v.data_ptr(), cache.k_exp.data_ptr(), cache.v_exp.data_ptr(), out_k.data_ptr(), out_v.data_ptr(),
+        block_tables.data_ptr(), ctx_lens.data_ptr(), 0 if q_start is None else q_start.data_ptr(), status.data_ptr(), _stream(), s, nkv, hd,
+        page_size, block_tables.shape[1], pages, window or 0, 2 if skip_single else 1, READ_BLOCKS, dtype_code(out_k.dtype))), "read_pages")
 
 
 class DecodeWorkspace:
@@ -179,15 +194,17 @@ class DecodeWorkspace:
     GPU alone) and counters that are zero between calls.  Calls that may overlap on the GPU must not share one."""
 
     def __init__(self, requests: int, num_heads: int, num_kv_heads: int, head_dim: int, device) -> None:
-        floats, words = _scratch_sizes(requests, num_heads, num_kv_heads, head_dim, _sms(device))
+        device = torch.device(device)
+        floats, words = _scratch_sizes(requests, num_heads, num_kv_heads, head_dim, _sm_count(device.index))
         self.floats = torch.empty(floats, dtype=torch.float32, device=device)
         self.words = torch.zeros(words, dtype=torch.int32, device=device)
 
 
-def _sms(device) -> int:
+@functools.lru_cache(maxsize=None)
+def _sm_count(index: int | None) -> int:
     from . import attention_fast
 
-    return attention_fast._sm_count(torch.device(device))
+    return attention_fast._sm_count(torch.device("cuda", index) if index is not None else None)
 
 
 @functools.lru_cache(maxsize=256)
@@ -201,23 +218,21 @@ def _scratch_sizes(requests: int, num_heads: int, num_kv_heads: int, head_dim: i
 _workspaces: dict = {}  # (device, stream) -> the scratch of calls that bring none
 
 
-def _workspace(workspace: DecodeWorkspace | None, requests: int, num_heads: int, num_kv_heads: int, head_dim: int, device: torch.device,
+def _workspace(workspace: DecodeWorkspace | None, requests: int, num_heads: int, num_kv_heads: int, head_dim: int, index: int,
                stream: int, sms: int) -> DecodeWorkspace:
     """The caller's workspace, or the one of the current stream, replaced by a larger one when a call needs more.  A call that is being
     captured and brings none gets one of its own in the graph's memory, cleared at every replay: graphs may be replayed on any
     stream."""
     floats, words = _scratch_sizes(requests, num_heads, num_kv_heads, head_dim, sms)
     if workspace is not None:
-        if workspace.floats.numel() < floats or workspace.words.numel() < words or workspace.floats.device != device:
+        if workspace.floats.numel() < floats or workspace.words.numel() < words or workspace.floats.get_device() != index:
             raise ValueError("the workspace was made for fewer requests, other heads or another device")
         return workspace
     if torch.cuda.is_current_stream_capturing():
-        return DecodeWorkspace(requests, num_heads, num_kv_heads, head_dim, device)
-    held = _workspaces.get((device.index, stream))
+        return DecodeWorkspace(requests, num_heads, num_kv_heads, head_dim, torch.device("cuda", index))
+    held = _workspaces.get((index, stream))
     if held is None or held.floats.numel() < floats or held.words.numel() < words:
-        held = _workspaces[device.index, stream] = DecodeWorkspace(max(requests, 256), num_heads, num_kv_heads, max(head_dim, 128), device)
-        if held.words.numel() < words or held.floats.numel() < floats:  # (heads of 128 come in other groups than larger ones)
-            held = _workspaces[device.index, stream] = DecodeWorkspace(requests, num_heads, num_kv_heads, head_dim, device)
+        held = _workspaces[index, stream] = DecodeWorkspace(max(requests, 256), num_heads, num_kv_heads, head_dim, torch.device("cuda", index))
     return held
 
 
@@ -232,8 +247,7 @@ def attention_decode(q: torch.Tensor, cache: E4M3Pages, block_tables: torch.Tens
     prompt portions; only requests with exactly one row are served, the others' rows are left alone.  ``workspace``: the call's scratch (default:
     one per stream)."""
     code = dtype_code(q.dtype)
-    check_pages(cache)
-    pages, page_size, nkv, hd = cache.k.shape
+    pages, page_size, nkv, hd = check_pages(cache)
     if q.dim() != 2 or q.shape[1] < num_heads * hd or q.stride(1) != 1:
         raise ValueError("q must be [rows, >= nh * hd] with unit column stride")
     if num_heads <= 0 or num_heads % nkv:
@@ -252,19 +266,22 @@ def attention_decode(q: torch.Tensor, cache: E4M3Pages, block_tables: torch.Tens
             raise ValueError("a flat batch needs the output tensor")
     elif q.shape[0] != s:
         raise ValueError(f"q has {q.shape[0]} rows for {s} requests")
-    if out is None:
-        out = torch.empty((s, num_heads * hd), dtype=q.dtype, device=q.device)
-    elif out.dtype != q.dtype or tuple(out.shape) != (q.shape[0], num_heads * hd) or not out.is_contiguous():
+    if out is not None and (out.dtype != q.dtype or out.shape != (q.shape[0], num_heads * hd) or not out.is_contiguous()):
         raise ValueError("out must be contiguous [rows, nh * hd] of q's type")
-    _same_place(q.device, cache=cache.k, block_tables=block_tables, ctx_lens=ctx_lens, q_start=q_start, out=out, status=status)
-    _check_device(q)
-    stride = q.stride(0) if q.shape[0] > 1 else max(q.stride(0), num_heads * hd)
-    stream, sms = _stream(), _sms(q.device)
-    scratch = _workspace(workspace, s, num_heads, nkv, hd, q.device, stream, sms) if code == 1 and hd % 32 == 0 else None
-    check(library().cw_attention_decode_e4m3(
-        _ptr(q), stride, _ptr(out), _ptr(cache.k), _ptr(cache.v), _ptr(cache.k_exp), _ptr(cache.v_exp), _ptr(block_tables),
-        _ptr(ctx_lens), _ptr(q_start), s, num_heads, nkv, hd, page_size, block_tables.shape[1], pages, int(window or 0), float(scale), code, sms,
-        scratch and scratch.floats.data_ptr(), scratch and scratch.words.data_ptr(), _ptr(status), stream), "attention_decode_e4m3")
+    index = q.get_device()
+    _elsewhere(index, cache=cache.k, block_tables=block_tables, ctx_lens=ctx_lens, q_start=q_start, out=out, status=status)
+    _check_device(index)
+    if out is None:
+        out = q.new_empty((s, num_heads * hd))
+    stream, sms, floats, words = _stream(), _sm_count(index), 0, 0
+    if code == 1 and hd % 32 == 0:
+        scratch = _workspace(workspace, s, num_heads, nkv, hd, index, stream, sms)
+        floats, words = scratch.floats.data_ptr(), scratch.words.data_ptr()
+    check(library().cw_attention_decode_e4m3(_DECODE_ARGS(
+        q.data_ptr(), out.data_ptr(), cache.k.data_ptr(), cache.v.data_ptr(), cache.k_exp.data_ptr(), cache.v_exp.data_ptr(),
+        block_tables.data_ptr(), ctx_lens.data_ptr(), 0 if q_start is None else q_start.data_ptr(), floats, words, status.data_ptr(), stream,
+        q.stride(0) if q.shape[0] > 1 else num_heads * hd, s, num_heads, nkv, hd, page_size, block_tables.shape[1], pages, window or 0, code,
+        sms, scale)), "attention_decode_e4m3")
     return out
 
 
@@ -340,8 +357,8 @@ def attention_portions(q: torch.Tensor, cache: E4M3Pages, block_tables: torch.Te
     from . import attention_ref
     from . import attention_fast as fast
 
-    check_pages(cache)
-    _, page_size, nkv, hd = cache.k.shape
+    _, page_size, nkv, hd = check_pages(cache)
+    _check_device(q.get_device())
     held = portion_scratch(cache, q.dtype)
     read_pages(cache, block_tables, ctx_lens, held.k, held.v, status, window=window, q_start=q_start)
     if q.dtype == torch.bfloat16 and hd in fast.PREFILL_HEAD_DIMS:

@@ -17,7 +17,7 @@ struct StoreParams {
     const int* positions; const int* slots;
     const float* inv_freq; const float* q_weight; const float* k_weight;
     void* k_cache; void* v_cache; uint8_t* k_exp; uint8_t* v_exp;  // k_exp null: a plain cache
-    int nh, nkv, hd, rot, page_size, num_slots;
+    int N, nh, nkv, hd, rot, page_size, num_slots;
     float eps;
     int* status;
 };
@@ -31,40 +31,55 @@ __device__ __forceinline__ void turn_of(float position, float freq, float& sn, f
     cs = c * less - s * e;
 }
 
-// A token per block.  LG neighbouring lanes share a head; a lane holds two quads of it: the two halves of four pairs that turn
-// together (the lanes below rot / 8), or eight entries behind them.  So pairs never leave a thread, the mean of squares and the
-// largest magnitude are shuffles among LG lanes, and all accesses are of 8 or 16 bytes.
-template <typename T, int LG>
-__global__ void norm_rotate_store_kernel(const StoreParams p) {
-    extern __shared__ float turn[];  // cos[rot / 2], sin[rot / 2]
+// TOKENS tokens per block, whose angles are worked out once for all heads.  LG neighbouring lanes share a head; a lane holds two
+// quads of it: the two halves of four pairs that turn together (the lanes below rot / 8), or eight entries behind them.  So pairs
+// never leave a thread, the mean of squares and the largest magnitude are shuffles among LG lanes, and all accesses are of 8 or 16
+// bytes.  A (token, head) is loaded while the one before it is worked on.
+template <typename T, int LG, int TOKENS>
+__global__ void __launch_bounds__(512) norm_rotate_store_kernel(const StoreParams p) {
+    extern __shared__ float turn[];  // per token: cos[rot / 2], sin[rot / 2]
+    __shared__ int slot_s[TOKENS], power_s[TOKENS];  // a token's slot (-1: none), and where head 0 has its power
     pdl_enter();
-    const int t = blockIdx.x, half = p.rot >> 1;
-    {
-        const float pos = (float)p.positions[t];
-        for (int j = threadIdx.x; j < half; j += blockDim.x) turn_of(pos, p.inv_freq[j], turn[half + j], turn[j]);
-    }
-    int slot = p.slots[t];
-    if (slot >= p.num_slots) {
-        if (threadIdx.x == 0) cw_report(p.status, CW_ST_SLOT_RANGE, t, slot);
-        slot = -1;
-    }
-    const int page = slot >= 0 ? slot / p.page_size : 0, off = slot >= 0 ? slot - page * p.page_size : 0;
-    __syncthreads();
-    const int heads = p.nh + 2 * p.nkv, l = threadIdx.x % LG, turning = p.rot >> 3;
+    const int t0 = blockIdx.x * TOKENS, tokens = min(TOKENS, p.N - t0), half = p.rot >> 1;
+    const int heads = p.nh + 2 * p.nkv, l = threadIdx.x % LG, turning = p.rot >> 3, each = blockDim.x / LG;
     const bool there = l < (p.hd >> 3), turns = l < turning;
     const int a_at = turns ? 4 * l : p.rot + 8 * (l - turning), b_at = turns ? half + 4 * l : a_at + 4;
-    const T* row = (const T*)p.qkv + (size_t)t * heads * p.hd;
-    for (int head0 = 0; head0 < heads; head0 += blockDim.x / LG) {  // (whole warps go round together: the shuffles below)
-        const int head = head0 + threadIdx.x / LG;
-        const bool live = head < heads && there, is_q = head < p.nh, is_v = head >= p.nh + p.nkv;
-        float4 a = make_float4(0.f, 0.f, 0.f, 0.f), b = a;
-        if (live) {
-            a = Vec4<T>::load(row + (size_t)head * p.hd + a_at);
-            b = Vec4<T>::load(row + (size_t)head * p.hd + b_at);
+    const T* rows = (const T*)p.qkv + (size_t)t0 * heads * p.hd;
+    const int items = tokens * heads;
+    int item = threadIdx.x / LG;
+    float4 a_next = make_float4(0.f, 0.f, 0.f, 0.f), b_next = a_next;
+    auto load = [&](int i) {
+        if (i < items && there) {
+            a_next = Vec4<T>::load(rows + (size_t)i * p.hd + a_at);
+            b_next = Vec4<T>::load(rows + (size_t)i * p.hd + b_at);
         }
+    };
+    load(item);
+    if (threadIdx.x < tokens) {
+        int slot = p.slots[t0 + threadIdx.x];
+        if (slot >= p.num_slots) {
+            cw_report(p.status, CW_ST_SLOT_RANGE, t0 + threadIdx.x, slot);
+            slot = -1;
+        }
+        const int page = max(slot, 0) / p.page_size;
+        slot_s[threadIdx.x] = slot;
+        power_s[threadIdx.x] = max(slot, 0) - page * p.page_size;  // (within the page; the page again below)
+    }
+    for (int i = threadIdx.x; i < tokens * half; i += blockDim.x) {
+        const int t = i / half, j = i - t * half;
+        turn_of((float)p.positions[t0 + t], p.inv_freq[j], turn[t * p.rot + half + j], turn[t * p.rot + j]);
+    }
+    __syncthreads();
+    for (; item - (int)(threadIdx.x % 32) / LG < items; item += each) {  // (whole warps go round together: the shuffles below)
+        float4 a = a_next, b = b_next;
+        load(item + each);
+        const int t = TOKENS == 1 ? 0 : item / heads, head = item - t * heads;
+        const bool live = item < items && there, is_q = head < p.nh, is_v = head >= p.nh + p.nkv;
+        const int slot = slot_s[TOKENS == 1 ? 0 : min(t, TOKENS - 1)];
         const float* weight = is_q ? p.q_weight : p.k_weight;
         if (p.q_weight != nullptr || p.k_weight != nullptr) {
             float sum = a.x * a.x + a.y * a.y + a.z * a.z + a.w * a.w + b.x * b.x + b.y * b.y + b.z * b.z + b.w * b.w;
+            if (!there) sum = 0.f;
 #pragma unroll
             for (int o = LG / 2; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
             if (live && !is_v && weight != nullptr) {
@@ -75,20 +90,22 @@ __global__ void norm_rotate_store_kernel(const StoreParams p) {
             }
         }
         if (live && !is_v && turns) {
-            const float4 cs = *reinterpret_cast<const float4*>(turn + 4 * l), sn = *reinterpret_cast<const float4*>(turn + half + 4 * l);
+            const float4 cs = *reinterpret_cast<const float4*>(turn + t * p.rot + 4 * l), sn = *reinterpret_cast<const float4*>(turn + t * p.rot + half + 4 * l);
             const float4 x = a, y = b;
             a.x = x.x * cs.x - y.x * sn.x; a.y = x.y * cs.y - y.y * sn.y; a.z = x.z * cs.z - y.z * sn.z; a.w = x.w * cs.w - y.w * sn.w;
             b.x = y.x * cs.x + x.x * sn.x; b.y = y.y * cs.y + x.y * sn.y; b.z = y.z * cs.z + x.z * sn.z; b.w = y.w * cs.w + x.w * sn.w;
         }
         if (live && is_q) {
-            T* out = (T*)p.q_out + ((size_t)t * p.nh + head) * p.hd;
+            T* out = (T*)p.q_out + ((size_t)(t0 + t) * p.nh + head) * p.hd;
             Vec4<T>::store(out + a_at, a);
             Vec4<T>::store(out + b_at, b);
         }
+        const bool stores = live && !is_q && slot >= 0;
+        if (!__any_sync(0xffffffffu, stores)) continue;
         const int kvh = is_v ? head - p.nh - p.nkv : head - p.nh;
-        const size_t at = ((size_t)(slot < 0 ? 0 : slot) * p.nkv + kvh) * p.hd;
+        const size_t at = ((size_t)max(slot, 0) * p.nkv + kvh) * p.hd;
         if (p.k_exp == nullptr) {
-            if (live && !is_q && slot >= 0) {
+            if (stores) {
                 T* out = (T*)(is_v ? p.v_cache : p.k_cache) + at;
                 Vec4<T>::store(out + a_at, a);
                 Vec4<T>::store(out + b_at, b);
@@ -99,16 +116,17 @@ __global__ void norm_rotate_store_kernel(const StoreParams p) {
         b.x = kv_clamped(b.x); b.y = kv_clamped(b.y); b.z = kv_clamped(b.z); b.w = kv_clamped(b.w);
         float big = fmaxf(fmaxf(fmaxf(fabsf(a.x), fabsf(a.y)), fmaxf(fabsf(a.z), fabsf(a.w))),
                           fmaxf(fmaxf(fabsf(b.x), fabsf(b.y)), fmaxf(fabsf(b.z), fabsf(b.w))));
-        big = fmaxf(big, 0.f);  // (a row of NaN alone)
+        big = there ? fmaxf(big, 0.f) : 0.f;  // (a row of NaN alone: 0)
 #pragma unroll
         for (int o = LG / 2; o > 0; o >>= 1) big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, o));
-        if (live && !is_q && slot >= 0) {
-            const int power = kv_power(big);
+        if (stores) {
+            const int power = kv_power(big), off = power_s[TOKENS == 1 ? 0 : t];
             const float d = kv_down(power);
             uint8_t* out = (uint8_t*)(is_v ? p.v_cache : p.k_cache) + at;
             *reinterpret_cast<uint32_t*>(out + a_at) = kv_codes(a.x * d, a.y * d, a.z * d, a.w * d);
             *reinterpret_cast<uint32_t*>(out + b_at) = kv_codes(b.x * d, b.y * d, b.z * d, b.w * d);
-            if (l == 0) (is_v ? p.v_exp : p.k_exp)[((size_t)page * p.nkv + kvh) * p.page_size + off] = (uint8_t)power;
+            // ((slot - off) / page_size, the page, times nkv rows of page_size powers)
+            if (l == 0) (is_v ? p.v_exp : p.k_exp)[(size_t)(slot - off) * p.nkv + (size_t)kvh * p.page_size + off] = (uint8_t)power;
         }
     }
 }
@@ -165,6 +183,21 @@ __global__ void norm_rotate_store_any_kernel(const StoreParams p) {
 
 static inline bool aligned(const void* p, int bytes) { return ((uintptr_t)p & (bytes - 1)) == 0; }
 
+#define STORE_FOUR_FROM 1776  // 3 * 148 * 4
+
+template <typename T, int TOKENS>
+static int store_tokens(const StoreParams& p, int lg, int threads, cudaStream_t stream) {
+    const dim3 grid((p.N + TOKENS - 1) / TOKENS), block(threads);
+    const size_t smem = (size_t)TOKENS * p.rot * sizeof(float);
+    switch (lg) {
+        case 2: return cw_launch(norm_rotate_store_kernel<T, 2, TOKENS>, grid, block, smem, stream, 1u, p);
+        case 4: return cw_launch(norm_rotate_store_kernel<T, 4, TOKENS>, grid, block, smem, stream, 1u, p);
+        case 8: return cw_launch(norm_rotate_store_kernel<T, 8, TOKENS>, grid, block, smem, stream, 1u, p);
+        case 16: return cw_launch(norm_rotate_store_kernel<T, 16, TOKENS>, grid, block, smem, stream, 1u, p);
+        default: return cw_launch(norm_rotate_store_kernel<T, 32, TOKENS>, grid, block, smem, stream, 1u, p);
+    }
+}
+
 template <typename T>
 static int store_launch(const StoreParams& p, int N, cudaStream_t stream) {
     const int heads = p.nh + 2 * p.nkv, smem = p.rot * (int)sizeof(float);
@@ -178,14 +211,9 @@ static int store_launch(const StoreParams& p, int N, cudaStream_t stream) {
     }
     int lg = 2;
     while (lg * 8 < p.hd) lg *= 2;
-    const int threads = min(512, (heads * lg + 31) / 32 * 32);
-    switch (lg) {
-        case 2: return cw_launch(norm_rotate_store_kernel<T, 2>, dim3(N), dim3(threads), smem, stream, 1u, p);
-        case 4: return cw_launch(norm_rotate_store_kernel<T, 4>, dim3(N), dim3(threads), smem, stream, 1u, p);
-        case 8: return cw_launch(norm_rotate_store_kernel<T, 8>, dim3(N), dim3(threads), smem, stream, 1u, p);
-        case 16: return cw_launch(norm_rotate_store_kernel<T, 16>, dim3(N), dim3(threads), smem, stream, 1u, p);
-        default: return cw_launch(norm_rotate_store_kernel<T, 32>, dim3(N), dim3(threads), smem, stream, 1u, p);
-    }
+    // Four tokens a block once that still gives every SM three blocks; fewer tokens: one each, so that more SMs have some.
+    if (N >= STORE_FOUR_FROM) return store_tokens<T, 4>(p, lg, min(512, (4 * heads * lg + 31) / 32 * 32), stream);
+    return store_tokens<T, 1>(p, lg, min(512, (heads * lg + 31) / 32 * 32), stream);
 }
 
 // q_out [N, nh * hd]; slots[t] < 0: the token is not stored.  k_exp and v_exp null: the cache is of the run's type.
@@ -208,7 +236,7 @@ extern "C" int cw_norm_rotate_store(const char* block) {
         (long long)num_pages * page_size > 0x7FFFFFFF || (rot > 0 && inv_freq == nullptr) || (k_exp == nullptr) != (v_exp == nullptr))
         return CW_ERR_BAD_SIZE;
     const StoreParams p = {qkv, q_out, positions, slots, inv_freq, q_weight, k_weight, k_cache, v_cache, k_exp, v_exp,
-                           nh, nkv, hd, rot, page_size, num_pages * page_size, eps, status};
+                           N, nh, nkv, hd, rot, page_size, num_pages * page_size, eps, status};
     if (dtype == 0) return store_launch<float>(p, N, stream);
     if (dtype == 1) return store_launch<bf16>(p, N, stream);
     return CW_ERR_BAD_DTYPE;
@@ -222,55 +250,80 @@ struct ReadParams {
     int* status;
 };
 
-// Units are pages of a request, keys and values apart.  A page's codes are one run of memory, and so is where they go; a thread
-// takes 16 codes at a time, whose row has one power.
+__device__ __forceinline__ void store8(float* at, float a, float b, float c, float d, float e, float f, float g, float h) {
+    *reinterpret_cast<float4*>(at) = make_float4(a, b, c, d);
+    *reinterpret_cast<float4*>(at + 4) = make_float4(e, f, g, h);
+}
+__device__ __forceinline__ void store8(bf16* at, float a, float b, float c, float d, float e, float f, float g, float h) {
+    const __nv_bfloat162 x[4] = {__floats2bfloat162_rn(a, b), __floats2bfloat162_rn(c, d), __floats2bfloat162_rn(e, f), __floats2bfloat162_rn(g, h)};
+    *reinterpret_cast<uint4*>(at) = *reinterpret_cast<const uint4*>(x);
+}
+
+// x / d for x * d < 2^32, by a multiplication.
+struct Quotient {
+    uint32_t d, magic;
+    static Quotient by(uint32_t d) { return {d, d == 1 ? 0u : (uint32_t)(((1ULL << 32) + d - 1) / d)}; }
+    __device__ __forceinline__ uint32_t of(uint32_t x) const { return d == 1 ? x : __umulhi(x, magic); }
+};
+
+// Units are pages of a request, keys and values apart, a warp to each, so that thousands are on their way at once.  A page's codes
+// are one run of memory, and so is where they go; a lane takes 8 codes at a time (they share a row and its power), so that a
+// warp writes whole lines.
+#define READ_AT_ONCE 8
 template <typename T>
-__global__ void __launch_bounds__(256) read_pages_kernel(const ReadParams p) {
+__global__ void __launch_bounds__(256) read_pages_kernel(const ReadParams p, const Quotient by_chunks, const Quotient by_heads) {
     __shared__ int sh[36];
     pdl_enter();
-    auto first_block = [&](int s, int ctx) { return p.window > 0 ? max(0, ctx - p.window) / p.page_size : 0; };
-    // (a portion's first row sees `window` keys before it: the window reaches back from there)
-    auto span = [&](int s, int& from) {
+    auto span = [&](int s, int& from) {  // a request's blocks that are read: how many, and the first
         int ctx = p.ctx_lens[s], first = ctx;
         if (p.q_start != nullptr) {
             const int rows = p.q_start[s + 1] - p.q_start[s];
             if (rows < p.least_rows) return 0;
-            first = ctx - rows + 1;
+            first = ctx - rows + 1;  // (a portion's first row sees `window` keys, its own among them: the window reaches back from there)
         }
-        from = first_block(s, first);
+        from = p.window > 0 ? max(0, first - p.window) / p.page_size : 0;
         return max(0, min((ctx + p.page_size - 1) / p.page_size, p.max_blocks) - from);
     };
-    const UnitRange r = units_of_block([&](int s) { int from; return 2 * span(s, from); }, p.requests, 1, gridDim.x, blockIdx.x, sh);
-    int s = r.request, at = r.offset;
-    const int chunks = p.hd >> 4, items = p.page_size * p.nkv * chunks;
-    for (int u = r.first; u < r.last; ++s, at = 0) {
-        int from = 0;
-        const int n = 2 * span(s, from), ctx = p.ctx_lens[s];
-        for (; at < n && u < r.last; ++at, ++u) {
-            const bool is_v = at & 1;
-            const int block = from + (at >> 1), page = p.block_tables[(size_t)s * p.max_blocks + block];
-            if (page < 0 || page >= p.num_pages) {
-                if (threadIdx.x == 0) cw_report(p.status, CW_ST_PAGE_RANGE, s, page);
-                continue;
-            }
-            const uint4* src = reinterpret_cast<const uint4*>(is_v ? p.v : p.k) + (size_t)page * items;
-            const uint8_t* powers = (is_v ? p.v_exp : p.k_exp) + (size_t)page * p.nkv * p.page_size;
-            T* dst = (T*)(is_v ? p.v_out : p.k_out) + (size_t)page * items * 16;
-            const int live = min(p.page_size, ctx - block * p.page_size);
-            for (int i = threadIdx.x; i < items; i += blockDim.x) {
-                const int row = i / chunks, token = row / p.nkv, head = row - token * p.nkv;
-                uint4 codes = make_uint4(0, 0, 0, 0);
-                float up = 0.f;
-                if (token < live) {
-                    codes = src[i];
-                    up = kv_up(powers[head * p.page_size + token]);
-                }
-                const uint32_t w[4] = {codes.x, codes.y, codes.z, codes.w};
+    const int warps = blockDim.x >> 5, lane = threadIdx.x & 31;
+    const UnitRange r = units_of_block([&](int s) { int from; return 2 * span(s, from); }, p.requests, warps, gridDim.x, blockIdx.x, sh);
+    const int chunks = p.page_size * p.nkv * (p.hd >> 3);
+    int s = r.request, at = r.offset + (threadIdx.x >> 5);  // units of a block go to its warps in turn
+    for (int u = r.first + (threadIdx.x >> 5); u < r.last; u += warps, at += warps) {
+        int from = 0, n = 2 * span(s, from);
+        while (at >= n && s + 1 < p.requests) {
+            at -= n;
+            n = 2 * span(++s, from);
+        }
+        const bool is_v = at & 1;
+        const int block = from + (at >> 1), page = block < p.max_blocks ? p.block_tables[(size_t)s * p.max_blocks + block] : -1;
+        if (page < 0 || page >= p.num_pages) {
+            if (lane == 0) cw_report(p.status, CW_ST_PAGE_RANGE, s, page);
+            continue;
+        }
+        const uint2* src = reinterpret_cast<const uint2*>(is_v ? p.v : p.k) + (size_t)page * chunks;
+        const uint8_t* powers = (is_v ? p.v_exp : p.k_exp) + (size_t)page * p.nkv * p.page_size;
+        T* dst = (T*)(is_v ? p.v_out : p.k_out) + (size_t)page * chunks * 8;
+        const int live = min(p.page_size, p.ctx_lens[s] - block * p.page_size) * p.nkv;  // rows that hold something
+        for (int i0 = lane; i0 < chunks; i0 += 32 * READ_AT_ONCE) {
+            uint2 codes[READ_AT_ONCE];
+            uint32_t power[READ_AT_ONCE];
 #pragma unroll
-                for (int q = 0; q < 4; ++q) {
-                    const float2 lo = kv_float2(w[q]), hi = kv_float2(w[q] >> 16);
-                    Vec4<T>::store(dst + (size_t)i * 16 + q * 4, make_float4(lo.x * up, lo.y * up, hi.x * up, hi.y * up));
+            for (int k = 0; k < READ_AT_ONCE; ++k) {
+                const int i = i0 + 32 * k, row = by_chunks.of(i), token = by_heads.of(row);
+                codes[k] = make_uint2(0, 0);
+                power[k] = 0;
+                if (i < chunks && row < live) {
+                    codes[k] = __ldcs(src + i);
+                    power[k] = powers[(row - token * p.nkv) * p.page_size + token];
                 }
+            }
+#pragma unroll
+            for (int k = 0; k < READ_AT_ONCE; ++k) {
+                const int i = i0 + 32 * k;
+                if (i >= chunks) break;
+                const float up = kv_up(power[k]);
+                const float2 x0 = kv_float2(codes[k].x), x1 = kv_float2(codes[k].x >> 16), x2 = kv_float2(codes[k].y), x3 = kv_float2(codes[k].y >> 16);
+                store8(dst + (size_t)i * 8, x0.x * up, x0.y * up, x1.x * up, x1.y * up, x2.x * up, x2.y * up, x3.x * up, x3.y * up);
             }
         }
     }
@@ -290,12 +343,13 @@ extern "C" int cw_read_pages(const char* block) {
     if (requests == 0) return CW_OK;
     if (requests < 0 || nkv <= 0 || hd <= 0 || hd % 16 || page_size <= 0 || max_blocks <= 0 || num_pages <= 0 || window < 0 || blocks <= 0 || least_rows < 1 ||
         !aligned(k, 16) || !aligned(v, 16) || !aligned(k_out, 16) || !aligned(v_out, 16) ||
-        (long long)page_size * nkv * (hd >> 4) > 0x7FFFFFFF)
+        (long long)page_size * nkv * (hd >> 3) * max(hd >> 3, nkv) > 0x7FFFFFFF)  // (Quotient's range)
         return CW_ERR_BAD_SIZE;
     const ReadParams p = {k, v, k_exp, v_exp, k_out, v_out, block_tables, ctx_lens, q_start, requests, nkv, hd, page_size,
                           max_blocks, num_pages, window, least_rows, status};
-    if (dtype == 0) return cw_launch(read_pages_kernel<float>, dim3(blocks), dim3(256), 0, stream, 1u, p);
-    if (dtype == 1) return cw_launch(read_pages_kernel<bf16>, dim3(blocks), dim3(256), 0, stream, 1u, p);
+    const Quotient by_chunks = Quotient::by(hd >> 3), by_heads = Quotient::by(nkv);
+    if (dtype == 0) return cw_launch(read_pages_kernel<float>, dim3(blocks), dim3(256), 0, stream, 1u, p, by_chunks, by_heads);
+    if (dtype == 1) return cw_launch(read_pages_kernel<bf16>, dim3(blocks), dim3(256), 0, stream, 1u, p, by_chunks, by_heads);
     return CW_ERR_BAD_DTYPE;
 }
 

@@ -31,101 +31,139 @@ __device__ __forceinline__ void turn_of(float position, float freq, float& sn, f
     cs = c * less - s * e;
 }
 
-// TOKENS tokens per block, whose angles are worked out once for all heads.  LG neighbouring lanes share a head; a lane holds two
-// quads of it: the two halves of four pairs that turn together (the lanes below rot / 8), or eight entries behind them.  So pairs
-// never leave a thread, the mean of squares and the largest magnitude are shuffles among LG lanes, and all accesses are of 8 or 16
-// bytes.  A (token, head) is loaded while the one before it is worked on.
-template <typename T, int LG, int TOKENS>
-__global__ void __launch_bounds__(512) norm_rotate_store_kernel(const StoreParams p) {
+// LG neighbouring lanes hold a head, a lane two octets of it (octet i, i < rot / 8: four entries and the four that turn with them;
+// behind those, eight neighbours), so that pairs never leave a thread, the mean of squares and the largest magnitude are shuffles
+// among LG lanes, and accesses are of 8 or 16 bytes.  A thread keeps its head and its entries for a block's tokens, whose rows are
+// loaded one ahead: weights, offsets and the kind of head are found out once.  Blocks have as many tokens as leave the SMs two
+// blocks each, eight at most.
+#define STORE_TOKENS 8
+template <typename T, int LG>
+__global__ void __launch_bounds__(512) norm_rotate_store_kernel(const StoreParams p, int most_tokens, int block_heads) {
     extern __shared__ float turn[];  // per token: cos[rot / 2], sin[rot / 2]
-    __shared__ int slot_s[TOKENS], power_s[TOKENS];  // a token's slot (-1: none), and where head 0 has its power
+    __shared__ int slot_s[STORE_TOKENS], off_s[STORE_TOKENS];  // a token's slot (-1: none) and its place in its page
     pdl_enter();
-    const int t0 = blockIdx.x * TOKENS, tokens = min(TOKENS, p.N - t0), half = p.rot >> 1;
-    const int heads = p.nh + 2 * p.nkv, l = threadIdx.x % LG, turning = p.rot >> 3, each = blockDim.x / LG;
-    const bool there = l < (p.hd >> 3), turns = l < turning;
-    const int a_at = turns ? 4 * l : p.rot + 8 * (l - turning), b_at = turns ? half + 4 * l : a_at + 4;
-    const T* rows = (const T*)p.qkv + (size_t)t0 * heads * p.hd;
-    const int items = tokens * heads;
-    int item = threadIdx.x / LG;
-    float4 a_next = make_float4(0.f, 0.f, 0.f, 0.f), b_next = a_next;
-    auto load = [&](int i) {
-        if (i < items && there) {
-            a_next = Vec4<T>::load(rows + (size_t)i * p.hd + a_at);
-            b_next = Vec4<T>::load(rows + (size_t)i * p.hd + b_at);
-        }
+    const int t0 = blockIdx.x * most_tokens, tokens = min(most_tokens, p.N - t0), half = p.rot >> 1;
+    const int heads = p.nh + 2 * p.nkv, l = threadIdx.x % LG, turning = p.rot >> 3;
+    const int own = threadIdx.x / LG, head = blockIdx.y * block_heads + own;
+    const bool live = own < block_heads && head < heads, is_q = head < p.nh, is_v = head >= p.nh + p.nkv;
+    int a_at[2], b_at[2];
+    bool there[2], turns[2];
+    float4 a_next[2], b_next[2];
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+        const int octet = l + e * LG;
+        there[e] = live && octet < (p.hd >> 3);
+        turns[e] = octet < turning && !is_v;
+        a_at[e] = octet < turning ? 4 * octet : p.rot + 8 * (octet - turning);
+        b_at[e] = octet < turning ? half + 4 * octet : a_at[e] + 4;
+        a_next[e] = b_next[e] = make_float4(0.f, 0.f, 0.f, 0.f);
+    }
+    const T* row = (const T*)p.qkv + ((size_t)t0 * heads + head) * p.hd;
+    auto load = [&]() {
+#pragma unroll
+        for (int e = 0; e < 2; ++e)
+            if (there[e]) {
+                a_next[e] = Vec4<T>::load(row + a_at[e]);
+                b_next[e] = Vec4<T>::load(row + b_at[e]);
+            }
+        row += (size_t)heads * p.hd;
     };
-    load(item);
+    load();
     if (threadIdx.x < tokens) {
         int slot = p.slots[t0 + threadIdx.x];
         if (slot >= p.num_slots) {
-            cw_report(p.status, CW_ST_SLOT_RANGE, t0 + threadIdx.x, slot);
+            if (blockIdx.y == 0) cw_report(p.status, CW_ST_SLOT_RANGE, t0 + threadIdx.x, slot);
             slot = -1;
         }
-        const int page = max(slot, 0) / p.page_size;
         slot_s[threadIdx.x] = slot;
-        power_s[threadIdx.x] = max(slot, 0) - page * p.page_size;  // (within the page; the page again below)
+        off_s[threadIdx.x] = max(slot, 0) % p.page_size;
     }
     for (int i = threadIdx.x; i < tokens * half; i += blockDim.x) {
         const int t = i / half, j = i - t * half;
         turn_of((float)p.positions[t0 + t], p.inv_freq[j], turn[t * p.rot + half + j], turn[t * p.rot + j]);
     }
+    const float* weight = is_v ? nullptr : is_q ? p.q_weight : p.k_weight;
+    float4 wa[2], wb[2];
+    if (weight != nullptr)
+#pragma unroll
+        for (int e = 0; e < 2; ++e)
+            if (there[e]) {
+                wa[e] = *reinterpret_cast<const float4*>(weight + a_at[e]);
+                wb[e] = *reinterpret_cast<const float4*>(weight + b_at[e]);
+            }
+    const float per_entry = 1.f / (float)p.hd;
+    const bool any_norm = __any_sync(0xffffffffu, live && weight != nullptr), any_kv = __any_sync(0xffffffffu, live && !is_q);
+    const int kvh = is_v ? head - p.nh - p.nkv : head - p.nh;
     __syncthreads();
-    for (; item - (int)(threadIdx.x % 32) / LG < items; item += each) {  // (whole warps go round together: the shuffles below)
-        float4 a = a_next, b = b_next;
-        load(item + each);
-        const int t = TOKENS == 1 ? 0 : item / heads, head = item - t * heads;
-        const bool live = item < items && there, is_q = head < p.nh, is_v = head >= p.nh + p.nkv;
-        const int slot = slot_s[TOKENS == 1 ? 0 : min(t, TOKENS - 1)];
-        const float* weight = is_q ? p.q_weight : p.k_weight;
-        if (p.q_weight != nullptr || p.k_weight != nullptr) {
-            float sum = a.x * a.x + a.y * a.y + a.z * a.z + a.w * a.w + b.x * b.x + b.y * b.y + b.z * b.z + b.w * b.w;
-            if (!there) sum = 0.f;
+    for (int t = 0; t < tokens; ++t) {
+        float4 a[2] = {a_next[0], a_next[1]}, b[2] = {b_next[0], b_next[1]};
+        if (t + 1 < tokens) load();
+        if (any_norm) {
+            float sum = 0.f;
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {  // (entries that there are not: zeros)
+                sum = fmaf(a[e].x, a[e].x, fmaf(a[e].y, a[e].y, fmaf(a[e].z, a[e].z, fmaf(a[e].w, a[e].w, sum))));
+                sum = fmaf(b[e].x, b[e].x, fmaf(b[e].y, b[e].y, fmaf(b[e].z, b[e].z, fmaf(b[e].w, b[e].w, sum))));
+            }
 #pragma unroll
             for (int o = LG / 2; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-            if (live && !is_v && weight != nullptr) {
-                const float r = rsqrtf(sum / (float)p.hd + p.eps);
-                const float4 wa = *reinterpret_cast<const float4*>(weight + a_at), wb = *reinterpret_cast<const float4*>(weight + b_at);
-                a.x *= r * wa.x; a.y *= r * wa.y; a.z *= r * wa.z; a.w *= r * wa.w;
-                b.x *= r * wb.x; b.y *= r * wb.y; b.z *= r * wb.z; b.w *= r * wb.w;
+            if (weight != nullptr) {
+                const float r = rsqrtf(fmaf(sum, per_entry, p.eps));
+#pragma unroll
+                for (int e = 0; e < 2; ++e)
+                    if (there[e]) {
+                        a[e].x *= r * wa[e].x; a[e].y *= r * wa[e].y; a[e].z *= r * wa[e].z; a[e].w *= r * wa[e].w;
+                        b[e].x *= r * wb[e].x; b[e].y *= r * wb[e].y; b[e].z *= r * wb[e].z; b[e].w *= r * wb[e].w;
+                    }
             }
         }
-        if (live && !is_v && turns) {
-            const float4 cs = *reinterpret_cast<const float4*>(turn + t * p.rot + 4 * l), sn = *reinterpret_cast<const float4*>(turn + t * p.rot + half + 4 * l);
-            const float4 x = a, y = b;
-            a.x = x.x * cs.x - y.x * sn.x; a.y = x.y * cs.y - y.y * sn.y; a.z = x.z * cs.z - y.z * sn.z; a.w = x.w * cs.w - y.w * sn.w;
-            b.x = y.x * cs.x + x.x * sn.x; b.y = y.y * cs.y + x.y * sn.y; b.z = y.z * cs.z + x.z * sn.z; b.w = y.w * cs.w + x.w * sn.w;
-        }
-        if (live && is_q) {
-            T* out = (T*)p.q_out + ((size_t)(t0 + t) * p.nh + head) * p.hd;
-            Vec4<T>::store(out + a_at, a);
-            Vec4<T>::store(out + b_at, b);
-        }
+#pragma unroll
+        for (int e = 0; e < 2; ++e)
+            if (turns[e]) {
+                const float* at = turn + t * p.rot + a_at[e];
+                const float4 cs = *reinterpret_cast<const float4*>(at), sn = *reinterpret_cast<const float4*>(at + half), x = a[e], y = b[e];
+                a[e].x = x.x * cs.x - y.x * sn.x; a[e].y = x.y * cs.y - y.y * sn.y; a[e].z = x.z * cs.z - y.z * sn.z; a[e].w = x.w * cs.w - y.w * sn.w;
+                b[e].x = y.x * cs.x + x.x * sn.x; b[e].y = y.y * cs.y + x.y * sn.y; b[e].z = y.z * cs.z + x.z * sn.z; b[e].w = y.w * cs.w + x.w * sn.w;
+            }
+        const int slot = slot_s[t];
         const bool stores = live && !is_q && slot >= 0;
-        if (!__any_sync(0xffffffffu, stores)) continue;
-        const int kvh = is_v ? head - p.nh - p.nkv : head - p.nh;
         const size_t at = ((size_t)max(slot, 0) * p.nkv + kvh) * p.hd;
-        if (p.k_exp == nullptr) {
-            if (stores) {
-                T* out = (T*)(is_v ? p.v_cache : p.k_cache) + at;
-                Vec4<T>::store(out + a_at, a);
-                Vec4<T>::store(out + b_at, b);
-            }
-            continue;
+        if ((live && is_q) || (stores && p.k_exp == nullptr)) {  // rows of the run's type
+            T* out = is_q ? (T*)p.q_out + ((size_t)(t0 + t) * p.nh + head) * p.hd : (T*)(is_v ? p.v_cache : p.k_cache) + at;
+#pragma unroll
+            for (int e = 0; e < 2; ++e)
+                if (there[e]) {
+                    Vec4<T>::store(out + a_at[e], a[e]);
+                    Vec4<T>::store(out + b_at[e], b[e]);
+                }
         }
-        a.x = kv_clamped(a.x); a.y = kv_clamped(a.y); a.z = kv_clamped(a.z); a.w = kv_clamped(a.w);
-        b.x = kv_clamped(b.x); b.y = kv_clamped(b.y); b.z = kv_clamped(b.z); b.w = kv_clamped(b.w);
-        float big = fmaxf(fmaxf(fmaxf(fabsf(a.x), fabsf(a.y)), fmaxf(fabsf(a.z), fabsf(a.w))),
-                          fmaxf(fmaxf(fabsf(b.x), fabsf(b.y)), fmaxf(fabsf(b.z), fabsf(b.w))));
-        big = there ? fmaxf(big, 0.f) : 0.f;  // (a row of NaN alone: 0)
+        if (!any_kv || p.k_exp == nullptr) continue;
+        float big = 0.f;  // (NaN has no say)
+#pragma unroll
+        for (int e = 0; e < 2; ++e)
+            big = fmaxf(big, fmaxf(fmaxf(fmaxf(fabsf(a[e].x), fabsf(a[e].y)), fmaxf(fabsf(a[e].z), fabsf(a[e].w))),
+                                   fmaxf(fmaxf(fabsf(b[e].x), fabsf(b[e].y)), fmaxf(fabsf(b[e].z), fabsf(b[e].w)))));
 #pragma unroll
         for (int o = LG / 2; o > 0; o >>= 1) big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, o));
+        if (big > KV_BIGGEST) {
+            big = KV_BIGGEST;
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                a[e].x = kv_clamped(a[e].x); a[e].y = kv_clamped(a[e].y); a[e].z = kv_clamped(a[e].z); a[e].w = kv_clamped(a[e].w);
+                b[e].x = kv_clamped(b[e].x); b[e].y = kv_clamped(b[e].y); b[e].z = kv_clamped(b[e].z); b[e].w = kv_clamped(b[e].w);
+            }
+        }
         if (stores) {
-            const int power = kv_power(big), off = power_s[TOKENS == 1 ? 0 : t];
+            const int power = kv_power(big), off = off_s[t];
             const float d = kv_down(power);
             uint8_t* out = (uint8_t*)(is_v ? p.v_cache : p.k_cache) + at;
-            *reinterpret_cast<uint32_t*>(out + a_at) = kv_codes(a.x * d, a.y * d, a.z * d, a.w * d);
-            *reinterpret_cast<uint32_t*>(out + b_at) = kv_codes(b.x * d, b.y * d, b.z * d, b.w * d);
-            // ((slot - off) / page_size, the page, times nkv rows of page_size powers)
+#pragma unroll
+            for (int e = 0; e < 2; ++e)
+                if (there[e]) {
+                    *reinterpret_cast<uint32_t*>(out + a_at[e]) = kv_codes(a[e].x * d, a[e].y * d, a[e].z * d, a[e].w * d);
+                    *reinterpret_cast<uint32_t*>(out + b_at[e]) = kv_codes(b[e].x * d, b[e].y * d, b[e].z * d, b[e].w * d);
+                }
+            // (slot - off: the page times page_size, and a page has nkv rows of page_size powers)
             if (l == 0) (is_v ? p.v_exp : p.k_exp)[(size_t)(slot - off) * p.nkv + (size_t)kvh * p.page_size + off] = (uint8_t)power;
         }
     }
@@ -183,21 +221,6 @@ __global__ void norm_rotate_store_any_kernel(const StoreParams p) {
 
 static inline bool aligned(const void* p, int bytes) { return ((uintptr_t)p & (bytes - 1)) == 0; }
 
-#define STORE_FOUR_FROM 1776  // 3 * 148 * 4
-
-template <typename T, int TOKENS>
-static int store_tokens(const StoreParams& p, int lg, int threads, cudaStream_t stream) {
-    const dim3 grid((p.N + TOKENS - 1) / TOKENS), block(threads);
-    const size_t smem = (size_t)TOKENS * p.rot * sizeof(float);
-    switch (lg) {
-        case 2: return cw_launch(norm_rotate_store_kernel<T, 2, TOKENS>, grid, block, smem, stream, 1u, p);
-        case 4: return cw_launch(norm_rotate_store_kernel<T, 4, TOKENS>, grid, block, smem, stream, 1u, p);
-        case 8: return cw_launch(norm_rotate_store_kernel<T, 8, TOKENS>, grid, block, smem, stream, 1u, p);
-        case 16: return cw_launch(norm_rotate_store_kernel<T, 16, TOKENS>, grid, block, smem, stream, 1u, p);
-        default: return cw_launch(norm_rotate_store_kernel<T, 32, TOKENS>, grid, block, smem, stream, 1u, p);
-    }
-}
-
 template <typename T>
 static int store_launch(const StoreParams& p, int N, cudaStream_t stream) {
     const int heads = p.nh + 2 * p.nkv, smem = p.rot * (int)sizeof(float);
@@ -209,11 +232,19 @@ static int store_launch(const StoreParams& p, int N, cudaStream_t stream) {
         const int threads = heads < 8 ? heads * 32 : 256;
         return cw_launch(norm_rotate_store_any_kernel<T>, dim3(N), dim3(threads), smem, stream, 1u, p);
     }
-    int lg = 2;
-    while (lg * 8 < p.hd) lg *= 2;
-    // Four tokens a block once that still gives every SM three blocks; fewer tokens: one each, so that more SMs have some.
-    if (N >= STORE_FOUR_FROM) return store_tokens<T, 4>(p, lg, min(512, (4 * heads * lg + 31) / 32 * 32), stream);
-    return store_tokens<T, 1>(p, lg, min(512, (heads * lg + 31) / 32 * 32), stream);
+    int lg = 1;
+    while (lg * 16 < p.hd) lg *= 2;
+    const int chunks = (heads * lg + 511) / 512, block_heads = (heads + chunks - 1) / chunks;
+    const int tokens = max(1, min(STORE_TOKENS, (N * chunks + 2 * 148 - 1) / (2 * 148)));
+    const dim3 grid((N + tokens - 1) / tokens, chunks), block((block_heads * lg + 31) / 32 * 32);
+    const size_t room = (size_t)tokens * smem;
+    switch (lg) {
+        case 1: return cw_launch(norm_rotate_store_kernel<T, 1>, grid, block, room, stream, 1u, p, tokens, block_heads);
+        case 2: return cw_launch(norm_rotate_store_kernel<T, 2>, grid, block, room, stream, 1u, p, tokens, block_heads);
+        case 4: return cw_launch(norm_rotate_store_kernel<T, 4>, grid, block, room, stream, 1u, p, tokens, block_heads);
+        case 8: return cw_launch(norm_rotate_store_kernel<T, 8>, grid, block, room, stream, 1u, p, tokens, block_heads);
+        default: return cw_launch(norm_rotate_store_kernel<T, 16>, grid, block, room, stream, 1u, p, tokens, block_heads);
+    }
 }
 
 // q_out [N, nh * hd]; slots[t] < 0: the token is not stored.  k_exp and v_exp null: the cache is of the run's type.

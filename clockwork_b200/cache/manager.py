@@ -14,7 +14,8 @@ a windowed group gives pages back as soon as the window has passed them.  A grou
 row per ``every`` positions instead of one per position (``PagedKVNeed.every``: summaries of whole
 blocks of positions); its tables are that much shorter and its pool that much smaller.  Mixers that
 keep a state of fixed size (``SlotStateNeed``) get a row per request in a slot tensor instead of
-pages.  A mixer may name several needs (a tuple): pages of one or two kinds and a state slot.
+pages.  A mixer may name several needs (a tuple): pages of one or two kinds and a state slot.  With ``kv_dtype`` "e4m3" pages
+hold 8-bit codes and a power of two per token and KV head (``ops.quantised``): about half of what bfloat16 takes.
 """
 
 from __future__ import annotations
@@ -27,34 +28,47 @@ from ..parts.base import PagedKVNeed, PagedView, SlotStateNeed, StateView
 from .allocator import OutOfPages, PageAllocator
 
 NO_PAGE = -1
+KV_DTYPES = ("auto", "e4m3")  # keys and values in the run's type, or in 8 bits
 
 
 class PageGroup:
     """Layers with identical needs: one allocator, one device tensor
-    ``[layers, planes (K, V; or one row per token), pages, page_size, kv_heads, head_dim]``."""
+    ``[layers, planes (K, V; or one row per token), pages, page_size, kv_heads, head_dim]``.  ``e4m3``: that holds codes, and
+    ``exps`` the powers of their rows, ``[layers, 2, pages, kv_heads, page_size]``."""
 
     def __init__(self, need: PagedKVNeed, cache_layers: list[int], num_pages: int, page_size: int,
-                 dtype: torch.dtype | None, device) -> None:
+                 dtype: torch.dtype | None, device, e4m3: bool = False) -> None:
         self.need = need
+        self.e4m3 = e4m3
         self.every = need.every  # positions per row
         self.cache_layers = list(cache_layers)
         self.page_size = page_size
         self.allocator = PageAllocator(num_pages, page_size)
         self.kv: torch.Tensor | None = None
+        self.exps: torch.Tensor | None = None
         if device is not None and dtype is not None:
             self.kv = torch.zeros(
                 (len(cache_layers), need.planes, num_pages, page_size, need.num_kv_heads, need.head_dim),
-                dtype=dtype, device=device,
+                dtype=torch.uint8 if e4m3 else dtype, device=device,
             )
+            if e4m3:
+                self.kv = self.kv.view(torch.float8_e4m3fn)
+                self.exps = torch.zeros((len(cache_layers), 2, num_pages, need.num_kv_heads, page_size), dtype=torch.uint8, device=device)
         self._index = {layer: i for i, layer in enumerate(self.cache_layers)}
 
     def layer_kv(self, cache_layer: int) -> tuple[torch.Tensor, torch.Tensor]:
         plane = self.kv[self._index[cache_layer]]
         return plane[0], plane[self.need.planes - 1]
 
+    def layer_exps(self, cache_layer: int) -> tuple[torch.Tensor | None, torch.Tensor | None]:
+        if self.exps is None:
+            return None, None
+        plane = self.exps[self._index[cache_layer]]
+        return plane[0], plane[1]
+
     def bytes_per_token(self) -> int:
-        elem = self.kv.element_size() if self.kv is not None else 2
-        return len(self.cache_layers) * self.need.planes * self.need.num_kv_heads * self.need.head_dim * elem
+        elem = self.kv.element_size() if self.kv is not None else 1 if self.e4m3 else 2
+        return len(self.cache_layers) * self.need.planes * self.need.num_kv_heads * (self.need.head_dim * elem + (1 if self.e4m3 else 0))
 
 
 @dataclass
@@ -135,7 +149,9 @@ class StateSlots:
 class CacheManager:
     def __init__(self, needs: dict[int, PagedKVNeed | SlotStateNeed], num_pages: int, page_size: int,
                  dtype: torch.dtype | None = None, device=None, num_state_slots: int = 64,
-                 watermark: float = 0.0) -> None:
+                 watermark: float = 0.0, kv_dtype: str = "auto") -> None:
+        if kv_dtype not in KV_DTYPES:
+            raise ValueError(f"unknown kv_dtype {kv_dtype!r}, expected one of {KV_DTYPES}")
         if watermark < 0:
             raise ValueError(f"watermark must be non-negative, got {watermark}")
         self.page_size = page_size
@@ -159,9 +175,14 @@ class CacheManager:
                 seen.append(need)
             if several:
                 self.view_order[layer] = tuple(seen)
+        if kv_dtype == "e4m3":
+            refused = [layer for need, layers in by_need.items() if not need.e4m3 for layer in layers]
+            if refused or not by_need:
+                raise ValueError("kv_dtype e4m3: " + (f"the mixers of cache layers {sorted(refused)} keep rows that cannot be held in 8 bits"
+                                                      if refused else "this model keeps no keys and values in pages"))
         # a group of one row per `every` positions holds 1/every of the rows, and up to one part-filled page a request more
         self.groups = [PageGroup(need, layers, num_pages if need.every == 1 else -(-num_pages // need.every) + num_state_slots,
-                                 page_size, dtype, device) for need, layers in by_need.items()]
+                                 page_size, dtype, device, kv_dtype == "e4m3") for need, layers in by_need.items()]
         self.group_of_need = {need: g for g, need in enumerate(by_need)}
         self.group_of_layer = {layer: g for g, group in reversed(list(enumerate(self.groups))) for layer in group.cache_layers}
         self.state = StateSlots(state_needs, num_state_slots, device)
@@ -277,6 +298,8 @@ class CacheManager:
         planes = group.kv.view(group.kv.shape[0] * group.kv.shape[1], *group.kv.shape[2:])
         pairs = torch.tensor([[src, dst]], dtype=torch.int32, device=group.kv.device)
         ops.copy_pages(planes, pairs, self.status)
+        if group.exps is not None:
+            group.exps[:, :, dst].copy_(group.exps[:, :, src])
 
     def release_behind_window(self, req: RequestCache, computed: int) -> int:
         """Give back pages of windowed groups that no later token can read: a query at position
@@ -368,7 +391,7 @@ class CacheManager:
 
         def paged(g: int, layer: int) -> PagedView:
             k, v = self.groups[g].layer_kv(layer)
-            return PagedView(k, v, block_tables[g], slots[g], True)
+            return PagedView(k, v, block_tables[g], slots[g], True, *self.groups[g].layer_exps(layer))
 
         def state(layer: int) -> StateView:
             return StateView(self.state.tensors[layer], state_slots, list(state_slots_host))

@@ -95,7 +95,7 @@ def _cmd_replay(args) -> int:
     from .engine.trace import main as trace_main
 
     return trace_main(["--model", args.model, "--dtype", args.dtype, "--out", args.out,
-                       "--max-tokens", str(args.max_tokens), "--page-size", str(args.page_size)])
+                       "--max-tokens", str(args.max_tokens), "--page-size", str(args.page_size), "--kv-dtype", args.kv_dtype])
 
 
 def main(argv: list[str] | None = None) -> int:
@@ -135,6 +135,7 @@ def main(argv: list[str] | None = None) -> int:
     t.add_argument("--out", required=True)
     t.add_argument("--max-tokens", type=int, required=True)
     t.add_argument("--page-size", type=int, default=16)
+    t.add_argument("--kv-dtype", default="auto", choices=["auto", "e4m3"])
     t.set_defaults(fn=_cmd_replay)
 
     args = parser.parse_args(argv)

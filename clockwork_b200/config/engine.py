@@ -5,7 +5,7 @@ The field names and meanings follow the reference's ``clockwork/config.py:17-87`
 YAML profiles load unchanged.  Fields that only made sense for a multi-backend
 engine (``device``, ``trust_remote_code``, ``attention_backend``) are accepted in a
 YAML file and ignored; new fields are ``prefill_chunk_size`` (the scheduler cuts
-prompts into portions, which the reference does not) and ``num_state_slots``.
+prompts into portions, which the reference does not), ``num_state_slots`` and ``kv_dtype``.
 """
 
 from __future__ import annotations
@@ -51,6 +51,7 @@ class CacheConfig:
     enable_prefix_cache: bool = True
     watermark: float = 0.01
     num_state_slots: int | None = None  # default: scheduler.max_num_seqs
+    kv_dtype: str = "auto"  # "e4m3": keys and values in 8 bits, a power of two per token and KV head (models of `attention` layers)
 
 
 @dataclass

@@ -66,6 +66,7 @@ class LLMEngine:
         self.cache = CacheManager(
             needs, num_pages=cfg.cache.num_blocks, page_size=cfg.cache.block_size, dtype=model.dtype, device=model.device,
             num_state_slots=cfg.cache.num_state_slots or cfg.scheduler.max_num_seqs, watermark=cfg.cache.watermark,
+            kv_dtype=cfg.cache.kv_dtype,
         )
         self.prefix_cache = None
         if self.cache.groups:

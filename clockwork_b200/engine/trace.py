@@ -35,7 +35,7 @@ import numpy as np
 import torch
 
 from ..cache.allocator import OutOfPages
-from ..cache.manager import CacheManager
+from ..cache.manager import KV_DTYPES, CacheManager
 from ..cache.prefix import PrefixCache
 from .loading import load_model
 from .step import ModelRunner, StepEntry
@@ -47,7 +47,7 @@ BUDGET_GRANULE = 64  # --max-tokens counts each request rounded up to a multiple
 class TraceSession:
     def __init__(self, model_dir: str | Path, dtype: str, max_tokens: int, page_size: int = 16,
                  device: str = "cuda:0", max_live: int = MAX_LIVE_REQUESTS, graphs: bool = True,
-                 prefix_cache: bool = False) -> None:
+                 prefix_cache: bool = False, kv_dtype: str = "auto") -> None:
         if max_tokens <= 0:
             raise ValueError("--max-tokens must be positive")
         if page_size <= 0:
@@ -59,7 +59,7 @@ class TraceSession:
             num_pages += max_live
         self.cache = CacheManager(
             self.model.cache_needs(), num_pages=num_pages, page_size=page_size, dtype=self.model.dtype,
-            device=device, num_state_slots=max_live, watermark=0.0,
+            device=device, num_state_slots=max_live, watermark=0.0, kv_dtype=kv_dtype,
         )
         self.runner = ModelRunner(self.model, self.cache)
         self.uses_graphs = graphs and self.runner.enable_graphs(max_ctx=num_pages * page_size, max_batch=max_live)
@@ -169,6 +169,7 @@ def main(argv: list[str] | None = None) -> int:
                         help="run single-token steps through the uncaptured step function too")
     parser.add_argument("--prefix-cache", action="store_true",
                         help="share whole pages of equal leading tokens between requests (see the module text)")
+    parser.add_argument("--kv-dtype", default="auto", choices=KV_DTYPES, help="e4m3: keys and values in 8 bits")
     parser.add_argument("--device", default="cuda:0")
     args = parser.parse_args(argv)
     if not torch.cuda.is_available():
@@ -177,7 +178,7 @@ def main(argv: list[str] | None = None) -> int:
     print("trace_run: loading model and kernels", file=sys.stderr, flush=True)
     try:
         session = TraceSession(args.model, args.dtype, args.max_tokens, args.page_size, args.device, args.max_live,
-                               graphs=not args.no_graphs, prefix_cache=args.prefix_cache)
+                               graphs=not args.no_graphs, prefix_cache=args.prefix_cache, kv_dtype=args.kv_dtype)
     except ValueError as exc:
         print(f"trace_run: {exc}", file=sys.stderr)
         return 1

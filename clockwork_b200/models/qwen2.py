@@ -47,6 +47,7 @@ class Qwen2Config:
     tie_word_embeddings: bool
     eos_token_ids: tuple[int, ...]
     max_position_embeddings: int | None
+    qk_norm: bool = False  # RMS norms over every query and key head (``q_norm.weight``, ``k_norm.weight`` of a layer's attention)
 
     @classmethod
     def from_raw(cls, raw: dict[str, Any]) -> "Qwen2Config":
@@ -94,6 +95,7 @@ class Qwen2Config:
             tie_word_embeddings=bool(raw.get("tie_word_embeddings", False)),
             eos_token_ids=eos_ids,
             max_position_embeddings=raw.get("max_position_embeddings"),
+            qk_norm=bool(raw.get("qk_norm", False)),
         )
 
     def to_raw(self) -> dict[str, Any]:
@@ -113,6 +115,8 @@ class Qwen2Config:
             "hidden_act": "silu",
             "use_sliding_window": False,
         }
+        if self.qk_norm:
+            raw["qk_norm"] = True
         if self.max_position_embeddings is not None:
             raw["max_position_embeddings"] = self.max_position_embeddings
         if self.eos_token_ids:
@@ -166,6 +170,7 @@ class Qwen2Architecture:
                 "scale": config.head_dim**-0.5,  # clockwork/engine/model.py:73
                 "window": None,  # full causal attention
                 "position": position,
+                **({"qk_norm": config.rms_norm_eps} if config.qk_norm else {}),
             },
         )
         ffn = PartSpec(

@@ -509,7 +509,8 @@ class _Prefill:
         return head_dim in PREFILL_HEAD_DIMS and ctx.q_start is not None
 
     @staticmethod
-    def run(ctx, qkv, view, num_heads, num_kv_heads, head_dim, scale, window) -> torch.Tensor:
+    def singles_apart(ctx, head_dim) -> int:
+        """How many requests, at most, bring a single token that another kernel than the portions' serves."""
         # Requests that bring a single token go to the decode kernel (a context split over CTAs, the query
         # heads of a KV head sharing every tile) instead of taking a 128-row query tile per head here; the
         # two kernels fill one output tensor.
@@ -517,13 +518,23 @@ class _Prefill:
         if captured is not None:
             # a captured step: how its tokens are divided is not known here; the work list is an array of
             # the step, and whether single tokens are served apart was fixed when the step was captured
-            singles = ctx.num_seqs if captured["singles"] and _route_single_tokens and head_dim in DECODE_HEAD_DIMS else 0
-        else:
-            singles = sum(1 for n in ctx.q_lens_host if n == 1) if _route_single_tokens and head_dim in DECODE_HEAD_DIMS else 0
-        item_seq, item_q0, item_split, items = _work_items(ctx, _cuts_for(num_heads, head_dim, view.k_cache.shape[1]), singles > 0)
-        out = attention_prefill(qkv, view.k_cache, view.v_cache, view.block_tables, ctx.q_start, ctx.ctx_lens,
-                                item_seq, item_q0, items, num_heads, num_kv_heads, head_dim, scale, window, ctx.status,
-                                item_split=item_split)
+            return ctx.num_seqs if captured["singles"] and _route_single_tokens and head_dim in DECODE_HEAD_DIMS else 0
+        return sum(1 for n in ctx.q_lens_host if n == 1) if _route_single_tokens and head_dim in DECODE_HEAD_DIMS else 0
+
+    @staticmethod
+    def portions(ctx, qkv, k_cache, v_cache, block_tables, num_heads, num_kv_heads, head_dim, scale, window, singles) -> torch.Tensor:
+        """Attention of the step's portions (with ``singles``: of those of more than one token)."""
+        item_seq, item_q0, item_split, items = _work_items(ctx, _cuts_for(num_heads, head_dim, k_cache.shape[1]), singles > 0)
+        return attention_prefill(qkv, k_cache, v_cache, block_tables, ctx.q_start, ctx.ctx_lens,
+                                 item_seq, item_q0, items, num_heads, num_kv_heads, head_dim, scale, window, ctx.status,
+                                 item_split=item_split)
+
+    @staticmethod
+    def run(ctx, qkv, view, num_heads, num_kv_heads, head_dim, scale, window) -> torch.Tensor:
+        captured = ctx.extras.get("captured_portions")
+        singles = _Prefill.singles_apart(ctx, head_dim)
+        out = _Prefill.portions(ctx, qkv, view.k_cache, view.v_cache, view.block_tables, num_heads, num_kv_heads, head_dim, scale, window,
+                                singles)
         if singles and captured is not None:
             # any of the step's requests may be one that brings a single token, with a context up to the
             # step's bound; how finely contexts are cut is a device scalar of the step

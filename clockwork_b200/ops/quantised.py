@@ -366,3 +366,50 @@ def attention_portions(q: torch.Tensor, cache: E4M3Pages, block_tables: torch.Te
                                       nkv, hd, scale, window, status, item_split=plan.item_split)
     return attention_ref(q, held.k, held.v, block_tables, plan.tok_seq, plan.positions, num_heads, nkv, hd, scale, window, status, q_start,
                          list(zip(plan.q_lens, plan.ctx_lens)))
+
+
+# ---- the attention of a step ---------------------------------------------------------------------------------------------------
+_step_workspaces: dict = {}
+
+
+def step_workspace(requests: int, num_heads: int, num_kv_heads: int, head_dim: int, index: int) -> DecodeWorkspace:
+    """The workspace that the layers of a device's engine steps share (steps run one after the other); replaced by a larger one
+    when a step brings more requests, and kept then, since captured steps point at it."""
+    key = (index, num_heads, num_kv_heads, head_dim)
+    held = _step_workspaces.get(key)
+    if held is None or held[0] < requests:
+        if torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("the workspace of a captured step must exist before it is captured: run the step once first")
+        if held is not None:
+            _retired_scratch.append(held)
+        room = max(requests, 256)
+        held = _step_workspaces[key] = (room, DecodeWorkspace(room, num_heads, num_kv_heads, head_dim, torch.device("cuda", index)))
+    return held[1]
+
+
+def paged_attention(ctx, q: torch.Tensor, cache: E4M3Pages, block_tables: torch.Tensor, num_heads: int, scale: float,
+                    window: int | None) -> torch.Tensor:
+    """Attention of a step of the engine over an 8-bit cache that already holds the step's keys and values: single tokens straight
+    from the codes; portions from their requests' pages read back into scratch pages, by the kernels of the run's type."""
+    from . import attention_ref
+    from .attention_fast import _Prefill
+
+    _, _, nkv, hd = cache.k.shape
+    index = q.get_device()
+
+    def singles(out=None):
+        scratch = step_workspace(ctx.num_seqs, num_heads, nkv, hd, index) if q.dtype == torch.bfloat16 and hd % 32 == 0 else None
+        return attention_decode(q, cache, block_tables, ctx.ctx_lens, num_heads, scale, ctx.status, window=window,
+                                q_start=None if out is None else ctx.q_start, out=out, workspace=scratch)
+
+    if ctx.all_single_token:
+        return singles()
+    held = portion_scratch(cache, q.dtype)
+    if q.dtype == torch.bfloat16 and _Prefill.accepts(ctx, None, num_heads, nkv, hd, window):
+        apart = _Prefill.singles_apart(ctx, hd)
+        read_pages(cache, block_tables, ctx.ctx_lens, held.k, held.v, ctx.status, window=window, q_start=ctx.q_start, skip_single=apart > 0)
+        out = _Prefill.portions(ctx, q, held.k, held.v, block_tables, num_heads, nkv, hd, scale, window, apart)
+        return singles(out) if apart else out
+    read_pages(cache, block_tables, ctx.ctx_lens, held.k, held.v, ctx.status, window=window, q_start=ctx.q_start)
+    return attention_ref(q, held.k, held.v, block_tables, ctx.tok_seq, ctx.positions, num_heads, nkv, hd, scale, window, ctx.status,
+                         ctx.q_start, list(zip(ctx.q_lens_host, ctx.ctx_lens_host)))

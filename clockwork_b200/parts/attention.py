@@ -4,10 +4,14 @@ Reference: ``clockwork/engine/model.py:66-128``: q/k/v projections (biased in Qw
 encoding on q and k, K/V written to the cache by slot before attention reads them, causal
 attention with the query aligned to the end of its request's context, output projection
 (bias-free in Qwen2).  Parameters: ``hidden_size, num_heads, num_kv_heads, head_dim, qkv_bias,
-o_bias, scale, window, position`` (a position-encoding spec).  Tensors (Hugging Face names):
-``q_proj/k_proj/v_proj.weight`` (+ ``.bias``), ``o_proj.weight`` (+ ``.bias``).
+o_bias, scale, window, position`` (a position-encoding spec), ``qk_norm`` (None, or the epsilon of RMS norms over the entries of
+every query and key head, before the rotation).  Tensors (Hugging Face names):
+``q_proj/k_proj/v_proj.weight`` (+ ``.bias``), ``o_proj.weight`` (+ ``.bias``), with ``qk_norm`` ``q_norm.weight``, ``k_norm.weight``.
 
 At load q, k and v rows are concatenated so that one product yields [q | k | v] per token.
+
+With normed heads, or over a cache that holds keys and values in 8 bits, one kernel norms, rotates and stores
+(``ops.quantised.norm_rotate_store``) and attention reads what it stored.
 """
 
 from __future__ import annotations
@@ -15,7 +19,7 @@ from __future__ import annotations
 import torch
 
 from .. import ops
-from ..ops import attention as attention_ops
+from ..ops import attention as attention_ops, quantised
 from ..weights.decl import TensorDecl
 from .base import Mixer, PagedKVNeed, PagedView, ResidualStream, StepContext
 from .linear import Linear
@@ -42,14 +46,20 @@ class Attention(Mixer):
             raise ValueError(f"head_dim {self.head_dim}: the attention kernels take multiples of 16 up to 256")
         if self.window is not None and int(self.window) <= 0:
             raise ValueError("window must be positive or None")
+        self.qk_norm = None if p.get("qk_norm") is None else float(p["qk_norm"])
         self.position = build_part("position", p["position"], prefix, dtype, device)
+        # (a position encoding that other kernels can apply: its frequencies and how many entries turn)
+        self.separable = hasattr(self.position, "fused_decode_args")
+        if self.qk_norm is not None and (self.qk_norm < 0 or not self.separable):
+            raise ValueError("qk_norm needs an epsilon that is not negative and a position encoding that hands its constants over")
+        self.q_norm = self.k_norm = None
         self.graph_safe = bool(self.position.graph_safe)
         self.graph_safe_portions = bool(getattr(self.position, "graph_safe_portions", False))
         self.qkv: Linear | None = None
         self.o: Linear | None = None
 
     def cache_need(self) -> PagedKVNeed:
-        return PagedKVNeed(self.num_kv_heads, self.head_dim, int(self.window) if self.window else None)
+        return PagedKVNeed(self.num_kv_heads, self.head_dim, int(self.window) if self.window else None, e4m3=self.separable)
 
     def step_scalars(self):
         """How finely the decode kernel cuts contexts is decided per step from the live requests."""
@@ -82,6 +92,9 @@ class Attention(Mixer):
         yield TensorDecl(self.name("o_proj.weight"), (self.hidden_size, q_out), "matrix", "linear")
         if self.o_bias:
             yield TensorDecl(self.name("o_proj.bias"), (self.hidden_size,), "vector", "bias")
+        if self.qk_norm is not None:
+            for norm in ("q_norm", "k_norm"):
+                yield TensorDecl(self.name(f"{norm}.weight"), (self.head_dim,), "vector", "norm")
         yield from self.position.tensor_decls()
 
     def load_weights(self, fetch) -> None:
@@ -91,10 +104,14 @@ class Attention(Mixer):
             b = torch.cat([fetch(self.name(f"{p}.bias")) for p in ("q_proj", "k_proj", "v_proj")], dim=0)
         self.qkv = Linear(w.contiguous(), b)
         self.o = Linear(fetch(self.name("o_proj.weight")), fetch(self.name("o_proj.bias")) if self.o_bias else None)
+        if self.qk_norm is not None:
+            self.q_norm, self.k_norm = fetch(self.name("q_norm.weight")), fetch(self.name("k_norm.weight"))
         self.position.load_weights(fetch)
 
     def forward(self, ctx: StepContext, x: torch.Tensor, view: PagedView, stream: ResidualStream):
         qkv = self.qkv(x)  # [N, (nh + 2 nkv) hd]
+        if self.qk_norm is not None or view.k_exp is not None:
+            return self.o.add_or_defer(self._store_and_attend(ctx, qkv, view), stream)
         # When every request decodes one token, the attention kernel itself rotates q and the new k and
         # stores the new k, v (one kernel less per layer), provided the position part can hand its
         # constants over; otherwise the position part runs its own kernel first.
@@ -107,6 +124,20 @@ class Attention(Mixer):
         out = attention_ops.paged_attention(ctx, qkv, view, self.num_heads, self.num_kv_heads,
                                             self.head_dim, self.scale, self.window, fused_position=fused)
         return self.o.add_or_defer(out, stream)
+
+
+    def _store_and_attend(self, ctx: StepContext, qkv: torch.Tensor, view: PagedView) -> torch.Tensor:
+        nh, nkv, hd = self.num_heads, self.num_kv_heads, self.head_dim
+        constants = self.position.fused_decode_args(hd) if self.separable else None
+        if constants is None or not view.write:
+            raise ValueError("normed heads and 8-bit caches need a rotation that fits the head and a cache that is written")
+        cache = quantised.PlainPages(view.k_cache, view.v_cache) if view.k_exp is None else quantised.E4M3Pages(
+            view.k_cache, view.v_cache, view.k_exp, view.v_exp)
+        q = quantised.norm_rotate_store(qkv, ctx.positions, view.slots, constants[0], cache, nh, nkv, hd, ctx.status, q_weight=self.q_norm,
+                                        k_weight=self.k_norm, eps=self.qk_norm or 0.0)
+        if view.k_exp is None:
+            return attention_ops.paged_attention(ctx, q, view, nh, nkv, hd, self.scale, self.window)
+        return quantised.paged_attention(ctx, q, cache, view.block_tables, nh, self.scale, self.window)
 
 
 register_mixer("attention", Attention, replace=True)

@@ -42,7 +42,8 @@ class PagedKVNeed:
     made from): its view's ``k_cache`` and ``v_cache`` are then the same tensor.  ``every``: the mixer keeps one row per
     ``every`` positions (a summary of each whole block of that many): row r belongs to positions r*every .. r*every +
     every - 1, and the slot that a step names for a token is the row of the token's block; no window.  ``keep_first``: beside
-    the window, the sequence's first ``keep_first`` tokens are read for ever (their pages are never given back)."""
+    the window, the sequence's first ``keep_first`` tokens are read for ever (their pages are never given back).  ``e4m3``: the
+    mixer can keep its keys and values in 8 bits (its view then has ``k_exp`` and ``v_exp``), if the cache is asked to."""
 
     num_kv_heads: int
     head_dim: int
@@ -51,6 +52,7 @@ class PagedKVNeed:
     block: int | None = None
     every: int = 1
     keep_first: int = 0
+    e4m3: bool = False
 
 
 @dataclass(frozen=True)
@@ -71,6 +73,8 @@ class PagedView:
     block_tables: torch.Tensor  # int32 [S, max_blocks] of this step's requests (-1: no page)
     slots: torch.Tensor  # int32 [N]: where each token's k/v go (page*page_size + offset)
     write: bool = True
+    k_exp: torch.Tensor | None = None  # 8-bit caches: powers, uint8 [pages, kv_heads, page_size]; k_cache and v_cache then hold
+    v_exp: torch.Tensor | None = None  # the codes, float8_e4m3fn
 
     @property
     def page_size(self) -> int:

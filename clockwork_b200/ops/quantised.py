@@ -106,20 +106,17 @@ def check_pages(cache: E4M3Pages) -> tuple[int, int, int, int]:
     return shape
 
 
-def norm_rotate_store(qkv: torch.Tensor, positions: torch.Tensor, slots: torch.Tensor, inv_freq: torch.Tensor | None, cache,
-                      num_heads: int, num_kv_heads: int, head_dim: int, status: torch.Tensor, *,
-                      q_weight: torch.Tensor | None = None, k_weight: torch.Tensor | None = None, eps: float = 0.0) -> torch.Tensor:
-    """What lies between the [q | k | v] product and attention, in one pass: ``qkv`` [N, (nh + 2 nkv) hd] (float32 or bfloat16;
-    left as it is), RMS norms of every query and key head with float32 ``q_weight``, ``k_weight`` [hd] (None: not normed), the
-    rotation of each head's leading ``2 * len(inv_freq)`` entries by ``positions`` (None: none turn; entry j pairs with
-    j + len(inv_freq)), and the write of k and v at ``slots`` (< 0: not stored) of ``cache`` (``E4M3Pages``, or ``PlainPages``
-    of qkv's type).  Returns q [N, nh * hd].  Everything up to the one rounding of each output is float32."""
-    code = dtype_code(qkv.dtype)
+def _check_rows(qkv: torch.Tensor, num_heads: int, num_kv_heads: int, head_dim: int) -> int:
+    """How many rows [q | k | v] has."""
     if qkv.dim() != 2 or not qkv.is_contiguous() or qkv.shape[1] != (num_heads + 2 * num_kv_heads) * head_dim:
         raise ValueError(f"qkv must be contiguous [N, (nh + 2 nkv) * hd], got {tuple(qkv.shape)}")
-    if not 0 < head_dim <= MAX_HEAD_DIM:
-        raise ValueError(f"head_dim {head_dim} must be positive and at most {MAX_HEAD_DIM}")
-    n = qkv.shape[0]
+    if not 0 < head_dim <= MAX_HEAD_DIM or num_heads <= 0 or num_kv_heads <= 0:
+        raise ValueError(f"head_dim {head_dim} must be positive and at most {MAX_HEAD_DIM}, and there must be heads")
+    return qkv.shape[0]
+
+
+def _store_call(qkv, n, positions, slots, inv_freq, cache, num_heads, num_kv_heads, head_dim, status, code, q_weight, k_weight, eps):
+    """The rest of ``norm_rotate_store``'s checks: (q, the entry point's words, the cache's shape, the device)."""
     _ints(positions, "positions", 1, n)
     _ints(slots, "slots", 1, n)
     _check_status(status)
@@ -148,11 +145,25 @@ def norm_rotate_store(qkv: torch.Tensor, positions: torch.Tensor, slots: torch.T
                status=status)
     _check_device(index)
     q = qkv.new_empty((n, num_heads * head_dim))
-    check(library().cw_norm_rotate_store(_STORE_ARGS(
+    words = _STORE_ARGS(
         qkv.data_ptr(), q.data_ptr(), positions.data_ptr(), slots.data_ptr(), inv_freq.data_ptr() if rot else 0,
         0 if q_weight is None else q_weight.data_ptr(), 0 if k_weight is None else k_weight.data_ptr(), cache.k.data_ptr(), cache.v.data_ptr(),
         cache.k_exp.data_ptr() if quantised else 0, cache.v_exp.data_ptr() if quantised else 0, status.data_ptr(), _stream(), n, num_heads,
-        num_kv_heads, head_dim, rot, shape[1], shape[0], code, eps)), "norm_rotate_store")
+        num_kv_heads, head_dim, rot, shape[1], shape[0], code, eps)
+    return q, words, shape, index
+
+
+def norm_rotate_store(qkv: torch.Tensor, positions: torch.Tensor, slots: torch.Tensor, inv_freq: torch.Tensor | None, cache,
+                      num_heads: int, num_kv_heads: int, head_dim: int, status: torch.Tensor, *,
+                      q_weight: torch.Tensor | None = None, k_weight: torch.Tensor | None = None, eps: float = 0.0) -> torch.Tensor:
+    """What lies between the [q | k | v] product and attention, in one pass: ``qkv`` [N, (nh + 2 nkv) hd] (float32 or bfloat16;
+    left as it is), RMS norms of every query and key head with float32 ``q_weight``, ``k_weight`` [hd] (None: not normed), the
+    rotation of each head's leading ``2 * len(inv_freq)`` entries by ``positions`` (None: none turn; entry j pairs with
+    j + len(inv_freq)), and the write of k and v at ``slots`` (< 0: not stored) of ``cache`` (``E4M3Pages``, or ``PlainPages``
+    of qkv's type).  Returns q [N, nh * hd].  Everything up to the one rounding of each output is float32."""
+    code, n = dtype_code(qkv.dtype), _check_rows(qkv, num_heads, num_kv_heads, head_dim)
+    q, words = _store_call(qkv, n, positions, slots, inv_freq, cache, num_heads, num_kv_heads, head_dim, status, code, q_weight, k_weight, eps)[:2]
+    check(library().cw_norm_rotate_store(words), "norm_rotate_store")
     return q
 
 
@@ -236,6 +247,20 @@ def _workspace(workspace: DecodeWorkspace | None, requests: int, num_heads: int,
     return held
 
 
+def _decode_call(q, out, cache, block_tables, ctx_lens, q_start, num_heads, shape, scale, window, code, status, index, workspace) -> None:
+    pages, page_size, nkv, hd = shape
+    s = block_tables.shape[0]
+    stream, sms, floats, words = _stream(), _sm_count(index), 0, 0
+    if code == 1 and hd % 32 == 0:
+        scratch = _workspace(workspace, s, num_heads, nkv, hd, index, stream, sms)
+        floats, words = scratch.floats.data_ptr(), scratch.words.data_ptr()
+    check(library().cw_attention_decode_e4m3(_DECODE_ARGS(
+        q.data_ptr(), out.data_ptr(), cache.k.data_ptr(), cache.v.data_ptr(), cache.k_exp.data_ptr(), cache.v_exp.data_ptr(),
+        block_tables.data_ptr(), ctx_lens.data_ptr(), 0 if q_start is None else q_start.data_ptr(), floats, words, status.data_ptr(), stream,
+        q.stride(0) if q.shape[0] > 1 else num_heads * hd, s, num_heads, nkv, hd, page_size, block_tables.shape[1], pages, window or 0, code,
+        sms, scale)), "attention_decode_e4m3")
+
+
 def attention_decode(q: torch.Tensor, cache: E4M3Pages, block_tables: torch.Tensor, ctx_lens: torch.Tensor, num_heads: int,
                      scale: float, status: torch.Tensor, *, window: int | None = None, q_start: torch.Tensor | None = None,
                      out: torch.Tensor | None = None, workspace: DecodeWorkspace | None = None) -> torch.Tensor:
@@ -273,15 +298,8 @@ def attention_decode(q: torch.Tensor, cache: E4M3Pages, block_tables: torch.Tens
     _check_device(index)
     if out is None:
         out = q.new_empty((s, num_heads * hd))
-    stream, sms, floats, words = _stream(), _sm_count(index), 0, 0
-    if code == 1 and hd % 32 == 0:
-        scratch = _workspace(workspace, s, num_heads, nkv, hd, index, stream, sms)
-        floats, words = scratch.floats.data_ptr(), scratch.words.data_ptr()
-    check(library().cw_attention_decode_e4m3(_DECODE_ARGS(
-        q.data_ptr(), out.data_ptr(), cache.k.data_ptr(), cache.v.data_ptr(), cache.k_exp.data_ptr(), cache.v_exp.data_ptr(),
-        block_tables.data_ptr(), ctx_lens.data_ptr(), 0 if q_start is None else q_start.data_ptr(), floats, words, status.data_ptr(), stream,
-        q.stride(0) if q.shape[0] > 1 else num_heads * hd, s, num_heads, nkv, hd, page_size, block_tables.shape[1], pages, window or 0, code,
-        sms, scale)), "attention_decode_e4m3")
+    _decode_call(q, out, cache, block_tables, ctx_lens, q_start, num_heads, (pages, page_size, nkv, hd), scale, window, code, status, index,
+                 workspace)
     return out
 
 
@@ -291,9 +309,22 @@ def decode_step(qkv: torch.Tensor, positions: torch.Tensor, slots: torch.Tensor,
                 eps: float = 0.0, window: int | None = None, workspace: DecodeWorkspace | None = None) -> torch.Tensor:
     """``norm_rotate_store`` of one new token per request, then ``attention_decode`` of it: what an attention layer does between
     its two products while every request decodes.  ``ctx_lens`` count the new tokens."""
-    q = norm_rotate_store(qkv, positions, slots, inv_freq, cache, num_heads, num_kv_heads, head_dim, status, q_weight=q_weight,
-                          k_weight=k_weight, eps=eps)
-    return attention_decode(q, cache, block_tables, ctx_lens, num_heads, scale, status, window=window, workspace=workspace)
+    code, n = dtype_code(qkv.dtype), _check_rows(qkv, num_heads, num_kv_heads, head_dim)
+    if not isinstance(cache, E4M3Pages):
+        raise ValueError(f"an 8-bit cache (E4M3Pages) is needed, got {type(cache).__name__}")
+    if num_heads % num_kv_heads or head_dim % 16:
+        raise ValueError(f"{num_heads} query heads over {num_kv_heads} KV heads of {head_dim}: a multiple of the KV heads, entries a multiple of 16")
+    _ints(block_tables, "block_tables", 2, n)
+    _ints(ctx_lens, "ctx_lens", 1, n)
+    if window is not None and window <= 0:
+        raise ValueError("window must be positive or None")
+    q, words, shape, index = _store_call(qkv, n, positions, slots, inv_freq, cache, num_heads, num_kv_heads, head_dim, status, code, q_weight,
+                                         k_weight, eps)
+    _elsewhere(index, block_tables=block_tables, ctx_lens=ctx_lens)
+    out = torch.empty_like(q)
+    check(library().cw_norm_rotate_store(words), "norm_rotate_store")
+    _decode_call(q, out, cache, block_tables, ctx_lens, None, num_heads, shape, scale, window, code, status, index, workspace)
+    return out
 
 
 # ---- prompt portions --------------------------------------------------------------------------------------------------------

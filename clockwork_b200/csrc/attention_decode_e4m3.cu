@@ -5,8 +5,8 @@
 // over the context's positions j (the last `window` of them), m their largest s_j; float32 but for what is said below.
 //
 // The step is a stream of codes from memory, 2 (hd + 1) bytes per token and KV head, so all query heads of a KV head (16 at
-// most, or 8) share what a block fetches.  Work is cut by the contexts themselves: requests, KV heads and tiles of 32 tokens
-// are numbered through, and every warp of a grid that fills the SMs once takes an equal run of tiles, wherever requests begin
+// most, or 8) share what a block fetches.  Work is cut by the contexts themselves: requests, KV heads and tiles of 16 to 64
+// tokens are numbered through, and every warp of a grid that fills the SMs once takes an equal run of tiles, wherever requests begin
 // and end in it (units_of_block); so contexts of any lengths fill the GPU, and no scratch grows with them.  Each warp has a ring
 // of tiles in shared memory of its own, filled by 16-byte asynchronous copies two or more tiles ahead and on into the next
 // request, so that warps never wait for one another while they stream.
@@ -46,7 +46,6 @@ struct DecodeE4m3Params {
     int* counters;           // [requests * nkv * groups] and [2 * blocks], zero between launches
 };
 
-#define TILE_TOKENS 32
 #define WARPS 4
 #define MERGE_AT_ONCE 8
 #ifndef LEAST_UNITS
@@ -74,9 +73,12 @@ __device__ __forceinline__ uint32_t half2_of(float a, float b) {
 
 template <int HD, int NT>
 struct Stream {
-    static constexpr int CH = HD / 16;                 // 16-byte chunks of a row
-    static constexpr int TILE_BYTES = TILE_TOKENS * HD;  // K or V of a tile
-    static constexpr int PER_SM = HD > 128 ? 1 : NT == 1 ? 3 : 2;  // blocks on an SM (registers: 168, 255)
+    static constexpr int CH = HD / 16;  // 16-byte chunks of a row
+    // Tokens of a tile: what a tile costs besides its products (looking up pages, the maxima's way over the lanes) is shared by
+    // more of them where rows are short, and rings stay deep enough for two blocks an SM where rows are long.
+    static constexpr int TOKENS = HD <= 64 ? 64 : HD <= 128 ? 32 : 16;
+    static constexpr int TILE_BYTES = TOKENS * HD;  // K or V of a tile
+    static constexpr int PER_SM = HD <= 128 && NT == 1 ? 3 : 2;  // blocks on an SM (registers: 168, 255)
     static constexpr int FIT = 196608 / PER_SM / (WARPS * 2 * TILE_BYTES);
     static constexpr int ST = FIT > 8 ? 8 : FIT;       // tiles in a warp's ring
     static constexpr int RING = WARPS * ST * 2 * TILE_BYTES;
@@ -120,11 +122,12 @@ struct Piece {
 template <int HD, int NT>
 __global__ void __launch_bounds__(WARPS * 32, Stream<HD, NT>::PER_SM) decode_e4m3_kernel(const DecodeE4m3Params p) {
     using C = Stream<HD, NT>;
-    constexpr int ROWS = 8 * NT, ST = C::ST, CH = C::CH;
+    constexpr int ROWS = 8 * NT, ST = C::ST, CH = C::CH, TOKENS = C::TOKENS;
+    constexpr int U = TOKENS / 16, HALVES = (TOKENS + 31) / 32;  // products' 16 tokens; a lane's tokens when pages are looked up
     constexpr int WORDS = HD / 32;  // a thread's 4-byte words of a V row
     extern __shared__ __align__(128) uint8_t ring_s[];
-    __shared__ uint32_t row_s[WARPS][ST][TILE_TOKENS];       // 16-byte chunk where a token's row begins; ~0: it does not count
-    __shared__ uint32_t power_at_s[WARPS][ST][TILE_TOKENS];  // where its powers are
+    __shared__ uint32_t row_s[WARPS][ST][TOKENS];       // 16-byte chunk where a token's row begins; ~0: it does not count
+    __shared__ uint32_t power_at_s[WARPS][ST][TOKENS];  // where its powers are
     __shared__ float m_s[2 * WARPS][ROWS], l_s[2 * WARPS][ROWS], f_s[2 * WARPS][ROWS];
     __shared__ Piece piece_s[2 * WARPS];  // of every warp: the end of a segment that began before its run, and what its run ends in
     __shared__ float top_s[2 * WARPS][ROWS], total_s[2 * WARPS][ROWS];  // of a group of pieces, at its first
@@ -138,7 +141,7 @@ __global__ void __launch_bounds__(WARPS * 32, Stream<HD, NT>::PER_SM) decode_e4m
     };
     auto begin_of = [&](int ctx) { return p.window > 0 ? max(0, ctx - p.window) : 0; };
     auto tiles_of = [&](int ctx) {
-        return ctx <= 0 ? 0 : (ctx + TILE_TOKENS - 1) / TILE_TOKENS - begin_of(ctx) / TILE_TOKENS;
+        return ctx <= 0 ? 0 : (ctx + TOKENS - 1) / TOKENS - begin_of(ctx) / TOKENS;
     };
     // A segment is its tiles and, before them, a unit for what changing to it costs (about a tile's time).  A block's run is a
     // whole number of equal runs for its warps.  Every warp finds its own: four neighbouring requests per lane, 128 at a time.
@@ -255,32 +258,42 @@ __global__ void __launch_bounds__(WARPS * 32, Stream<HD, NT>::PER_SM) decode_e4m
     const uint32_t my_ring_addr = smem_addr(my_ring);
     // ---- fetching: ST - 1 tiles ahead of the products, through the segments' ends ----
     Walk ahead = at;
-    int fetch_stage = 0, ahead_page = -1, ahead_pos = 0;
+    int fetch_stage = 0, ahead_page[HALVES], ahead_pos = 0;
     const int copy_lane = C::at(lane / CH, lane % CH);
-    auto look_up = [&]() {  // the page of this lane's token of the tile that is fetched next
-        ahead_page = -1;
+    auto look_up = [&]() {  // the pages of this lane's tokens of the tile that is fetched next
         if (ahead.left <= 0) return;
-        ahead_pos = (ahead.begin / TILE_TOKENS + ahead.tile) * TILE_TOKENS + lane;
-        if (ahead_pos >= ahead.begin && ahead_pos < ahead.ctx)
-            ahead_page = p.block_tables[(size_t)ahead.s * p.max_blocks + (p.page_shift >= 0 ? ahead_pos >> p.page_shift : ahead_pos / p.page_size)];
+        ahead_pos = (ahead.begin / TOKENS + ahead.tile) * TOKENS + lane;
+#pragma unroll
+        for (int h = 0; h < HALVES; ++h) {
+            const int pos = ahead_pos + 32 * h;
+            ahead_page[h] = -1;
+            if ((TOKENS >= 32 || lane < TOKENS) && pos >= ahead.begin && pos < ahead.ctx)
+                ahead_page[h] = p.block_tables[(size_t)ahead.s * p.max_blocks + (p.page_shift >= 0 ? pos >> p.page_shift : pos / p.page_size)];
+        }
     };
     auto fetch = [&]() {
         if (ahead.left > 0) {
             const int kvh = p.groups == 1 ? ahead.seg : ahead.seg / p.groups;
-            uint32_t row = ~0u, power_at = 0;
-            if (ahead_page >= 0 && ahead_page < p.num_pages) {
-                const int off = p.page_shift >= 0 ? ahead_pos & (p.page_size - 1) : ahead_pos % p.page_size;
-                row = ((uint32_t)(ahead_page * p.page_size + off) * p.nkv + kvh) * CH;
-                power_at = ((uint32_t)ahead_page * p.nkv + kvh) * p.page_size + off;
-            } else if (ahead_pos >= ahead.begin && ahead_pos < ahead.ctx) {
-                cw_report(p.status, CW_ST_PAGE_RANGE, ahead.s, ahead_page);
+#pragma unroll
+            for (int h = 0; h < HALVES; ++h) {
+                const int pos = ahead_pos + 32 * h, page = ahead_page[h];
+                uint32_t row = ~0u, power_at = 0;
+                if (page >= 0 && page < p.num_pages) {
+                    const int off = p.page_shift >= 0 ? pos & (p.page_size - 1) : pos % p.page_size;
+                    row = ((uint32_t)(page * p.page_size + off) * p.nkv + kvh) * CH;
+                    power_at = ((uint32_t)page * p.nkv + kvh) * p.page_size + off;
+                } else if ((TOKENS >= 32 || lane < TOKENS) && pos >= ahead.begin && pos < ahead.ctx) {
+                    cw_report(p.status, CW_ST_PAGE_RANGE, ahead.s, page);
+                }
+                if (TOKENS >= 32 || lane < TOKENS) {
+                    row_s[warp][fetch_stage][32 * h + lane] = row;
+                    power_at_s[warp][fetch_stage][32 * h + lane] = power_at;
+                }
             }
-            row_s[warp][fetch_stage][lane] = row;
-            power_at_s[warp][fetch_stage][lane] = power_at;
             __syncwarp();
             const uint32_t base = my_ring_addr + fetch_stage * 2 * C::TILE_BYTES;
 #pragma unroll
-            for (int j = 0; j < CH; ++j) {
+            for (int j = 0; j < TOKENS * CH / 32; ++j) {
                 const int i = j * 32 + lane;
                 const uint32_t from = row_s[warp][fetch_stage][32 % CH == 0 ? j * (32 / CH) + lane / CH : i / CH];
                 const bool there = from != ~0u;
@@ -296,13 +309,17 @@ __global__ void __launch_bounds__(WARPS * 32, Stream<HD, NT>::PER_SM) decode_e4m
         }
         cp_async_commit();
     };
-    // a lane looks up the powers of token 8 t + g a tile ahead of their use: K's, V's, and whether the token counts
-    uint32_t k_power = 0, v_power = 0, counts = 0;
+    // a lane looks up the powers of token 8 t + g (and 32 further) a tile ahead of their use: K's, V's, and whether the token counts
+    uint32_t k_power[HALVES], v_power[HALVES], counts[HALVES];
     auto look_at_powers = [&](int stage) {
-        const uint32_t i = power_at_s[warp][stage][8 * t + g];
-        counts = row_s[warp][stage][8 * t + g];
-        k_power = p.k_exp[i];
-        v_power = p.v_exp[i];
+#pragma unroll
+        for (int h = 0; h < HALVES; ++h) {
+            const int token = 32 * h + 8 * (TOKENS >= 32 ? t : t & 1) + g;
+            const uint32_t i = power_at_s[warp][stage][token];
+            counts[h] = row_s[warp][stage][token];
+            k_power[h] = p.k_exp[i];
+            v_power[h] = p.v_exp[i];
+        }
     };
     look_up();
     if (at.left > 0) call_queries(at);
@@ -364,20 +381,22 @@ __global__ void __launch_bounds__(WARPS * 32, Stream<HD, NT>::PER_SM) decode_e4m
             cp_async_wait<ST - 1>();
             __syncwarp();
             const int next = stage + 1 == ST ? 0 : stage + 1;
-            const uint32_t powers = counts == ~0u ? 0u : k_power | v_power << 8 | 1u << 16;
+            uint32_t powers[HALVES];
+#pragma unroll
+            for (int h = 0; h < HALVES; ++h) powers[h] = counts[h] == ~0u ? 0u : k_power[h] | v_power[h] << 8 | 1u << 16;
             if (i + 1 < n_tiles || ahead.left > 0 || fetch_stage != next) look_at_powers(next);
             const uint8_t* kt = my_ring + stage * 2 * C::TILE_BYTES;
             const uint8_t* vt = kt + C::TILE_BYTES;
-            float sc[NT][2][4];
+            float sc[NT][U][4];
 #pragma unroll
             for (int n = 0; n < NT; ++n)
 #pragma unroll
-                for (int u = 0; u < 2; ++u) sc[n][u][0] = sc[n][u][1] = sc[n][u][2] = sc[n][u][3] = 0.f;
+                for (int u = 0; u < U; ++u) sc[n][u][0] = sc[n][u][1] = sc[n][u][2] = sc[n][u][3] = 0.f;
 #pragma unroll
             for (int b = 0; b < PIECES; ++b) {
                 const uint8_t* kb = kt + (HD % 128 == 0 ? (k_at ^ ((b & 1) << 6)) + (b >> 1) * 128 : k_at + b * 4 * PIECE);
 #pragma unroll
-                for (int u = 0; u < 2; ++u) {
+                for (int u = 0; u < U; ++u) {
                     uint32_t lo[STEPS], hi[STEPS];  // rows g and g + 8
                     if (PIECE == 16) {
                         const uint4 x = *reinterpret_cast<const uint4*>(kb + 16 * u * HD), y = *reinterpret_cast<const uint4*>(kb + (16 * u + 8) * HD);
@@ -399,10 +418,10 @@ __global__ void __launch_bounds__(WARPS * 32, Stream<HD, NT>::PER_SM) decode_e4m
                 }
             }
             // scores of tokens 8 x + g (x = 2 u, 2 u + 1) for heads 2 t, 2 t + 1
-            float vs[4];  // 2^(127 - Ev)
+            float vs[2 * U];  // 2^(127 - Ev)
 #pragma unroll
-            for (int x = 0; x < 4; ++x) {
-                const uint32_t w = __shfl_sync(0xffffffffu, powers, (lane & ~3) | x);
+            for (int x = 0; x < 2 * U; ++x) {
+                const uint32_t w = __shfl_sync(0xffffffffu, powers[x >> 2], (lane & ~3) | (x & 3));
                 const float kf = kv_up(w & 255), ev = (w >> 16) != 0 ? (float)((int)((w >> 8) & 255) - 127) : -INFINITY;
                 vs[x] = kv_down((w >> 8) & 255);
 #pragma unroll
@@ -410,13 +429,15 @@ __global__ void __launch_bounds__(WARPS * 32, Stream<HD, NT>::PER_SM) decode_e4m
 #pragma unroll
                     for (int e = 0; e < 2; ++e) sc[n][x >> 1][2 * (x & 1) + e] = fmaf(sc[n][x >> 1][2 * (x & 1) + e] * qf[n][e], kf, ev);
             }
-            uint32_t pb[NT][2][2];
+            uint32_t pb[NT][U][2];
 #pragma unroll
             for (int n = 0; n < NT; ++n) {
                 float keep[2];
 #pragma unroll
                 for (int e = 0; e < 2; ++e) {
-                    float top = fmaxf(fmaxf(sc[n][0][e], sc[n][0][2 + e]), fmaxf(sc[n][1][e], sc[n][1][2 + e]));
+                    float top = -INFINITY;
+#pragma unroll
+                    for (int u = 0; u < U; ++u) top = fmaxf(top, fmaxf(sc[n][u][e], sc[n][u][2 + e]));
 #pragma unroll
                     for (int d = 4; d < 32; d <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
                     const float m_new = fmaxf(m[n][e], top), ref = m_new == -INFINITY ? 0.f : m_new - 14.f;
@@ -424,7 +445,7 @@ __global__ void __launch_bounds__(WARPS * 32, Stream<HD, NT>::PER_SM) decode_e4m
                     m[n][e] = m_new;
                     float sum = 0.f;
 #pragma unroll
-                    for (int u = 0; u < 2; ++u)
+                    for (int u = 0; u < U; ++u)
 #pragma unroll
                         for (int r = 0; r < 2; ++r) {
                             const float w = fast_exp2(sc[n][u][2 * r + e] - ref);
@@ -440,14 +461,14 @@ __global__ void __launch_bounds__(WARPS * 32, Stream<HD, NT>::PER_SM) decode_e4m
                     }
                 }
 #pragma unroll
-                for (int u = 0; u < 2; ++u)
+                for (int u = 0; u < U; ++u)
 #pragma unroll
                     for (int r = 0; r < 2; ++r) pb[n][u][r] = transposed(half2_of(sc[n][u][2 * r], sc[n][u][2 * r + 1]));
             }
             // O^T += V^T P^T: a thread pairs tokens (2 t, 2 t + 1) and (2 t + 8, 2 t + 9); its words of a row: 16 bytes of every
             // 128, then 8 of 64 and 4 of 32
 #pragma unroll
-            for (int u = 0; u < 2; ++u) {
+            for (int u = 0; u < U; ++u) {
                 uint32_t w[4][WORDS];
 #pragma unroll
                 for (int x = 0; x < 4; ++x) {
@@ -852,7 +873,7 @@ extern "C" int cw_attention_decode_e4m3(const char* block) {
                           max_blocks, num_pages, window, scale, status};
     const int groups = ((uintptr_t)q % 4 || q_stride % 2) ? 0 : groups_of(nh, nkv, hd, dtype);  // (queries are read in pairs)
     if (groups && floats != nullptr && words != nullptr && (long long)num_pages * page_size * nkv * (hd / 16) < 0xFFFFFFFFLL &&
-        (long long)requests * nkv * groups * ((long long)max_blocks * page_size / TILE_TOKENS + 2) < 0x7FFFFFFF) {
+        (long long)requests * nkv * groups * ((long long)max_blocks * page_size / 16 + 2) < 0x7FFFFFFF) {
         p.page_shift = (page_size & (page_size - 1)) == 0 ? __builtin_ctz(page_size) : -1;
         p.groups = groups;
         p.heads_each = (nh / nkv + groups - 1) / groups;

@@ -39,18 +39,19 @@ struct DecodeE4m3Params {
     int* status;
     // the streaming kernel
     int page_shift;          // log2 of the page size, or -1
+    int teams;               // KV heads that long walks take side by side
     int groups, heads_each;  // groups of query heads per KV head, heads in a group (the last may have fewer)
     float* heads_o;          // [4 * blocks][8 or 16][hd]: ends of segments that an earlier warp began
-    float* part_o;           // [2 * blocks][8 or 16][hd]
-    float* part_ml;          // [2 * blocks][8 or 16][2]
-    int* counters;           // [requests * nkv * groups] and [2 * blocks], zero between launches
+    float* part_o;           // [blocks][teams][2][8 or 16][hd]
+    float* part_ml;          // [blocks][teams][2][8 or 16][2]
+    int* counters;           // [requests * nkv * groups] and [blocks][teams][2], zero between launches
 };
 
 #define WARPS 4
 #define MERGE_AT_ONCE 8
-#ifndef LEAST_UNITS
-#define LEAST_UNITS 2
-#endif
+#define MOST_TEAMS 4
+#define TEAMS_FROM_BYTES 170000000LL
+#define LEAST_UNITS 2  // a warp's run: 8 requests of 1,024 tokens 16.4 us with 1 (nine pieces a segment to add up), 14.4 with 2
 
 __device__ __forceinline__ void mma_half(float* d, const uint32_t* a, uint32_t b0, uint32_t b1) {
     asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
@@ -116,6 +117,7 @@ struct Walk {
 struct Piece {
     int segment;           // -1: there is none
     int row, head, heads;  // where its outputs go
+    int team;
     int first_block, blocks;  // which blocks have pieces of it
 };
 
@@ -131,10 +133,10 @@ __global__ void __launch_bounds__(WARPS * 32, Stream<HD, NT>::PER_SM) decode_e4m
     __shared__ float m_s[2 * WARPS][ROWS], l_s[2 * WARPS][ROWS], f_s[2 * WARPS][ROWS];
     __shared__ Piece piece_s[2 * WARPS];  // of every warp: the end of a segment that began before its run, and what its run ends in
     __shared__ float top_s[2 * WARPS][ROWS], total_s[2 * WARPS][ROWS];  // of a group of pieces, at its first
-    __shared__ int last_s[2], final_s;
+    __shared__ int shared_s[2 * MOST_TEAMS], last_s[2 * MOST_TEAMS], final_s;
     pdl_enter();
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
-    const int per_request = p.nkv * p.groups;
+
     auto context_of = [&](int s) -> int {  // -1: not served here
         if (p.q_start != nullptr && p.q_start[s + 1] - p.q_start[s] != 1) return -1;
         return min(p.ctx_lens[s], p.max_blocks * p.page_size);
@@ -143,23 +145,36 @@ __global__ void __launch_bounds__(WARPS * 32, Stream<HD, NT>::PER_SM) decode_e4m
     auto tiles_of = [&](int ctx) {
         return ctx <= 0 ? 0 : (ctx + TOKENS - 1) / TOKENS - begin_of(ctx) / TOKENS;
     };
+    // Units are numbered through requests, teams' worth of KV heads, groups and tiles; every team of a block has the same ones.
     // A segment is its tiles and, before them, a unit for what changing to it costs (about a tile's time).  A block's run is a
-    // whole number of equal runs for its warps.  Every warp finds its own: four neighbouring requests per lane, 128 at a time.
-    auto units_of = [&](int tiles) { return tiles > 0 ? per_request * (tiles + 1) : 0; };
-    const int warps = gridDim.x * WARPS, chunks = (p.requests + 127) / 128;
+    // whole number of equal runs for a team's warps.  Every warp finds its own: four neighbouring requests per lane, 128 at a time.
+    const int chunks = (p.requests + 127) / 128;
     int context[4], total = 0;
     for (int c = chunks - 1; c >= 0; --c) {  // (the last one looked at is the first: what it holds is used again below)
         int units = 0;
 #pragma unroll
         for (int j = 0; j < 4; ++j) context[j] = c * 128 + 4 * lane + j < p.requests ? context_of(c * 128 + 4 * lane + j) : -1;
 #pragma unroll
-        for (int j = 0; j < 4; ++j) units += units_of(tiles_of(context[j]));
+        for (int j = 0; j < 4; ++j) {
+            const int tiles = tiles_of(context[j]);
+            if (tiles > 0) units += tiles + 1;
+        }
         total += units;
     }
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
-    const int quota = max(LEAST_UNITS, (total + warps - 1) / warps), block_units = quota * WARPS;
-    const int first = (int)min((long long)(blockIdx.x * WARPS + warp) * quota, (long long)total);
+    // Rows that are no multiple of 128 bytes share lines with their neighbours' rows (p.teams > 1), and the L2 fetches whole lines:
+    // as many KV heads, neighbours in memory, are walked at the same time by teams of the block's warps, so that a line comes once.
+    // Not where all that is read stays in the L2 (126 MB) until the neighbour comes anyway: one team's four warps leave a segment
+    // in fewer pieces.  Measured, cold, one team and two: 16 KV heads of 64, 100 MB 36.7 and 39.0 us, 200 MB 76.5 and 56.2, 400 MB 154 and
+    // 90; 2 of 96, 200 MB 53.6 and 59.4, 400 MB 137 and 92; 4 of 32 (four teams), 100 MB 50.9 and 65.0, 200 MB 106 and 93.
+    const int teams = (long long)total * p.nkv * p.groups * 2 * C::TILE_BYTES >= TEAMS_FROM_BYTES ? p.teams : 1;
+    const int of_team = WARPS / teams, team = warp / of_team, member = warp - team * of_team, warps = gridDim.x * of_team;
+    const int per_request = p.nkv / teams * p.groups;
+    total *= per_request;
+    auto units_of = [&](int tiles) { return tiles > 0 ? per_request * (tiles + 1) : 0; };
+    const int quota = max(LEAST_UNITS, (total + warps - 1) / warps), block_units = quota * of_team;
+    const int first = (int)min((long long)(blockIdx.x * of_team + member) * quota, (long long)total);
     auto zeros = [&]() {  // the rows of requests without a context
         for (int s = blockIdx.x; s < p.requests; s += gridDim.x) {
             if (context_of(s) != 0) continue;
@@ -229,10 +244,10 @@ __global__ void __launch_bounds__(WARPS * 32, Stream<HD, NT>::PER_SM) decode_e4m
     };
     // where a segment's queries are, and how many heads it has
     auto query_row = [&](const Walk& w) { return p.q_start != nullptr ? p.q_start[w.s] : w.s; };
-    auto first_head = [&](const Walk& w) {
-        return p.groups == 1 ? w.seg * p.heads_each : w.seg / p.groups * (p.nh / p.nkv) + w.seg % p.groups * p.heads_each;
-    };
-    auto heads_of = [&](const Walk& w) { return p.groups == 1 ? p.heads_each : min(p.heads_each, p.nh / p.nkv - w.seg % p.groups * p.heads_each); };
+    auto kv_head = [&](const Walk& w) { return (p.groups == 1 ? w.seg : w.seg / p.groups) * teams + team; };
+    auto part_of = [&](const Walk& w) { return p.groups == 1 ? 0 : w.seg % p.groups; };
+    auto first_head = [&](const Walk& w) { return kv_head(w) * (p.nh / p.nkv) + part_of(w) * p.heads_each; };
+    auto heads_of = [&](const Walk& w) { return min(p.heads_each, p.nh / p.nkv - part_of(w) * p.heads_each); };
     auto call_queries = [&](const Walk& w) {  // brings a segment's queries near, ahead of their use
         const bf16* q = (const bf16*)p.q + (size_t)query_row(w) * p.q_stride + (size_t)first_head(w) * HD;
         for (int i = lane * 16; i < heads_of(w) * HD; i += 512) {  // a sector each
@@ -273,7 +288,7 @@ __global__ void __launch_bounds__(WARPS * 32, Stream<HD, NT>::PER_SM) decode_e4m
     };
     auto fetch = [&]() {
         if (ahead.left > 0) {
-            const int kvh = p.groups == 1 ? ahead.seg : ahead.seg / p.groups;
+            const int kvh = kv_head(ahead);
 #pragma unroll
             for (int h = 0; h < HALVES; ++h) {
                 const int pos = ahead_pos + 32 * h, page = ahead_page[h];
@@ -524,7 +539,8 @@ __global__ void __launch_bounds__(WARPS * 32, Stream<HD, NT>::PER_SM) decode_e4m
                 }
             if (lane == 0) {
                 const int first_block = (seg_unit + 1) / block_units;
-                piece_s[piece] = {at.s * per_request + at.seg, row, h0, rows, first_block, (seg_unit + at.tiles) / block_units - first_block + 1};
+                piece_s[piece] = {(at.s * p.nkv + kv_head(at)) * p.groups + part_of(at), row, h0, rows, team, first_block,
+                                  (seg_unit + at.tiles) / block_units - first_block + 1};
             }
         }
         if (!ends) cp_async_wait<0>();  // (nothing is in flight any more: the run is over)
@@ -577,7 +593,9 @@ __global__ void __launch_bounds__(WARPS * 32, Stream<HD, NT>::PER_SM) decode_e4m
         total_s[x][r] = sum;
     }
     __syncthreads();
-    int came = -1, goes = -1;  // first pieces of the two segments, at most, that blocks before and after this one have pieces of as well
+    // the first pieces of segments that other blocks have pieces of as well: of every team one that came from before, one that goes on
+    if (tid < 2 * MOST_TEAMS) shared_s[tid] = -1;
+    __syncthreads();
 #pragma unroll 1
     for (uint32_t todo = leads; todo != 0; todo &= todo - 1) {
         const int x = __ffs(todo) - 1;
@@ -585,8 +603,9 @@ __global__ void __launch_bounds__(WARPS * 32, Stream<HD, NT>::PER_SM) decode_e4m
         const int head = __ffs(group & 0x55) - 1;  // the one piece, if any, that lies in global memory
         const Piece& s = piece_s[x];
         const bool whole = s.blocks == 1, begins_here = blockIdx.x == s.first_block;
-        if (!whole) (begins_here ? goes : came) = x;
-        float* part = p.part_o + (size_t)(2 * blockIdx.x + begins_here) * ROWS * HD;
+        const size_t piece = (size_t)2 * (blockIdx.x * teams + s.team) + begins_here;
+        if (!whole && tid == 0) shared_s[2 * s.team + begins_here] = x;
+        float* part = p.part_o + piece * ROWS * HD;
         const int items = s.heads * (HD / 4);
 #pragma unroll 1
         for (int i0 = tid; i0 < items; i0 += 2 * WARPS * 32) {  // four outputs each, two such at a time: all loads before their use
@@ -617,20 +636,16 @@ __global__ void __launch_bounds__(WARPS * 32, Stream<HD, NT>::PER_SM) decode_e4m
                     Vec4<bf16>::store((bf16*)p.out + ((size_t)s.row * p.nh + s.head) * HD + i * 4, make_float4(sum.x * inv, sum.y * inv, sum.z * inv, sum.w * inv));
                 } else {
                     *reinterpret_cast<float4*>(part + i * 4) = sum;
-                    if (i % (HD / 4) == 0) *reinterpret_cast<float2*>(p.part_ml + ((size_t)(2 * blockIdx.x + begins_here) * ROWS + r) * 2) = make_float2(top_s[x][r], total);
+                    if (i % (HD / 4) == 0) *reinterpret_cast<float2*>(p.part_ml + (piece * ROWS + r) * 2) = make_float2(top_s[x][r], total);
                 }
             }
         }
     }
     zeros();
-    if (came < 0 && goes < 0) {
-        cw_trace_end();
-        return;
-    }
-    // ---- segments that other blocks have pieces of: thread e counts this block in at segment e's counter ----
+    // ---- segments that other blocks have pieces of: thread e counts this block in at its counter ----
     // (pieces by number: y is of block first_block + y, its second one where the segment begins in it)
     auto by_eights = [&](const Piece& s) { return s.blocks > 3 * MERGE_AT_ONCE; };  // added up by eights first
-    auto place = [&](const Piece& s, int y) { return (size_t)2 * (s.first_block + y) + (y == 0 ? 1 : 0); };
+    auto place = [&](const Piece& s, int y) { return (size_t)2 * ((s.first_block + y) * teams + s.team) + (y == 0 ? 1 : 0); };
     // the barrier orders all threads' stores before the release; the last block's acquire, followed by the next barrier, its
     // threads' loads behind everybody's stores
     auto count_in = [&](int* counter, int count) {
@@ -640,14 +655,14 @@ __global__ void __launch_bounds__(WARPS * 32, Stream<HD, NT>::PER_SM) decode_e4m
         return before == count - 1;
     };
     __syncthreads();
-    if (tid < 2) {
-        const int x = tid == 0 ? came : goes;
+    if (tid < 2 * teams) {
+        const int x = shared_s[tid];
         bool is_last = false;
         if (x >= 0) {
             const Piece& s = piece_s[x];
             const int y = blockIdx.x - s.first_block, from = y - y % MERGE_AT_ONCE;
             if (by_eights(s))
-                is_last = count_in(p.counters + p.requests * per_request + place(s, from), min(MERGE_AT_ONCE, s.blocks - from));
+                is_last = count_in(p.counters + p.requests * p.nkv * p.groups + place(s, from), min(MERGE_AT_ONCE, s.blocks - from));
             else
                 is_last = count_in(p.counters + s.segment, s.blocks);
         }
@@ -655,9 +670,9 @@ __global__ void __launch_bounds__(WARPS * 32, Stream<HD, NT>::PER_SM) decode_e4m
     }
     __syncthreads();
 #pragma unroll 1
-    for (int e = 0; e < 2; ++e) {
+    for (int e = 0; e < 2 * teams; ++e) {
         if (!last_s[e]) continue;
-        const Piece s = piece_s[e == 0 ? came : goes];
+        const Piece s = piece_s[shared_s[e]];
         const int y = blockIdx.x - s.first_block;
         bool final = !by_eights(s);
         int from = final ? 0 : y - y % MERGE_AT_ONCE, count = final ? s.blocks : min(MERGE_AT_ONCE, s.blocks - from), stride = 1;
@@ -673,7 +688,7 @@ __global__ void __launch_bounds__(WARPS * 32, Stream<HD, NT>::PER_SM) decode_e4m
                     float2 ml[2][MERGE_AT_ONCE];
                     float4 v[2][MERGE_AT_ONCE];
                     // (in units of a piece's rows; the segment's very first piece lies one further)
-                    size_t at_piece = (size_t)2 * (s.first_block + from + y0 * stride);
+                    size_t at_piece = (size_t)2 * ((s.first_block + from + y0 * stride) * teams + s.team);
 #pragma unroll
                     for (int k = 0; k < MERGE_AT_ONCE; ++k) {
                         const size_t here = (at_piece + (k == 0 && from + y0 == 0 ? 1 : 0)) * ROWS;
@@ -687,7 +702,7 @@ __global__ void __launch_bounds__(WARPS * 32, Stream<HD, NT>::PER_SM) decode_e4m
                                 v[e][k] = __ldcg(reinterpret_cast<const float4*>(p.part_o + here * HD) + i);
                             }
                         }
-                        at_piece += 2 * stride;
+                        at_piece += 2 * teams * stride;
                     }
 #pragma unroll
                     for (int e = 0; e < 2; ++e) {
@@ -845,8 +860,8 @@ static int groups_of(int nh, int nkv, int hd, int dtype) {
 extern "C" int cw_attention_decode_e4m3_scratch(int requests, int nh, int nkv, int hd, int dtype, int sms, long long* floats, int* words) {
     if (requests < 0 || nh <= 0 || nkv <= 0 || nh % nkv || hd <= 0 || hd > 256 || sms <= 0) return CW_ERR_BAD_SIZE;
     const int groups = groups_of(nh, nkv, hd, dtype);
-    const long long pieces = groups ? 6LL * sms : 0;  // three blocks an SM at most, two pieces a block
-    *floats = pieces * 16 * (hd + 2) + 2 * pieces * 16 * hd;
+    const long long pieces = groups ? 6LL * sms * MOST_TEAMS : 0;  // three blocks an SM at most, two pieces a team
+    *floats = pieces * 16 * (hd + 2) + 12LL * sms * 16 * hd;
     *words = groups ? (int)(requests * nkv * groups + pieces) : 0;
     return CW_OK;
 }
@@ -877,9 +892,10 @@ extern "C" int cw_attention_decode_e4m3(const char* block) {
         p.page_shift = (page_size & (page_size - 1)) == 0 ? __builtin_ctz(page_size) : -1;
         p.groups = groups;
         p.heads_each = (nh / nkv + groups - 1) / groups;
+        p.teams = hd == 32 && nkv % 4 == 0 ? 4 : hd < 128 && nkv % 2 == 0 ? 2 : 1;
         p.part_o = floats;
-        p.heads_o = floats + 6LL * sms * 16 * hd;
-        p.part_ml = p.heads_o + 12LL * sms * 16 * hd;
+        p.part_ml = floats + 6LL * sms * MOST_TEAMS * 16 * hd;
+        p.heads_o = p.part_ml + 6LL * sms * MOST_TEAMS * 16 * 2;
         p.counters = words;
         switch (hd) {
             case 32: return stream_launch_heads<32>(p, sms, stream);

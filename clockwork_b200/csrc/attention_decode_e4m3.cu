@@ -44,7 +44,8 @@ struct DecodeE4m3Params {
     float* heads_o;          // [4 * blocks][8 or 16][hd]: ends of segments that an earlier warp began
     float* part_o;           // [blocks][teams][2][8 or 16][hd]
     float* part_ml;          // [blocks][teams][2][8 or 16][2]
-    int* counters;           // [requests * nkv * groups] and [blocks][teams][2], zero between launches
+    int* counters;           // [blocks][4] (by the block that a segment begins in: one of a team goes on) and [blocks][4][2], zero between launches
+    int least_rows, most_rows;  // portions: the requests that are served
 };
 
 #define WARPS 4
@@ -109,21 +110,24 @@ __device__ __forceinline__ void halves_of(uint32_t word, uint32_t& lo, uint32_t&
 // A run of tiles through requests and segments: which tile it stands at.
 struct Walk {
     int s, ctx, begin, tiles;  // the request, its context, the first position it sees, its tiles
+    int n, groups;             // tokens that it brings, groups of their query heads per KV head
     int seg, tile;             // KV head and group; tile of it
     int left;                  // units of the run that are left
 };
 
 // Part of a segment that several warps share.
 struct Piece {
-    int segment;           // -1: there is none
-    int row, head, heads;  // where its outputs go
+    int segment;     // the unit before its tiles, and the team; -1: there is none
+    int row, head;   // the request's first row, the KV head's first query head
+    int first, rows; // its rows (of token and head in the group of query heads)
     int team;
     int first_block, blocks;  // which blocks have pieces of it
 };
 
-template <int HD, int NT>
+template <int HD, int NT, bool PORTIONS>
 __global__ void __launch_bounds__(WARPS * 32, Stream<HD, NT>::PER_SM) decode_e4m3_kernel(const DecodeE4m3Params p) {
     using C = Stream<HD, NT>;
+    static_assert(!PORTIONS || 8 * NT <= 32, "a lane to a row");
     constexpr int ROWS = 8 * NT, ST = C::ST, CH = C::CH, TOKENS = C::TOKENS;
     constexpr int U = TOKENS / 16, HALVES = (TOKENS + 31) / 32;  // products' 16 tokens; a lane's tokens when pages are looked up
     constexpr int WORDS = HD / 32;  // a thread's 4-byte words of a V row
@@ -133,33 +137,43 @@ __global__ void __launch_bounds__(WARPS * 32, Stream<HD, NT>::PER_SM) decode_e4m
     __shared__ float m_s[2 * WARPS][ROWS], l_s[2 * WARPS][ROWS], f_s[2 * WARPS][ROWS];
     __shared__ Piece piece_s[2 * WARPS];  // of every warp: the end of a segment that began before its run, and what its run ends in
     __shared__ float top_s[2 * WARPS][ROWS], total_s[2 * WARPS][ROWS];  // of a group of pieces, at its first
+    __shared__ int limit_s[WARPS][PORTIONS ? ROWS : 1];
     __shared__ int shared_s[2 * MOST_TEAMS], last_s[2 * MOST_TEAMS], final_s;
     pdl_enter();
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
 
-    auto context_of = [&](int s) -> int {  // -1: not served here
-        if (p.q_start != nullptr && p.q_start[s + 1] - p.q_start[s] != 1) return -1;
-        return min(p.ctx_lens[s], p.max_blocks * p.page_size);
+    const int each = p.nh / p.nkv;  // query heads of a KV head
+    auto tokens_of = [&](int s) -> int {  // that request s brings; 0: it is not served here
+        if (!PORTIONS) return p.q_start == nullptr || p.q_start[s + 1] - p.q_start[s] == 1 ? 1 : 0;
+        const int n = p.q_start[s + 1] - p.q_start[s];
+        return n >= p.least_rows && n <= p.most_rows ? n : 0;
     };
-    auto begin_of = [&](int ctx) { return p.window > 0 ? max(0, ctx - p.window) : 0; };
-    auto tiles_of = [&](int ctx) {
-        return ctx <= 0 ? 0 : (ctx + TOKENS - 1) / TOKENS - begin_of(ctx) / TOKENS;
+    auto context_of = [&](int s) -> int { return min(p.ctx_lens[s], p.max_blocks * p.page_size); };
+    auto begin_of = [&](int ctx, int n) { return p.window > 0 ? max(0, ctx - (PORTIONS ? n : 1) + 1 - p.window) : 0; };
+    auto tiles_of = [&](int ctx, int n) {
+        return ctx <= 0 || n <= 0 ? 0 : (ctx + TOKENS - 1) / TOKENS - begin_of(ctx, n) / TOKENS;
     };
+    auto groups_of = [&](int n) { return PORTIONS ? (n * each + ROWS - 1) / ROWS : p.groups; };
     // Units are numbered through requests, teams' worth of KV heads, groups and tiles; every team of a block has the same ones.
     // A segment is its tiles and, before them, a unit for what changing to it costs (about a tile's time).  A block's run is a
     // whole number of equal runs for a team's warps.  Every warp finds its own: four neighbouring requests per lane, 128 at a time.
     const int chunks = (p.requests + 127) / 128;
-    int context[4], total = 0;
-    for (int c = chunks - 1; c >= 0; --c) {  // (the last one looked at is the first: what it holds is used again below)
-        int units = 0;
-#pragma unroll
-        for (int j = 0; j < 4; ++j) context[j] = c * 128 + 4 * lane + j < p.requests ? context_of(c * 128 + 4 * lane + j) : -1;
+    int context[4], tokens[4], total = 0;
+    auto look_at = [&](int c) {
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-            const int tiles = tiles_of(context[j]);
-            if (tiles > 0) units += tiles + 1;
+            const int s = c * 128 + 4 * lane + j;
+            tokens[j] = s < p.requests ? tokens_of(s) : 0;
+            context[j] = tokens[j] > 0 ? context_of(s) : -1;
         }
-        total += units;
+    };
+    for (int c = chunks - 1; c >= 0; --c) {  // (the last one looked at is the first: what it holds is used again below)
+        look_at(c);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const int tiles = tiles_of(context[j], tokens[j]);
+            if (tiles > 0) total += groups_of(tokens[j]) * (tiles + 1);
+        }
     }
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
@@ -168,16 +182,15 @@ __global__ void __launch_bounds__(WARPS * 32, Stream<HD, NT>::PER_SM) decode_e4m
     // Not where all that is read stays in the L2 (126 MB) until the neighbour comes anyway: one team's four warps leave a segment
     // in fewer pieces.  Measured, cold, one team and two: 16 KV heads of 64, 100 MB 36.7 and 39.0 us, 200 MB 76.5 and 56.2, 400 MB 154 and
     // 90; 2 of 96, 200 MB 53.6 and 59.4, 400 MB 137 and 92; 4 of 32 (four teams), 100 MB 50.9 and 65.0, 200 MB 106 and 93.
-    const int teams = (long long)total * p.nkv * p.groups * 2 * C::TILE_BYTES >= TEAMS_FROM_BYTES ? p.teams : 1;
+    const int teams = !PORTIONS && (long long)total * p.nkv * 2 * C::TILE_BYTES >= TEAMS_FROM_BYTES ? p.teams : 1;
     const int of_team = WARPS / teams, team = warp / of_team, member = warp - team * of_team, warps = gridDim.x * of_team;
-    const int per_request = p.nkv / teams * p.groups;
-    total *= per_request;
-    auto units_of = [&](int tiles) { return tiles > 0 ? per_request * (tiles + 1) : 0; };
+    const int kv_units = p.nkv / teams;
+    total *= kv_units;
     const int quota = max(LEAST_UNITS, (total + warps - 1) / warps), block_units = quota * of_team;
     const int first = (int)min((long long)(blockIdx.x * of_team + member) * quota, (long long)total);
     auto zeros = [&]() {  // the rows of requests without a context
         for (int s = blockIdx.x; s < p.requests; s += gridDim.x) {
-            if (context_of(s) != 0) continue;
+            if (PORTIONS || tokens_of(s) == 0 || context_of(s) > 0) continue;
             const int row = p.q_start != nullptr ? p.q_start[s] : s;
             for (int i = tid; i < p.nh * HD; i += blockDim.x) ((bf16*)p.out)[(size_t)row * p.nh * HD + i] = __float2bfloat16_rn(0.f);
         }
@@ -192,11 +205,12 @@ __global__ void __launch_bounds__(WARPS * 32, Stream<HD, NT>::PER_SM) decode_e4m
     if (at.left > 0) {
         int before = 0, skip = 0;
         for (int c = 0; c < chunks; ++c) {
+            if (c > 0) look_at(c);
             int units[4], sum = 0;
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
-                if (c > 0) context[j] = c * 128 + 4 * lane + j < p.requests ? context_of(c * 128 + 4 * lane + j) : -1;
-                units[j] = units_of(tiles_of(context[j]));
+                const int tiles = tiles_of(context[j], tokens[j]);
+                units[j] = tiles > 0 ? kv_units * groups_of(tokens[j]) * (tiles + 1) : 0;
                 sum += units[j];
             }
             int upto = sum;
@@ -207,24 +221,27 @@ __global__ void __launch_bounds__(WARPS * 32, Stream<HD, NT>::PER_SM) decode_e4m
             }
             const int chunk = __shfl_sync(0xffffffffu, upto, 31);
             if (first < before + chunk) {
-                int from = before + upto - sum, mine = 0, ctx = context[0];
+                int from = before + upto - sum, mine = 0, ctx = context[0], n = tokens[0];
 #pragma unroll
                 for (int j = 0; j < 3; ++j)
                     if (mine == j && first >= from + units[j]) {
                         from += units[j];
                         mine = j + 1;
                         ctx = context[j + 1];
+                        n = tokens[j + 1];
                     }
                 const int who = __ffs(__ballot_sync(0xffffffffu, first < before + upto)) - 1;
                 skip = first - __shfl_sync(0xffffffffu, from, who);
                 at.s = c * 128 + 4 * who + __shfl_sync(0xffffffffu, mine, who);
                 at.ctx = __shfl_sync(0xffffffffu, ctx, who);
+                at.n = __shfl_sync(0xffffffffu, n, who);
                 break;
             }
             before += chunk;
         }
-        at.tiles = max(1, tiles_of(at.ctx));
-        at.begin = begin_of(at.ctx);
+        at.tiles = max(1, tiles_of(at.ctx, at.n));
+        at.begin = begin_of(at.ctx, at.n);
+        at.groups = groups_of(at.n);
         at.seg = skip / (at.tiles + 1);
         skip -= at.seg * (at.tiles + 1);
         seg_unit = first - skip;
@@ -234,25 +251,30 @@ __global__ void __launch_bounds__(WARPS * 32, Stream<HD, NT>::PER_SM) decode_e4m
     auto enter = [&](Walk& w, int s) {  // the next request from s on that has tiles
         for (; s < p.requests; ++s) {
             w.s = s;
+            w.n = tokens_of(s);
             w.ctx = context_of(s);
-            w.tiles = tiles_of(w.ctx);
-            w.begin = begin_of(w.ctx);
+            w.tiles = tiles_of(w.ctx, w.n);
+            w.begin = begin_of(w.ctx, w.n);
+            w.groups = groups_of(w.n);
             if (w.tiles > 0) return;
         }
         w.ctx = 0;  // (lengths that change under the call: tokens that do not count)
         w.tiles = 0x7FFFFFFF;
     };
-    // where a segment's queries are, and how many heads it has
+    // A segment's rows: of single tokens the query heads of a group; of portions (token, head of the KV head's) in this order, 16
+    // to a group.  Row x of a KV head is that of token x / each and head x % each.
     auto query_row = [&](const Walk& w) { return p.q_start != nullptr ? p.q_start[w.s] : w.s; };
-    auto kv_head = [&](const Walk& w) { return (p.groups == 1 ? w.seg : w.seg / p.groups) * teams + team; };
-    auto part_of = [&](const Walk& w) { return p.groups == 1 ? 0 : w.seg % p.groups; };
-    auto first_head = [&](const Walk& w) { return kv_head(w) * (p.nh / p.nkv) + part_of(w) * p.heads_each; };
-    auto heads_of = [&](const Walk& w) { return min(p.heads_each, p.nh / p.nkv - part_of(w) * p.heads_each); };
+    auto kv_head = [&](const Walk& w) { return (!PORTIONS && p.groups == 1 ? w.seg : w.seg / w.groups) * teams + team; };
+    auto first_of = [&](const Walk& w) { return !PORTIONS && p.groups == 1 ? 0 : w.seg % w.groups * (PORTIONS ? ROWS : p.heads_each); };
+    auto rows_of = [&](const Walk& w) { return PORTIONS ? min(ROWS, w.n * each - first_of(w)) : min(p.heads_each, each - first_of(w)); };
+    auto row_at = [&](int row, int head, int x, int stride) {  // where row x of a KV head begins in q or out
+        return PORTIONS ? (size_t)(row + x / each) * stride + (size_t)(head + x % each) * HD : (size_t)row * stride + (size_t)(head + x) * HD;
+    };
     auto call_queries = [&](const Walk& w) {  // brings a segment's queries near, ahead of their use
-        const bf16* q = (const bf16*)p.q + (size_t)query_row(w) * p.q_stride + (size_t)first_head(w) * HD;
-        for (int i = lane * 16; i < heads_of(w) * HD; i += 512) {  // a sector each
+        const int row = query_row(w), head = kv_head(w) * each, x0 = first_of(w), rows = rows_of(w);
+        for (int i = lane; i < rows * (HD / 16); i += 32) {  // a sector each
             uint32_t unused;
-            asm volatile("ld.global.u32 %0, [%1];" : "=r"(unused) : "l"(q + i));
+            asm volatile("ld.global.u32 %0, [%1];" : "=r"(unused) : "l"((const bf16*)p.q + row_at(row, head, x0 + i / (HD / 16), p.q_stride) + i % (HD / 16) * 16));
         }
     };
     auto step = [&](Walk& w, int tiles) {  // so many tiles on within its segment, and on to the next one's first
@@ -261,7 +283,7 @@ __global__ void __launch_bounds__(WARPS * 32, Stream<HD, NT>::PER_SM) decode_e4m
         if (w.tile == w.tiles) {
             w.tile = 0;
             --w.left;
-            if (++w.seg == per_request) {
+            if (++w.seg == kv_units * w.groups) {
                 w.seg = 0;
                 if (w.left > 0) enter(w, w.s + 1);
             }
@@ -348,14 +370,14 @@ __global__ void __launch_bounds__(WARPS * 32, Stream<HD, NT>::PER_SM) decode_e4m
     const int k_at = C::at(g, HD % 64 == 0 ? t : t >> 1) + (HD % 64 == 0 ? 0 : 8 * (t & 1));
     constexpr int PIECE = HD % 64 == 0 ? 16 : 8, STEPS = PIECE / 4, PIECES = HD / (4 * PIECE);
     while (at.left > 0) {
-        const int row = query_row(at), h0 = first_head(at), rows = heads_of(at);
+        const int row = query_row(at), head = kv_head(at) * each, x0 = first_of(at), rows = rows_of(at);
         const int n_tiles = min(at.tiles - at.tile, at.left);
         // ---- the group's queries, as B fragments over the entries that a lane's pieces of K hold: half precision, a power of two out ----
         uint32_t qb[NT][PIECES][STEPS][2];
         float qf[NT][2], m[NT][2], l[NT][2], o[NT][HD / 16][4];
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
-            const bf16* q = (const bf16*)p.q + (size_t)row * p.q_stride + (size_t)(h0 + 8 * n + g) * HD;
+            const bf16* q = (const bf16*)p.q + row_at(row, head, x0 + min(8 * n + g, rows - 1), p.q_stride);
             float big = 0.f;
 #pragma unroll
             for (int b = 0; b < PIECES; ++b)
@@ -391,7 +413,14 @@ __global__ void __launch_bounds__(WARPS * 32, Stream<HD, NT>::PER_SM) decode_e4m
 #pragma unroll
             for (int j = 0; j < HD / 16; ++j) o[n][j][0] = o[n][j][1] = o[n][j][2] = o[n][j][3] = 0.f;
         }
-        for (int i = 0; i < n_tiles; ++i) {
+        // (portions) the last position that row x sees: of token x / each
+        const int before = at.ctx - at.n, seen_by_all = before + x0 / each, seen_by_any = before + (x0 + rows - 1) / each;
+        int pos0 = (at.begin / TOKENS + at.tile) * TOKENS;
+        if (PORTIONS) {
+            if (lane < ROWS) limit_s[warp][lane] = before + min(x0 + lane, x0 + rows - 1) / each;
+            __syncwarp();
+        }
+        for (int i = 0; i < n_tiles; ++i, pos0 += TOKENS) {
             fetch();
             cp_async_wait<ST - 1>();
             __syncwarp();
@@ -402,6 +431,11 @@ __global__ void __launch_bounds__(WARPS * 32, Stream<HD, NT>::PER_SM) decode_e4m
             if (i + 1 < n_tiles || ahead.left > 0 || fetch_stage != next) look_at_powers(next);
             const uint8_t* kt = my_ring + stage * 2 * C::TILE_BYTES;
             const uint8_t* vt = kt + C::TILE_BYTES;
+            stage = next;
+            if (PORTIONS && (pos0 > seen_by_any || (p.window > 0 && pos0 + TOKENS - 1 <= seen_by_all - p.window))) {
+                __syncwarp();  // no row sees any of the tile
+                continue;
+            }
             float sc[NT][U][4];
 #pragma unroll
             for (int n = 0; n < NT; ++n)
@@ -428,7 +462,8 @@ __global__ void __launch_bounds__(WARPS * 32, Stream<HD, NT>::PER_SM) decode_e4m
                         halves_of(lo[k], a[0], a[2]);
                         halves_of(hi[k], a[1], a[3]);
 #pragma unroll
-                        for (int n = 0; n < NT; ++n) mma_half(sc[n][u], a, qb[n][b][k][0], qb[n][b][k][1]);
+                        for (int n = 0; n < NT; ++n)
+                            if (!PORTIONS || 8 * n < rows) mma_half(sc[n][u], a, qb[n][b][k][0], qb[n][b][k][1]);
                     }
                 }
             }
@@ -444,9 +479,23 @@ __global__ void __launch_bounds__(WARPS * 32, Stream<HD, NT>::PER_SM) decode_e4m
 #pragma unroll
                     for (int e = 0; e < 2; ++e) sc[n][x >> 1][2 * (x & 1) + e] = fmaf(sc[n][x >> 1][2 * (x & 1) + e] * qf[n][e], kf, ev);
             }
+            if (PORTIONS && (pos0 + TOKENS - 1 > seen_by_all || p.window > 0)) {
+#pragma unroll
+                for (int n = 0; n < NT; ++n)
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) {
+                        const int seen = limit_s[warp][8 * n + 2 * t + e], from = p.window > 0 ? seen - p.window : -1;
+#pragma unroll
+                        for (int x = 0; x < 2 * U; ++x) {
+                            const int pos = pos0 + 8 * x + g;
+                            if (pos > seen || pos <= from) sc[n][x >> 1][2 * (x & 1) + e] = -INFINITY;
+                        }
+                    }
+            }
             uint32_t pb[NT][U][2];
 #pragma unroll
             for (int n = 0; n < NT; ++n) {
+                if (PORTIONS && 8 * n >= rows) continue;  // (an eight of rows that there is not)
                 float keep[2];
 #pragma unroll
                 for (int e = 0; e < 2; ++e) {
@@ -512,12 +561,12 @@ __global__ void __launch_bounds__(WARPS * 32, Stream<HD, NT>::PER_SM) decode_e4m
                     halves_of(__byte_perm(w[2][j], w[3][j], 0x7362), odd[2], odd[3]);
 #pragma unroll
                     for (int n = 0; n < NT; ++n) {
+                        if (PORTIONS && 8 * n >= rows) continue;
                         mma_half(o[n][2 * j], even, pb[n][u][0], pb[n][u][1]);
                         mma_half(o[n][2 * j + 1], odd, pb[n][u][0], pb[n][u][1]);
                     }
                 }
             }
-            stage = next;
             __syncwarp();  // the stage is free
         }
         // ---- the run has left the segment, or ends in it ----
@@ -539,7 +588,7 @@ __global__ void __launch_bounds__(WARPS * 32, Stream<HD, NT>::PER_SM) decode_e4m
                 }
             if (lane == 0) {
                 const int first_block = (seg_unit + 1) / block_units;
-                piece_s[piece] = {(at.s * p.nkv + kv_head(at)) * p.groups + part_of(at), row, h0, rows, team, first_block,
+                piece_s[piece] = {seg_unit | team << 29, row, head, x0, rows, team, first_block,
                                   (seg_unit + at.tiles) / block_units - first_block + 1};
             }
         }
@@ -560,7 +609,7 @@ __global__ void __launch_bounds__(WARPS * 32, Stream<HD, NT>::PER_SM) decode_e4m
                     if (begins && ends) {
                         const float inv = l[n][e] == 0.f ? 0.f : 1.f / l[n][e];
                         if (r < rows)
-                            Vec4<bf16>::store((bf16*)p.out + ((size_t)row * p.nh + h0 + r) * HD + d, make_float4(x.x * inv, x.y * inv, x.z * inv, x.w * inv));
+                            Vec4<bf16>::store((bf16*)p.out + row_at(row, head, x0 + r, p.nh * HD) + d, make_float4(x.x * inv, x.y * inv, x.z * inv, x.w * inv));
                     } else {
                         *reinterpret_cast<float4*>(sums + r * HD + d) = x;
                     }
@@ -606,7 +655,7 @@ __global__ void __launch_bounds__(WARPS * 32, Stream<HD, NT>::PER_SM) decode_e4m
         const size_t piece = (size_t)2 * (blockIdx.x * teams + s.team) + begins_here;
         if (!whole && tid == 0) shared_s[2 * s.team + begins_here] = x;
         float* part = p.part_o + piece * ROWS * HD;
-        const int items = s.heads * (HD / 4);
+        const int items = s.rows * (HD / 4);
 #pragma unroll 1
         for (int i0 = tid; i0 < items; i0 += 2 * WARPS * 32) {  // four outputs each, two such at a time: all loads before their use
             float4 v[2][WARPS + 1];
@@ -633,7 +682,7 @@ __global__ void __launch_bounds__(WARPS * 32, Stream<HD, NT>::PER_SM) decode_e4m
                 const float total = total_s[x][r];
                 if (whole) {
                     const float inv = total == 0.f ? 0.f : 1.f / total;
-                    Vec4<bf16>::store((bf16*)p.out + ((size_t)s.row * p.nh + s.head) * HD + i * 4, make_float4(sum.x * inv, sum.y * inv, sum.z * inv, sum.w * inv));
+                    Vec4<bf16>::store((bf16*)p.out + row_at(s.row, s.head, s.first + r, p.nh * HD) + i % (HD / 4) * 4, make_float4(sum.x * inv, sum.y * inv, sum.z * inv, sum.w * inv));
                 } else {
                     *reinterpret_cast<float4*>(part + i * 4) = sum;
                     if (i % (HD / 4) == 0) *reinterpret_cast<float2*>(p.part_ml + (piece * ROWS + r) * 2) = make_float2(top_s[x][r], total);
@@ -662,9 +711,9 @@ __global__ void __launch_bounds__(WARPS * 32, Stream<HD, NT>::PER_SM) decode_e4m
             const Piece& s = piece_s[x];
             const int y = blockIdx.x - s.first_block, from = y - y % MERGE_AT_ONCE;
             if (by_eights(s))
-                is_last = count_in(p.counters + p.requests * p.nkv * p.groups + place(s, from), min(MERGE_AT_ONCE, s.blocks - from));
+                is_last = count_in(p.counters + gridDim.x * MOST_TEAMS + place(s, from), min(MERGE_AT_ONCE, s.blocks - from));
             else
-                is_last = count_in(p.counters + s.segment, s.blocks);
+                is_last = count_in(p.counters + s.first_block * teams + s.team, s.blocks);
         }
         last_s[tid] = is_last;
     }
@@ -678,7 +727,7 @@ __global__ void __launch_bounds__(WARPS * 32, Stream<HD, NT>::PER_SM) decode_e4m
         int from = final ? 0 : y - y % MERGE_AT_ONCE, count = final ? s.blocks : min(MERGE_AT_ONCE, s.blocks - from), stride = 1;
 #pragma unroll 1
         for (;;) {
-            const int items = s.heads * (HD / 4);
+            const int items = s.rows * (HD / 4);
 #pragma unroll 1
             for (int i0 = tid; i0 < items; i0 += 2 * WARPS * 32) {  // two at a time, eight pieces of each: one trip to the L2
                 float top[2] = {-INFINITY, -INFINITY}, total[2] = {0.f, 0.f};
@@ -727,7 +776,7 @@ __global__ void __launch_bounds__(WARPS * 32, Stream<HD, NT>::PER_SM) decode_e4m
                     if (i >= items) break;
                     if (final) {
                         const float inv = total[e] == 0.f ? 0.f : 1.f / total[e];
-                        Vec4<bf16>::store((bf16*)p.out + ((size_t)s.row * p.nh + s.head) * HD + i * 4,
+                        Vec4<bf16>::store((bf16*)p.out + row_at(s.row, s.head, s.first + i / (HD / 4), p.nh * HD) + i % (HD / 4) * 4,
                                           make_float4(sum[e].x * inv, sum[e].y * inv, sum[e].z * inv, sum[e].w * inv));
                     } else {  // over the first of the eight, whose four sums this thread alone reads and writes
                         *reinterpret_cast<float4*>(p.part_o + place(s, from) * ROWS * HD + i * 4) = sum[e];
@@ -740,13 +789,13 @@ __global__ void __launch_bounds__(WARPS * 32, Stream<HD, NT>::PER_SM) decode_e4m
             }
             __syncthreads();  // (maxima and sums of the pieces are read by all; top_s and total_s are free)
             if (final) break;
-            if (tid < s.heads) *reinterpret_cast<float2*>(p.part_ml + (place(s, from) * ROWS + tid) * 2) = make_float2(top_s[0][tid], total_s[0][tid]);
+            if (tid < s.rows) *reinterpret_cast<float2*>(p.part_ml + (place(s, from) * ROWS + tid) * 2) = make_float2(top_s[0][tid], total_s[0][tid]);
             from = 0;
             count = (s.blocks + MERGE_AT_ONCE - 1) / MERGE_AT_ONCE;
             stride = MERGE_AT_ONCE;
             final = true;
             __syncthreads();
-            if (tid == 0) final_s = count_in(p.counters + s.segment, count);
+            if (tid == 0) final_s = count_in(p.counters + s.first_block * teams + s.team, count);
             __syncthreads();
             if (final_s == 0) break;
         }
@@ -829,23 +878,23 @@ __global__ void __launch_bounds__(ANY_TOKENS) decode_e4m3_any_kernel(const Decod
         if (tid + e * ANY_TOKENS < p.hd) out[tid + e * ANY_TOKENS] = from_f<T>(l > 0.f ? acc[e] / l : (l == l ? 0.f : l));
 }
 
-template <int HD, int NT>
+template <int HD, int NT, bool PORTIONS>
 static int stream_launch(const DecodeE4m3Params& p, int sms, cudaStream_t stream) {
     using C = Stream<HD, NT>;
     static bool configured[64] = {};  // (per device)
     int device = 0;
     cudaGetDevice(&device);
     if (device < 0 || device >= 64 || !configured[device]) {
-        const cudaError_t e = cudaFuncSetAttribute(decode_e4m3_kernel<HD, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::RING);
+        const cudaError_t e = cudaFuncSetAttribute(decode_e4m3_kernel<HD, NT, PORTIONS>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::RING);
         if (e != cudaSuccess) return (int)e;
         if (device >= 0 && device < 64) configured[device] = true;
     }
-    return cw_launch(decode_e4m3_kernel<HD, NT>, dim3(sms * C::PER_SM), dim3(WARPS * 32), C::RING, stream, 1u, p);
+    return cw_launch(decode_e4m3_kernel<HD, NT, PORTIONS>, dim3(sms * C::PER_SM), dim3(WARPS * 32), C::RING, stream, 1u, p);
 }
 template <int HD>
 static int stream_launch_heads(const DecodeE4m3Params& p, int sms, cudaStream_t stream) {
-    if (p.heads_each <= 8) return stream_launch<HD, 1>(p, sms, stream);
-    return stream_launch<(HD <= 128 ? HD : 32), 2>(p, sms, stream);  // (head sizes beyond 128 come in groups of 8)
+    if (p.heads_each <= 8) return stream_launch<HD, 1, false>(p, sms, stream);
+    return stream_launch<(HD <= 128 ? HD : 32), 2, false>(p, sms, stream);  // (head sizes beyond 128 come in groups of 8)
 }
 
 // How a KV head's query heads are shared out: groups of 16 at most, of 8 where heads are so large that the sums of 16 would not
@@ -856,14 +905,26 @@ static int groups_of(int nh, int nkv, int hd, int dtype) {
     return (each + most - 1) / most;
 }
 
-// Scratch of the call: float32 words and zeroed int32 words (which are zero again when it has run).
-extern "C" int cw_attention_decode_e4m3_scratch(int requests, int nh, int nkv, int hd, int dtype, int sms, long long* floats, int* words) {
-    if (requests < 0 || nh <= 0 || nkv <= 0 || nh % nkv || hd <= 0 || hd > 256 || sms <= 0) return CW_ERR_BAD_SIZE;
-    const int groups = groups_of(nh, nkv, hd, dtype);
-    const long long pieces = groups ? 6LL * sms * MOST_TEAMS : 0;  // three blocks an SM at most, two pieces a team
-    *floats = pieces * 16 * (hd + 2) + 12LL * sms * 16 * hd;
-    *words = groups ? (int)(requests * nkv * groups + pieces) : 0;
+// Scratch of the calls: float32 words, and zeroed int32 words (which are zero again when a call has run).  It goes by the GPU and the
+// head size alone: two pieces per block and team, the ends of segments per warp; 16 rows of three blocks an SM with four teams.
+#define SCRATCH_PIECES(sms) (6LL * (sms) * MOST_TEAMS)
+extern "C" int cw_attention_e4m3_scratch(int hd, int sms, long long* floats, int* words) {
+    if (hd <= 0 || hd > 256 || sms <= 0) return CW_ERR_BAD_SIZE;
+    *floats = SCRATCH_PIECES(sms) * 16 * (hd + 2) + 12LL * sms * 16 * hd;
+    *words = (int)(3 * sms * MOST_TEAMS + SCRATCH_PIECES(sms));
     return CW_OK;
+}
+
+static bool streams(DecodeE4m3Params& p, long long groups, int sms, float* floats, int* words) {
+    const long long slots = (long long)p.num_pages * p.page_size, tiles = (long long)p.max_blocks * p.page_size / 16 + 2;
+    if (floats == nullptr || words == nullptr || (uintptr_t)p.q % 4 || p.q_stride % 2) return false;  // (queries are read in pairs)
+    if (slots * p.nkv * (p.hd / 16) >= 0xFFFFFFFFLL || p.nkv * groups * tiles >= 1LL << 29) return false;
+    p.page_shift = (p.page_size & (p.page_size - 1)) == 0 ? __builtin_ctz(p.page_size) : -1;
+    p.part_o = floats;
+    p.part_ml = p.part_o + SCRATCH_PIECES(sms) * 16 * p.hd;
+    p.heads_o = p.part_ml + SCRATCH_PIECES(sms) * 16 * 2;
+    p.counters = words;
+    return true;
 }
 
 // q [rows, q_stride >= nh * hd], out [rows, nh * hd]; request s owns row s, or with q_start rows q_start[s] .. q_start[s + 1], and
@@ -886,17 +947,11 @@ extern "C" int cw_attention_decode_e4m3(const char* block) {
         return CW_ERR_BAD_SIZE;
     DecodeE4m3Params p = {q, q_stride, out, k, v, k_exp, v_exp, block_tables, ctx_lens, q_start, requests, nh, nkv, hd, page_size,
                           max_blocks, num_pages, window, scale, status};
-    const int groups = ((uintptr_t)q % 4 || q_stride % 2) ? 0 : groups_of(nh, nkv, hd, dtype);  // (queries are read in pairs)
-    if (groups && floats != nullptr && words != nullptr && (long long)num_pages * page_size * nkv * (hd / 16) < 0xFFFFFFFFLL &&
-        (long long)requests * nkv * groups * ((long long)max_blocks * page_size / 16 + 2) < 0x7FFFFFFF) {
-        p.page_shift = (page_size & (page_size - 1)) == 0 ? __builtin_ctz(page_size) : -1;
+    const int groups = groups_of(nh, nkv, hd, dtype);
+    if (groups && streams(p, (long long)requests * groups, sms, floats, words)) {
         p.groups = groups;
         p.heads_each = (nh / nkv + groups - 1) / groups;
         p.teams = hd == 32 && nkv % 4 == 0 ? 4 : hd < 128 && nkv % 2 == 0 ? 2 : 1;
-        p.part_o = floats;
-        p.part_ml = floats + 6LL * sms * MOST_TEAMS * 16 * hd;
-        p.heads_o = p.part_ml + 6LL * sms * MOST_TEAMS * 16 * 2;
-        p.counters = words;
         switch (hd) {
             case 32: return stream_launch_heads<32>(p, sms, stream);
             case 64: return stream_launch_heads<64>(p, sms, stream);
@@ -911,6 +966,41 @@ extern "C" int cw_attention_decode_e4m3(const char* block) {
     if (dtype == 0) return cw_launch(decode_e4m3_any_kernel<float>, dim3(nh, requests), dim3(ANY_TOKENS), 0, stream, 1u, p);
     if (dtype == 1) return cw_launch(decode_e4m3_any_kernel<bf16>, dim3(nh, requests), dim3(ANY_TOKENS), 0, stream, 1u, p);
     return CW_ERR_BAD_DTYPE;
+}
+
+// Causal attention of the portions of requests that bring `least_rows` to `most_rows` rows, q_start[s] .. q_start[s + 1] of q and out
+// (other rows are left alone), the last of the ctx_lens[s] tokens that each has in the cache; `rows`: the most rows that all of them
+// bring together.  bfloat16, head sizes 32, 64, 96 and 128.
+extern "C" int cw_attention_portions_e4m3(const char* block) {
+    ArgumentWords w(block);
+    const void* q = w.pointer(); void* out = w.pointer();
+    const uint8_t *k = (const uint8_t*)w.pointer(), *v = (const uint8_t*)w.pointer(), *k_exp = (const uint8_t*)w.pointer(), *v_exp = (const uint8_t*)w.pointer();
+    const int *block_tables = (const int*)w.pointer(), *ctx_lens = (const int*)w.pointer(), *q_start = (const int*)w.pointer();
+    float* floats = (float*)w.pointer();
+    int *words = (int*)w.pointer(), *status = (int*)w.pointer();
+    const cudaStream_t stream = (cudaStream_t)w.pointer();
+    const int q_stride = w.number(), requests = w.number(), nh = w.number(), nkv = w.number(), hd = w.number(), page_size = w.number(),
+              max_blocks = w.number(), num_pages = w.number(), window = w.number(), sms = w.number(), rows = w.number(), least_rows = w.number(),
+              most_rows = w.number();
+    const float scale = (float)w.real();
+    if (requests == 0 || rows == 0) return CW_OK;
+    if (requests < 0 || nh <= 0 || nkv <= 0 || nh % nkv || page_size <= 0 || max_blocks <= 0 || num_pages <= 0 || window < 0 ||
+        q_stride < nh * hd || ((uintptr_t)k | (uintptr_t)v) % 16 || sms <= 0 || rows < 0 || least_rows < 1 || most_rows < least_rows ||
+        q_start == nullptr || (long long)num_pages * page_size > 0x7FFFFFFF || (long long)max_blocks * page_size > 0x7FFFFFFF)
+        return CW_ERR_BAD_SIZE;
+    DecodeE4m3Params p = {q, q_stride, out, k, v, k_exp, v_exp, block_tables, ctx_lens, q_start, requests, nh, nkv, hd, page_size,
+                          max_blocks, num_pages, window, scale, status};
+    p.groups = p.teams = 1;
+    p.least_rows = least_rows;
+    p.most_rows = most_rows;
+    if (!streams(p, (long long)rows * (nh / nkv) / 16 + requests, sms, floats, words)) return CW_ERR_UNSUPPORTED;
+    switch (hd) {
+        case 32: return stream_launch<32, 2, true>(p, sms, stream);
+        case 64: return stream_launch<64, 2, true>(p, sms, stream);
+        case 96: return stream_launch<96, 2, true>(p, sms, stream);
+        case 128: return stream_launch<128, 2, true>(p, sms, stream);
+    }
+    return CW_ERR_UNSUPPORTED;
 }
 
 CW_TRACE_TU(attention_decode_e4m3)

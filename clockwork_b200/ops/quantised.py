@@ -16,6 +16,7 @@ import functools
 import struct
 from typing import NamedTuple
 
+import numpy as np
 import torch
 
 from . import _stream, dtype_code
@@ -26,6 +27,7 @@ from .library import check, library
 _STORE_ARGS = struct.Struct("21qd").pack
 _READ_ARGS = struct.Struct("21q").pack
 _DECODE_ARGS = struct.Struct("24qd").pack
+_PORTION_ARGS = struct.Struct("26qd").pack
 
 CODES = torch.float8_e4m3fn
 MAX_HEAD_DIM = 256
@@ -171,12 +173,12 @@ READ_BLOCKS = 148 * 4
 
 
 def read_pages(cache: E4M3Pages, block_tables: torch.Tensor, ctx_lens: torch.Tensor, out_k: torch.Tensor, out_v: torch.Tensor,
-               status: torch.Tensor, *, window: int | None = None, q_start: torch.Tensor | None = None, skip_single: bool = False) -> None:
+               status: torch.Tensor, *, window: int | None = None, q_start: torch.Tensor | None = None, least_rows: int = 1) -> None:
     """The keys and values of positions [0, ctx_lens[s]) of every request, through ``block_tables`` [S, max_blocks], into plain
     pages ``out_k``, ``out_v`` [pages, page_size, nkv, hd] (float32 or bfloat16) at the same pages and slots.  What is left of a
     request's last page becomes zero; no other page is touched.  ``window``: from the page on that a query at the request's last
     position sees with that window.  ``q_start`` [S + 1] (the rows that the requests bring to a step): only requests that bring
-    rows are read (``skip_single``: more than one row), and the window is that of their first row."""
+    at least ``least_rows`` rows are read, and the window is that of their first row."""
     pages, page_size, nkv, hd = check_pages(cache)
     for name, t in (("out_k", out_k), ("out_v", out_v)):
         if t.shape != cache.k.shape or not t.is_contiguous() or t.dtype != out_k.dtype or t.data_ptr() % 16:
@@ -190,6 +192,8 @@ def read_pages(cache: E4M3Pages, block_tables: torch.Tensor, ctx_lens: torch.Ten
         raise ValueError(f"head_dim {hd} must be a multiple of 16")
     if window is not None and window <= 0:
         raise ValueError("window must be positive or None")
+    if least_rows < 1:
+        raise ValueError("least_rows must be at least 1")
     _check_status(status)
     index = cache.k.get_device()
     _elsewhere(index, out_k=out_k, out_v=out_v, block_tables=block_tables, ctx_lens=ctx_lens, q_start=q_start, status=status)
@@ -197,16 +201,18 @@ def read_pages(cache: E4M3Pages, block_tables: torch.Tensor, ctx_lens: torch.Ten
     check(library().cw_read_pages(_READ_ARGS(
         cache.k.data_ptr(), cache.v.data_ptr(), cache.k_exp.data_ptr(), cache.v_exp.data_ptr(), out_k.data_ptr(), out_v.data_ptr(),
         block_tables.data_ptr(), ctx_lens.data_ptr(), 0 if q_start is None else q_start.data_ptr(), status.data_ptr(), _stream(), s, nkv, hd,
-        page_size, block_tables.shape[1], pages, window or 0, 2 if skip_single else 1, READ_BLOCKS, dtype_code(out_k.dtype))), "read_pages")
+        page_size, block_tables.shape[1], pages, window or 0, least_rows, READ_BLOCKS, dtype_code(out_k.dtype))), "read_pages")
 
 
 class DecodeWorkspace:
-    """Scratch of ``attention_decode`` for up to ``requests`` requests of these heads: partial results (of a size that goes by the
-    GPU alone) and counters that are zero between calls.  Calls that may overlap on the GPU must not share one."""
+    """Scratch of ``attention_decode`` and ``attention_portions`` for heads of ``head_dim`` entries: partial results and counters that
+    are zero between calls, of a size that goes by the GPU and the head size alone.  Calls that may overlap on the GPU must not
+    share one."""
 
-    def __init__(self, requests: int, num_heads: int, num_kv_heads: int, head_dim: int, device) -> None:
+    def __init__(self, head_dim: int, device) -> None:
         device = torch.device(device)
-        floats, words = _scratch_sizes(requests, num_heads, num_kv_heads, head_dim, _sm_count(device.index))
+        floats, words = _scratch_sizes(head_dim, _sm_count(device.index))
+        self.head_dim = head_dim
         self.floats = torch.empty(floats, dtype=torch.float32, device=device)
         self.words = torch.zeros(words, dtype=torch.int32, device=device)
 
@@ -219,31 +225,27 @@ def _sm_count(index: int | None) -> int:
 
 
 @functools.lru_cache(maxsize=256)
-def _scratch_sizes(requests: int, num_heads: int, num_kv_heads: int, head_dim: int, sms: int) -> tuple[int, int]:
+def _scratch_sizes(head_dim: int, sms: int) -> tuple[int, int]:
     floats, words = ctypes.c_longlong(0), ctypes.c_int(0)
-    check(library().cw_attention_decode_e4m3_scratch(requests, num_heads, num_kv_heads, head_dim, 1, sms, ctypes.addressof(floats),
-                                                     ctypes.addressof(words)), "attention_decode_e4m3_scratch")
+    check(library().cw_attention_e4m3_scratch(head_dim, sms, ctypes.addressof(floats), ctypes.addressof(words)), "attention_e4m3_scratch")
     return floats.value, words.value
 
 
-_workspaces: dict = {}  # (device, stream) -> the scratch of calls that bring none
+_workspaces: dict = {}  # (device, stream, head size) -> the scratch of calls that bring none
 
 
-def _workspace(workspace: DecodeWorkspace | None, requests: int, num_heads: int, num_kv_heads: int, head_dim: int, index: int,
-               stream: int, sms: int) -> DecodeWorkspace:
-    """The caller's workspace, or the one of the current stream, replaced by a larger one when a call needs more.  A call that is being
-    captured and brings none gets one of its own in the graph's memory, cleared at every replay: graphs may be replayed on any
-    stream."""
-    floats, words = _scratch_sizes(requests, num_heads, num_kv_heads, head_dim, sms)
+def _workspace(workspace: DecodeWorkspace | None, head_dim: int, index: int, stream: int) -> DecodeWorkspace:
+    """The caller's workspace, or the one of the current stream.  A call that is being captured and brings none gets one of its own
+    in the graph's memory, cleared at every replay: graphs may be replayed on any stream."""
     if workspace is not None:
-        if workspace.floats.numel() < floats or workspace.words.numel() < words or workspace.floats.get_device() != index:
-            raise ValueError("the workspace was made for fewer requests, other heads or another device")
+        if workspace.head_dim < head_dim or workspace.floats.get_device() != index:
+            raise ValueError("the workspace was made for smaller heads or another device")
         return workspace
     if torch.cuda.is_current_stream_capturing():
-        return DecodeWorkspace(requests, num_heads, num_kv_heads, head_dim, torch.device("cuda", index))
-    held = _workspaces.get((index, stream))
-    if held is None or held.floats.numel() < floats or held.words.numel() < words:
-        held = _workspaces[index, stream] = DecodeWorkspace(max(requests, 256), num_heads, num_kv_heads, head_dim, torch.device("cuda", index))
+        return DecodeWorkspace(head_dim, torch.device("cuda", index))
+    held = _workspaces.get((index, stream, head_dim))
+    if held is None:
+        held = _workspaces[index, stream, head_dim] = DecodeWorkspace(head_dim, torch.device("cuda", index))
     return held
 
 
@@ -252,7 +254,7 @@ def _decode_call(q, out, cache, block_tables, ctx_lens, q_start, num_heads, shap
     s = block_tables.shape[0]
     stream, sms, floats, words = _stream(), _sm_count(index), 0, 0
     if code == 1 and hd % 32 == 0:
-        scratch = _workspace(workspace, s, num_heads, nkv, hd, index, stream, sms)
+        scratch = _workspace(workspace, hd, index, stream)
         floats, words = scratch.floats.data_ptr(), scratch.words.data_ptr()
     check(library().cw_attention_decode_e4m3(_DECODE_ARGS(
         q.data_ptr(), out.data_ptr(), cache.k.data_ptr(), cache.v.data_ptr(), cache.k_exp.data_ptr(), cache.v_exp.data_ptr(),
@@ -328,36 +330,75 @@ def decode_step(qkv: torch.Tensor, positions: torch.Tensor, slots: torch.Tensor,
 
 
 # ---- prompt portions --------------------------------------------------------------------------------------------------------
+SHORT_HEAD_DIMS = (32, 64, 96, 128)
+
+
+def short_rows(num_heads: int, num_kv_heads: int, head_dim: int) -> int:
+    """Requests that bring up to this many rows are attended straight from the codes, sixteen (row, query head) pairs of a KV head to a
+    warp; with more pairs the tensor cores' rate counts, and the kernel of whole tiles over pages read back is faster.  Measured
+    (us, read back and straight): 6 heads to a KV head, 2 KV heads of 128, 12,000 tokens behind one request of 2 rows 34.9 and 22.3, of
+    16 (96 pairs) 34.9 and 35.0, of 32 34.9 and 39.2; 5 to 8 KV heads, four requests of 16 rows 227 and 126, of 32 (160 pairs) 229 and 229;
+    1 to 16 KV heads of 64, one of 64 rows 41.0 and 41.0, four of 64 behind 2,000 35.3 and 33.2."""
+    return SHORT_PAIRS // (num_heads // num_kv_heads) if head_dim in SHORT_HEAD_DIMS else 0
+
+
+SHORT_PAIRS = 96
+
+
 class PortionPlan(NamedTuple):
     """How the portions of a step are cut into work for ``attention_portions``; made once per step, shared by layers of the same
     heads."""
 
     q_lens: tuple
     ctx_lens: tuple
+    short: int           # rows of the requests that bring `least_rows` to `most_rows` of them
+    least_rows: int
+    most_rows: int
+    items: int           # work items of the others
     item_seq: torch.Tensor
     item_q0: torch.Tensor
     item_split: torch.Tensor | None
-    items: int
     tok_seq: torch.Tensor
     positions: torch.Tensor
 
 
-def plan_portions(q_lens, ctx_lens, num_heads: int, num_kv_heads: int, head_dim: int, page_size: int, device) -> PortionPlan:
-    """``q_lens``: the rows that each request brings; ``ctx_lens``: its tokens in the cache with them (both on the host)."""
+def plan_portions(q_lens, ctx_lens, num_heads: int, num_kv_heads: int, head_dim: int, page_size: int, device,
+                  most_rows: int | None = None, least_rows: int = 1) -> PortionPlan:
+    """``q_lens``: the rows that each request brings; ``ctx_lens``: its tokens in the cache with them (both on the host).
+    ``most_rows``: see ``short_rows``, which decides by default.  bfloat16 requests that bring fewer than ``least_rows`` rows are
+    left alone."""
     from . import attention_fast as fast
 
     q_lens, ctx_lens = tuple(int(n) for n in q_lens), tuple(int(c) for c in ctx_lens)
     if len(q_lens) != len(ctx_lens) or any(n < 0 or c < n for n, c in zip(q_lens, ctx_lens)):
         raise ValueError("every request has a length and a context that holds its rows")
+    if most_rows is None:
+        most_rows = short_rows(num_heads, num_kv_heads, head_dim)
+    short = sum(n for n in q_lens if least_rows <= n <= most_rows)
     cuts = fast._cuts_for(num_heads, head_dim, page_size)
-    seqs, q0s, words = fast.prefill_work_items(q_lens, ctx_lens, cuts, fast._sm_count(torch.device(device)) if cuts else 0)
-    rows = [(s, c - n + r) for s, (n, c) in enumerate(zip(q_lens, ctx_lens)) for r in range(n)]
-    n = len(seqs)
-    host = torch.tensor(seqs + q0s + words + [r[0] for r in rows] + [r[1] for r in rows], dtype=torch.int32)
-    dev = host.to(device)
+    seqs, q0s, words = fast.prefill_work_items([n if n > max(most_rows, least_rows - 1) else 0 for n in q_lens], ctx_lens, cuts,
+                                               fast._sm_count(torch.device(device)) if cuts else 0)
+    lens = np.array(q_lens, dtype=np.int32)
+    starts = np.cumsum(lens, dtype=np.int32) - lens
+    tok_seq = np.repeat(np.arange(len(lens), dtype=np.int32), lens)
+    positions = np.arange(lens.sum(), dtype=np.int32) + np.repeat(np.array(ctx_lens, dtype=np.int32) - lens - starts, lens)
+    n, rows = len(seqs), len(tok_seq)
+    dev = torch.from_numpy(np.concatenate([np.array(seqs + q0s + words, dtype=np.int32), tok_seq, positions])).to(device)
     cut = any(w & 0xFF != 1 for w in words)
-    return PortionPlan(q_lens, ctx_lens, dev[:n], dev[n : 2 * n], dev[2 * n : 3 * n] if cut else None, n, dev[3 * n : 3 * n + len(rows)],
-                       dev[3 * n + len(rows) :])
+    return PortionPlan(q_lens, ctx_lens, short, least_rows, most_rows, n, dev[:n], dev[n : 2 * n], dev[2 * n : 3 * n] if cut else None,
+                       dev[3 * n : 3 * n + rows], dev[3 * n + rows :])
+
+
+def _short_call(q, out, cache, block_tables, ctx_lens, q_start, num_heads, shape, scale, window, rows, least_rows, most_rows, status, index,
+                workspace) -> None:
+    pages, page_size, nkv, hd = shape
+    stream = _stream()
+    scratch = _workspace(workspace, hd, index, stream)
+    check(library().cw_attention_portions_e4m3(_PORTION_ARGS(
+        q.data_ptr(), out.data_ptr(), cache.k.data_ptr(), cache.v.data_ptr(), cache.k_exp.data_ptr(), cache.v_exp.data_ptr(),
+        block_tables.data_ptr(), ctx_lens.data_ptr(), q_start.data_ptr(), scratch.floats.data_ptr(), scratch.words.data_ptr(),
+        status.data_ptr(), stream, q.stride(0) if q.shape[0] > 1 else num_heads * hd, block_tables.shape[0], num_heads, nkv, hd, page_size,
+        block_tables.shape[1], pages, window or 0, _sm_count(index), rows, least_rows, most_rows, scale)), "attention_portions_e4m3")
 
 
 _read_scratch: dict = {}
@@ -380,67 +421,111 @@ def portion_scratch(cache: E4M3Pages, dtype: torch.dtype) -> PlainPages:
 
 
 def attention_portions(q: torch.Tensor, cache: E4M3Pages, block_tables: torch.Tensor, q_start: torch.Tensor, ctx_lens: torch.Tensor,
-                       plan: PortionPlan, num_heads: int, scale: float, status: torch.Tensor, *, window: int | None = None) -> torch.Tensor:
+                       plan: PortionPlan, num_heads: int, scale: float, status: torch.Tensor, *, window: int | None = None,
+                       workspace: DecodeWorkspace | None = None) -> torch.Tensor:
     """Causal attention of prompt portions over an 8-bit cache: ``q`` [N, >= nh * hd]; request s owns rows
-    q_start[s]:q_start[s + 1] and has ctx_lens[s] tokens in the cache, its rows' among them, at the end.  Returns [N, nh * hd]
-    (rows behind the last request's: undefined).  The contexts are read back into scratch pages that calls on a device share:
-    calls that may overlap on the GPU (different streams) must be serialised."""
+    q_start[s]:q_start[s + 1] and has ctx_lens[s] tokens in the cache, its rows' among them, at the end (``plan`` holds the same
+    numbers).  Returns [N, nh * hd] (rows behind the last request's: undefined).  bfloat16 requests of few rows are attended
+    straight from the codes; the contexts of the others are read back into scratch pages that calls on a device share: calls that
+    may overlap on the GPU (different streams) must be serialised."""
     from . import attention_ref
     from . import attention_fast as fast
 
-    _, page_size, nkv, hd = check_pages(cache)
-    _check_device(q.get_device())
+    code, shape = dtype_code(q.dtype), check_pages(cache)
+    _, page_size, nkv, hd = shape
+    if q.dim() != 2 or q.shape[1] < num_heads * hd or q.stride(1) != 1:
+        raise ValueError("q must be [rows, >= nh * hd] with unit column stride")
+    if num_heads <= 0 or num_heads % nkv or hd % 16 or hd > MAX_HEAD_DIM:
+        raise ValueError(f"{num_heads} query heads over {nkv} KV heads of {hd}: a multiple of the KV heads, entries a multiple of 16 up to {MAX_HEAD_DIM}")
+    _ints(block_tables, "block_tables", 2)
+    s = block_tables.shape[0]
+    _ints(ctx_lens, "ctx_lens", 1, s)
+    _ints(q_start, "q_start", 1, s + 1)
+    if len(plan.q_lens) != s or sum(plan.q_lens) > q.shape[0]:
+        raise ValueError(f"the plan is for {len(plan.q_lens)} requests of {sum(plan.q_lens)} rows, the call has {s} and {q.shape[0]}")
+    if window is not None and window <= 0:
+        raise ValueError("window must be positive or None")
+    _check_status(status)
+    index = q.get_device()
+    _elsewhere(index, cache=cache.k, block_tables=block_tables, ctx_lens=ctx_lens, q_start=q_start, plan=plan.tok_seq, status=status)
+    _check_device(index)
+    if code == 1 and hd in fast.PREFILL_HEAD_DIMS:
+        out = q.new_empty((q.shape[0], num_heads * hd))
+        if plan.items:
+            held = portion_scratch(cache, q.dtype)
+            read_pages(cache, block_tables, ctx_lens, held.k, held.v, status, window=window, q_start=q_start,
+                       least_rows=max(plan.most_rows + 1, plan.least_rows))
+            fast.attention_prefill(q, held.k, held.v, block_tables, q_start, ctx_lens, plan.item_seq, plan.item_q0, plan.items, num_heads,
+                                   nkv, hd, scale, window, status, item_split=plan.item_split, out=out)
+        if plan.short:
+            _short_call(q, out, cache, block_tables, ctx_lens, q_start, num_heads, shape, scale, window, plan.short, plan.least_rows, plan.most_rows, status,
+                        index, workspace)
+        return out
+    rows = sum(plan.q_lens)
     held = portion_scratch(cache, q.dtype)
     read_pages(cache, block_tables, ctx_lens, held.k, held.v, status, window=window, q_start=q_start)
-    if q.dtype == torch.bfloat16 and hd in fast.PREFILL_HEAD_DIMS:
-        return fast.attention_prefill(q, held.k, held.v, block_tables, q_start, ctx_lens, plan.item_seq, plan.item_q0, plan.items, num_heads,
-                                      nkv, hd, scale, window, status, item_split=plan.item_split)
-    return attention_ref(q, held.k, held.v, block_tables, plan.tok_seq, plan.positions, num_heads, nkv, hd, scale, window, status, q_start,
-                         list(zip(plan.q_lens, plan.ctx_lens)))
+    out = attention_ref(q[:rows], held.k, held.v, block_tables, plan.tok_seq, plan.positions, num_heads, nkv, hd, scale, window, status, q_start,
+                        list(zip(plan.q_lens, plan.ctx_lens)))
+    return out if rows == q.shape[0] else torch.cat([out, out.new_empty((q.shape[0] - rows, out.shape[1]))])
 
 
 # ---- the attention of a step ---------------------------------------------------------------------------------------------------
 _step_workspaces: dict = {}
 
 
-def step_workspace(requests: int, num_heads: int, num_kv_heads: int, head_dim: int, index: int) -> DecodeWorkspace:
-    """The workspace that the layers of a device's engine steps share (steps run one after the other); replaced by a larger one
-    when a step brings more requests, and kept then, since captured steps point at it."""
-    key = (index, num_heads, num_kv_heads, head_dim)
-    held = _step_workspaces.get(key)
-    if held is None or held[0] < requests:
+def step_workspace(head_dim: int, index: int) -> DecodeWorkspace:
+    """The workspace that the layers of a device's engine steps share (steps run one after the other, captured ones too)."""
+    held = _step_workspaces.get((index, head_dim))
+    if held is None:
         if torch.cuda.is_current_stream_capturing():
             raise RuntimeError("the workspace of a captured step must exist before it is captured: run the step once first")
-        if held is not None:
-            _retired_scratch.append(held)
-        room = max(requests, 256)
-        held = _step_workspaces[key] = (room, DecodeWorkspace(room, num_heads, num_kv_heads, head_dim, torch.device("cuda", index)))
-    return held[1]
+        held = _step_workspaces[index, head_dim] = DecodeWorkspace(head_dim, torch.device("cuda", index))
+    return held
 
 
 def paged_attention(ctx, q: torch.Tensor, cache: E4M3Pages, block_tables: torch.Tensor, num_heads: int, scale: float,
                     window: int | None) -> torch.Tensor:
-    """Attention of a step of the engine over an 8-bit cache that already holds the step's keys and values: single tokens straight
-    from the codes; portions from their requests' pages read back into scratch pages, by the kernels of the run's type."""
+    """Attention of a step of the engine over an 8-bit cache that already holds the step's keys and values: single tokens and short
+    portions straight from the codes; longer ones from their requests' pages read back into scratch pages, by the kernels of the
+    run's type."""
     from . import attention_ref
     from .attention_fast import _Prefill
 
-    _, _, nkv, hd = cache.k.shape
+    shape = cache.k.shape
+    _, _, nkv, hd = shape
     index = q.get_device()
+    streams = q.dtype == torch.bfloat16 and hd % 32 == 0
+    scratch = step_workspace(hd, index) if streams else None
 
     def singles(out=None):
-        scratch = step_workspace(ctx.num_seqs, num_heads, nkv, hd, index) if q.dtype == torch.bfloat16 and hd % 32 == 0 else None
         return attention_decode(q, cache, block_tables, ctx.ctx_lens, num_heads, scale, ctx.status, window=window,
                                 q_start=None if out is None else ctx.q_start, out=out, workspace=scratch)
 
     if ctx.all_single_token:
         return singles()
-    held = portion_scratch(cache, q.dtype)
     if q.dtype == torch.bfloat16 and _Prefill.accepts(ctx, None, num_heads, nkv, hd, window):
         apart = _Prefill.singles_apart(ctx, hd)
-        read_pages(cache, block_tables, ctx.ctx_lens, held.k, held.v, ctx.status, window=window, q_start=ctx.q_start, skip_single=apart > 0)
+        least = 2 if apart else 1
+        if ctx.extras.get("captured_portions") is None:
+            key = ("e4m3 portions", num_heads, nkv, hd, shape[1], least)
+            plan = ctx.extras.get(key)
+            if plan is None:
+                plan = ctx.extras[key] = plan_portions(ctx.q_lens_host, ctx.ctx_lens_host, num_heads, nkv, hd, shape[1], ctx.device, least_rows=least)
+            out = attention_portions(q, cache, block_tables, ctx.q_start, ctx.ctx_lens, plan, num_heads, scale, ctx.status, window=window,
+                                     workspace=scratch)
+            return singles(out) if apart else out
+        # a captured step: how its rows are divided among its requests is not known here, but that none brings more than there are
+        most = short_rows(num_heads, nkv, hd) if streams else 0
+        if ctx.num_tokens <= most:
+            out = q.new_empty((q.shape[0], num_heads * hd))
+            _short_call(q, out, cache, block_tables, ctx.ctx_lens, ctx.q_start, num_heads, shape, scale, window, ctx.num_tokens, least, most,
+                        ctx.status, index, scratch)
+            return singles(out) if apart else out
+        held = portion_scratch(cache, q.dtype)
+        read_pages(cache, block_tables, ctx.ctx_lens, held.k, held.v, ctx.status, window=window, q_start=ctx.q_start, least_rows=least)
         out = _Prefill.portions(ctx, q, held.k, held.v, block_tables, num_heads, nkv, hd, scale, window, apart)
         return singles(out) if apart else out
+    held = portion_scratch(cache, q.dtype)
     read_pages(cache, block_tables, ctx.ctx_lens, held.k, held.v, ctx.status, window=window, q_start=ctx.q_start)
     return attention_ref(q, held.k, held.v, block_tables, ctx.tok_seq, ctx.positions, num_heads, nkv, hd, scale, window, ctx.status,
                          ctx.q_start, list(zip(ctx.q_lens_host, ctx.ctx_lens_host)))

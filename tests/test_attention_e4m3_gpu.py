@@ -131,26 +131,32 @@ def test_decode_reports_pages_outside_the_pool():
 
 PORTIONS = [  # heads, rows of each request, tokens behind them, page size, window
     ((12, 2, 128), [130], [0], 16, None), ((12, 2, 128), [64, 1, 200], [300, 40, 0], 16, None), ((4, 4, 64), [150, 0, 7], [0, 9, 1000], 8, 60),
-    ((4, 2, 16), [33], [12], 4, None), ((6, 2, 96), [20, 50], [5, 0], 16, None), ((2, 1, 256), [40], [77], 16, None)]
+    ((4, 2, 16), [33], [12], 4, None), ((6, 2, 96), [20, 50], [5, 0], 16, None), ((2, 1, 256), [40], [77], 16, None),
+    ((28, 4, 128), [5, 17, 2], [3000, 0, 64], 16, None), ((9, 3, 32), [11, 100], [70, 31], 7, 20), ((16, 16, 64), [2] * 40, [90] * 40, 16, None),
+    ((70, 2, 64), [3, 40], [200, 1], 16, None), ((4, 1, 128), [60, 1, 61], [2000, 500, 4000], 64, 700), ((40, 8, 128), [16], [5000], 16, None)]
 
 
-@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("dtype, most", [(torch.bfloat16, None), (torch.bfloat16, 0), (torch.bfloat16, 10000), (torch.float32, None)])
 @pytest.mark.parametrize("heads, new, behind, page, window", PORTIONS)
-def test_portions(heads, new, behind, page, window, dtype):
+def test_portions(heads, new, behind, page, window, dtype, most):
+    """``most``: requests of up to so many rows straight from the codes (None: as the operator chooses)."""
     nh, nkv, hd = heads
+    if most and hd not in quantised.SHORT_HEAD_DIMS:
+        pytest.skip("this head size is read back")
     ctx = [a + b for a, b in zip(new, behind)]
     g = torch.Generator().manual_seed(sum(ctx) + hd)
     cache, tables = filled_pages(ctx, page, nkv, hd, g)
     starts = [sum(new[:i]) for i in range(len(new) + 1)]
-    q = torch.randn(starts[-1], nh * hd, generator=g).to(dtype)
+    q = torch.randn(starts[-1] + 2, nh * hd, generator=g).to(dtype)  # (two rows behind the last request's)
     status = ops.new_status(DEV)
-    plan = quantised.plan_portions(new, ctx, nh, nkv, hd, page, torch.device(DEV))
-    out = quantised.attention_portions(q.to(DEV), quantised.E4M3Pages(*_on(*cache)), *_on(tables, torch.tensor(starts, dtype=torch.int32),
-                                       torch.tensor(ctx, dtype=torch.int32)), plan, nh, hd**-0.5, status, window=window)
+    plan = quantised.plan_portions(new, ctx, nh, nkv, hd, page, torch.device(DEV), most_rows=most)
+    out = quantised.attention_portions(q.to(DEV), quantised.E4M3Pages(*_on(*cache)),
+                                       *_on(tables, torch.tensor(starts, dtype=torch.int32), torch.tensor(ctx, dtype=torch.int32)), plan, nh,
+                                       hd**-0.5, status, window=window)
     ops.raise_on_status(status)
-    # (the bfloat16 kernels hold a weight in that type: half a step, 2^-8 of it)
+    # (the bfloat16 kernels over pages read back hold a weight in that type: half a step, 2^-8 of it)
     _check(out, q, cache, tables, ctx, [(s, starts[s], n, ctx[s] - n) for s, n in enumerate(new) if n], page, window, hd**-0.5, dtype,
-           8 if dtype == torch.bfloat16 else 24)
+           24 if dtype == torch.float32 else WEIGHT_BITS if most == 10000 else 8)
 
 
 @pytest.mark.parametrize("norm", [False, True])

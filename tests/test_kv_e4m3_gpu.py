@@ -212,9 +212,9 @@ def test_read_pages(ctx, page, nkv, hd, window, dtype):
         assert dtype == torch.float32 or torch.equal(want.to(dtype).double(), want)  # bfloat16 holds every held number
 
 
-@pytest.mark.parametrize("skip", [False, True])
-def test_read_pages_of_the_requests_that_bring_rows(skip):
-    """With q_start only requests of rows (``skip_single``: of several) are read, from the page on that their first row's window reaches."""
+@pytest.mark.parametrize("least", [1, 2, 11])
+def test_read_pages_of_the_requests_that_bring_rows(least):
+    """With q_start only requests of at least so many rows are read, from the page on that their first row's window reaches."""
     ctx, new, page, window = [100, 90, 64, 50], [10, 1, 0, 40], 8, 16
     g = torch.Generator().manual_seed(8)
     cache, tables = filled_pages(ctx, page, 2, 32, g)
@@ -222,12 +222,12 @@ def test_read_pages_of_the_requests_that_bring_rows(skip):
     out = [torch.full(cache[0].shape, 3.0, device=DEV) for _ in range(2)]
     starts = torch.tensor([0, 10, 11, 11, 51], dtype=torch.int32)
     quantised.read_pages(quantised.E4M3Pages(*_on(*cache)), *_on(tables, torch.tensor(ctx, dtype=torch.int32)), *out, status, window=window,
-                         q_start=starts.to(DEV), skip_single=skip)
+                         q_start=starts.to(DEV), least_rows=least)
     ops.raise_on_status(status)
     read = (out[0] != 3.0).flatten(1).any(1).cpu()
     want = torch.zeros_like(read)
     for s, (c, n) in enumerate(zip(ctx, new)):
-        if n > (1 if skip else 0):
+        if n >= least:
             want[tables[s, max(0, c - n + 1 - window) // page : -(-c // page)].long()] = True
     assert torch.equal(read, want)
 

@@ -580,12 +580,22 @@ def attention_prefill(q, k_cache, v_cache, block_tables, q_start, ctx_lens, item
         raise ValueError("out must be a contiguous bfloat16 [N, nh*hd] tensor")
     if use_tc is None:
         use_tc = prefill_tc_takes(head_dim, k_cache.shape[1])
-    if item_split is not None and not use_tc:
-        raise ValueError("only the tcgen05 kernel takes work items that are parts")
+    if item_split is not None:
+        if not use_tc:
+            raise ValueError("only the tcgen05 kernel takes work items that are parts")
+        _need(item_split, torch.int32, "item_split", 1)
+    launch_prefill(q, k_cache, v_cache, block_tables, q_start, ctx_lens, item_seq, item_q0, items, num_heads, num_kv_heads, head_dim, scale,
+                   window, status, use_tc, item_split, out)
+    return out
+
+
+def launch_prefill(q, k_cache, v_cache, block_tables, q_start, ctx_lens, item_seq, item_q0, items, num_heads, num_kv_heads, head_dim, scale,
+                   window, status, use_tc, item_split, out) -> None:
+    """The launch of ``attention_prefill``, its arguments as that has checked them."""
+    _configure()
     if use_tc:
         st = {"part_o": None, "part_ml": None, "counters": None}
         if item_split is not None:
-            _need(item_split, torch.int32, "item_split", 1)
             st = _prefill_scratch(q.device, items, num_heads, head_dim)
         check(library().cw_attention_prefill_tc(
             _ptr(q), q.stride(0), q.shape[1], q.shape[0], _ptr(out), _ptr(k_cache), _ptr(v_cache), _ptr(block_tables),
@@ -593,12 +603,11 @@ def attention_prefill(q, k_cache, v_cache, block_tables, q_start, ctx_lens, item
             _ptr(st["part_ml"]), _ptr(st["counters"]), items, num_heads, num_kv_heads, head_dim,
             k_cache.shape[1], block_tables.shape[1], k_cache.shape[0], float(scale), int(window or 0), _ptr(status),
             _stream()), "attention_prefill_tc")
-        return out
+        return
     check(library().cw_attention_prefill(
         _ptr(q), q.stride(0), _ptr(out), _ptr(k_cache), _ptr(v_cache), _ptr(block_tables), _ptr(q_start), _ptr(ctx_lens),
         _ptr(item_seq), _ptr(item_q0), items, num_heads, num_kv_heads, head_dim, k_cache.shape[1], block_tables.shape[1],
         k_cache.shape[0], float(scale), int(window or 0), _ptr(status), _stream()), "attention_prefill")
-    return out
 
 
 def enable() -> None:

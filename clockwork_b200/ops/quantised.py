@@ -172,6 +172,14 @@ def norm_rotate_store(qkv: torch.Tensor, positions: torch.Tensor, slots: torch.T
 READ_BLOCKS = 148 * 4
 
 
+def _read_call(cache, shape, block_tables, ctx_lens, q_start, out_k, out_v, window, least_rows, code, status) -> None:
+    pages, page_size, nkv, hd = shape
+    check(library().cw_read_pages(_READ_ARGS(
+        cache.k.data_ptr(), cache.v.data_ptr(), cache.k_exp.data_ptr(), cache.v_exp.data_ptr(), out_k.data_ptr(), out_v.data_ptr(),
+        block_tables.data_ptr(), ctx_lens.data_ptr(), 0 if q_start is None else q_start.data_ptr(), status.data_ptr(), _stream(), block_tables.shape[0], nkv, hd,
+        page_size, block_tables.shape[1], pages, window or 0, least_rows, READ_BLOCKS, code)), "read_pages")
+
+
 def read_pages(cache: E4M3Pages, block_tables: torch.Tensor, ctx_lens: torch.Tensor, out_k: torch.Tensor, out_v: torch.Tensor,
                status: torch.Tensor, *, window: int | None = None, q_start: torch.Tensor | None = None, least_rows: int = 1) -> None:
     """The keys and values of positions [0, ctx_lens[s]) of every request, through ``block_tables`` [S, max_blocks], into plain
@@ -198,10 +206,7 @@ def read_pages(cache: E4M3Pages, block_tables: torch.Tensor, ctx_lens: torch.Ten
     index = cache.k.get_device()
     _elsewhere(index, out_k=out_k, out_v=out_v, block_tables=block_tables, ctx_lens=ctx_lens, q_start=q_start, status=status)
     _check_device(index)
-    check(library().cw_read_pages(_READ_ARGS(
-        cache.k.data_ptr(), cache.v.data_ptr(), cache.k_exp.data_ptr(), cache.v_exp.data_ptr(), out_k.data_ptr(), out_v.data_ptr(),
-        block_tables.data_ptr(), ctx_lens.data_ptr(), 0 if q_start is None else q_start.data_ptr(), status.data_ptr(), _stream(), s, nkv, hd,
-        page_size, block_tables.shape[1], pages, window or 0, least_rows, READ_BLOCKS, dtype_code(out_k.dtype))), "read_pages")
+    _read_call(cache, (pages, page_size, nkv, hd), block_tables, ctx_lens, q_start, out_k, out_v, window, least_rows, dtype_code(out_k.dtype), status)
 
 
 class DecodeWorkspace:
@@ -453,10 +458,9 @@ def attention_portions(q: torch.Tensor, cache: E4M3Pages, block_tables: torch.Te
         out = q.new_empty((q.shape[0], num_heads * hd))
         if plan.items:
             held = portion_scratch(cache, q.dtype)
-            read_pages(cache, block_tables, ctx_lens, held.k, held.v, status, window=window, q_start=q_start,
-                       least_rows=max(plan.most_rows + 1, plan.least_rows))
-            fast.attention_prefill(q, held.k, held.v, block_tables, q_start, ctx_lens, plan.item_seq, plan.item_q0, plan.items, num_heads,
-                                   nkv, hd, scale, window, status, item_split=plan.item_split, out=out)
+            _read_call(cache, shape, block_tables, ctx_lens, q_start, held.k, held.v, window, max(plan.most_rows + 1, plan.least_rows), code, status)
+            fast.launch_prefill(q, held.k, held.v, block_tables, q_start, ctx_lens, plan.item_seq, plan.item_q0, plan.items, num_heads, nkv, hd,
+                                scale, window, status, fast.prefill_tc_takes(hd, page_size), plan.item_split, out)
         if plan.short:
             _short_call(q, out, cache, block_tables, ctx_lens, q_start, num_heads, shape, scale, window, plan.short, plan.least_rows, plan.most_rows, status,
                         index, workspace)

@@ -1,0 +1,164 @@
+"""The 8-bit cache's operators as programs use them: captured in graphs, on two streams at once, with and without a workspace of their
+own, called again and again on one workspace, at the ends of their ranges."""
+
+import pytest
+import torch
+
+from clockwork_b200 import ops
+from clockwork_b200.ops import quantised
+from tests.e4m3_tools import filled_pages
+from tests.gpu_tools import DEV
+
+pytestmark = pytest.mark.gpu
+NH, NKV, HD, PAGE = 12, 2, 128, 16
+
+
+def _problem(ctx, seed, nh=NH, nkv=NKV, hd=HD):
+    g = torch.Generator().manual_seed(seed)
+    cache, tables = filled_pages(ctx, PAGE, nkv, hd, g)
+    q = torch.randn(len(ctx), nh * hd, generator=g).bfloat16()
+    return (q.to(DEV), quantised.E4M3Pages(*(t.to(DEV) for t in cache)), tables.to(DEV), torch.tensor(ctx, dtype=torch.int32, device=DEV))
+
+
+def _run(problem, status, nh=NH, **kwargs):
+    q, cache, tables, ctx = problem
+    return quantised.attention_decode(q, cache, tables, ctx, nh, 0.09, status, **kwargs)
+
+
+@pytest.mark.parametrize("own", [False, True])
+def test_captured_calls_give_the_bits_of_plain_ones(own):
+    """Replayed many times, with the lengths changed between replays, and two graphs one after the other."""
+    status = ops.new_status(DEV)
+    workspace = quantised.DecodeWorkspace(HD, DEV) if own else None
+    problems = [_problem([700, 3, 2000, 64], 1), _problem([5000], 2)]
+    want = [_run(p, status) for p in problems]
+    graphs, outs = [], []
+    for p in problems:
+        _run(p, status, workspace=workspace)
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            outs.append(_run(p, status, workspace=workspace))
+        graphs.append(graph)
+    for _ in range(3):
+        for graph, out, w in zip(graphs, outs, want):
+            out.zero_()
+            graph.replay()
+            assert torch.equal(out, w)
+    lengths = problems[0][3]
+    lengths.copy_(torch.tensor([1, 0, 1999, 33], dtype=torch.int32))
+    shorter = _run(problems[0], status)
+    graphs[0].replay()
+    assert torch.equal(outs[0], shorter) and (shorter[1] == 0).all() and not torch.equal(shorter, want[0])
+    ops.raise_on_status(status)
+
+
+def test_two_streams_and_two_graphs_at_once():
+    """Calls that bring no workspace may overlap on the GPU: every stream, and every captured call, has scratch of its own."""
+    status = [ops.new_status(DEV), ops.new_status(DEV)]
+    problems = [_problem([9000, 8000], 3), _problem([20000], 4)]
+    want = [_run(p, s) for p, s in zip(problems, status)]
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    torch.cuda.synchronize()
+    got = [[], []]
+    for _ in range(20):
+        for i in range(2):
+            with torch.cuda.stream(streams[i]):
+                got[i].append(_run(problems[i], status[i]))
+    graphs, outs = [], []
+    torch.cuda.synchronize()
+    for i in range(2):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            outs.append(_run(problems[i], status[i]))
+        graphs.append(graph)
+    for _ in range(20):
+        for i in range(2):
+            with torch.cuda.stream(streams[i]):
+                graphs[i].replay()
+    torch.cuda.synchronize()
+    for i in range(2):
+        ops.raise_on_status(status[i])
+        assert all(torch.equal(x, want[i]) for x in got[i]) and torch.equal(outs[i], want[i])
+
+
+def test_one_workspace_serves_calls_of_every_shape():
+    """Counters are zero again after each call, whatever its heads, lengths and pieces."""
+    workspace, status = quantised.DecodeWorkspace(HD, DEV), ops.new_status(DEV)
+    shapes = [([100000], 12, 2, 128), ([5] * 300, 12, 2, 128), ([3000, 1], 16, 16, 64), ([40, 7000, 0, 900], 24, 2, 128), ([12345] * 3, 8, 4, 32)]
+    problems = [(_problem(ctx, 5 + i, nh, nkv, hd), nh) for i, (ctx, nh, nkv, hd) in enumerate(shapes)]
+    want = [_run(p, status, nh) for p, nh in problems]
+    for _ in range(3):
+        for (p, nh), w in zip(problems, want):
+            assert torch.equal(_run(p, status, nh, workspace=workspace), w)
+    assert (workspace.words == 0).all()
+    with pytest.raises(ValueError, match="workspace"):
+        _run(_problem([40], 9, 2, 1, 256), status, 2, workspace=workspace)
+    ops.raise_on_status(status)
+
+
+def test_portions_in_a_graph():
+    status = ops.new_status(DEV)
+    ctx, new = [300, 2000, 90], [7, 150, 1]
+    g = torch.Generator().manual_seed(11)
+    cache, tables = filled_pages(ctx, PAGE, NKV, HD, g)
+    cache, tables = quantised.E4M3Pages(*(t.to(DEV) for t in cache)), tables.to(DEV)
+    q = torch.randn(sum(new), NH * HD, generator=g).bfloat16().to(DEV)
+    starts = torch.tensor([0, 7, 157, 158], dtype=torch.int32, device=DEV)
+    lens = torch.tensor(ctx, dtype=torch.int32, device=DEV)
+    plan = quantised.plan_portions(new, ctx, NH, NKV, HD, PAGE, torch.device(DEV))
+    assert plan.short == 8 and plan.items > 0  # both kernels
+
+    def run():
+        return quantised.attention_portions(q, cache, tables, starts, lens, plan, NH, 0.09, status)
+
+    want = run()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = run()
+    for _ in range(3):
+        out.zero_()
+        graph.replay()
+        assert torch.equal(out, want)
+    ops.raise_on_status(status)
+
+
+def test_the_same_page_in_two_requests_and_twice_in_one():
+    """Block tables may name a page more than once (a shared prefix; a request that repeats a page)."""
+    q, cache, tables, ctx = _problem([64, 64, 64], 12)
+    tables[1, :2] = tables[0, :2]
+    tables[2, 1] = tables[2, 0]
+    status = ops.new_status(DEV)
+    out = quantised.attention_decode(q, cache, tables, ctx, NH, 0.09, status)
+    out_k, out_v = (torch.zeros(cache.k.shape, dtype=torch.bfloat16, device=DEV) for _ in range(2))
+    quantised.read_pages(cache, tables, ctx, out_k, out_v, status)
+    ops.raise_on_status(status)
+    from clockwork_b200.ops.attention_fast import attention_decode
+
+    plain = attention_decode(q, out_k, out_v, tables, ctx, NH, NKV, HD, 0.09, None, 64, status)
+    # two kernels over the same numbers: weights in 11 and 8 bits, outputs in 8
+    size = out_v.float().abs().max()
+    assert (out.float() - plain.float()).abs().max() <= (2.0**-8 + 2.0**-8 + 2.0**-10) * size
+
+
+def test_queries_that_are_not_aligned_for_pairs():
+    """Rows that begin at an odd entry go to the kernel that reads entry by entry."""
+    q, cache, tables, ctx = _problem([200, 31], 13)
+    wide = torch.zeros(2, NH * HD + 3, dtype=torch.bfloat16, device=DEV)
+    wide[:, 1 : 1 + NH * HD] = q
+    status = ops.new_status(DEV)
+    a = quantised.attention_decode(wide[:, 1 : 1 + NH * HD], cache, tables, ctx, NH, 0.09, status)
+    b = quantised.attention_decode(q, cache, tables, ctx, NH, 0.09, status)
+    ops.raise_on_status(status)
+    assert (a.float() - b.float()).abs().max() <= 2.0**-7 * b.float().abs().max()
+
+
+def test_no_rows_at_all():
+    status = ops.new_status(DEV)
+    cache = quantised.allocate_pages(2, PAGE, NKV, HD, DEV)
+    none = torch.zeros(0, dtype=torch.int32, device=DEV)
+    q = quantised.norm_rotate_store(torch.zeros(0, (NH + 2 * NKV) * HD, dtype=torch.bfloat16, device=DEV), none, none, None, cache, NH, NKV, HD, status)
+    assert q.shape == (0, NH * HD)
+    out = quantised.attention_decode(q, cache, torch.zeros(0, 1, dtype=torch.int32, device=DEV), none, NH, 0.09, status)
+    assert out.shape == (0, NH * HD)
+    ops.raise_on_status(status)

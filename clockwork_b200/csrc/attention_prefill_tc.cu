@@ -37,9 +37,9 @@
 // (request, first query row) work items, one per 128 query tokens; a decoded token is a portion of
 // length one and may ride along.
 //
-// Key slots past the end of a request's context are fetched from page 0 and multiplied by
-// probabilities that are exactly zero; the cache pool is zero-initialised and only ever holds
-// finite values, so they cannot leak.  Every wait is bounded (CW_ST_WAIT_TIMEOUT in the status
+// Pages of a tile that lie wholly past the last visible key or before the window are not looked up (their table entries may name
+// nothing): the request's last visible page stands in for them.  What is fetched and not visible is multiplied by probabilities
+// that are exactly zero; the cache pool is zero-initialised and only ever holds finite values, so it cannot leak.  Every wait is bounded (CW_ST_WAIT_TIMEOUT in the status
 // words, then the kernel frees TMEM and returns).
 #include <type_traits>
 #include "tc_attention.cuh"
@@ -199,11 +199,12 @@ attn_prefill_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
         }
         const int* table = p.block_tables + (size_t)s * p.max_blocks;
         const int pages_per_tile = AK >> p.page_shift;  // at most 16
+        const int own = table[min((kv_hi - 1) >> p.page_shift, p.max_blocks - 1)];
         auto page_of = [&](int j) -> int {
-            // slots past the context: any finite data will do, their probabilities are zero
+            // pages without a visible key: any finite data of the request's own will do, their probabilities are zero
             const int pos = tile_lo + j * AK + lane * p.page_size;
             const int blk = pos >> p.page_shift;
-            return (j < ntiles && lane < pages_per_tile && pos < kv_hi && blk < p.max_blocks) ? table[blk] : 0;
+            return (j < ntiles && lane < pages_per_tile && pos < kv_hi && pos + p.page_size > kv_lo && blk < p.max_blocks) ? table[blk] : own;
         };
         int pg_v = page_of(0), pg_1 = page_of(1), pg_2 = page_of(2);  // this lane's page of tiles j, j+1, j+2
         asm volatile("griddepcontrol.wait;" ::: "memory");

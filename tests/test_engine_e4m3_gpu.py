@@ -32,7 +32,7 @@ class Untouched:
 
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("kv_dtype, norm", [("e4m3", None), ("e4m3", 1e-5), ("auto", 1e-5)])
-@pytest.mark.parametrize("heads, window", [((6, 2, 48), None), ((8, 2, 64), None), ((4, 1, 32), 20), ((3, 3, 128), None), ((2, 1, 256), 33)])
+@pytest.mark.parametrize("heads, window", [((6, 2, 48), None), ((8, 2, 64), None), ((8, 2, 64), 16), ((4, 1, 32), 20), ((2, 2, 128), 9), ((3, 3, 128), None), ((2, 1, 256), 33)])
 def test_attention_part(heads, window, kv_dtype, norm, dtype):
     """Portions, single tokens and both in one step.  q and what the cache holds are checked in the kernels' own tests; here they are
     taken from the kernel and the cache, and attention of every row is worked out from them in float64."""

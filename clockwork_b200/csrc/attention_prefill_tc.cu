@@ -31,6 +31,10 @@
 // owner, 2..9 and 10..17 the softmax sets (warp w owns TMEM lanes 32 (w % 4) .. +31; two warps of a
 // set share a lane quarter and split the columns).
 //
+// Packed rows (`each` > 1): a CTA's 128 rows are the `each` query heads of a KV head for 128 / each tokens (row r: token r / each, head
+// r % each), so that a portion of few tokens fills its tiles, and the diagonal costs a tile less; q comes by a map of rank 3, whose box
+// of [tokens][heads] rows lies in that order.  Otherwise a CTA has one head and a row is a token.
+//
 // Reference: clockwork/kernels/attention.py:68-96 (gather the context through one block table, then
 // dense causal attention with the query aligned to the end of the context, :45-65) and
 // clockwork/engine/model.py:103-118.  One launch covers every portion of the batch: the host lists
@@ -61,6 +65,7 @@ struct PrefillTcParams {
     // in counters[first * nh + head] (zero between launches); the last one to arrive merges them all.
     const int* item_split; float* part_o; float* part_ml; int* counters;
     int nh, nkv, page_size, page_shift, max_blocks, num_pages;
+    int each;  // query heads that share a CTA: 1, or those of a KV head
     float scale; int window;
     int* status;
 };
@@ -85,6 +90,12 @@ __device__ __forceinline__ void tma_load_5d(uint32_t dst, const CUtensorMap* map
     asm volatile(
         "cp.async.bulk.tensor.5d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6, %7}], [%2];"
         ::"r"(dst), "l"(map), "r"(bar), "r"(x), "r"(y), "r"(z), "r"(w), "r"(v)
+        : "memory");
+}
+__device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap* map, int x, int y, int z, uint32_t bar) {
+    asm volatile(
+        "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];"
+        ::"r"(dst), "l"(map), "r"(bar), "r"(x), "r"(y), "r"(z)
         : "memory");
 }
 // K-major operand, 128-byte swizzle, with the groups of 8 rows `group_bytes` apart (tc_common's form has 1024).
@@ -112,7 +123,7 @@ __device__ __forceinline__ bool bar_and(int id, int n, bool pred) {
                  : "memory");
     return all != 0;
 }
-template <int HD>
+template <int HD, bool PACKED>
 __global__ void __launch_bounds__(A_THREADS, 1)  // (18 warps: five on one scheduler, whose 16,384 registers allow 96 per thread)
 attn_prefill_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
                        const __grid_constant__ CUtensorMap map_v, const PrefillTcParams p) {
@@ -138,15 +149,17 @@ attn_prefill_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
     // So everything up to the first TMA load runs while the preceding kernel finishes, and only the
     // producer warp, whose loads are the kernel's only reads of that data, waits for it.
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-    const int h = blockIdx.x, item = blockIdx.y;
+    const int h = blockIdx.x, heads = gridDim.x, item = blockIdx.y;  // (h: of the head, or of the KV head whose heads are packed)
     const int s = p.item_seq[item], q0 = p.item_q0[item];
     if (s < 0) return;  // an unused entry of a work list of fixed length (captured steps): nothing is set up yet
-    const int kvh = h / (p.nh / p.nkv);
+    const int each = PACKED ? p.each : 1, tile_tokens = AQ / each;
+    const int kvh = PACKED ? h : h / (p.nh / p.nkv);
     const int row0 = p.q_start[s], q_len = p.q_start[s + 1] - row0;
     const int ctx = p.ctx_lens[s];
     const int pos0 = ctx - q_len + q0;           // position of the tile's first query
-    const int nq = min(AQ, q_len - q0);          // query rows in this tile
-    const int kv_hi = pos0 + nq;                 // keys [.., kv_hi) are visible to the last row
+    const int nt = min(tile_tokens, q_len - q0); // tokens in this tile
+    const int nq = nt * each;                  // and its query rows
+    const int kv_hi = pos0 + nt;                 // keys [.., kv_hi) are visible to the last row
     const int kv_lo = p.window > 0 ? max(0, pos0 + 1 - p.window) : 0;
     int tile_lo = kv_lo / AK * AK;               // key tiles start at multiples of 128 whatever the portion
     int ntiles = (kv_hi - tile_lo + AK - 1) / AK;
@@ -209,9 +222,13 @@ attn_prefill_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
         int pg_v = page_of(0), pg_1 = page_of(1), pg_2 = page_of(2);  // this lane's page of tiles j, j+1, j+2
         asm volatile("griddepcontrol.wait;" ::: "memory");
         if (lane == 0) {
-            mbar_expect_tx(q_full, C::Q_BYTES);
-            for (int cb = 0; cb < C::CB; ++cb)
-                tma_load_2d(smem_u32(q_s + cb * C::BLOCK_BYTES), &map_q, h * HD + cb * 64, row0 + q0, q_full);
+            mbar_expect_tx(q_full, C::CB * tile_tokens * each * 128);
+            for (int cb = 0; cb < C::CB; ++cb) {
+                if (!PACKED)
+                    tma_load_2d(smem_u32(q_s + cb * C::BLOCK_BYTES), &map_q, h * HD + cb * 64, row0 + q0, q_full);
+                else
+                    tma_load_3d(smem_u32(q_s + cb * C::BLOCK_BYTES), &map_q, cb * 64, h * each, row0 + q0, q_full);
+            }
         }
         int t = 0;
         auto load = [&](int page, bool is_v) -> bool {
@@ -323,7 +340,8 @@ attn_prefill_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
         constexpr int SC = AK / 2;   // S columns per thread
         constexpr int OC = HD / 2;   // O columns per thread
         const uint32_t lane_addr = tmem_base + ((uint32_t)(quarter * 32) << 16);
-        const int qp = pos0 + row;                                     // this row's position
+        const int token = PACKED ? row / each : row, head = PACKED ? h * each + (row - token * each) : h;
+        const int qp = pos0 + token;                                   // this row's position
         const int lo = p.window > 0 ? max(0, qp + 1 - p.window) : 0;   // its first visible key
         const float scale_log2 = p.scale * 1.4426950408889634f;        // softmax in base 2
         const int pair_bar = 1 + 4 * set + quarter;                    // named barrier of the 64 threads of a quarter
@@ -339,7 +357,7 @@ attn_prefill_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
             ok = mbar_wait(s_full0 + 8 * set, (j >> 1) & 1, give_up);
             ok = __all_sync(0xffffffffu, ok);  // one decision per warp: the TMEM accesses below are warp-wide
             // tiles wholly visible to all 128 rows skip the per-element test
-            const bool all_visible = tile0 + AK - 1 <= pos0 && (p.window <= 0 || tile0 > pos0 + AQ - 1 - p.window);
+            const bool all_visible = tile0 + AK - 1 <= pos0 && (p.window <= 0 || tile0 > pos0 + tile_tokens - 1 - p.window);
             // this thread's half row of S, read from TMEM once and held in registers
             float sv[SC];
             if (ok) {
@@ -457,7 +475,7 @@ attn_prefill_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
                     for (int i = 0; i < 32; ++i) v[i] *= w0;
                 }
             };
-            bf16* o = p.out + ((size_t)(row0 + q0 + row) * p.nh + h) * HD + half * OC;
+            bf16* o = p.out + ((size_t)(row0 + q0 + token) * p.nh + head) * HD + half * OC;
             if (parts == 1) {
                 if (ok) {
                     const float inv = L > 0.f ? 1.f / L : 0.f;
@@ -482,8 +500,8 @@ attn_prefill_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
                 // ---- one part of a cut row of keys: leave (m, l, unnormalised O), the last part to arrive merges ----
                 // part_o is [item][head][column][row]: a warp's 32 rows lie side by side, so that its stores
                 // here and its loads in the merge are whole 128-byte lines
-                float* my_o = p.part_o + (((size_t)item * p.nh + h) * HD + half * OC) * AQ + row;
-                float* my_ml = p.part_ml + (((size_t)item * p.nh + h) * AQ + row) * 2;
+                float* my_o = p.part_o + (((size_t)item * heads + h) * HD + half * OC) * AQ + row;
+                float* my_ml = p.part_ml + (((size_t)item * heads + h) * AQ + row) * 2;
 #pragma unroll
                 for (int c = 0; c < OC / 32; ++c) {
                     float v[32];
@@ -504,7 +522,7 @@ attn_prefill_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
                 // thread 64's release, and its acquire before every thread's loads of the other parts.
                 asm volatile("bar.sync 10, 256;" ::: "memory");
                 if (tid == 64) {
-                    int* counter = p.counters + (size_t)first_item * p.nh + h;
+                    int* counter = p.counters + (size_t)first_item * heads + h;
                     int prev;
                     asm volatile("atom.add.acq_rel.gpu.global.s32 %0, [%1], 1;" : "=r"(prev) : "l"(counter) : "memory");
                     *last_part = (prev == parts - 1);
@@ -514,9 +532,9 @@ attn_prefill_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
                 if (*last_part && row < nq) {
                     // every load of a round is in flight before the first is used: the (m, l) of all parts,
                     // then O in rounds of 16 or 8 columns of KP parts each (in part order whoever came last)
-                    const size_t stride_o = (size_t)p.nh * AQ * HD, stride_ml = (size_t)p.nh * AQ * 2;
-                    const float* ml0 = p.part_ml + (((size_t)first_item * p.nh + h) * AQ + row) * 2;
-                    const float* o0 = p.part_o + (((size_t)first_item * p.nh + h) * HD + half * OC) * AQ + row;
+                    const size_t stride_o = (size_t)heads * AQ * HD, stride_ml = (size_t)heads * AQ * 2;
+                    const float* ml0 = p.part_ml + (((size_t)first_item * heads + h) * AQ + row) * 2;
+                    const float* o0 = p.part_o + (((size_t)first_item * heads + h) * HD + half * OC) * AQ + row;
                     float2 ml[PREFILL_MAX_PARTS];
 #pragma unroll
                     for (int k = 0; k < PREFILL_MAX_PARTS; ++k)
@@ -573,18 +591,18 @@ attn_prefill_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
 // ---------------------------------------------------------------------------------------------
 // host side
 // ---------------------------------------------------------------------------------------------
-template <int HD>
+template <int HD, bool PACKED>
 static int launch_prefill_tc(const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMap& mv,
                              const PrefillTcParams& p, int items, cudaStream_t stream) {
     using C = ACfg<HD>;
     static bool configured = false;
     if (!configured) {
-        if (cudaFuncSetAttribute(attn_prefill_tc_kernel<HD>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+        if (cudaFuncSetAttribute(attn_prefill_tc_kernel<HD, PACKED>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                  C::SMEM_BYTES) != cudaSuccess)
             return (int)cudaGetLastError();
         configured = true;
     }
-    return cw_launch(attn_prefill_tc_kernel<HD>, dim3(p.nh, items), dim3(A_THREADS), C::SMEM_BYTES, stream, 1, mq, mk, mv, p);
+    return cw_launch(attn_prefill_tc_kernel<HD, PACKED>, dim3(p.nh / p.each, items), dim3(A_THREADS), C::SMEM_BYTES, stream, 1, mq, mk, mv, p);
 }
 
 // q: [q_rows, q_cols] rows of the flat batch (row stride q_stride, head h at columns h*hd..), out:
@@ -593,14 +611,13 @@ static int launch_prefill_tc(const CUtensorMap& mq, const CUtensorMap& mk, const
 // items * nh * 256 and counters items * nh zeros, which the kernel leaves zero).  Takes head sizes
 // 64 and 128 and pages of 8..128 tokens (a power of two); CW_ERR_UNSUPPORTED otherwise, so that the
 // caller can use the mma.sync kernel.
-extern "C" int cw_attention_prefill_tc(const void* q, int q_stride, int q_cols, int q_rows, void* out,
-                                       const void* k_cache, const void* v_cache, const int* block_tables,
-                                       const int* q_start, const int* ctx_lens, const int* item_seq,
-                                       const int* item_q0, const int* item_split, float* part_o, float* part_ml,
-                                       int* counters, int items, int nh, int nkv, int hd, int page_size,
-                                       int max_blocks, int num_pages, float scale, int window, int* status,
-                                       cudaStream_t stream) {
+// `each` > 1: the query heads of a KV head packed into a tile's rows (items are then cut at multiples of 128 / each tokens).
+static int prefill_tc(const void* q, int q_stride, int q_cols, int q_rows, void* out, const void* k_cache, const void* v_cache,
+                      const int* block_tables, const int* q_start, const int* ctx_lens, const int* item_seq, const int* item_q0,
+                      const int* item_split, float* part_o, float* part_ml, int* counters, int items, int nh, int nkv, int hd,
+                      int page_size, int max_blocks, int num_pages, float scale, int window, int each, int* status, cudaStream_t stream) {
     if (items == 0) return CW_OK;
+    if (each < 1 || each > AQ || (each > 1 && (nkv <= 0 || each != nh / nkv))) return CW_ERR_BAD_SIZE;
     if (items < 0 || nh <= 0 || nkv <= 0 || nh % nkv != 0 || page_size <= 0 || max_blocks <= 0 || num_pages <= 0 ||
         q_rows <= 0 || q_cols < nh * hd)
         return CW_ERR_BAD_SIZE;
@@ -613,7 +630,16 @@ extern "C" int cw_attention_prefill_tc(const void* q, int q_stride, int q_cols, 
     if (nh > 65535 || items > 65535) return CW_ERR_BAD_SIZE;
     if (load_encode() != 0) return CW_ERR_UNSUPPORTED;
     CUtensorMap mq, mk, mv;
-    {
+    if (each > 1) {
+        const cuuint64_t dims[3] = {(cuuint64_t)hd, (cuuint64_t)nh, (cuuint64_t)q_rows};
+        const cuuint64_t strides[2] = {(cuuint64_t)hd * 2, (cuuint64_t)q_stride * 2};
+        const cuuint32_t box[3] = {64, (cuuint32_t)each, (cuuint32_t)(AQ / each)};
+        const cuuint32_t elem[3] = {1, 1, 1};
+        if (g_encode(&mq, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void*>(q), dims, strides, box, elem,
+                     CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                     CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
+            return CW_ERR_UNSUPPORTED;
+    } else {
         const cuuint64_t dims[2] = {(cuuint64_t)q_cols, (cuuint64_t)q_rows};
         const cuuint64_t strides[1] = {(cuuint64_t)q_stride * 2};
         const cuuint32_t box[2] = {64, AQ};
@@ -655,8 +681,30 @@ extern "C" int cw_attention_prefill_tc(const void* q, int q_stride, int q_cols, 
     p.item_split = item_split; p.part_o = part_o; p.part_ml = part_ml; p.counters = counters;
     p.nh = nh; p.nkv = nkv; p.page_size = page_size; p.page_shift = __builtin_ctz(page_size);
     p.max_blocks = max_blocks; p.num_pages = num_pages;
-    p.scale = scale; p.window = window; p.status = status;
-    return hd == 64 ? launch_prefill_tc<64>(mq, mk, mv, p, items, stream) : launch_prefill_tc<128>(mq, mk, mv, p, items, stream);
+    p.scale = scale; p.window = window; p.status = status; p.each = each;
+    if (each > 1) return hd == 64 ? launch_prefill_tc<64, true>(mq, mk, mv, p, items, stream) : launch_prefill_tc<128, true>(mq, mk, mv, p, items, stream);
+    return hd == 64 ? launch_prefill_tc<64, false>(mq, mk, mv, p, items, stream) : launch_prefill_tc<128, false>(mq, mk, mv, p, items, stream);
+}
+
+extern "C" int cw_attention_prefill_tc(const void* q, int q_stride, int q_cols, int q_rows, void* out,
+                                       const void* k_cache, const void* v_cache, const int* block_tables,
+                                       const int* q_start, const int* ctx_lens, const int* item_seq,
+                                       const int* item_q0, const int* item_split, float* part_o, float* part_ml,
+                                       int* counters, int items, int nh, int nkv, int hd, int page_size,
+                                       int max_blocks, int num_pages, float scale, int window, int* status,
+                                       cudaStream_t stream) {
+    return prefill_tc(q, q_stride, q_cols, q_rows, out, k_cache, v_cache, block_tables, q_start, ctx_lens, item_seq, item_q0, item_split, part_o,
+                      part_ml, counters, items, nh, nkv, hd, page_size, max_blocks, num_pages, scale, window, 1, status, stream);
+}
+extern "C" int cw_attention_prefill_tc_packed(const void* q, int q_stride, int q_cols, int q_rows, void* out,
+                                              const void* k_cache, const void* v_cache, const int* block_tables,
+                                              const int* q_start, const int* ctx_lens, const int* item_seq,
+                                              const int* item_q0, const int* item_split, float* part_o, float* part_ml,
+                                              int* counters, int items, int nh, int nkv, int hd, int page_size,
+                                              int max_blocks, int num_pages, float scale, int window, int each, int* status,
+                                              cudaStream_t stream) {
+    return prefill_tc(q, q_stride, q_cols, q_rows, out, k_cache, v_cache, block_tables, q_start, ctx_lens, item_seq, item_q0, item_split, part_o,
+                      part_ml, counters, items, nh, nkv, hd, page_size, max_blocks, num_pages, scale, window, each, status, stream);
 }
 
 CW_TRACE_TU(attention_prefill_tc)

@@ -45,6 +45,8 @@ def _configure() -> None:
     lib.cw_attention_prefill.restype = c_int
     lib.cw_attention_prefill_tc.argtypes = [P, I, I, I, P, P, P, P, P, P, P, P, P, P, P, P, I, I, I, I, I, I, I, F, I, P, P]
     lib.cw_attention_prefill_tc.restype = c_int
+    lib.cw_attention_prefill_tc_packed.argtypes = [P, I, I, I, P, P, P, P, P, P, P, P, P, P, P, P, I, I, I, I, I, I, I, F, I, I, P, P]
+    lib.cw_attention_prefill_tc_packed.restype = c_int
     _configured = True
 
 
@@ -281,7 +283,8 @@ MAX_PARTS = 8                   # (the kernel's limit)
 
 
 def prefill_work_items(q_lens, ctx_lens, num_heads: int = 0, sm_count: int = 0,
-                       skip_single: bool = False, max_items: int | None = None) -> tuple[list[int], list[int], list[int]]:
+                       skip_single: bool = False, max_items: int | None = None,
+                       tile: int = QUERY_TILE) -> tuple[list[int], list[int], list[int]]:
     """Work items of a step's portions: (request index, first query row, split word) per 128 query rows,
     longest first (CTAs are handed to SMs in this order, so the short ones fill the tail).
 
@@ -291,13 +294,16 @@ def prefill_work_items(q_lens, ctx_lens, num_heads: int = 0, sm_count: int = 0,
     (a CTA costs several microseconds besides its keys, so a second round of CTAs would cost more
     than it saves).  A step with more tiles x heads than SMs has its rows cut when that evens out the
     rounds of CTAs (``_cut_for_even_rounds``; never more than ``max_items`` items then).  A part's item repeats its tile's (request, row); the split
-    word is (index of the tile's first item) << 8 | parts."""
+    word is (index of the tile's first item) << 8 | parts.
+
+    ``tile``: rows per tile; fewer than 128 where a tile's rows are the query heads of a KV head for that many tokens (``num_heads`` is
+    then the number of KV heads)."""
     groups = []  # [keys the tile's last row sees, request, first row, parts]
     for s, (n, c) in enumerate(zip(q_lens, ctx_lens)):
         if skip_single and n == 1:
             continue  # (requests that bring a single token are the decode kernel's)
-        for q0 in range(0, n, QUERY_TILE):
-            groups.append([c - n + min(q0 + QUERY_TILE, n), s, q0, 1])
+        for q0 in range(0, n, tile):
+            groups.append([c - n + min(q0 + tile, n), s, q0, 1])
     if num_heads > 0 and sm_count > 0 and groups:
         room = sm_count // num_heads - len(groups)  # items that can be added within one round of CTAs
         while room > 0:
@@ -590,13 +596,22 @@ def attention_prefill(q, k_cache, v_cache, block_tables, q_start, ctx_lens, item
 
 
 def launch_prefill(q, k_cache, v_cache, block_tables, q_start, ctx_lens, item_seq, item_q0, items, num_heads, num_kv_heads, head_dim, scale,
-                   window, status, use_tc, item_split, out) -> None:
-    """The launch of ``attention_prefill``, its arguments as that has checked them."""
+                   window, status, use_tc, item_split, out, each: int = 1) -> None:
+    """The launch of ``attention_prefill``, its arguments as that has checked them.  ``each``: the query heads of a KV head, packed
+    into the tiles' rows (tcgen05 kernel; the items are then those of tiles of 128 // each tokens)."""
     _configure()
     if use_tc:
         st = {"part_o": None, "part_ml": None, "counters": None}
         if item_split is not None:
             st = _prefill_scratch(q.device, items, num_heads, head_dim)
+        if each > 1:
+            check(library().cw_attention_prefill_tc_packed(
+                _ptr(q), q.stride(0), q.shape[1], q.shape[0], _ptr(out), _ptr(k_cache), _ptr(v_cache), _ptr(block_tables),
+                _ptr(q_start), _ptr(ctx_lens), _ptr(item_seq), _ptr(item_q0), _ptr(item_split), _ptr(st["part_o"]),
+                _ptr(st["part_ml"]), _ptr(st["counters"]), items, num_heads, num_kv_heads, head_dim,
+                k_cache.shape[1], block_tables.shape[1], k_cache.shape[0], float(scale), int(window or 0), each, _ptr(status),
+                _stream()), "attention_prefill_tc_packed")
+            return
         check(library().cw_attention_prefill_tc(
             _ptr(q), q.stride(0), q.shape[1], q.shape[0], _ptr(out), _ptr(k_cache), _ptr(v_cache), _ptr(block_tables),
             _ptr(q_start), _ptr(ctx_lens), _ptr(item_seq), _ptr(item_q0), _ptr(item_split), _ptr(st["part_o"]),

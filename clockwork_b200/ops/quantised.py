@@ -360,6 +360,7 @@ class PortionPlan(NamedTuple):
     least_rows: int
     most_rows: int
     items: int           # work items of the others
+    each: int            # query heads that share their tiles' rows
     item_seq: torch.Tensor
     item_q0: torch.Tensor
     item_split: torch.Tensor | None
@@ -368,10 +369,10 @@ class PortionPlan(NamedTuple):
 
 
 def plan_portions(q_lens, ctx_lens, num_heads: int, num_kv_heads: int, head_dim: int, page_size: int, device,
-                  most_rows: int | None = None, least_rows: int = 1) -> PortionPlan:
+                  most_rows: int | None = None, least_rows: int = 1, packed: bool | None = None) -> PortionPlan:
     """``q_lens``: the rows that each request brings; ``ctx_lens``: its tokens in the cache with them (both on the host).
     ``most_rows``: see ``short_rows``, which decides by default.  bfloat16 requests that bring fewer than ``least_rows`` rows are
-    left alone."""
+    left alone.  ``packed``: whether the query heads of a KV head share the longer portions' tiles (default: where that leaves fewer of them)."""
     from . import attention_fast as fast
 
     q_lens, ctx_lens = tuple(int(n) for n in q_lens), tuple(int(c) for c in ctx_lens)
@@ -380,9 +381,20 @@ def plan_portions(q_lens, ctx_lens, num_heads: int, num_kv_heads: int, head_dim:
     if most_rows is None:
         most_rows = short_rows(num_heads, num_kv_heads, head_dim)
     short = sum(n for n in q_lens if least_rows <= n <= most_rows)
-    cuts = fast._cuts_for(num_heads, head_dim, page_size)
-    seqs, q0s, words = fast.prefill_work_items([n if n > max(most_rows, least_rows - 1) else 0 for n in q_lens], ctx_lens, cuts,
-                                               fast._sm_count(torch.device(device)) if cuts else 0)
+    long = [n if n > max(most_rows, least_rows - 1) else 0 for n in q_lens]
+    each = num_heads // num_kv_heads
+    if not 1 < each <= fast.QUERY_TILE or not fast.prefill_tc_takes(head_dim, page_size):
+        each = 1
+    # Packed where that leaves fewer tiles (measured, us, a head to a tile and packed: 17, 33, 60 and 100 rows behind 2,000, 40 heads over 8
+    # 65.5 and 43.1, 28 over 4 37.4 and 30.8; 1,003, 64 and 200 rows, 40 over 8 318 and 304; 2,048 rows behind 30,000, 12 over 2, where
+    # packing only moves the cuts, 412 and 552)
+    tiles = [sum(-(-n // t) for n in long) for t in (fast.QUERY_TILE, fast.QUERY_TILE // each)]
+    if packed is None:
+        packed = num_kv_heads * tiles[1] <= 0.95 * num_heads * tiles[0]
+    each = each if packed else 1
+    cuts = fast._cuts_for(num_kv_heads if each > 1 else num_heads, head_dim, page_size)
+    seqs, q0s, words = fast.prefill_work_items(long, ctx_lens, cuts,
+                                               fast._sm_count(torch.device(device)) if cuts else 0, tile=fast.QUERY_TILE // each)
     lens = np.array(q_lens, dtype=np.int32)
     starts = np.cumsum(lens, dtype=np.int32) - lens
     tok_seq = np.repeat(np.arange(len(lens), dtype=np.int32), lens)
@@ -390,7 +402,7 @@ def plan_portions(q_lens, ctx_lens, num_heads: int, num_kv_heads: int, head_dim:
     n, rows = len(seqs), len(tok_seq)
     dev = torch.from_numpy(np.concatenate([np.array(seqs + q0s + words, dtype=np.int32), tok_seq, positions])).to(device)
     cut = any(w & 0xFF != 1 for w in words)
-    return PortionPlan(q_lens, ctx_lens, short, least_rows, most_rows, n, dev[:n], dev[n : 2 * n], dev[2 * n : 3 * n] if cut else None,
+    return PortionPlan(q_lens, ctx_lens, short, least_rows, most_rows, n, each, dev[:n], dev[n : 2 * n], dev[2 * n : 3 * n] if cut else None,
                        dev[3 * n : 3 * n + rows], dev[3 * n + rows :])
 
 
@@ -460,7 +472,7 @@ def attention_portions(q: torch.Tensor, cache: E4M3Pages, block_tables: torch.Te
             held = portion_scratch(cache, q.dtype)
             _read_call(cache, shape, block_tables, ctx_lens, q_start, held.k, held.v, window, max(plan.most_rows + 1, plan.least_rows), code, status)
             fast.launch_prefill(q, held.k, held.v, block_tables, q_start, ctx_lens, plan.item_seq, plan.item_q0, plan.items, num_heads, nkv, hd,
-                                scale, window, status, fast.prefill_tc_takes(hd, page_size), plan.item_split, out)
+                                scale, window, status, fast.prefill_tc_takes(hd, page_size), plan.item_split, out, plan.each)
         if plan.short:
             _short_call(q, out, cache, block_tables, ctx_lens, q_start, num_heads, shape, scale, window, plan.short, plan.least_rows, plan.most_rows, status,
                         index, workspace)

@@ -133,13 +133,15 @@ PORTIONS = [  # heads, rows of each request, tokens behind them, page size, wind
     ((12, 2, 128), [130], [0], 16, None), ((12, 2, 128), [64, 1, 200], [300, 40, 0], 16, None), ((4, 4, 64), [150, 0, 7], [0, 9, 1000], 8, 60),
     ((4, 2, 16), [33], [12], 4, None), ((6, 2, 96), [20, 50], [5, 0], 16, None), ((2, 1, 256), [40], [77], 16, None),
     ((28, 4, 128), [5, 17, 2], [3000, 0, 64], 16, None), ((9, 3, 32), [11, 100], [70, 31], 7, 20), ((16, 16, 64), [2] * 40, [90] * 40, 16, None),
-    ((70, 2, 64), [3, 40], [200, 1], 16, None), ((4, 1, 128), [60, 1, 61], [2000, 500, 4000], 64, 700), ((40, 8, 128), [16], [5000], 16, None)]
+    ((70, 2, 64), [3, 40], [200, 1], 16, None), ((12, 2, 128), [300, 22], [3000, 9000], 16, None), ((14, 2, 64), [18, 19, 37], [1000, 0, 64], 8, 130), ((4, 1, 128), [60, 1, 61], [2000, 500, 4000], 64, 700), ((40, 8, 128), [16], [5000], 16, None)]
 
 
-@pytest.mark.parametrize("dtype, most", [(torch.bfloat16, None), (torch.bfloat16, 0), (torch.bfloat16, 10000), (torch.float32, None)])
+@pytest.mark.parametrize("dtype, most, packed", [(torch.bfloat16, None, None), (torch.bfloat16, 0, False), (torch.bfloat16, 0, True),
+                                                 (torch.bfloat16, 10000, None), (torch.float32, None, None)])
 @pytest.mark.parametrize("heads, new, behind, page, window", PORTIONS)
-def test_portions(heads, new, behind, page, window, dtype, most):
-    """``most``: requests of up to so many rows straight from the codes (None: as the operator chooses)."""
+def test_portions(heads, new, behind, page, window, dtype, most, packed):
+    """``most``: requests of up to so many rows straight from the codes (None: as the operator chooses); ``packed``: the heads of a KV
+    head in the tiles of the others, or a head to a tile."""
     nh, nkv, hd = heads
     if most and hd not in quantised.SHORT_HEAD_DIMS:
         pytest.skip("this head size is read back")
@@ -149,7 +151,7 @@ def test_portions(heads, new, behind, page, window, dtype, most):
     starts = [sum(new[:i]) for i in range(len(new) + 1)]
     q = torch.randn(starts[-1] + 2, nh * hd, generator=g).to(dtype)  # (two rows behind the last request's)
     status = ops.new_status(DEV)
-    plan = quantised.plan_portions(new, ctx, nh, nkv, hd, page, torch.device(DEV), most_rows=most)
+    plan = quantised.plan_portions(new, ctx, nh, nkv, hd, page, torch.device(DEV), most_rows=most, packed=packed)
     out = quantised.attention_portions(q.to(DEV), quantised.E4M3Pages(*_on(*cache)),
                                        *_on(tables, torch.tensor(starts, dtype=torch.int32), torch.tensor(ctx, dtype=torch.int32)), plan, nh,
                                        hd**-0.5, status, window=window)

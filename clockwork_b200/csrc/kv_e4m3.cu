@@ -4,9 +4,9 @@
 //     q, k:  x <- x * rsqrt(mean(x^2) + eps) * w        (where the layer norms its heads)
 //            (x_j, x_{j + rot/2}) turned by position * inv_freq[j], j < rot/2
 // q is rounded once to the run's type and handed on; k (float32, not rounded before) and v become rows of the cache: 8-bit rows
-// (kv_e4m3.cuh) or rows of the run's type.  The angle is position * inv_freq as a product of two floats with its rounding error
-// made good: sin(p + e) = sin p (1 - e^2/2) + e cos p with p + e the exact product, |e| <= 2^-24 p, so that a position of a million is
-// still turned to a few 2^-24.
+// (kv_e4m3.cuh) or rows of the run's type.  Angles, their sines and cosines are worked out in float64 and
+// rounded once: position * inv_freq is exact there, so that a position of a million is turned as exactly as the first, and a key's
+// last bits, which decide between two codes, are not the sine's.  (An angle serves all heads: 64 of them beside 4,608 entries.)
 //
 // read_pages: code * 2^(E - 127) in bfloat16 (exact) or float32 for the positions of every request's context, at the same page
 // and slot of a plain cache; the rest of a request's last page becomes zero.  Both are streams over memory.
@@ -22,13 +22,18 @@ struct StoreParams {
     int* status;
 };
 
-__device__ __forceinline__ void turn_of(float position, float freq, float& sn, float& cs) {
-    const float p = position * freq, e = fmaf(position, freq, -p);
-    float s, c;
-    sincosf(p, &s, &c);
-    const float less = 1.f - 0.5f * e * e;
-    sn = s * less + c * e;
-    cs = c * less - s * e;
+// sin and cos of position * freq (a product that float64 holds exactly), rounded once: the angle less the nearest multiple k of pi/2,
+// which leaves |x| <= pi/4, then the Taylor sums to x^11 and x^10 (the next terms are below 2^-33), turned by k quarters.
+__device__ __forceinline__ void turn_of(int position, float freq, float& sn, float& cs) {
+    const double angle = (double)position * (double)freq, k = rint(angle * 0.63661977236758134308);
+    // pi/2 as a float64 and what that leaves of it
+    const double x = fma(-k, 6.123233995736766e-17, fma(-k, 1.5707963267948966, angle)), y = x * x;
+    const double s = x * fma(y, fma(y, fma(y, fma(y, fma(y, -1.0 / 39916800, 1.0 / 362880), -1.0 / 5040), 1.0 / 120), -1.0 / 6), 1.0);
+    const double c = fma(y, fma(y, fma(y, fma(y, fma(y, -1.0 / 3628800, 1.0 / 40320), -1.0 / 720), 1.0 / 24), -0.5), 1.0);
+    const int quarter = (int)((long long)k & 3);
+    const float a = (float)(quarter & 1 ? c : s), b = (float)(quarter & 1 ? s : c);
+    sn = quarter & 2 ? -a : a;
+    cs = (quarter == 1 || quarter == 2) ? -b : b;
 }
 
 // LG neighbouring lanes hold a head, a lane two octets of it (octet i, i < rot / 8: four entries and the four that turn with them;
@@ -80,7 +85,7 @@ __global__ void __launch_bounds__(512) norm_rotate_store_kernel(const StoreParam
     }
     for (int i = threadIdx.x; i < tokens * half; i += blockDim.x) {
         const int t = i / half, j = i - t * half;
-        turn_of((float)p.positions[t0 + t], p.inv_freq[j], turn[t * p.rot + half + j], turn[t * p.rot + j]);
+        turn_of(p.positions[t0 + t], p.inv_freq[j], turn[t * p.rot + half + j], turn[t * p.rot + j]);
     }
     const float* weight = is_v ? nullptr : is_q ? p.q_weight : p.k_weight;
     float4 wa[2], wb[2];
@@ -91,7 +96,6 @@ __global__ void __launch_bounds__(512) norm_rotate_store_kernel(const StoreParam
                 wa[e] = *reinterpret_cast<const float4*>(weight + a_at[e]);
                 wb[e] = *reinterpret_cast<const float4*>(weight + b_at[e]);
             }
-    const float per_entry = 1.f / (float)p.hd;
     const bool any_norm = __any_sync(0xffffffffu, live && weight != nullptr), any_kv = __any_sync(0xffffffffu, live && !is_q);
     const int kvh = is_v ? head - p.nh - p.nkv : head - p.nh;
     __syncthreads();
@@ -108,7 +112,7 @@ __global__ void __launch_bounds__(512) norm_rotate_store_kernel(const StoreParam
 #pragma unroll
             for (int o = LG / 2; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
             if (weight != nullptr) {
-                const float r = rsqrtf(fmaf(sum, per_entry, p.eps));
+                const float r = __frcp_rn(__fsqrt_rn(__fdiv_rn(sum, (float)p.hd) + p.eps));
 #pragma unroll
                 for (int e = 0; e < 2; ++e)
                     if (there[e]) {
@@ -175,7 +179,7 @@ __global__ void norm_rotate_store_any_kernel(const StoreParams p) {
     extern __shared__ float turn[];
     pdl_enter();
     const int t = blockIdx.x, half = p.rot >> 1, lane = threadIdx.x & 31;
-    const float pos = (float)p.positions[t];
+    const int pos = p.positions[t];
     for (int j = threadIdx.x; j < half; j += blockDim.x) turn_of(pos, p.inv_freq[j], turn[half + j], turn[j]);
     int slot = p.slots[t];
     if (slot >= p.num_slots) {
@@ -193,7 +197,7 @@ __global__ void norm_rotate_store_any_kernel(const StoreParams p) {
         if (weight != nullptr) {
             float sum = 0.f;
             for (int j = lane; j < p.hd; j += 32) sum += to_f(x[j]) * to_f(x[j]);
-            r = rsqrtf(warp_sum(sum) / (float)p.hd + p.eps);
+            r = __frcp_rn(__fsqrt_rn(__fdiv_rn(warp_sum(sum), (float)p.hd) + p.eps));
         }
         auto normed = [&](int j) { return weight != nullptr ? to_f(x[j]) * (r * weight[j]) : to_f(x[j]); };
         auto entry = [&](int j) {

@@ -131,17 +131,18 @@ def test_only_one_of_the_norms_and_unaligned_rows():
     ops.raise_on_status(status)
 
 
-def test_far_positions_are_turned_exactly():
-    """Positions of a million: float32 angles would be off by hundredths of a radian."""
+@pytest.mark.parametrize("top", [64, 1 << 20, (1 << 31) - 1])
+def test_far_positions_are_turned_exactly(top):
+    """Positions of a million and a billion: float32 angles would be off by hundredths of a radian, and by many turns."""
     g = torch.Generator().manual_seed(4)
-    qkv, pos, slots, freq, _ = _inputs((4, 2, 128), 64, torch.float32, 128, False, g, 16, 5, pos_top=1 << 20)
+    qkv, pos, slots, freq, _ = _inputs((4, 2, 128), 64, torch.float32, 128, False, g, 16, 5, pos_top=top)
     cache = _cache("plain", torch.float32, 5, 16, 2, 128)
     status = ops.new_status(DEV)
     q = quantised.norm_rotate_store(qkv.to(DEV), *_on(pos, slots, freq), cache, 4, 2, 128, status)
     want, off = _exact_rows(qkv.view(64, 8, 128)[:, :4], None, 0.0, pos, freq)
-    # (the error of the product, up to 2^-4 of a radian here, is made good up to its third power: 2^-12 / 6 at the very most
-    # where position * freq is near a million; freq 1 is exact and the next is 0.87, whose product's error is 2^-5: 2^-15 / 6 < 2^-17)
-    assert ((q.double().cpu().view(64, 4, 128) - want).abs() <= 2.0**-24 * want.abs() + off + 2.0**-17 * want.abs().amax(-1, keepdim=True)).all()
+    # (both sides' angles are off by float64's last bit at most: 2^-53 of 2^31, 2^-22, here and there, for the farthest)
+    far = 2.0**-21 if top > 1 << 20 else 2.0**-32
+    assert ((q.double().cpu().view(64, 4, 128) - want).abs() <= 2.0**-24 * want.abs() + off + far * want.abs().amax(-1, keepdim=True)).all()
 
 
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])

@@ -37,6 +37,7 @@ struct DecodeE4m3Params {
     int requests, nh, nkv, hd, page_size, max_blocks, num_pages, window;
     float scale;
     int* status;
+    int early;               // lengths, tables and all of the cache but the newest tokens' rows are older than the kernel in front
     // the streaming kernel
     int page_shift;          // log2 of the page size, or -1
     int teams;               // KV heads that long walks take side by side
@@ -139,9 +140,17 @@ __global__ void __launch_bounds__(WARPS * 32, Stream<HD, NT>::PER_SM) decode_e4m
     __shared__ float top_s[2 * WARPS][ROWS], total_s[2 * WARPS][ROWS];  // of a group of pieces, at its first
     __shared__ int limit_s[WARPS][PORTIONS ? ROWS : 1];
     __shared__ int shared_s[2 * MOST_TEAMS], last_s[2 * MOST_TEAMS], final_s;
-    pdl_enter();
+    // (early: what the kernel in front writes, queries and the newest rows, is waited for only where it is first needed)
+    bool waited = PORTIONS || !p.early;
+    if (waited)
+        pdl_enter();
+    else
+        pdl_launch_dependents();
+    auto wait = [&]() {
+        if (!waited) pdl_wait();
+        waited = true;
+    };
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
-
     const int each = p.nh / p.nkv;  // query heads of a KV head
     auto tokens_of = [&](int s) -> int {  // that request s brings; 0: it is not served here
         if (!PORTIONS) return p.q_start == nullptr || p.q_start[s + 1] - p.q_start[s] == 1 ? 1 : 0;
@@ -196,6 +205,7 @@ __global__ void __launch_bounds__(WARPS * 32, Stream<HD, NT>::PER_SM) decode_e4m
         }
     };
     if ((long long)blockIdx.x * block_units >= total) {
+        wait();
         zeros();
         return;
     }
@@ -310,6 +320,7 @@ __global__ void __launch_bounds__(WARPS * 32, Stream<HD, NT>::PER_SM) decode_e4m
     };
     auto fetch = [&]() {
         if (ahead.left > 0) {
+            if (ahead.tile == ahead.tiles - 1) wait();  // (the request's newest row is in this tile)
             const int kvh = kv_head(ahead);
 #pragma unroll
             for (int h = 0; h < HALVES; ++h) {
@@ -342,7 +353,10 @@ __global__ void __launch_bounds__(WARPS * 32, Stream<HD, NT>::PER_SM) decode_e4m
             if (++fetch_stage == ST) fetch_stage = 0;
             const bool other = step(ahead, 1);
             look_up();
-            if (other) call_queries(ahead);
+            if (other) {
+                wait();
+                call_queries(ahead);
+            }
         }
         cp_async_commit();
     };
@@ -359,10 +373,11 @@ __global__ void __launch_bounds__(WARPS * 32, Stream<HD, NT>::PER_SM) decode_e4m
         }
     };
     look_up();
-    if (at.left > 0) call_queries(at);
+    if (at.left > 0 && waited) call_queries(at);
 #pragma unroll 1
     for (int i = 0; i < ST - 1; ++i) fetch();
     __syncwarp();
+    wait();
     int stage = 0;
     if (at.left > 0) look_at_powers(0);
     if (lane < 2) piece_s[2 * warp + lane].segment = -1;
@@ -938,7 +953,8 @@ extern "C" int cw_attention_decode_e4m3(const char* block) {
     int *words = (int*)w.pointer(), *status = (int*)w.pointer();
     const cudaStream_t stream = (cudaStream_t)w.pointer();
     const int q_stride = w.number(), requests = w.number(), nh = w.number(), nkv = w.number(), hd = w.number(), page_size = w.number(),
-              max_blocks = w.number(), num_pages = w.number(), window = w.number(), dtype = w.number(), sms = w.number();
+              max_blocks = w.number(), num_pages = w.number(), window = w.number(), dtype = w.number(), sms = w.number(),
+              early = w.number();
     const float scale = (float)w.real();
     if (requests == 0) return CW_OK;
     if (requests < 0 || nh <= 0 || nkv <= 0 || nh % nkv || hd <= 0 || hd % 16 || hd > 256 || page_size <= 0 || max_blocks <= 0 ||
@@ -947,6 +963,7 @@ extern "C" int cw_attention_decode_e4m3(const char* block) {
         return CW_ERR_BAD_SIZE;
     DecodeE4m3Params p = {q, q_stride, out, k, v, k_exp, v_exp, block_tables, ctx_lens, q_start, requests, nh, nkv, hd, page_size,
                           max_blocks, num_pages, window, scale, status};
+    p.early = early;
     const int groups = groups_of(nh, nkv, hd, dtype);
     if (groups && streams(p, (long long)requests * groups, sms, floats, words)) {
         p.groups = groups;

@@ -19,6 +19,7 @@ struct StoreParams {
     void* k_cache; void* v_cache; uint8_t* k_exp; uint8_t* v_exp;  // k_exp null: a plain cache
     int N, nh, nkv, hd, rot, page_size, num_slots;
     float eps;
+    int early;  // positions, slots and frequencies are older than the kernel in front: angles are worked out while that one finishes
     int* status;
 };
 
@@ -46,7 +47,10 @@ template <typename T, int LG>
 __global__ void __launch_bounds__(512) norm_rotate_store_kernel(const StoreParams p, int most_tokens, int block_heads) {
     extern __shared__ float turn[];  // per token: cos[rot / 2], sin[rot / 2]
     __shared__ int slot_s[STORE_TOKENS], off_s[STORE_TOKENS];  // a token's slot (-1: none) and its place in its page
-    pdl_enter();
+    if (p.early)
+        pdl_launch_dependents();
+    else
+        pdl_enter();
     const int t0 = blockIdx.x * most_tokens, tokens = min(most_tokens, p.N - t0), half = p.rot >> 1;
     const int heads = p.nh + 2 * p.nkv, l = threadIdx.x % LG, turning = p.rot >> 3;
     const int own = threadIdx.x / LG, head = blockIdx.y * block_heads + own;
@@ -73,7 +77,7 @@ __global__ void __launch_bounds__(512) norm_rotate_store_kernel(const StoreParam
             }
         row += (size_t)heads * p.hd;
     };
-    load();
+    if (!p.early) load();
     if (threadIdx.x < tokens) {
         int slot = p.slots[t0 + threadIdx.x];
         if (slot >= p.num_slots) {
@@ -98,6 +102,10 @@ __global__ void __launch_bounds__(512) norm_rotate_store_kernel(const StoreParam
             }
     const bool any_norm = __any_sync(0xffffffffu, live && weight != nullptr), any_kv = __any_sync(0xffffffffu, live && !is_q);
     const int kvh = is_v ? head - p.nh - p.nkv : head - p.nh;
+    if (p.early) {
+        pdl_wait();
+        load();
+    }
     __syncthreads();
     for (int t = 0; t < tokens; ++t) {
         float4 a[2] = {a_next[0], a_next[1]}, b[2] = {b_next[0], b_next[1]};
@@ -264,14 +272,14 @@ extern "C" int cw_norm_rotate_store(const char* block) {
     int* status = (int*)w.pointer();
     const cudaStream_t stream = (cudaStream_t)w.pointer();
     const int N = w.number(), nh = w.number(), nkv = w.number(), hd = w.number(), rot = w.number(), page_size = w.number(), num_pages = w.number(),
-              dtype = w.number();
+              dtype = w.number(), early = w.number();
     const float eps = (float)w.real();
     if (N == 0) return CW_OK;
     if (N < 0 || nh <= 0 || nkv <= 0 || hd <= 0 || hd > 256 || rot < 0 || rot > hd || rot % 2 || page_size <= 0 || num_pages <= 0 ||
         (long long)num_pages * page_size > 0x7FFFFFFF || (rot > 0 && inv_freq == nullptr) || (k_exp == nullptr) != (v_exp == nullptr))
         return CW_ERR_BAD_SIZE;
     const StoreParams p = {qkv, q_out, positions, slots, inv_freq, q_weight, k_weight, k_cache, v_cache, k_exp, v_exp,
-                           N, nh, nkv, hd, rot, page_size, num_pages * page_size, eps, status};
+                           N, nh, nkv, hd, rot, page_size, num_pages * page_size, eps, early, status};
     if (dtype == 0) return store_launch<float>(p, N, stream);
     if (dtype == 1) return store_launch<bf16>(p, N, stream);
     return CW_ERR_BAD_DTYPE;

@@ -24,9 +24,9 @@ from .library import check, library
 
 # The entry points of this module take one block of words (pointers and whole numbers, then the floats), which costs a third of what
 # as many ctypes arguments do: 2 of 5 us of a call whose kernel may take 4.
-_STORE_ARGS = struct.Struct("21qd").pack
+_STORE_ARGS = struct.Struct("22qd").pack
 _READ_ARGS = struct.Struct("21q").pack
-_DECODE_ARGS = struct.Struct("24qd").pack
+_DECODE_ARGS = struct.Struct("25qd").pack
 _PORTION_ARGS = struct.Struct("26qd").pack
 
 CODES = torch.float8_e4m3fn
@@ -117,7 +117,8 @@ def _check_rows(qkv: torch.Tensor, num_heads: int, num_kv_heads: int, head_dim: 
     return qkv.shape[0]
 
 
-def _store_call(qkv, n, positions, slots, inv_freq, cache, num_heads, num_kv_heads, head_dim, status, code, q_weight, k_weight, eps):
+def _store_call(qkv, n, positions, slots, inv_freq, cache, num_heads, num_kv_heads, head_dim, status, code, q_weight, k_weight, eps,
+                early=False):
     """The rest of ``norm_rotate_store``'s checks: (q, the entry point's words, the cache's shape, the device)."""
     _ints(positions, "positions", 1, n)
     _ints(slots, "slots", 1, n)
@@ -151,20 +152,25 @@ def _store_call(qkv, n, positions, slots, inv_freq, cache, num_heads, num_kv_hea
         qkv.data_ptr(), q.data_ptr(), positions.data_ptr(), slots.data_ptr(), inv_freq.data_ptr() if rot else 0,
         0 if q_weight is None else q_weight.data_ptr(), 0 if k_weight is None else k_weight.data_ptr(), cache.k.data_ptr(), cache.v.data_ptr(),
         cache.k_exp.data_ptr() if quantised else 0, cache.v_exp.data_ptr() if quantised else 0, status.data_ptr(), _stream(), n, num_heads,
-        num_kv_heads, head_dim, rot, shape[1], shape[0], code, eps)
+        num_kv_heads, head_dim, rot, shape[1], shape[0], code, early, eps)
     return q, words, shape, index
 
 
 def norm_rotate_store(qkv: torch.Tensor, positions: torch.Tensor, slots: torch.Tensor, inv_freq: torch.Tensor | None, cache,
                       num_heads: int, num_kv_heads: int, head_dim: int, status: torch.Tensor, *,
-                      q_weight: torch.Tensor | None = None, k_weight: torch.Tensor | None = None, eps: float = 0.0) -> torch.Tensor:
+                      q_weight: torch.Tensor | None = None, k_weight: torch.Tensor | None = None, eps: float = 0.0,
+                      early: bool = False) -> torch.Tensor:
     """What lies between the [q | k | v] product and attention, in one pass: ``qkv`` [N, (nh + 2 nkv) hd] (float32 or bfloat16;
     left as it is), RMS norms of every query and key head with float32 ``q_weight``, ``k_weight`` [hd] (None: not normed), the
     rotation of each head's leading ``2 * len(inv_freq)`` entries by ``positions`` (None: none turn; entry j pairs with
     j + len(inv_freq)), and the write of k and v at ``slots`` (< 0: not stored) of ``cache`` (``E4M3Pages``, or ``PlainPages``
-    of qkv's type).  Returns q [N, nh * hd].  Everything up to the one rounding of each output is float32."""
+    of qkv's type).  Returns q [N, nh * hd].  Everything up to the one rounding of each output is float32.
+
+    ``early``: a promise that ``positions``, ``slots`` and ``inv_freq`` were complete before the kernel in front of this call was
+    launched, as a step's inputs are; the call then begins while that kernel finishes."""
     code, n = dtype_code(qkv.dtype), _check_rows(qkv, num_heads, num_kv_heads, head_dim)
-    q, words = _store_call(qkv, n, positions, slots, inv_freq, cache, num_heads, num_kv_heads, head_dim, status, code, q_weight, k_weight, eps)[:2]
+    q, words = _store_call(qkv, n, positions, slots, inv_freq, cache, num_heads, num_kv_heads, head_dim, status, code, q_weight, k_weight, eps,
+                           early)[:2]
     check(library().cw_norm_rotate_store(words), "norm_rotate_store")
     return q
 
@@ -254,7 +260,8 @@ def _workspace(workspace: DecodeWorkspace | None, head_dim: int, index: int, str
     return held
 
 
-def _decode_call(q, out, cache, block_tables, ctx_lens, q_start, num_heads, shape, scale, window, code, status, index, workspace) -> None:
+def _decode_call(q, out, cache, block_tables, ctx_lens, q_start, num_heads, shape, scale, window, code, status, index, workspace,
+                 early=False) -> None:
     pages, page_size, nkv, hd = shape
     s = block_tables.shape[0]
     stream, sms, floats, words = _stream(), _sm_count(index), 0, 0
@@ -265,19 +272,21 @@ def _decode_call(q, out, cache, block_tables, ctx_lens, q_start, num_heads, shap
         q.data_ptr(), out.data_ptr(), cache.k.data_ptr(), cache.v.data_ptr(), cache.k_exp.data_ptr(), cache.v_exp.data_ptr(),
         block_tables.data_ptr(), ctx_lens.data_ptr(), 0 if q_start is None else q_start.data_ptr(), floats, words, status.data_ptr(), stream,
         q.stride(0) if q.shape[0] > 1 else num_heads * hd, s, num_heads, nkv, hd, page_size, block_tables.shape[1], pages, window or 0, code,
-        sms, scale)), "attention_decode_e4m3")
+        sms, early, scale)), "attention_decode_e4m3")
 
 
 def attention_decode(q: torch.Tensor, cache: E4M3Pages, block_tables: torch.Tensor, ctx_lens: torch.Tensor, num_heads: int,
                      scale: float, status: torch.Tensor, *, window: int | None = None, q_start: torch.Tensor | None = None,
-                     out: torch.Tensor | None = None, workspace: DecodeWorkspace | None = None) -> torch.Tensor:
+                     out: torch.Tensor | None = None, workspace: DecodeWorkspace | None = None, early: bool = False) -> torch.Tensor:
     """One query token per request over an 8-bit cache: ``q`` [S, >= nh * hd] (float32 or bfloat16, unit column stride; row s
     belongs to request s), ``ctx_lens`` [S] the tokens of each request in the cache, its own included.  ``window``: a request sees
     its last ``window`` tokens only.  Returns [S, nh * hd]; a request of no tokens gets zeros.
 
     ``q_start`` (int32 [S + 1]) with ``out`` ([N, nh * hd]): the requests are those of a flat batch of N rows that also holds
     prompt portions; only requests with exactly one row are served, the others' rows are left alone.  ``workspace``: the call's scratch (default:
-    one per stream)."""
+    one per stream).  ``early``: a promise that ``ctx_lens``, ``block_tables``, ``q_start`` and all of the cache but the requests' newest rows
+    were complete before the kernel in front of this call was launched, as they are in a step whose inputs were uploaded before
+    it; the call then begins to read while that kernel finishes."""
     code = dtype_code(q.dtype)
     pages, page_size, nkv, hd = check_pages(cache)
     if q.dim() != 2 or q.shape[1] < num_heads * hd or q.stride(1) != 1:
@@ -306,16 +315,16 @@ def attention_decode(q: torch.Tensor, cache: E4M3Pages, block_tables: torch.Tens
     if out is None:
         out = q.new_empty((s, num_heads * hd))
     _decode_call(q, out, cache, block_tables, ctx_lens, q_start, num_heads, (pages, page_size, nkv, hd), scale, window, code, status, index,
-                 workspace)
+                 workspace, early)
     return out
 
 
 def decode_step(qkv: torch.Tensor, positions: torch.Tensor, slots: torch.Tensor, inv_freq: torch.Tensor | None, cache: E4M3Pages,
                 block_tables: torch.Tensor, ctx_lens: torch.Tensor, num_heads: int, num_kv_heads: int, head_dim: int, scale: float,
                 status: torch.Tensor, *, q_weight: torch.Tensor | None = None, k_weight: torch.Tensor | None = None,
-                eps: float = 0.0, window: int | None = None, workspace: DecodeWorkspace | None = None) -> torch.Tensor:
+                eps: float = 0.0, window: int | None = None, workspace: DecodeWorkspace | None = None, early: bool = False) -> torch.Tensor:
     """``norm_rotate_store`` of one new token per request, then ``attention_decode`` of it: what an attention layer does between
-    its two products while every request decodes.  ``ctx_lens`` count the new tokens."""
+    its two products while every request decodes.  ``ctx_lens`` count the new tokens.  ``early``: the promises of both."""
     code, n = dtype_code(qkv.dtype), _check_rows(qkv, num_heads, num_kv_heads, head_dim)
     if not isinstance(cache, E4M3Pages):
         raise ValueError(f"an 8-bit cache (E4M3Pages) is needed, got {type(cache).__name__}")
@@ -326,11 +335,11 @@ def decode_step(qkv: torch.Tensor, positions: torch.Tensor, slots: torch.Tensor,
     if window is not None and window <= 0:
         raise ValueError("window must be positive or None")
     q, words, shape, index = _store_call(qkv, n, positions, slots, inv_freq, cache, num_heads, num_kv_heads, head_dim, status, code, q_weight,
-                                         k_weight, eps)
+                                         k_weight, eps, early)
     _elsewhere(index, block_tables=block_tables, ctx_lens=ctx_lens)
     out = torch.empty_like(q)
     check(library().cw_norm_rotate_store(words), "norm_rotate_store")
-    _decode_call(q, out, cache, block_tables, ctx_lens, None, num_heads, shape, scale, window, code, status, index, workspace)
+    _decode_call(q, out, cache, block_tables, ctx_lens, None, num_heads, shape, scale, window, code, status, index, workspace, early)
     return out
 
 
@@ -515,7 +524,7 @@ def paged_attention(ctx, q: torch.Tensor, cache: E4M3Pages, block_tables: torch.
 
     def singles(out=None):
         return attention_decode(q, cache, block_tables, ctx.ctx_lens, num_heads, scale, ctx.status, window=window,
-                                q_start=None if out is None else ctx.q_start, out=out, workspace=scratch)
+                                q_start=None if out is None else ctx.q_start, out=out, workspace=scratch, early=True)
 
     if ctx.all_single_token:
         return singles()

@@ -134,7 +134,7 @@ class Attention(Mixer):
         cache = quantised.PlainPages(view.k_cache, view.v_cache) if view.k_exp is None else quantised.E4M3Pages(
             view.k_cache, view.v_cache, view.k_exp, view.v_exp)
         q = quantised.norm_rotate_store(qkv, ctx.positions, view.slots, constants[0], cache, nh, nkv, hd, ctx.status, q_weight=self.q_norm,
-                                        k_weight=self.k_norm, eps=self.qk_norm or 0.0)
+                                        k_weight=self.k_norm, eps=self.qk_norm or 0.0, early=True)
         if view.k_exp is None:
             return attention_ops.paged_attention(ctx, q, view, nh, nkv, hd, self.scale, self.window)
         return quantised.paged_attention(ctx, q, cache, view.block_tables, nh, self.scale, self.window)

@@ -28,6 +28,8 @@ _STORE_ARGS = struct.Struct("22qd").pack
 _READ_ARGS = struct.Struct("21q").pack
 _DECODE_ARGS = struct.Struct("25qd").pack
 _PORTION_ARGS = struct.Struct("26qd").pack
+_STEP_ARGS = struct.Struct("26qdd").pack
+_UNSUPPORTED = -3
 
 CODES = torch.float8_e4m3fn
 MAX_HEAD_DIM = 256
@@ -117,9 +119,8 @@ def _check_rows(qkv: torch.Tensor, num_heads: int, num_kv_heads: int, head_dim: 
     return qkv.shape[0]
 
 
-def _store_call(qkv, n, positions, slots, inv_freq, cache, num_heads, num_kv_heads, head_dim, status, code, q_weight, k_weight, eps,
-                early=False):
-    """The rest of ``norm_rotate_store``'s checks: (q, the entry point's words, the cache's shape, the device)."""
+def _check_store(qkv, n, positions, slots, inv_freq, cache, num_kv_heads, head_dim, status, q_weight, k_weight):
+    """What ``norm_rotate_store`` looks at besides its rows; returns the cache's shape."""
     _ints(positions, "positions", 1, n)
     _ints(slots, "slots", 1, n)
     _check_status(status)
@@ -133,27 +134,29 @@ def _store_call(qkv, n, positions, slots, inv_freq, cache, num_heads, num_kv_hea
         shape = cache.k.shape
     if shape[2] != num_kv_heads or shape[3] != head_dim:
         raise ValueError(f"the cache holds {tuple(shape[2:])} KV heads and entries, expected {(num_kv_heads, head_dim)}")
-    rot = 0
     if inv_freq is not None:
         if inv_freq.dtype != torch.float32 or inv_freq.dim() != 1 or not inv_freq.is_contiguous():
             raise ValueError("inv_freq must be a contiguous float32 vector")
-        rot = 2 * inv_freq.shape[0]
-        if rot > head_dim:
-            raise ValueError(f"inv_freq turns {rot} entries of heads of {head_dim}")
+        if 2 * inv_freq.shape[0] > head_dim:
+            raise ValueError(f"inv_freq turns {2 * inv_freq.shape[0]} entries of heads of {head_dim}")
     for name, w in (("q_weight", q_weight), ("k_weight", k_weight)):
         if w is not None and (w.dtype != torch.float32 or tuple(w.shape) != (head_dim,) or not w.is_contiguous()):
             raise ValueError(f"{name} must be contiguous float32 [{head_dim}]")
-    index = qkv.get_device()
-    _elsewhere(index, positions=positions, slots=slots, inv_freq=inv_freq, q_weight=q_weight, k_weight=k_weight, cache=cache.k, values=cache.v,
-               status=status)
-    _check_device(index)
+    _elsewhere(qkv.get_device(), positions=positions, slots=slots, inv_freq=inv_freq, q_weight=q_weight, k_weight=k_weight, cache=cache.k,
+               values=cache.v, status=status)
+    return shape
+
+
+def _store_words(qkv, n, positions, slots, inv_freq, cache, num_heads, num_kv_heads, head_dim, shape, status, code, q_weight, k_weight, eps,
+                 early):
+    """The query rows' tensor and the entry point's words."""
+    quantised, rot = isinstance(cache, E4M3Pages), 0 if inv_freq is None else 2 * inv_freq.shape[0]
     q = qkv.new_empty((n, num_heads * head_dim))
-    words = _STORE_ARGS(
+    return q, _STORE_ARGS(
         qkv.data_ptr(), q.data_ptr(), positions.data_ptr(), slots.data_ptr(), inv_freq.data_ptr() if rot else 0,
         0 if q_weight is None else q_weight.data_ptr(), 0 if k_weight is None else k_weight.data_ptr(), cache.k.data_ptr(), cache.v.data_ptr(),
         cache.k_exp.data_ptr() if quantised else 0, cache.v_exp.data_ptr() if quantised else 0, status.data_ptr(), _stream(), n, num_heads,
         num_kv_heads, head_dim, rot, shape[1], shape[0], code, early, eps)
-    return q, words, shape, index
 
 
 def norm_rotate_store(qkv: torch.Tensor, positions: torch.Tensor, slots: torch.Tensor, inv_freq: torch.Tensor | None, cache,
@@ -169,8 +172,10 @@ def norm_rotate_store(qkv: torch.Tensor, positions: torch.Tensor, slots: torch.T
     ``early``: a promise that ``positions``, ``slots`` and ``inv_freq`` were complete before the kernel in front of this call was
     launched, as a step's inputs are; the call then begins while that kernel finishes."""
     code, n = dtype_code(qkv.dtype), _check_rows(qkv, num_heads, num_kv_heads, head_dim)
-    q, words = _store_call(qkv, n, positions, slots, inv_freq, cache, num_heads, num_kv_heads, head_dim, status, code, q_weight, k_weight, eps,
-                           early)[:2]
+    shape = _check_store(qkv, n, positions, slots, inv_freq, cache, num_kv_heads, head_dim, status, q_weight, k_weight)
+    _check_device(qkv.get_device())
+    q, words = _store_words(qkv, n, positions, slots, inv_freq, cache, num_heads, num_kv_heads, head_dim, shape, status, code, q_weight, k_weight,
+                            eps, early)
     check(library().cw_norm_rotate_store(words), "norm_rotate_store")
     return q
 
@@ -319,12 +324,18 @@ def attention_decode(q: torch.Tensor, cache: E4M3Pages, block_tables: torch.Tens
     return out
 
 
+STEP_HEAD_DIMS = (64, 128, 256)
+
+
 def decode_step(qkv: torch.Tensor, positions: torch.Tensor, slots: torch.Tensor, inv_freq: torch.Tensor | None, cache: E4M3Pages,
                 block_tables: torch.Tensor, ctx_lens: torch.Tensor, num_heads: int, num_kv_heads: int, head_dim: int, scale: float,
                 status: torch.Tensor, *, q_weight: torch.Tensor | None = None, k_weight: torch.Tensor | None = None,
                 eps: float = 0.0, window: int | None = None, workspace: DecodeWorkspace | None = None, early: bool = False) -> torch.Tensor:
-    """``norm_rotate_store`` of one new token per request, then ``attention_decode`` of it: what an attention layer does between
-    its two products while every request decodes.  ``ctx_lens`` count the new tokens.  ``early``: the promises of both."""
+    """``norm_rotate_store`` of one new token per request and ``attention_decode`` of it: what an attention layer does between its two
+    products while every request decodes.  ``slots`` name the places of the new tokens, the last of their requests' ``ctx_lens``, in the
+    block tables (< 0: not stored, and whether it is attended is left open).  ``early``: the promises of both; two kernels run then, each of
+    which begins while the one in front finishes.  Without it one does it all in bfloat16, for heads of 64, 128 and 256 entries that
+    turn whole or not at all."""
     code, n = dtype_code(qkv.dtype), _check_rows(qkv, num_heads, num_kv_heads, head_dim)
     if not isinstance(cache, E4M3Pages):
         raise ValueError(f"an 8-bit cache (E4M3Pages) is needed, got {type(cache).__name__}")
@@ -334,11 +345,26 @@ def decode_step(qkv: torch.Tensor, positions: torch.Tensor, slots: torch.Tensor,
     _ints(ctx_lens, "ctx_lens", 1, n)
     if window is not None and window <= 0:
         raise ValueError("window must be positive or None")
-    q, words, shape, index = _store_call(qkv, n, positions, slots, inv_freq, cache, num_heads, num_kv_heads, head_dim, status, code, q_weight,
-                                         k_weight, eps, early)
+    shape = _check_store(qkv, n, positions, slots, inv_freq, cache, num_kv_heads, head_dim, status, q_weight, k_weight)
+    index = qkv.get_device()
     _elsewhere(index, block_tables=block_tables, ctx_lens=ctx_lens)
-    out = torch.empty_like(q)
+    _check_device(index)
+    if not early and code == 1 and head_dim in STEP_HEAD_DIMS and (inv_freq is None or 2 * inv_freq.shape[0] == head_dim):
+        out, stream = qkv.new_empty((n, num_heads * head_dim)), _stream()
+        scratch = _workspace(workspace, head_dim, index, stream)
+        result = library().cw_decode_step_e4m3(_STEP_ARGS(
+            qkv.data_ptr(), out.data_ptr(), positions.data_ptr(), slots.data_ptr(), 0 if inv_freq is None else inv_freq.data_ptr(),
+            0 if q_weight is None else q_weight.data_ptr(), 0 if k_weight is None else k_weight.data_ptr(), cache.k.data_ptr(), cache.v.data_ptr(),
+            cache.k_exp.data_ptr(), cache.v_exp.data_ptr(), block_tables.data_ptr(), ctx_lens.data_ptr(), scratch.floats.data_ptr(),
+            scratch.words.data_ptr(), status.data_ptr(), stream, n, num_heads, num_kv_heads, head_dim, shape[1], block_tables.shape[1], shape[0],
+            window or 0, _sm_count(index), scale, eps))
+        if result != _UNSUPPORTED:  # (sizes and addresses that only the two kernels take)
+            check(result, "decode_step_e4m3")
+            return out
+    q, words = _store_words(qkv, n, positions, slots, inv_freq, cache, num_heads, num_kv_heads, head_dim, shape, status, code, q_weight, k_weight,
+                            eps, early)
     check(library().cw_norm_rotate_store(words), "norm_rotate_store")
+    out = torch.empty_like(q)
     _decode_call(q, out, cache, block_tables, ctx_lens, None, num_heads, shape, scale, window, code, status, index, workspace, early)
     return out
 
@@ -510,8 +536,8 @@ def step_workspace(head_dim: int, index: int) -> DecodeWorkspace:
 
 def paged_attention(ctx, q: torch.Tensor, cache: E4M3Pages, block_tables: torch.Tensor, num_heads: int, scale: float,
                     window: int | None) -> torch.Tensor:
-    """Attention of a step of the engine over an 8-bit cache that already holds the step's keys and values: single tokens and short
-    portions straight from the codes; longer ones from their requests' pages read back into scratch pages, by the kernels of the
+    """Attention of a step of the engine that brings prompt portions, over an 8-bit cache that already holds the step's keys and
+    values: single tokens and short portions straight from the codes; longer ones from their requests' pages read back into scratch pages, by the kernels of the
     run's type."""
     from . import attention_ref
     from .attention_fast import _Prefill
@@ -522,12 +548,10 @@ def paged_attention(ctx, q: torch.Tensor, cache: E4M3Pages, block_tables: torch.
     streams = q.dtype == torch.bfloat16 and hd % 32 == 0
     scratch = step_workspace(hd, index) if streams else None
 
-    def singles(out=None):
-        return attention_decode(q, cache, block_tables, ctx.ctx_lens, num_heads, scale, ctx.status, window=window,
-                                q_start=None if out is None else ctx.q_start, out=out, workspace=scratch, early=True)
+    def singles(out):
+        return attention_decode(q, cache, block_tables, ctx.ctx_lens, num_heads, scale, ctx.status, window=window, q_start=ctx.q_start,
+                                out=out, workspace=scratch, early=True)
 
-    if ctx.all_single_token:
-        return singles()
     if q.dtype == torch.bfloat16 and _Prefill.accepts(ctx, None, num_heads, nkv, hd, window):
         apart = _Prefill.singles_apart(ctx, hd)
         least = 2 if apart else 1

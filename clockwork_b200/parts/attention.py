@@ -133,8 +133,12 @@ class Attention(Mixer):
             raise ValueError("normed heads and 8-bit caches need a rotation that fits the head and a cache that is written")
         cache = quantised.PlainPages(view.k_cache, view.v_cache) if view.k_exp is None else quantised.E4M3Pages(
             view.k_cache, view.v_cache, view.k_exp, view.v_exp)
-        q = quantised.norm_rotate_store(qkv, ctx.positions, view.slots, constants[0], cache, nh, nkv, hd, ctx.status, q_weight=self.q_norm,
-                                        k_weight=self.k_norm, eps=self.qk_norm or 0.0, early=True)
+        norms = {"q_weight": self.q_norm, "k_weight": self.k_norm, "eps": self.qk_norm or 0.0}
+        if view.k_exp is not None and ctx.all_single_token:
+            return quantised.decode_step(qkv, ctx.positions, view.slots, constants[0], cache, view.block_tables, ctx.ctx_lens, nh, nkv, hd,
+                                         self.scale, ctx.status, window=self.window, early=True, **norms,
+                                         workspace=quantised.step_workspace(hd, qkv.get_device()) if qkv.dtype == torch.bfloat16 and hd % 32 == 0 else None)
+        q = quantised.norm_rotate_store(qkv, ctx.positions, view.slots, constants[0], cache, nh, nkv, hd, ctx.status, early=True, **norms)
         if view.k_exp is None:
             return attention_ops.paged_attention(ctx, q, view, nh, nkv, hd, self.scale, self.window)
         return quantised.paged_attention(ctx, q, cache, view.block_tables, nh, self.scale, self.window)

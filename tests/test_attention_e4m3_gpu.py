@@ -5,7 +5,7 @@ import torch
 
 from clockwork_b200 import ops
 from clockwork_b200.ops import quantised
-from tests.e4m3_tools import attention, attention_bound, context, filled_pages
+from tests.e4m3_tools import CODES, attention, attention_bound, context, filled_pages
 from tests.gpu_tools import DEV
 
 pytestmark = pytest.mark.gpu
@@ -126,6 +126,106 @@ def test_decode_reports_pages_outside_the_pool():
                                      *_on(tables, torch.tensor([100, 60], dtype=torch.int32)), 1, 0.1, status)
     assert out.isfinite().all()  # (the tokens of such pages count for nothing)
     with pytest.raises(RuntimeError, match="page id"):
+        ops.raise_on_status(status)
+
+
+STEPS = [  # heads, contexts, page size, window, entries that turn, norms, type
+    ((12, 2, 128), [1], 16, None, 128, False, torch.bfloat16), ((12, 2, 128), [1024] * 8, 16, None, 128, True, torch.bfloat16),
+    ((28, 4, 128), [1, 2, 31, 32, 33, 0, 63, 64, 65, 500, 4000], 16, None, 128, False, torch.bfloat16),
+    ((16, 16, 64), [5, 700, 128, 0], 8, 100, 64, True, torch.bfloat16), ((24, 1, 128), [300, 1], 5, None, 128, True, torch.bfloat16),
+    ((48, 2, 64), [257, 12, 64, 65], 16, 1, 64, False, torch.bfloat16), ((32, 2, 256), [70, 1, 513, 16], 16, None, 256, True, torch.bfloat16),
+    ((14, 2, 64), [1, 129], 1, None, 0, True, torch.bfloat16), ((4, 4, 128), [0, 0], 16, None, 128, False, torch.bfloat16),
+    ((12, 2, 128), [20000, 3, 9000], 16, None, 128, True, torch.bfloat16), ((16, 16, 64), [200] * 900, 16, None, 64, False, torch.bfloat16),
+    ((6, 2, 96), [200, 41, 0], 8, None, 96, True, torch.bfloat16), ((12, 2, 128), [77, 0], 16, None, 64, True, torch.bfloat16),
+    ((12, 2, 128), [77, 64, 0], 16, 40, 128, True, torch.float32)]
+
+
+def _turned(x, w, eps, at, freq):
+    """Heads [n, heads, hd] normed and turned in float64, and the sums of the sizes of each result's terms."""
+    x = x.double()
+    if w is not None:
+        x = x / (x.square().mean(-1, keepdim=True) + eps).sqrt() * w.double()
+    size = x.abs()
+    if freq is not None:
+        angle = at.double()[:, None] * freq.double()
+        c, s, h = angle.cos()[:, None], angle.sin()[:, None], len(freq)
+        a, b = x[..., :h], x[..., h : 2 * h]
+        size = torch.cat([(a * c).abs() + (b * s).abs(), (b * c).abs() + (a * s).abs(), x[..., 2 * h :].abs()], -1)
+        x = torch.cat([a * c - b * s, b * c + a * s, x[..., 2 * h :]], -1)
+    return x, size
+
+
+@pytest.mark.parametrize("early", [False, True])
+@pytest.mark.parametrize("heads, ctx, page, window, rot, norm, dtype", STEPS)
+def test_whole_step(heads, ctx, page, window, rot, norm, dtype, early):
+    """One call of norms, rotation, store and attention: the rows that it stores (contexts of 0 too, whose output is 0), against the
+    formulas; its output over the cache that it leaves; nothing else in the cache changes; without slots nothing does."""
+    nh, nkv, hd = heads
+    n, g = len(ctx), torch.Generator().manual_seed(sum(ctx) + nh * hd + rot)
+    before, tables = filled_pages(ctx, page, nkv, hd, g)
+    owned = sum(-(-c // page) for c in ctx)
+    spare = [p for p in range(owned + 2) if p not in set(tables.flatten().tolist())]
+    slots = torch.tensor([int(tables[s, (c - 1) // page]) * page + (c - 1) % page if c else spare[s % 2] * page + s // 2 % page
+                          for s, c in enumerate(ctx)], dtype=torch.int32)
+    at = (torch.tensor(ctx) - 1 + torch.randint(0, 50, (n,), generator=g)).clamp(min=0).to(torch.int32)
+    qkv = torch.randn(n, (nh + 2 * nkv) * hd, generator=g).to(dtype)
+    freq = (10000.0 ** -(torch.arange(0, rot, 2).double() / max(rot, 1))).float() if rot else None
+    w = [1.0 + 0.2 * torch.randn(hd, generator=g) if norm else None for _ in range(2)]
+    w_on, scale, status = _on(*w), hd**-0.5, ops.new_status(DEV)
+    lens = torch.tensor(ctx, dtype=torch.int32)
+
+    def run(where, cache):
+        out = quantised.decode_step(*_on(qkv, at, where, freq), cache, *_on(tables, lens), nh, nkv, hd, scale, status, q_weight=w_on[0],
+                                    k_weight=w_on[1], eps=1e-6, window=window, early=early)
+        ops.raise_on_status(status)
+        return out
+
+    cache = quantised.E4M3Pages(*_on(*before))
+    out = run(slots, cache)
+    after = tuple(t.cpu() for t in cache)
+    rows = qkv.view(n, -1, hd)
+    q, q_size = _turned(rows[:, :nh], w[0], 1e-6, at, freq)
+    k, k_size = _turned(rows[:, nh : nh + nkv], w[1], 1e-6, at, freq)
+    page_at, off = slots.long() // page, slots.long() % page
+    off_by = (hd + 16) * 2.0**-24  # float32 roundings of sums of squares, a root, a quotient, a weight, an angle, two products
+    for i, (want, size) in enumerate(((k, k_size), (rows[:, nh + nkv :].double(), 0.0))):
+        codes, power = after[i].view(torch.uint8)[page_at, off].view(CODES).double(), after[2 + i][page_at, :, off].double()
+        up = torch.exp2(power - 127)[..., None]
+        # half a step of a code: 2^-4 of it, or 2^-10 of the power below the smallest whole one
+        assert ((codes * up - want).abs() <= torch.maximum(want.abs() * 2.0**-4, up * 2.0**-10) * 1.0001 + off_by * size).all()
+        big = want.abs().amax(-1)
+        assert (big <= 448.001 * up[..., 0]).all() and (big >= 223.99 * up[..., 0]).all()
+        for was, now in ((before[i].view(torch.uint8), after[i].view(torch.uint8)), (before[2 + i].transpose(1, 2), after[2 + i].transpose(1, 2))):
+            was, now = was.clone(), now.clone()
+            was[page_at, off] = now[page_at, off] = 0
+            assert torch.equal(was, now)
+    assert all((out[s] == 0).all() for s, c in enumerate(ctx) if c == 0)
+    # queries are rounded to the run's type; where float32's errors leave open which way, by so much either way
+    low, high = (q - off_by * q_size).to(dtype).double(), (q + off_by * q_size).to(dtype).double()
+    q = q.to(dtype).double()
+    for s in [s for s, c in enumerate(ctx) if c][:40]:
+        keys, values = (context(after[i], after[2 + i], tables[s], ctx[s], page) for i in (0, 1))
+        want, size, score = attention(q[s : s + 1], keys, values, ctx[s] - 1, window, scale)
+        open_by = scale * ((high - low)[s] * keys.abs().amax(0).repeat_interleave(nh // nkv, 0)).sum(-1)[None, :, None]
+        bound = attention_bound(want, size, score, hd, dtype, WEIGHT_BITS) + 2.5 * open_by * size
+        got = out[s].double().cpu().view(1, nh, hd)
+        assert got.isfinite().all() and float(((got - want).abs() / bound).max()) <= 1.0, f"request {s}"
+    if not early and dtype == torch.bfloat16 and hd in quantised.STEP_HEAD_DIMS and rot in (0, hd):
+        cache = quantised.E4M3Pages(*_on(*before))
+        assert torch.equal(run(torch.full_like(slots, -1), cache), out)
+        assert all(torch.equal(a.cpu().view(torch.uint8), b.view(torch.uint8)) for a, b in zip(cache, before))
+
+
+def test_whole_step_reports_slots_outside_the_pool():
+    """Such tokens are attended and not stored."""
+    g = torch.Generator().manual_seed(16)
+    cache, tables = filled_pages([33, 5], 16, 1, 64, g)
+    status, held = ops.new_status(DEV), quantised.E4M3Pages(*_on(*cache))
+    slots = torch.tensor([cache[0].shape[0] * 16, 2**31 - 1], dtype=torch.int32, device=DEV)
+    out = quantised.decode_step(torch.ones(2, 4 * 64, dtype=torch.bfloat16, device=DEV), *_on(torch.tensor([32, 4], dtype=torch.int32)), slots, None,
+                                held, *_on(tables, torch.tensor([33, 5], dtype=torch.int32)), 2, 1, 64, 0.1, status)
+    assert out.isfinite().all() and all(torch.equal(a.cpu().view(torch.uint8), b.view(torch.uint8)) for a, b in zip(held, cache))
+    with pytest.raises(RuntimeError, match="slot"):
         ops.raise_on_status(status)
 
 

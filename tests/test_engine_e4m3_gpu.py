@@ -48,13 +48,18 @@ def test_attention_part(heads, window, kv_dtype, norm, dtype):
     builder = StepBuilder(cache, dtype, DEV, cache.status)
     g = torch.Generator().manual_seed(hd)
     seen = {}
-    original = ops.quantised.norm_rotate_store
+    original, whole = ops.quantised.norm_rotate_store, ops.quantised.decode_step
 
     def noting(*args, **kwargs):
         seen["q"] = original(*args, **kwargs)
         return seen["q"]
 
-    ops.quantised.norm_rotate_store = noting
+    def noting_step(qkv, positions, slots, inv_freq, cache, tables, ctx, nh, nkv, hd, scale, status, **kwargs):
+        norms = {name: kwargs[name] for name in ("q_weight", "k_weight", "eps")}
+        seen["q"] = original(qkv, positions, torch.full_like(slots, -1), inv_freq, cache, nh, nkv, hd, status, **norms)  # (stored nowhere)
+        return whole(qkv, positions, slots, inv_freq, cache, tables, ctx, nh, nkv, hd, scale, status, **kwargs)
+
+    ops.quantised.norm_rotate_store, ops.quantised.decode_step = noting, noting_step
     try:
         for step in ({"a": 21}, {"b": 40, "a": 1}, {"a": 1, "b": 1}, {"c": 5, "a": 9, "b": 1}, {"a": 1, "b": 1, "c": 1}):
             entries = []
@@ -83,7 +88,7 @@ def test_attention_part(heads, window, kv_dtype, norm, dtype):
                 at += n
             builder.commit(prepared)
     finally:
-        ops.quantised.norm_rotate_store = original
+        ops.quantised.norm_rotate_store, ops.quantised.decode_step = original, whole
 
 
 @pytest.fixture(scope="module")

@@ -66,10 +66,10 @@ def _check_device(index: int) -> None:
         raise ValueError(f"the tensors are on cuda:{index}, the current device is cuda:{torch.cuda.current_device()}")
 
 
-def _elsewhere(index: int, **tensors) -> None:
-    for name, t in tensors.items():
+def _elsewhere(index: int, *tensors) -> None:
+    for t in tensors:
         if t is not None and t.get_device() != index:
-            raise ValueError(f"{name} is on {t.device}, the others are not")
+            raise ValueError(f"a tensor of {tuple(t.shape)} is on {t.device}, the call's first one on {'the CPU' if index < 0 else f'cuda:{index}'}")
 
 
 def _ints(t: torch.Tensor, name: str, ndim: int, entries: int | None = None) -> None:
@@ -139,11 +139,10 @@ def _check_store(qkv, n, positions, slots, inv_freq, cache, num_kv_heads, head_d
             raise ValueError("inv_freq must be a contiguous float32 vector")
         if 2 * inv_freq.shape[0] > head_dim:
             raise ValueError(f"inv_freq turns {2 * inv_freq.shape[0]} entries of heads of {head_dim}")
-    for name, w in (("q_weight", q_weight), ("k_weight", k_weight)):
-        if w is not None and (w.dtype != torch.float32 or tuple(w.shape) != (head_dim,) or not w.is_contiguous()):
-            raise ValueError(f"{name} must be contiguous float32 [{head_dim}]")
-    _elsewhere(qkv.get_device(), positions=positions, slots=slots, inv_freq=inv_freq, q_weight=q_weight, k_weight=k_weight, cache=cache.k,
-               values=cache.v, status=status)
+    for w in (q_weight, k_weight):
+        if w is not None and (w.dtype is not torch.float32 or w.shape != (head_dim,) or not w.is_contiguous()):
+            raise ValueError(f"{'q_weight' if w is q_weight else 'k_weight'} must be contiguous float32 [{head_dim}]")
+    _elsewhere(qkv.get_device(), positions, slots, inv_freq, q_weight, k_weight, cache.k, cache.v, status)
     return shape
 
 
@@ -215,7 +214,7 @@ def read_pages(cache: E4M3Pages, block_tables: torch.Tensor, ctx_lens: torch.Ten
         raise ValueError("least_rows must be at least 1")
     _check_status(status)
     index = cache.k.get_device()
-    _elsewhere(index, out_k=out_k, out_v=out_v, block_tables=block_tables, ctx_lens=ctx_lens, q_start=q_start, status=status)
+    _elsewhere(index, out_k, out_v, block_tables, ctx_lens, q_start, status)
     _check_device(index)
     _read_call(cache, (pages, page_size, nkv, hd), block_tables, ctx_lens, q_start, out_k, out_v, window, least_rows, dtype_code(out_k.dtype), status)
 
@@ -315,7 +314,7 @@ def attention_decode(q: torch.Tensor, cache: E4M3Pages, block_tables: torch.Tens
     if out is not None and (out.dtype != q.dtype or out.shape != (q.shape[0], num_heads * hd) or not out.is_contiguous()):
         raise ValueError("out must be contiguous [rows, nh * hd] of q's type")
     index = q.get_device()
-    _elsewhere(index, cache=cache.k, block_tables=block_tables, ctx_lens=ctx_lens, q_start=q_start, out=out, status=status)
+    _elsewhere(index, cache.k, block_tables, ctx_lens, q_start, out, status)
     _check_device(index)
     if out is None:
         out = q.new_empty((s, num_heads * hd))
@@ -347,7 +346,7 @@ def decode_step(qkv: torch.Tensor, positions: torch.Tensor, slots: torch.Tensor,
         raise ValueError("window must be positive or None")
     shape = _check_store(qkv, n, positions, slots, inv_freq, cache, num_kv_heads, head_dim, status, q_weight, k_weight)
     index = qkv.get_device()
-    _elsewhere(index, block_tables=block_tables, ctx_lens=ctx_lens)
+    _elsewhere(index, block_tables, ctx_lens)
     _check_device(index)
     if not early and code == 1 and head_dim in STEP_HEAD_DIMS and (inv_freq is None or 2 * inv_freq.shape[0] == head_dim):
         out, stream = qkv.new_empty((n, num_heads * head_dim)), _stream()
@@ -499,7 +498,7 @@ def attention_portions(q: torch.Tensor, cache: E4M3Pages, block_tables: torch.Te
         raise ValueError("window must be positive or None")
     _check_status(status)
     index = q.get_device()
-    _elsewhere(index, cache=cache.k, block_tables=block_tables, ctx_lens=ctx_lens, q_start=q_start, plan=plan.tok_seq, status=status)
+    _elsewhere(index, cache.k, block_tables, ctx_lens, q_start, plan.tok_seq, status)
     _check_device(index)
     if code == 1 and hd in fast.PREFILL_HEAD_DIMS:
         out = q.new_empty((q.shape[0], num_heads * hd))

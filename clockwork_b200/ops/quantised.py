@@ -390,6 +390,7 @@ class PortionPlan(NamedTuple):
 
     q_lens: tuple
     ctx_lens: tuple
+    shape: tuple         # heads, KV heads, entries, page size
     short: int           # rows of the requests that bring `least_rows` to `most_rows` of them
     least_rows: int
     most_rows: int
@@ -410,6 +411,8 @@ def plan_portions(q_lens, ctx_lens, num_heads: int, num_kv_heads: int, head_dim:
     from . import attention_fast as fast
 
     q_lens, ctx_lens = tuple(int(n) for n in q_lens), tuple(int(c) for c in ctx_lens)
+    if num_kv_heads <= 0 or num_heads <= 0 or num_heads % num_kv_heads or page_size <= 0:
+        raise ValueError(f"{num_heads} query heads over {num_kv_heads} KV heads in pages of {page_size}")
     if len(q_lens) != len(ctx_lens) or any(n < 0 or c < n for n, c in zip(q_lens, ctx_lens)):
         raise ValueError("every request has a length and a context that holds its rows")
     if most_rows is None:
@@ -436,7 +439,7 @@ def plan_portions(q_lens, ctx_lens, num_heads: int, num_kv_heads: int, head_dim:
     n, rows = len(seqs), len(tok_seq)
     dev = torch.from_numpy(np.concatenate([np.array(seqs + q0s + words, dtype=np.int32), tok_seq, positions])).to(device)
     cut = any(w & 0xFF != 1 for w in words)
-    return PortionPlan(q_lens, ctx_lens, short, least_rows, most_rows, n, each, dev[:n], dev[n : 2 * n], dev[2 * n : 3 * n] if cut else None,
+    return PortionPlan(q_lens, ctx_lens, (num_heads, num_kv_heads, head_dim, page_size), short, least_rows, most_rows, n, each, dev[:n], dev[n : 2 * n], dev[2 * n : 3 * n] if cut else None,
                        dev[3 * n : 3 * n + rows], dev[3 * n + rows :])
 
 
@@ -494,6 +497,8 @@ def attention_portions(q: torch.Tensor, cache: E4M3Pages, block_tables: torch.Te
     _ints(q_start, "q_start", 1, s + 1)
     if len(plan.q_lens) != s or sum(plan.q_lens) > q.shape[0]:
         raise ValueError(f"the plan is for {len(plan.q_lens)} requests of {sum(plan.q_lens)} rows, the call has {s} and {q.shape[0]}")
+    if plan.shape != (num_heads, nkv, hd, page_size):
+        raise ValueError(f"the plan is for {plan.shape} heads, KV heads, entries and page size, the call has {(num_heads, nkv, hd, page_size)}")
     if window is not None and window <= 0:
         raise ValueError("window must be positive or None")
     _check_status(status)

@@ -75,11 +75,45 @@ def test_read_refuses(change, words):
         quantised.read_pages(**{**args, **change})
 
 
+STEP = [*((change, words) for change, words in STORE if "cache" not in change), (dict(cache=quantised.PlainPages(torch.zeros(4, 8, 2, 32), torch.zeros(4, 8, 2, 32))), "8-bit cache"),
+        (dict(block_tables=torch.zeros(2, 2, dtype=torch.int32)), "block_tables"), (dict(block_tables=torch.zeros(3, 2)), "block_tables"),
+        (dict(ctx_lens=torch.zeros(3, dtype=torch.int64)), "ctx_lens"), (dict(window=0), "window"),
+        (dict(num_heads=3, qkv=torch.zeros(3, 224, dtype=torch.bfloat16)), "multiple"),
+        (dict(cache=_args(hd=24)["cache"], head_dim=24, qkv=torch.zeros(3, 192, dtype=torch.bfloat16), inv_freq=None), "multiple of 16")]
+
+
+@pytest.mark.parametrize("change, words", STEP)
+def test_step_refuses(change, words):
+    args = dict(**_args(), block_tables=torch.zeros(3, 2, dtype=torch.int32), ctx_lens=torch.zeros(3, dtype=torch.int32), scale=1.0)
+    for early in (False, True):
+        with pytest.raises(ValueError, match=words):
+            quantised.decode_step(**{**args, **change}, early=early)
+
+
+PORTIONS = [(dict(q=torch.zeros(5, 100, dtype=torch.bfloat16)), "q must"), (dict(q=torch.zeros(5, 128, dtype=torch.float16)), "dtype"),
+            (dict(q=torch.zeros(5, 256, dtype=torch.bfloat16)[:, ::2]), "stride"), (dict(num_heads=3), "multiple"), (dict(num_heads=0), "multiple"),
+            (dict(num_heads=2), "plan is for"), (dict(q=torch.zeros(4, 128, dtype=torch.bfloat16)), "plan is for"),
+            (dict(q_start=torch.zeros(3, dtype=torch.int32)), "q_start"), (dict(ctx_lens=torch.zeros(3)), "ctx_lens"),
+            (dict(block_tables=torch.zeros(2, 2, dtype=torch.int32), ctx_lens=torch.zeros(2, dtype=torch.int32), q_start=torch.zeros(3, dtype=torch.int32)), "plan is for"),
+            (dict(cache=_args(page=16)["cache"]), "plan is for"), (dict(window=-2), "window"), (dict(status=torch.zeros(4)), "status"), ({}, "CUDA")]
+
+
+@pytest.mark.parametrize("change, words", PORTIONS)
+def test_portions_refuse(change, words):
+    args = dict(q=torch.zeros(5, 128, dtype=torch.bfloat16), cache=_args()["cache"], block_tables=torch.zeros(3, 2, dtype=torch.int32),
+                q_start=torch.tensor([0, 2, 2, 5], dtype=torch.int32), ctx_lens=torch.tensor([2, 0, 9], dtype=torch.int32),
+                plan=quantised.plan_portions([2, 0, 3], [2, 0, 9], 4, 2, 32, 8, "cpu"), num_heads=4, scale=1.0, status=torch.zeros(4, dtype=torch.int32))
+    with pytest.raises(ValueError, match=words):
+        quantised.attention_portions(**{**args, **change})
+
+
 def test_plans_of_impossible_portions_are_refused():
     with pytest.raises(ValueError, match="context"):
         quantised.plan_portions([3, 2], [5, 1], 4, 2, 32, 8, "cpu")
     with pytest.raises(ValueError, match="context"):
         quantised.plan_portions([3], [5, 1], 4, 2, 32, 8, "cpu")
+    with pytest.raises(ValueError, match="KV heads"):
+        quantised.plan_portions([3], [5], 5, 2, 32, 8, "cpu")
 
 
 def test_the_oracle_rounds_as_the_type_does():

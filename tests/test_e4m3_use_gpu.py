@@ -162,3 +162,87 @@ def test_no_rows_at_all():
     out = quantised.attention_decode(q, cache, torch.zeros(0, 1, dtype=torch.int32, device=DEV), none, NH, 0.09, status)
     assert out.shape == (0, NH * HD)
     ops.raise_on_status(status)
+    out = quantised.decode_step(torch.zeros(0, (NH + 2 * NKV) * HD, dtype=torch.bfloat16, device=DEV), none, none, None, cache,
+                                torch.zeros(0, 1, dtype=torch.int32, device=DEV), none, NH, NKV, HD, 0.09, status)
+    assert out.shape == (0, NH * HD)
+
+
+def _steps(seed, start, steps, nh=NH, nkv=NKV, hd=HD):
+    """Requests that grow by a token a step: (cache, tables, qkv [steps, requests, ..], slots and contexts [steps, requests])."""
+    g = torch.Generator().manual_seed(seed)
+    cache, tables = filled_pages([c + steps for c in start], PAGE, nkv, hd, g)
+    ctx = torch.tensor(start, dtype=torch.int32) + 1 + torch.arange(steps, dtype=torch.int32)[:, None]
+    slots = torch.stack([tables[s, (ctx[:, s].long() - 1) // PAGE] * PAGE + (ctx[:, s] - 1) % PAGE for s in range(len(start))], 1).to(torch.int32)
+    qkv = torch.randn(steps, len(start), (nh + 2 * nkv) * hd, generator=g).bfloat16()
+    return (lambda: quantised.E4M3Pages(*(t.to(DEV) for t in cache))), tables.to(DEV), qkv.to(DEV), slots.to(DEV), ctx.to(DEV)
+
+
+@pytest.mark.parametrize("early", [False, True])
+def test_captured_steps_give_the_bits_of_plain_ones(early):
+    """Two layers' whole steps in one graph, replayed while the contexts grow over the ends of pages and tiles."""
+    status, steps = ops.new_status(DEV), 40
+    fresh, tables, qkv, slots, ctx = _steps(21, [1, 30, 1000, 0], steps)
+    freq = (10000.0 ** -(torch.arange(0, HD, 2).double() / HD)).float().to(DEV)
+    now = {"qkv": qkv[0].clone(), "slots": slots[0].clone(), "ctx": ctx[0].clone(), "at": ctx[0] - 1}
+
+    def run(layers):
+        return [quantised.decode_step(now["qkv"], now["at"], now["slots"], freq, layer, tables, now["ctx"], NH, NKV, HD, 0.09, status,
+                                      early=early) for layer in layers]
+
+    def bring(i):
+        for name, t in (("qkv", qkv[i]), ("slots", slots[i]), ("ctx", ctx[i]), ("at", ctx[i] - 1)):
+            now[name].copy_(t)
+
+    plain, layers, want = [fresh(), fresh()], [fresh(), fresh()], []
+    for i in range(steps):
+        bring(i)
+        want.append([out.clone() for out in run(plain)])
+    bring(0)
+    run([fresh()])
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        outs = run(layers)
+    for i in range(steps):
+        bring(i)
+        graph.replay()
+        assert all(torch.equal(a, b) for a, b in zip(outs, want[i])), i
+    for a, b in zip(plain, layers):
+        assert all(torch.equal(x.view(torch.uint8), y.view(torch.uint8)) for x, y in zip(a, b))
+    ops.raise_on_status(status)
+
+
+def test_whole_steps_on_two_streams():
+    status = [ops.new_status(DEV), ops.new_status(DEV)]
+    problems = [_steps(22, [9000, 8000], 10), _steps(23, [20000], 10)]
+
+    def run(i, cache):
+        _, tables, qkv, slots, ctx = problems[i]
+        return [quantised.decode_step(qkv[j], ctx[j] - 1, slots[j], None, cache, tables, ctx[j], NH, NKV, HD, 0.09, status[i]) for j in range(10)]
+
+    caches = [p[0]() for p in problems]
+    want = [run(i, p[0]()) for i, p in enumerate(problems)]
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    torch.cuda.synchronize()
+    got = []
+    for i in range(2):
+        with torch.cuda.stream(streams[i]):
+            got.append(run(i, caches[i]))
+    torch.cuda.synchronize()
+    for i in range(2):
+        ops.raise_on_status(status[i])
+        assert all(torch.equal(a, b) for a, b in zip(got[i], want[i]))
+
+
+def test_steps_whose_rows_begin_at_an_odd_entry():
+    """They go to the two kernels that read entry by entry, and hold the same rows."""
+    status = ops.new_status(DEV)
+    fresh, tables, qkv, slots, ctx = _steps(24, [200, 31], 1)
+    odd = torch.zeros(qkv[0].numel() + 1, dtype=torch.bfloat16, device=DEV)[1:].view_as(qkv[0])
+    odd.copy_(qkv[0])
+    caches, outs = [fresh(), fresh()], []
+    for rows, cache in zip((qkv[0], odd), caches):
+        outs.append(quantised.decode_step(rows, ctx[0] - 1, slots[0], None, cache, tables, ctx[0], NH, NKV, HD, 0.09, status))
+    ops.raise_on_status(status)
+    assert all(torch.equal(x.view(torch.uint8), y.view(torch.uint8)) for x, y in zip(*caches))
+    assert torch.equal(*outs)  # (their queries are the same bits: neither is normed nor turned)

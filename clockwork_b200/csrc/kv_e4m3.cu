@@ -23,15 +23,76 @@ struct StoreParams {
     int* status;
 };
 
+// Two float32 products, or products and sums, at a time.
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+    unsigned long long d;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(*reinterpret_cast<unsigned long long*>(&a)), "l"(*reinterpret_cast<unsigned long long*>(&b)));
+    return *reinterpret_cast<float2*>(&d);
+}
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+    unsigned long long d;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(*reinterpret_cast<unsigned long long*>(&a)),
+        "l"(*reinterpret_cast<unsigned long long*>(&b)), "l"(*reinterpret_cast<unsigned long long*>(&c)));
+    return *reinterpret_cast<float2*>(&d);
+}
+
+// Four neighbouring entries in float32.
+struct Pairs {
+    float2 x, y;
+    __device__ Pairs() {}
+    __device__ explicit Pairs(const float* at) {
+        const float4 v = *reinterpret_cast<const float4*>(at);
+        x = make_float2(v.x, v.y);
+        y = make_float2(v.z, v.w);
+    }
+    __device__ float4 four() const { return make_float4(x.x, x.y, y.x, y.y); }
+    __device__ float largest() const { return fmaxf(fmaxf(fabsf(x.x), fabsf(x.y)), fmaxf(fabsf(y.x), fabsf(y.y))); }
+    __device__ void clamp() {
+        x = make_float2(kv_clamped(x.x), kv_clamped(x.y));
+        y = make_float2(kv_clamped(y.x), kv_clamped(y.y));
+    }
+    __device__ uint32_t codes(float2 down) const {
+        const float2 u = mul2(x, down), v = mul2(y, down);
+        return kv_codes(u.x, u.y, v.x, v.y);
+    }
+};
+
+// The same as they lie in memory.
+template <typename T>
+struct Four;
+template <>
+struct Four<float> {
+    float4 v = {0.f, 0.f, 0.f, 0.f};
+    __device__ void load(const float* at) { v = *reinterpret_cast<const float4*>(at); }
+    __device__ Pairs pairs() const {
+        Pairs r;
+        r.x = make_float2(v.x, v.y);
+        r.y = make_float2(v.z, v.w);
+        return r;
+    }
+};
+template <>
+struct Four<bf16> {
+    uint2 v = {0u, 0u};
+    __device__ void load(const bf16* at) { v = *reinterpret_cast<const uint2*>(at); }
+    __device__ Pairs pairs() const {
+        Pairs r;
+        r.x = make_float2(__uint_as_float(v.x << 16), __uint_as_float(v.x & 0xFFFF0000u));
+        r.y = make_float2(__uint_as_float(v.y << 16), __uint_as_float(v.y & 0xFFFF0000u));
+        return r;
+    }
+};
+
 // LG neighbouring lanes hold a head, a lane two octets of it (octet i, i < rot / 8: four entries and the four that turn with them;
 // behind those, eight neighbours), so that pairs never leave a thread, the mean of squares and the largest magnitude are shuffles
 // among LG lanes, and accesses are of 8 or 16 bytes.  A thread keeps its head and its entries for a block's tokens, whose rows are
-// loaded one ahead: weights, offsets and the kind of head are found out once.  Blocks have as many tokens as leave the SMs two
-// blocks each, eight at most.
+// loaded one ahead: weights, offsets and the kind of head are found out once.  Bound by its instructions (304 a warp and token,
+// half of the issue slots taken at 78 registers a thread), which is why products go two at a time and the root is an estimate and
+// a step: 2,048 tokens of 36 normed heads of 128 13.7 -> 10.9 us (in the L2), 8,192 64 -> 38; what the bytes take: 5.5 and 22.
 #define STORE_TOKENS 8
 template <typename T, int LG>
 __global__ void __launch_bounds__(512) norm_rotate_store_kernel(const StoreParams p, int most_tokens, int block_heads) {
-    extern __shared__ float turn[];  // per token: cos[rot / 2], sin[rot / 2]
+    extern __shared__ float turn[];  // per token: cosines [rot / 2], sines and their opposites
     __shared__ int slot_s[STORE_TOKENS], off_s[STORE_TOKENS];  // a token's slot (-1: none) and its place in its page
     if (p.early)
         pdl_launch_dependents();
@@ -43,7 +104,8 @@ __global__ void __launch_bounds__(512) norm_rotate_store_kernel(const StoreParam
     const bool live = own < block_heads && head < heads, is_q = head < p.nh, is_v = head >= p.nh + p.nkv;
     int a_at[2], b_at[2];
     bool there[2], turns[2];
-    float4 a_next[2], b_next[2];
+    const T* row = (const T*)p.qkv + ((size_t)t0 * heads + head) * p.hd;
+    Four<T> a_next[2], b_next[2];  // the row of the next token (of entries that there are not: zeros)
 #pragma unroll
     for (int e = 0; e < 2; ++e) {
         const int octet = l + e * LG;
@@ -51,15 +113,13 @@ __global__ void __launch_bounds__(512) norm_rotate_store_kernel(const StoreParam
         turns[e] = octet < turning && !is_v;
         a_at[e] = octet < turning ? 4 * octet : p.rot + 8 * (octet - turning);
         b_at[e] = octet < turning ? half + 4 * octet : a_at[e] + 4;
-        a_next[e] = b_next[e] = make_float4(0.f, 0.f, 0.f, 0.f);
     }
-    const T* row = (const T*)p.qkv + ((size_t)t0 * heads + head) * p.hd;
     auto load = [&]() {
 #pragma unroll
         for (int e = 0; e < 2; ++e)
             if (there[e]) {
-                a_next[e] = Vec4<T>::load(row + a_at[e]);
-                b_next[e] = Vec4<T>::load(row + b_at[e]);
+                a_next[e].load(row + a_at[e]);
+                b_next[e].load(row + b_at[e]);
             }
         row += (size_t)heads * p.hd;
     };
@@ -75,16 +135,19 @@ __global__ void __launch_bounds__(512) norm_rotate_store_kernel(const StoreParam
     }
     for (int i = threadIdx.x; i < tokens * half; i += blockDim.x) {
         const int t = i / half, j = i - t * half;
-        turn_of(p.positions[t0 + t], p.inv_freq[j], turn[t * p.rot + half + j], turn[t * p.rot + j]);
+        float sn;
+        turn_of(p.positions[t0 + t], p.inv_freq[j], sn, turn[t * 3 * half + j]);
+        turn[t * 3 * half + half + j] = sn;
+        turn[t * 3 * half + 2 * half + j] = -sn;
     }
     const float* weight = is_v ? nullptr : is_q ? p.q_weight : p.k_weight;
-    float4 wa[2], wb[2];
+    Pairs wa[2], wb[2];
     if (weight != nullptr)
 #pragma unroll
         for (int e = 0; e < 2; ++e)
             if (there[e]) {
-                wa[e] = *reinterpret_cast<const float4*>(weight + a_at[e]);
-                wb[e] = *reinterpret_cast<const float4*>(weight + b_at[e]);
+                wa[e] = Pairs(weight + a_at[e]);
+                wb[e] = Pairs(weight + b_at[e]);
             }
     const bool any_norm = __any_sync(0xffffffffu, live && weight != nullptr), any_kv = __any_sync(0xffffffffu, live && !is_q);
     const int kvh = is_v ? head - p.nh - p.nkv : head - p.nh;
@@ -93,73 +156,94 @@ __global__ void __launch_bounds__(512) norm_rotate_store_kernel(const StoreParam
         load();
     }
     __syncthreads();
+    const float inv_hd = 1.f / (float)p.hd;
+    T* q_to = (T*)p.q_out + ((size_t)t0 * p.nh + head) * p.hd;
+#pragma unroll 1
     for (int t = 0; t < tokens; ++t) {
-        float4 a[2] = {a_next[0], a_next[1]}, b[2] = {b_next[0], b_next[1]};
+        Pairs a[2], b[2];
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+            a[e] = a_next[e].pairs();
+            b[e] = b_next[e].pairs();
+        }
         if (t + 1 < tokens) load();
         if (any_norm) {
-            float sum = 0.f;
-#pragma unroll
-            for (int e = 0; e < 2; ++e) {  // (entries that there are not: zeros)
-                sum = fmaf(a[e].x, a[e].x, fmaf(a[e].y, a[e].y, fmaf(a[e].z, a[e].z, fmaf(a[e].w, a[e].w, sum))));
-                sum = fmaf(b[e].x, b[e].x, fmaf(b[e].y, b[e].y, fmaf(b[e].z, b[e].z, fmaf(b[e].w, b[e].w, sum))));
-            }
+            float2 sums = mul2(a[0].x, a[0].x);
+            sums = fma2(a[0].y, a[0].y, sums);
+            float2 more = mul2(b[0].x, b[0].x);
+            more = fma2(b[0].y, b[0].y, more);
+            sums = fma2(a[1].x, a[1].x, sums);
+            more = fma2(b[1].x, b[1].x, more);
+            sums = fma2(a[1].y, a[1].y, sums);
+            more = fma2(b[1].y, b[1].y, more);
+            float sum = (sums.x + sums.y) + (more.x + more.y);
 #pragma unroll
             for (int o = LG / 2; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
             if (weight != nullptr) {
-                const float r = __frcp_rn(__fsqrt_rn(__fdiv_rn(sum, (float)p.hd) + p.eps));
+                // 1 / sqrt by an estimate (off by two last places at most) and a step of Newton's, which leaves less than one
+                const float mean = fmaf(sum, inv_hd, p.eps), y = rsqrtf(mean), z = mean * y, nearer = fmaf(0.5f * y, fmaf(-z, y, 1.f), y);
+                const float r = z - z == 0.f ? nearer : y;  // (means of 0 and infinity)
+                const float2 rr = make_float2(r, r);
 #pragma unroll
-                for (int e = 0; e < 2; ++e)
-                    if (there[e]) {
-                        a[e].x *= r * wa[e].x; a[e].y *= r * wa[e].y; a[e].z *= r * wa[e].z; a[e].w *= r * wa[e].w;
-                        b[e].x *= r * wb[e].x; b[e].y *= r * wb[e].y; b[e].z *= r * wb[e].z; b[e].w *= r * wb[e].w;
-                    }
+                for (int e = 0; e < 2; ++e) {
+                    a[e].x = mul2(a[e].x, mul2(rr, wa[e].x)); a[e].y = mul2(a[e].y, mul2(rr, wa[e].y));
+                    b[e].x = mul2(b[e].x, mul2(rr, wb[e].x)); b[e].y = mul2(b[e].y, mul2(rr, wb[e].y));
+                }
             }
         }
 #pragma unroll
         for (int e = 0; e < 2; ++e)
             if (turns[e]) {
-                const float* at = turn + t * p.rot + a_at[e];
-                const float4 cs = *reinterpret_cast<const float4*>(at), sn = *reinterpret_cast<const float4*>(at + half), x = a[e], y = b[e];
-                a[e].x = x.x * cs.x - y.x * sn.x; a[e].y = x.y * cs.y - y.y * sn.y; a[e].z = x.z * cs.z - y.z * sn.z; a[e].w = x.w * cs.w - y.w * sn.w;
-                b[e].x = y.x * cs.x + x.x * sn.x; b[e].y = y.y * cs.y + x.y * sn.y; b[e].z = y.z * cs.z + x.z * sn.z; b[e].w = y.w * cs.w + x.w * sn.w;
+                const float* at = turn + t * 3 * half + a_at[e];
+                const Pairs cs(at), sn(at + half), minus(at + 2 * half), x = a[e], y = b[e];
+                a[e].x = fma2(x.x, cs.x, mul2(y.x, minus.x)); a[e].y = fma2(x.y, cs.y, mul2(y.y, minus.y));
+                b[e].x = fma2(y.x, cs.x, mul2(x.x, sn.x)); b[e].y = fma2(y.y, cs.y, mul2(x.y, sn.y));
             }
-        const int slot = slot_s[t];
-        const bool stores = live && !is_q && slot >= 0;
-        const size_t at = ((size_t)max(slot, 0) * p.nkv + kvh) * p.hd;
-        if ((live && is_q) || (stores && p.k_exp == nullptr)) {  // rows of the run's type
-            T* out = is_q ? (T*)p.q_out + ((size_t)(t0 + t) * p.nh + head) * p.hd : (T*)(is_v ? p.v_cache : p.k_cache) + at;
+        if (live && is_q) {
 #pragma unroll
             for (int e = 0; e < 2; ++e)
                 if (there[e]) {
-                    Vec4<T>::store(out + a_at[e], a[e]);
-                    Vec4<T>::store(out + b_at[e], b[e]);
+                    Vec4<T>::store(q_to + a_at[e], a[e].four());
+                    Vec4<T>::store(q_to + b_at[e], b[e].four());
                 }
         }
-        if (!any_kv || p.k_exp == nullptr) continue;
+        q_to += (size_t)p.nh * p.hd;
+        if (!any_kv) continue;
+        const int slot = slot_s[t];
+        const bool stores = live && !is_q && slot >= 0;
+        const size_t at = ((size_t)max(slot, 0) * p.nkv + kvh) * p.hd;
+        if (p.k_exp == nullptr) {  // rows of the run's type
+            T* out = (T*)(is_v ? p.v_cache : p.k_cache) + at;
+#pragma unroll
+            for (int e = 0; e < 2; ++e)
+                if (stores && there[e]) {
+                    Vec4<T>::store(out + a_at[e], a[e].four());
+                    Vec4<T>::store(out + b_at[e], b[e].four());
+                }
+            continue;
+        }
         float big = 0.f;  // (NaN has no say)
 #pragma unroll
-        for (int e = 0; e < 2; ++e)
-            big = fmaxf(big, fmaxf(fmaxf(fmaxf(fabsf(a[e].x), fabsf(a[e].y)), fmaxf(fabsf(a[e].z), fabsf(a[e].w))),
-                                   fmaxf(fmaxf(fabsf(b[e].x), fabsf(b[e].y)), fmaxf(fabsf(b[e].z), fabsf(b[e].w)))));
+        for (int e = 0; e < 2; ++e) big = fmaxf(big, fmaxf(a[e].largest(), b[e].largest()));
 #pragma unroll
         for (int o = LG / 2; o > 0; o >>= 1) big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, o));
         if (big > KV_BIGGEST) {
             big = KV_BIGGEST;
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
-                a[e].x = kv_clamped(a[e].x); a[e].y = kv_clamped(a[e].y); a[e].z = kv_clamped(a[e].z); a[e].w = kv_clamped(a[e].w);
-                b[e].x = kv_clamped(b[e].x); b[e].y = kv_clamped(b[e].y); b[e].z = kv_clamped(b[e].z); b[e].w = kv_clamped(b[e].w);
+                a[e].clamp();
+                b[e].clamp();
             }
         }
         if (stores) {
             const int power = kv_power(big), off = off_s[t];
-            const float d = kv_down(power);
+            const float2 down = make_float2(kv_down(power), kv_down(power));
             uint8_t* out = (uint8_t*)(is_v ? p.v_cache : p.k_cache) + at;
 #pragma unroll
             for (int e = 0; e < 2; ++e)
                 if (there[e]) {
-                    *reinterpret_cast<uint32_t*>(out + a_at[e]) = kv_codes(a[e].x * d, a[e].y * d, a[e].z * d, a[e].w * d);
-                    *reinterpret_cast<uint32_t*>(out + b_at[e]) = kv_codes(b[e].x * d, b[e].y * d, b[e].z * d, b[e].w * d);
+                    *reinterpret_cast<uint32_t*>(out + a_at[e]) = a[e].codes(down);
+                    *reinterpret_cast<uint32_t*>(out + b_at[e]) = b[e].codes(down);
                 }
             // (slot - off: the page times page_size, and a page has nkv rows of page_size powers)
             if (l == 0) (is_v ? p.v_exp : p.k_exp)[(size_t)(slot - off) * p.nkv + (size_t)kvh * p.page_size + off] = (uint8_t)power;
@@ -233,9 +317,20 @@ static int store_launch(const StoreParams& p, int N, cudaStream_t stream) {
     int lg = 1;
     while (lg * 16 < p.hd) lg *= 2;
     const int chunks = (heads * lg + 511) / 512, block_heads = (heads + chunks - 1) / chunks;
-    const int tokens = max(1, min(STORE_TOKENS, (N * chunks + 2 * 148 - 1) / (2 * 148)));
-    const dim3 grid((N + tokens - 1) / tokens, chunks), block((block_heads * lg + 31) / 32 * 32);
-    const size_t room = (size_t)tokens * smem;
+    // tokens of a block: as many as end soonest, if a round of the blocks that fit on the SMs (80 registers a thread) takes what two
+    // tokens and each of its tokens do
+    const int threads = (block_heads * lg + 31) / 32 * 32, resident = 148 * max(1, 65536 / 80 / threads);
+    int tokens = 1;
+    long long least = 1LL << 62;
+    for (int t = 1; t <= STORE_TOKENS; ++t) {
+        const long long blocks = (long long)((N + t - 1) / t) * chunks, cost = (blocks + resident - 1) / resident * (t + 2);
+        if (cost < least) {
+            least = cost;
+            tokens = t;
+        }
+    }
+    const dim3 grid((N + tokens - 1) / tokens, chunks), block(threads);
+    const size_t room = (size_t)tokens * smem / 2 * 3;
     switch (lg) {
         case 1: return cw_launch(norm_rotate_store_kernel<T, 1>, grid, block, room, stream, 1u, p, tokens, block_heads);
         case 2: return cw_launch(norm_rotate_store_kernel<T, 2>, grid, block, room, stream, 1u, p, tokens, block_heads);

@@ -603,7 +603,7 @@ def launch_prefill(q, k_cache, v_cache, block_tables, q_start, ctx_lens, item_se
     if use_tc:
         st = {"part_o": None, "part_ml": None, "counters": None}
         if item_split is not None:
-            st = _prefill_scratch(q.device, items, num_heads, head_dim)
+            st = _prefill_scratch(q.device, items, num_heads // each, head_dim)
         if each > 1:
             check(library().cw_attention_prefill_tc_packed(
                 _ptr(q), q.stride(0), q.shape[1], q.shape[0], _ptr(out), _ptr(k_cache), _ptr(v_cache), _ptr(block_tables),

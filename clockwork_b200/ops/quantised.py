@@ -422,16 +422,17 @@ def plan_portions(q_lens, ctx_lens, num_heads: int, num_kv_heads: int, head_dim:
     each = num_heads // num_kv_heads
     if not 1 < each <= fast.QUERY_TILE or not fast.prefill_tc_takes(head_dim, page_size):
         each = 1
-    # Packed where that leaves fewer tiles (measured, us, a head to a tile and packed: 17, 33, 60 and 100 rows behind 2,000, 40 heads over 8
-    # 65.5 and 43.1, 28 over 4 37.4 and 30.8; 1,003, 64 and 200 rows, 40 over 8 318 and 304; 2,048 rows behind 30,000, 12 over 2, where
-    # packing only moves the cuts, 412 and 552)
+    # Packed where that leaves fewer tiles (measured, us, a head to a tile and packed: 17, 33, 60 and 100 rows behind 2,000, 28 heads over 4
+    # 39.0 and 31.2, 40 over 8 65.3 and 60.3; 391 rows and 130 behind 5,170, 14 over 2 of 64 30.8 and 24.4; where it leaves as many there is nothing
+    # in it: 2,048 rows behind 30,000, 12 over 2 412.8 and 412.2; 1,003 behind 9,001, 64 and 200, 14 over 2 of 64, 154 tiles and 144, 104 and 113)
     tiles = [sum(-(-n // t) for n in long) for t in (fast.QUERY_TILE, fast.QUERY_TILE // each)]
     if packed is None:
         packed = num_kv_heads * tiles[1] <= 0.95 * num_heads * tiles[0]
     each = each if packed else 1
     cuts = fast._cuts_for(num_kv_heads if each > 1 else num_heads, head_dim, page_size)
     seqs, q0s, words = fast.prefill_work_items(long, ctx_lens, cuts,
-                                               fast._sm_count(torch.device(device)) if cuts else 0, tile=fast.QUERY_TILE // each)
+                                               fast._sm_count(torch.device(device)) if cuts else 0, tile=fast.QUERY_TILE // each,
+                                               max_items=fast.ROUNDS_MAX_ITEMS * each)  # (as much scratch whichever way)
     lens = np.array(q_lens, dtype=np.int32)
     starts = np.cumsum(lens, dtype=np.int32) - lens
     tok_seq = np.repeat(np.arange(len(lens), dtype=np.int32), lens)

@@ -7,9 +7,14 @@
 // The step is a stream of codes from memory, 2 (hd + 1) bytes per token and KV head, so all query heads of a KV head (16 at
 // most, or 8) share what a block fetches.  Work is cut by the contexts themselves: requests, KV heads and tiles of 16 to 64
 // tokens are numbered through, and every warp of a grid that fills the SMs once takes an equal run of tiles, wherever requests begin
-// and end in it (units_of_block); so contexts of any lengths fill the GPU, and no scratch grows with them.  Each warp has a ring
-// of tiles in shared memory of its own, filled by 16-byte asynchronous copies two or more tiles ahead and on into the next
-// request, so that warps never wait for one another while they stream.
+// and end in it; so contexts of any lengths fill the GPU, and no scratch grows with them.  Each warp has a ring
+// of tiles in shared memory of its own, filled by 16-byte asynchronous copies one to three tiles ahead (twelve warps an SM have 96 KB or more under way) and on into the
+// next request, so that warps never wait for one another while they stream.
+//
+// Bound by memory while it streams, and by latency before and after that.  Measured, us, and what the bytes take at the rate of a copy: 64
+// requests of 1 to 7,650 tokens, 28 heads over 4 of 128, 251 MB 55.5 and 38.9 (the stream itself 36; the first tiles come after 6,
+// the last pieces are added up 8 after the last tile); four of 65,536 to 131,072, 40 heads over 8, 861 MB 160 and 133; 8 of 1,024, 12 over
+// 2, 4.3 MB 11 and 0.7: lengths, block table and rows are three trips to memory one after the other, and joining the pieces is four.
 //
 // Codes become half-precision numbers exactly (cvt) on their way into mma.sync.m16n8k16, which costs less here than it could
 // save elsewhere: at the rate of memory the tensor cores are a fifth busy.  Tokens are the M side of S^T = K Q^T and the codes'
@@ -251,10 +256,11 @@ __device__ __forceinline__ uint32_t row_of_step(const DecodeE4m3Params& p, const
 
 // MODE: single tokens whose queries and rows are ready (TOKENS_READY), portions of few rows (PORTION_ROWS), or whole steps of single
 // tokens (WHOLE_STEP): norms and rotation as a warp takes up a segment's queries, the new key and value by the warp that walks the
-// segment's last tile, into its ring and into the cache.  Whole steps are for callers that launch one call after the other: 2 requests of
-// a few hundred tokens 26.8 us as two calls, 19.8 as one (the host's time, mostly).  In a captured step two kernels are faster, because
-// this one's rings find no room beside the matrix product in front of it, while a store does and this one's beginning then hides behind
-// that (8 layers with 12 heads over 2 of 128, products and all: 8 x 1,024 tokens 465 us as two, 498 as one; 64 x 4,096 703 and 718).
+// segment's last tile, into its ring and into the cache.  Whole steps are for callers that launch one call after the other,
+// whose time is mostly the host's (us a call, one kernel and two: 12 heads over 2 of 128, 8 requests of 1,000 tokens 16.7 and 25.2, 64 of 300 18.1
+// and 25.3, 64 of 4,000 39.1 and 37.4; 16 heads of 64, 64 of 4,000 115 and 118).  In a captured step two kernels are faster: this one's
+// rings find no room beside the matrix product in front of it, while a store does, and attention's beginning hides behind that (8 layers,
+// products and all: 8 x 1,024 tokens 461 us as two, 498 as one; 64 x 4,096 702 and 718).
 #define TOKENS_READY 0
 #define PORTION_ROWS 1
 #define WHOLE_STEP 2

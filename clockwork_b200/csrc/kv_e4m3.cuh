@@ -76,66 +76,3 @@ __device__ __forceinline__ void turn_of(int position, float freq, float& sn, flo
     sn = quarter & 2 ? -a : a;
     cs = (quarter == 1 || quarter == 2) ? -b : b;
 }
-
-// The requests' work, cut evenly over the blocks of a grid: request s brings units(s) units, numbered through all requests;
-// block b owns units [b * quota, (b + 1) * quota), quota = ceil(total / blocks), at least `least`.  Every block works this out
-// from the lengths on the device (so that a captured launch follows them).  All threads of the block call it; `sh`: 36 words
-// of shared memory, free again after a barrier of the caller's.
-struct UnitRange {
-    int total, quota;
-    int first, last;     // this block's units [first, last)
-    int request, offset; // where unit `first` lies: request and unit within it
-};
-template <class F>
-__device__ __forceinline__ UnitRange units_of_block(F units, int requests, int least, int blocks, int block, int* sh) {
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = (blockDim.x + 31) >> 5;
-    UnitRange r;
-    int sum = 0;
-    const int mine = threadIdx.x < requests ? units(threadIdx.x) : 0;  // (looked up once where a thread per request suffices)
-    sum = mine;
-    for (int s = threadIdx.x + blockDim.x; s < requests; s += blockDim.x) sum += units(s);
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-    if (lane == 0) sh[warp] = sum;
-    __syncthreads();
-    r.total = 0;
-    for (int w = 0; w < warps; ++w) r.total += sh[w];
-    r.quota = max(least, (r.total + blocks - 1) / blocks);
-    r.first = (int)min((long long)block * r.quota, (long long)r.total);
-    r.last = min(r.total, r.first + r.quota);
-    r.request = r.offset = 0;
-    if (r.first >= r.last) return r;
-    int base = 0;
-    for (int s0 = 0; s0 < requests; s0 += blockDim.x) {
-        const int s = s0 + threadIdx.x;
-        const int n = s0 == 0 ? mine : s < requests ? units(s) : 0;
-        int upto = n;  // units of this chunk's requests up to and with s
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-            const int v = __shfl_up_sync(0xffffffffu, upto, o);
-            if (lane >= o) upto += v;
-        }
-        __syncthreads();  // (the words of the round before are read)
-        if (lane == 31) sh[warp] = upto;
-        if (threadIdx.x == 0) sh[32] = -1;
-        __syncthreads();
-        int before = base, chunk = 0;
-        for (int w = 0; w < warps; ++w) {
-            if (w < warp) before += sh[w];
-            chunk += sh[w];
-        }
-        const int from = before + upto - n;
-        if (from <= r.first && r.first < from + n) {
-            sh[32] = s;
-            sh[33] = r.first - from;
-        }
-        __syncthreads();
-        if (sh[32] >= 0) {
-            r.request = sh[32];
-            r.offset = sh[33];
-            break;
-        }
-        base += chunk;
-    }
-    return r;
-}

@@ -7,9 +7,9 @@
 // The step is a stream of codes from memory, 2 (hd + 1) bytes per token and KV head, so all query heads of a KV head (16 at
 // most, or 8) share what a block fetches.  Work is cut by the contexts themselves: requests, KV heads and tiles of 16 to 64
 // tokens are numbered through, and every warp of a grid that fills the SMs once takes an equal run of tiles, wherever requests begin
-// and end in it; so contexts of any lengths fill the GPU, and no scratch grows with them.  Each warp has a ring
-// of tiles in shared memory of its own, filled by 16-byte asynchronous copies one to three tiles ahead (twelve warps an SM have 96 KB or more under way) and on into the
-// next request, so that warps never wait for one another while they stream.
+// and end in it; so contexts of any lengths fill the GPU, and no scratch grows with them.  Each warp has a ring of tiles in shared
+// memory of its own, filled by 16-byte asynchronous copies one to three tiles ahead (the warps of an SM have 96 KB or more under
+// way) and on into the next request, so that warps never wait for one another while they stream.
 //
 // Bound by memory while it streams, and by latency before and after that.  Measured, us, and what the bytes take at the rate of a copy: 64
 // requests of 1 to 7,650 tokens, 28 heads over 4 of 128, 251 MB 55.5 and 38.9 (the stream itself 36; the first tiles come after 6,

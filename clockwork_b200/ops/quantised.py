@@ -110,6 +110,10 @@ def check_pages(cache: E4M3Pages) -> tuple[int, int, int, int]:
     return shape
 
 
+def _new_rows(like: torch.Tensor, rows: int, width: int) -> torch.Tensor:
+    return like.new_empty_strided((rows, width), (width, 1))  # (1.4 us of host time; new_empty 1.8, empty 2.4)
+
+
 def _check_rows(qkv: torch.Tensor, num_heads: int, num_kv_heads: int, head_dim: int) -> int:
     """How many rows [q | k | v] has."""
     if qkv.dim() != 2 or not qkv.is_contiguous() or qkv.shape[1] != (num_heads + 2 * num_kv_heads) * head_dim:
@@ -150,7 +154,7 @@ def _store_words(qkv, n, positions, slots, inv_freq, cache, num_heads, num_kv_he
                  early):
     """The query rows' tensor and the entry point's words."""
     quantised, rot = isinstance(cache, E4M3Pages), 0 if inv_freq is None else 2 * inv_freq.shape[0]
-    q = qkv.new_empty((n, num_heads * head_dim))
+    q = _new_rows(qkv, n, num_heads * head_dim)
     return q, _STORE_ARGS(
         qkv.data_ptr(), q.data_ptr(), positions.data_ptr(), slots.data_ptr(), inv_freq.data_ptr() if rot else 0,
         0 if q_weight is None else q_weight.data_ptr(), 0 if k_weight is None else k_weight.data_ptr(), cache.k.data_ptr(), cache.v.data_ptr(),
@@ -317,7 +321,7 @@ def attention_decode(q: torch.Tensor, cache: E4M3Pages, block_tables: torch.Tens
     _elsewhere(index, cache.k, block_tables, ctx_lens, q_start, out, status)
     _check_device(index)
     if out is None:
-        out = q.new_empty((s, num_heads * hd))
+        out = _new_rows(q, s, num_heads * hd)
     _decode_call(q, out, cache, block_tables, ctx_lens, q_start, num_heads, (pages, page_size, nkv, hd), scale, window, code, status, index,
                  workspace, early)
     return out
@@ -349,7 +353,7 @@ def decode_step(qkv: torch.Tensor, positions: torch.Tensor, slots: torch.Tensor,
     _elsewhere(index, block_tables, ctx_lens)
     _check_device(index)
     if not early and code == 1 and head_dim in STEP_HEAD_DIMS and (inv_freq is None or 2 * inv_freq.shape[0] == head_dim):
-        out, stream = qkv.new_empty((n, num_heads * head_dim)), _stream()
+        out, stream = _new_rows(qkv, n, num_heads * head_dim), _stream()
         scratch = _workspace(workspace, head_dim, index, stream)
         result = library().cw_decode_step_e4m3(_STEP_ARGS(
             qkv.data_ptr(), out.data_ptr(), positions.data_ptr(), slots.data_ptr(), 0 if inv_freq is None else inv_freq.data_ptr(),
@@ -507,7 +511,7 @@ def attention_portions(q: torch.Tensor, cache: E4M3Pages, block_tables: torch.Te
     _elsewhere(index, cache.k, block_tables, ctx_lens, q_start, plan.tok_seq, status)
     _check_device(index)
     if code == 1 and hd in fast.PREFILL_HEAD_DIMS:
-        out = q.new_empty((q.shape[0], num_heads * hd))
+        out = _new_rows(q, q.shape[0], num_heads * hd)
         if plan.items:
             held = portion_scratch(cache, q.dtype)
             _read_call(cache, shape, block_tables, ctx_lens, q_start, held.k, held.v, window, max(plan.most_rows + 1, plan.least_rows), code, status)
@@ -571,7 +575,7 @@ def paged_attention(ctx, q: torch.Tensor, cache: E4M3Pages, block_tables: torch.
         # a captured step: how its rows are divided among its requests is not known here, but that none brings more than there are
         most = short_rows(num_heads, nkv, hd) if streams else 0
         if ctx.num_tokens <= most:
-            out = q.new_empty((q.shape[0], num_heads * hd))
+            out = _new_rows(q, q.shape[0], num_heads * hd)
             _short_call(q, out, cache, block_tables, ctx.ctx_lens, ctx.q_start, num_heads, shape, scale, window, ctx.num_tokens, least, most,
                         ctx.status, index, scratch)
             return singles(out) if apart else out

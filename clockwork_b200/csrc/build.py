@@ -6,6 +6,9 @@ library's path.  It is what the first use of a kernel calls, so a fresh checkout
 itself; it prints a progress line per file to stderr.  No Python or torch headers are
 involved: the library exports plain ``extern "C"`` functions loaded with ctypes.
 
+``ensure_calls_built()`` compiles ``quantised_calls.cpp``, host code over torch's headers through which the shortest calls reach
+the library's functions, into a Python module beside it (the host compiler, 15 s).
+
     python -m clockwork_b200.csrc.build          # build now
     python -m clockwork_b200.csrc.build --ptxas  # also print registers / spills / shared memory
 """
@@ -17,6 +20,7 @@ import os
 import shutil
 import subprocess
 import sys
+import sysconfig
 import tempfile
 import time
 from concurrent.futures import ThreadPoolExecutor, as_completed
@@ -129,6 +133,37 @@ def ensure_built(force: bool = False, ptxas_verbose: bool = False) -> Path:
     return lib
 
 
+CALLS_NAME = "quantised_calls"
+
+
+def ensure_calls_built() -> Path:
+    import torch
+
+    src, out_dir = CSRC / f"{CALLS_NAME}.cpp", build_dir()
+    lib, stamp = out_dir / f"{CALLS_NAME}.so", out_dir / f"{CALLS_NAME}.so.digest"
+    digest = hashlib.sha256(src.read_bytes() + f"{torch.__version__} {sys.version}".encode()).hexdigest()
+    if lib.is_file() and stamp.is_file() and stamp.read_text().strip() == digest:
+        return lib
+    compiler = os.environ.get("CXX") or shutil.which("g++") or shutil.which("c++")
+    if compiler is None:
+        raise RuntimeError("no C++ compiler found")
+    _log(f"compiling {src.name} into {out_dir} (first use)")
+    t0, tmp = time.time(), out_dir / f".{CALLS_NAME}.{os.getpid()}"
+    root = Path(torch.__file__).parent
+    cuda = Path(find_nvcc()).resolve().parent.parent
+    includes = [root / "include", root / "include/torch/csrc/api/include", cuda / "include", sysconfig.get_path("include")]
+    proc = subprocess.run([compiler, "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+                           *[f"-I{d}" for d in includes], str(src), "-o", str(tmp), f"-L{root / 'lib'}", "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch_python"],
+                          capture_output=True, text=True)
+    if proc.returncode != 0:
+        raise RuntimeError(f"{compiler} failed on {src.name}:\n{proc.stdout}\n{proc.stderr}")
+    os.replace(tmp, lib)
+    stamp.write_text(digest)
+    _log(f"built {lib.name} in {time.time() - t0:.1f} s")
+    return lib
+
+
 if __name__ == "__main__":
     path = ensure_built(force=True, ptxas_verbose="--ptxas" in sys.argv)
     print(path)
+    print(ensure_calls_built())

@@ -155,6 +155,12 @@ class serial_launch:
 
 
 
+def counted() -> None:
+    """A launch that was made through the library without ``check``."""
+    global _launches
+    _launches += 1
+
+
 def launch_count() -> int:
     """Kernel launches made through this library so far (each entry point launches one kernel)."""
     return _launches

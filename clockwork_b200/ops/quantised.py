@@ -20,7 +20,7 @@ import numpy as np
 import torch
 
 from . import _stream, dtype_code
-from .library import check, library
+from .library import KernelLibraryError, check, counted, library
 
 # The entry points of this module take one block of words (pointers and whole numbers, then the floats), which costs a third of what
 # as many ctypes arguments do: 2 of 5 us of a call whose kernel may take 4.
@@ -49,6 +49,33 @@ class E4M3Pages(NamedTuple):
     v: torch.Tensor
     k_exp: torch.Tensor
     v_exp: torch.Tensor
+
+
+_calls_module = None
+
+
+def _calls():
+    """``csrc/quantised_calls.cpp``: the common calls without the interpreter's share (the store of 8 tokens 12 us of host time in
+    Python, 5 there).  Its functions do nothing and return None where they find anything amiss; the code below then says what."""
+    global _calls_module
+    if _calls_module is None:
+        from importlib.machinery import ExtensionFileLoader
+        from importlib.util import module_from_spec, spec_from_loader
+
+        from ..csrc.build import CALLS_NAME, ensure_calls_built
+
+        lib = library()
+        try:
+            loader = ExtensionFileLoader(CALLS_NAME, str(ensure_calls_built()))
+            module = module_from_spec(spec_from_loader(CALLS_NAME, loader))
+            loader.exec_module(module)
+        except Exception as exc:  # noqa: BLE001
+            raise KernelLibraryError(f"the module of the 8-bit cache's calls is unavailable ({exc})") from exc
+        entries = [ctypes.cast(f, ctypes.c_void_p).value for f in (lib.cw_norm_rotate_store, lib.cw_read_pages, lib.cw_attention_decode_e4m3,
+                                                                   lib.cw_decode_step_e4m3)]
+        module.bind(*entries, E4M3Pages, PlainPages)
+        _calls_module = module
+    return _calls_module
 
 
 def allocate_pages(num_pages: int, page_size: int, num_kv_heads: int, head_dim: int, device) -> E4M3Pages:
@@ -174,6 +201,11 @@ def norm_rotate_store(qkv: torch.Tensor, positions: torch.Tensor, slots: torch.T
 
     ``early``: a promise that ``positions``, ``slots`` and ``inv_freq`` were complete before the kernel in front of this call was
     launched, as a step's inputs are; the call then begins while that kernel finishes."""
+    if qkv.is_cuda:
+        q = _calls().store(qkv, positions, slots, inv_freq, cache, num_heads, num_kv_heads, head_dim, status, q_weight, k_weight, eps, early)
+        if q is not None:
+            counted()
+            return q
     code, n = dtype_code(qkv.dtype), _check_rows(qkv, num_heads, num_kv_heads, head_dim)
     shape = _check_store(qkv, n, positions, slots, inv_freq, cache, num_kv_heads, head_dim, status, q_weight, k_weight)
     _check_device(qkv.get_device())
@@ -201,6 +233,10 @@ def read_pages(cache: E4M3Pages, block_tables: torch.Tensor, ctx_lens: torch.Ten
     request's last page becomes zero; no other page is touched.  ``window``: from the page on that a query at the request's last
     position sees with that window.  ``q_start`` [S + 1] (the rows that the requests bring to a step): only requests that bring
     at least ``least_rows`` rows are read, and the window is that of their first row."""
+    if q_start is None and least_rows == 1 and out_k.is_cuda and _calls().read(cache, block_tables, ctx_lens, out_k, out_v, status, window,
+                                                                               READ_BLOCKS):
+        counted()
+        return
     pages, page_size, nkv, hd = check_pages(cache)
     for name, t in (("out_k", out_k), ("out_v", out_v)):
         if t.shape != cache.k.shape or not t.is_contiguous() or t.dtype != out_k.dtype or t.data_ptr() % 16:
@@ -234,6 +270,7 @@ class DecodeWorkspace:
         self.head_dim = head_dim
         self.floats = torch.empty(floats, dtype=torch.float32, device=device)
         self.words = torch.zeros(words, dtype=torch.int32, device=device)
+        self.pointers = (self.floats.data_ptr(), self.words.data_ptr(), head_dim, self.floats.get_device())
 
 
 @functools.lru_cache(maxsize=None)
@@ -268,6 +305,15 @@ def _workspace(workspace: DecodeWorkspace | None, head_dim: int, index: int, str
     return held
 
 
+def _scratch_of(workspace: DecodeWorkspace | None, cache) -> tuple | None:
+    """The pointers of a call's workspace, if it is there already."""
+    if workspace is None:
+        if type(cache) is not E4M3Pages or torch.cuda.is_current_stream_capturing():
+            return None
+        workspace = _workspaces.get((cache.k.get_device(), _stream(), cache.k.shape[-1]))
+    return None if workspace is None else workspace.pointers
+
+
 def _decode_call(q, out, cache, block_tables, ctx_lens, q_start, num_heads, shape, scale, window, code, status, index, workspace,
                  early=False) -> None:
     pages, page_size, nkv, hd = shape
@@ -295,6 +341,13 @@ def attention_decode(q: torch.Tensor, cache: E4M3Pages, block_tables: torch.Tens
     one per stream).  ``early``: a promise that ``ctx_lens``, ``block_tables``, ``q_start`` and all of the cache but the requests' newest rows
     were complete before the kernel in front of this call was launched, as they are in a step whose inputs were uploaded before
     it; the call then begins to read while that kernel finishes."""
+    if q_start is None and out is None and q.is_cuda:
+        scratch = _scratch_of(workspace, cache)
+        if scratch is not None:
+            out = _calls().decode(q, cache, block_tables, ctx_lens, num_heads, scale, status, window, scratch, _sm_count(q.get_device()), early)
+            if out is not None:
+                counted()
+                return out
     code = dtype_code(q.dtype)
     pages, page_size, nkv, hd = check_pages(cache)
     if q.dim() != 2 or q.shape[1] < num_heads * hd or q.stride(1) != 1:
@@ -339,6 +392,14 @@ def decode_step(qkv: torch.Tensor, positions: torch.Tensor, slots: torch.Tensor,
     block tables (< 0: not stored, and whether it is attended is left open).  ``early``: the promises of both; two kernels run then, each of
     which begins while the one in front finishes.  Without it one does it all in bfloat16, for heads of 64, 128 and 256 entries that
     turn whole or not at all."""
+    if not early and qkv.is_cuda and head_dim in STEP_HEAD_DIMS:
+        scratch = _scratch_of(workspace, cache)
+        if scratch is not None:
+            out = _calls().step(qkv, positions, slots, inv_freq, cache, num_heads, num_kv_heads, head_dim, status, q_weight, k_weight, eps,
+                                block_tables, ctx_lens, scale, window, scratch, _sm_count(qkv.get_device()))
+            if out is not None:
+                counted()
+                return out
     code, n = dtype_code(qkv.dtype), _check_rows(qkv, num_heads, num_kv_heads, head_dim)
     if not isinstance(cache, E4M3Pages):
         raise ValueError(f"an 8-bit cache (E4M3Pages) is needed, got {type(cache).__name__}")

@@ -1,11 +1,14 @@
 """The 8-bit cache's operators as programs use them: captured in graphs, on two streams at once, with and without a workspace of their
 own, called again and again on one workspace, at the ends of their ranges."""
 
+import ctypes
+
 import pytest
 import torch
 
 from clockwork_b200 import ops
 from clockwork_b200.ops import quantised
+from tests import test_e4m3_refusals as refusals
 from tests.e4m3_tools import filled_pages
 from tests.gpu_tools import DEV
 
@@ -246,3 +249,64 @@ def test_steps_whose_rows_begin_at_an_odd_entry():
     ops.raise_on_status(status)
     assert all(torch.equal(x.view(torch.uint8), y.view(torch.uint8)) for x, y in zip(*caches))
     assert torch.equal(*outs)  # (their queries are the same bits: neither is normed nor turned)
+
+
+def _moved(x):
+    if isinstance(x, torch.Tensor):
+        return x.to(DEV) if x.is_contiguous() else x.t().contiguous().to(DEV).t() if x.dim() == 2 and x.t().is_contiguous() else \
+            torch.repeat_interleave(x.to(DEV), 2, -1)[..., ::2]
+    return type(x)(*map(_moved, x)) if isinstance(x, tuple) else x
+
+
+@pytest.fixture
+def entry_points():
+    """The module of common calls with entry points that only count how often they are reached (nothing is launched)."""
+    module, reached = quantised._calls(), []
+    entry = ctypes.CFUNCTYPE(ctypes.c_int, ctypes.c_void_p)(lambda words: reached.append(words) or 0)
+    address = ctypes.cast(entry, ctypes.c_void_p).value
+    module.bind(address, address, address, address, quantised.E4M3Pages, quantised.PlainPages)
+    yield module, reached
+    quantised._calls_module = None  # (bound anew by the next call)
+
+
+def test_common_calls_refuse_what_the_others_name(entry_points):
+    """Every call that the checks in Python refuse, on the GPU's tensors, and mixtures of devices: the short way finds it too."""
+    module, reached = entry_points
+    base = {k: _moved(v) for k, v in refusals._args().items()}
+    ints = lambda *shape: torch.zeros(*shape, dtype=torch.int32, device=DEV)  # noqa: E731
+    scratch = quantised.DecodeWorkspace(128, DEV).pointers
+    names = ("qkv", "positions", "slots", "inv_freq", "cache", "num_heads", "num_kv_heads", "head_dim", "status", "q_weight", "k_weight", "eps")
+    store = {**base, "q_weight": None, "k_weight": None, "eps": 1e-6, "early": False}
+    step = {**store, "block_tables": ints(3, 2), "ctx_lens": ints(3), "scale": 1.0, "window": None, "scratch": scratch, "sms": 148}
+    decode = dict(q=torch.zeros(3, 128, dtype=torch.bfloat16, device=DEV), cache=base["cache"], block_tables=ints(3, 2), ctx_lens=ints(3), num_heads=4,
+                  scale=1.0, status=base["status"], window=None, scratch=scratch, sms=148, early=False)
+    plain = torch.zeros(4, 8, 2, 32, device=DEV)
+    read = dict(cache=base["cache"], block_tables=ints(3, 2), ctx_lens=ints(3), out_k=plain, out_v=plain.clone(), status=base["status"], window=None, blocks=4)
+    forms = [(module.store, store, (*names, "early"), refusals.STORE),
+             (module.step, step, (*names, "block_tables", "ctx_lens", "scale", "window", "scratch", "sms"), refusals.STEP),
+             (module.decode, decode, tuple(decode), [c for c in refusals.DECODE if not {"q_start", "out"} & set(c[0])]),
+             (module.read, read, tuple(read), [c for c in refusals.READ if "q_start" not in c[0]])]
+    for call, good, order, refused in forms:
+        assert call(*(good[name] for name in order)) is not None and len(reached) == 1
+        reached.clear()
+        cases = [{k: _moved(v) for k, v in change.items()} for change, _ in refused if change]
+        for name, value in good.items():  # a tensor elsewhere, of another type, of other sizes; what is no tensor at all
+            if isinstance(value, torch.Tensor):
+                cases += [{name: value.cpu()}, {name: value.to(torch.float16)}, {name: value[1:]}, {name: value[None]}, {name: "x"}, {name: None}]
+            elif isinstance(value, tuple) and name == "cache":
+                cases += [{name: value._replace(**{f: getattr(value, f).cpu()})} for f in value._fields]
+                cases += [{name: value._replace(**{f: getattr(value, f)[:, 1:].contiguous()})} for f in value._fields]
+                cases += [{name: tuple(value)}, {name: None}]
+            elif name == "scratch":
+                cases += [{name: (*value[:2], 16, 0)}, {name: (*value[:3], 1)}, {name: None}]
+            elif isinstance(value, int) and name not in ("early", "sms", "blocks"):
+                cases += [{name: value + 1}, {name: -value}, {name: 0}, {name: 1 << 40}, {name: 1 << 70}, {name: 1.5}]
+        for case in cases:
+            if (case.keys() & {"inv_freq", "q_weight", "k_weight"}) and list(case.values())[0] is None or case.keys() == {"inv_freq"} and \
+                    isinstance(case["inv_freq"], torch.Tensor) and call is module.store and case["inv_freq"].shape == (15,):
+                continue  # (those may be left out, and fewer entries may turn)
+            if case.keys() == {"status"} and isinstance(case["status"], torch.Tensor) and case["status"].shape[:1] == (1,) and case["status"].is_cuda and \
+                    case["status"].dtype == torch.int32:
+                continue  # (four words of any shape)
+            result = call(*({**good, **case}[name] for name in order))
+            assert result is None and not reached, (call, case.keys(), [getattr(v, "shape", v) for v in case.values()])

@@ -52,9 +52,6 @@ struct DecodeE4m3Params {
     float* part_ml;          // [blocks][teams][2][8 or 16][2]
     int* counters;           // [blocks][4] (by the block that a segment begins in: one of a team goes on) and [blocks][4][2], zero between launches
     int least_rows, most_rows;  // portions: the requests that are served
-    // whole steps: q are rows [q | k | v] as the product left them; heads are normed and turned here, the new token stored
-    const int* positions; const int* slots; const float* inv_freq; const float* q_weight; const float* k_weight;
-    float eps;
 };
 
 #define WARPS 4
@@ -133,141 +130,9 @@ struct Piece {
     int first_block, blocks;  // which blocks have pieces of it
 };
 
-// One row of queries, as four lanes hold it in pairs of bfloat16 ([piece][step][pair]: entries 4 PIECE piece + PIECE t + 4 step + 2 pair and
-// the next), normed and turned in float32 and rounded once.  An entry's partner, half a head on, is in the same lane's other pieces,
-// or with heads of 64 (one piece) in lane t ^ 2.
-template <int HD, int PIECES, int STEPS>
-__device__ __forceinline__ void queries_of_step(uint32_t (&w)[PIECES][STEPS][2], const DecodeE4m3Params& p, const float2* turn, int t) {
-    constexpr int PIECE = 4 * STEPS;
-    auto lo = [](uint32_t x) { return __uint_as_float(x << 16); };
-    auto hi = [](uint32_t x) { return __uint_as_float(x & 0xFFFF0000u); };
-    float r = 1.f;
-    if (p.q_weight != nullptr) {
-        float sum = 0.f;
-#pragma unroll
-        for (int b = 0; b < PIECES; ++b)
-#pragma unroll
-            for (int i = 0; i < STEPS; ++i)
-#pragma unroll
-                for (int e = 0; e < 2; ++e) sum = fmaf(lo(w[b][i][e]), lo(w[b][i][e]), fmaf(hi(w[b][i][e]), hi(w[b][i][e]), sum));
-        sum += __shfl_xor_sync(0xffffffffu, sum, 1);
-        sum += __shfl_xor_sync(0xffffffffu, sum, 2);
-        r = __frcp_rn(__fsqrt_rn(__fdiv_rn(sum, (float)HD) + p.eps));
-    }
-    auto normed = [&](uint32_t x, int d) {
-        float2 v = make_float2(lo(x), hi(x));
-        if (p.q_weight != nullptr) {
-            const float2 weight = *reinterpret_cast<const float2*>(p.q_weight + d);
-            v.x *= r * weight.x;
-            v.y *= r * weight.y;
-        }
-        return v;
-    };
-    constexpr int HALF = PIECES > 1 ? PIECES / 2 : 1;
-#pragma unroll
-    for (int b = 0; b < HALF; ++b)
-#pragma unroll
-        for (int i = 0; i < STEPS; ++i)
-#pragma unroll
-            for (int e = 0; e < 2; ++e) {
-                const int d = b * 4 * PIECE + t * PIECE + 4 * i + 2 * e;
-                float2 x = normed(w[b][i][e], d);
-                if (PIECES > 1) {
-                    float2 y = normed(w[(b + HALF) % PIECES][i][e], d + HD / 2);
-                    if (p.inv_freq != nullptr) {
-                        const float4 cs = *reinterpret_cast<const float4*>(turn + d);  // cosine, sine, and the next pair's
-                        const float2 a = x, c = y;
-                        x = make_float2(a.x * cs.x - c.x * cs.y, a.y * cs.z - c.y * cs.w);
-                        y = make_float2(c.x * cs.x + a.x * cs.y, c.y * cs.z + a.y * cs.w);
-                    }
-                    w[(b + HALF) % PIECES][i][e] = pack_bf16(y.x, y.y);
-                } else if (p.inv_freq != nullptr) {
-                    const float2 other = make_float2(__shfl_xor_sync(0xffffffffu, x.x, 2), __shfl_xor_sync(0xffffffffu, x.y, 2));
-                    const float4 cs = *reinterpret_cast<const float4*>(turn + d % (HD / 2));
-                    const float sign = t < 2 ? -1.f : 1.f;
-                    x = make_float2(x.x * cs.x + sign * other.x * cs.y, x.y * cs.z + sign * other.y * cs.w);
-                }
-                w[b][i][e] = pack_bf16(x.x, x.y);
-            }
-}
-
-// The new token's key and value of a KV head by one warp, HD / 32 neighbouring entries a lane (an entry's partner: lane ^ 16): normed,
-// turned, held in 8 bits, put at `k_to` and `v_to` (this lane's bytes of a tile in shared memory, or null) and, if `store`, into the cache.
-// Returns the powers, K's and 256 times V's.
-template <int HD>
-__device__ __forceinline__ uint32_t row_of_step(const DecodeE4m3Params& p, const float2* turn, int row, int kvh, bool store, uint8_t* k_to,
-                                                uint8_t* v_to, int lane) {
-    constexpr int E = HD / 32;
-    const bf16* from = (const bf16*)p.q + (size_t)row * p.q_stride + (size_t)(p.nh + kvh) * HD + lane * E;
-    float x[2][E];
-#pragma unroll
-    for (int i = 0; i < E; i += 2) {
-        const uint32_t k = *reinterpret_cast<const uint32_t*>(from + i), v = *reinterpret_cast<const uint32_t*>(from + (size_t)p.nkv * HD + i);
-        x[0][i] = __uint_as_float(k << 16); x[0][i + 1] = __uint_as_float(k & 0xFFFF0000u);
-        x[1][i] = __uint_as_float(v << 16); x[1][i + 1] = __uint_as_float(v & 0xFFFF0000u);
-    }
-    if (p.k_weight != nullptr) {
-        float sum = 0.f;
-#pragma unroll
-        for (int i = 0; i < E; ++i) sum = fmaf(x[0][i], x[0][i], sum);
-        const float r = __frcp_rn(__fsqrt_rn(__fdiv_rn(warp_sum(sum), (float)HD) + p.eps));
-#pragma unroll
-        for (int i = 0; i < E; ++i) x[0][i] *= r * p.k_weight[lane * E + i];
-    }
-    if (p.inv_freq != nullptr)
-#pragma unroll
-        for (int i = 0; i < E; ++i) {
-            const float2 cs = turn[(lane & 15) * E + i];
-            const float other = __shfl_xor_sync(0xffffffffu, x[0][i], 16);
-            x[0][i] = lane < 16 ? x[0][i] * cs.x - other * cs.y : x[0][i] * cs.x + other * cs.y;
-        }
-    int slot = store ? p.slots[row] : -1;
-    if (slot >= p.num_pages * p.page_size) {
-        if (lane == 0) cw_report(p.status, CW_ST_SLOT_RANGE, row, slot);
-        slot = -1;
-    }
-    uint32_t powers = 0;
-#pragma unroll
-    for (int e = 0; e < 2; ++e) {
-        float big = 0.f;
-#pragma unroll
-        for (int i = 0; i < E; ++i) {
-            x[e][i] = kv_clamped(x[e][i]);
-            big = fmaxf(big, fabsf(x[e][i]));
-        }
-        const int power = kv_power(warp_max(big));
-        const float down = kv_down(power);
-        uint8_t* to = e == 0 ? k_to : v_to;
-        uint8_t* codes = (uint8_t*)(e == 0 ? p.k : p.v) + ((size_t)max(slot, 0) * p.nkv + kvh) * HD + lane * E;
-#pragma unroll
-        for (int i = 0; i < E; i += 2) {
-            const uint16_t two = __nv_cvt_float2_to_fp8x2(make_float2(x[e][i] * down, x[e][i + 1] * down), __NV_SATFINITE, __NV_E4M3);
-            if (to != nullptr) *reinterpret_cast<uint16_t*>(to + i) = two;
-            if (slot >= 0) *reinterpret_cast<uint16_t*>(codes + i) = two;
-        }
-        if (slot >= 0 && lane == 0) {
-            const int off = slot % p.page_size;
-            ((uint8_t*)(e == 0 ? p.k_exp : p.v_exp))[(size_t)(slot - off) * p.nkv + (size_t)kvh * p.page_size + off] = (uint8_t)power;
-        }
-        powers |= (uint32_t)power << (8 * e);
-    }
-    return powers;
-}
-
-// MODE: single tokens whose queries and rows are ready (TOKENS_READY), portions of few rows (PORTION_ROWS), or whole steps of single
-// tokens (WHOLE_STEP): norms and rotation as a warp takes up a segment's queries, the new key and value by the warp that walks the
-// segment's last tile, into its ring and into the cache.  Whole steps are for callers that launch one call after the other,
-// whose time is mostly the host's (us a call, one kernel and two: 12 heads over 2 of 128, 8 requests of 1,000 tokens 16.7 and 25.2, 64 of 300 18.1
-// and 25.3, 64 of 4,000 39.1 and 37.4; 16 heads of 64, 64 of 4,000 115 and 118).  In a captured step two kernels are faster: this one's
-// rings find no room beside the matrix product in front of it, while a store does, and attention's beginning hides behind that (8 layers,
-// products and all: 8 x 1,024 tokens 461 us as two, 498 as one; 64 x 4,096 702 and 718).
-#define TOKENS_READY 0
-#define PORTION_ROWS 1
-#define WHOLE_STEP 2
-template <int HD, int NT, int MODE>
+template <int HD, int NT, bool PORTIONS>
 __global__ void __launch_bounds__(WARPS * 32, Stream<HD, NT>::PER_SM) decode_e4m3_kernel(const DecodeE4m3Params p) {
     using C = Stream<HD, NT>;
-    constexpr bool PORTIONS = MODE == PORTION_ROWS, STEP = MODE == WHOLE_STEP;
     static_assert(!PORTIONS || 8 * NT <= 32, "a lane to a row");
     constexpr int ROWS = 8 * NT, ST = C::ST, CH = C::CH, TOKENS = C::TOKENS;
     constexpr int U = TOKENS / 16, HALVES = (TOKENS + 31) / 32;  // products' 16 tokens; a lane's tokens when pages are looked up
@@ -279,10 +144,9 @@ __global__ void __launch_bounds__(WARPS * 32, Stream<HD, NT>::PER_SM) decode_e4m
     __shared__ Piece piece_s[2 * WARPS];  // of every warp: the end of a segment that began before its run, and what its run ends in
     __shared__ float top_s[2 * WARPS][ROWS], total_s[2 * WARPS][ROWS];  // of a group of pieces, at its first
     __shared__ int limit_s[WARPS][PORTIONS ? ROWS : 1];
-    __shared__ __align__(16) float2 turn_s[STEP ? WARPS : 1][STEP ? HD / 2 : 1];  // cosine and sine of every pair at a warp's request
     __shared__ int shared_s[2 * MOST_TEAMS], last_s[2 * MOST_TEAMS], final_s;
     // (early: what the kernel in front writes, queries and the newest rows, is waited for only where it is first needed)
-    bool waited = MODE != TOKENS_READY || !p.early;
+    bool waited = PORTIONS || !p.early;
     if (waited)
         pdl_enter();
     else
@@ -338,24 +202,11 @@ __global__ void __launch_bounds__(WARPS * 32, Stream<HD, NT>::PER_SM) decode_e4m
     total *= kv_units;
     const int quota = max(LEAST_UNITS, (total + warps - 1) / warps), block_units = quota * of_team;
     const int first = (int)min((long long)(blockIdx.x * of_team + member) * quota, (long long)total);
-    // (whole steps) a request's cosines and sines
-    int turned = -1;
-    auto turn = [&](int s) {
-        if (!STEP || p.inv_freq == nullptr || turned == s) return;
-        turned = s;
-        __syncwarp();
-        for (int j = lane; j < HD / 2; j += 32) turn_of(p.positions[s], p.inv_freq[j], turn_s[warp][j].y, turn_s[warp][j].x);
-        __syncwarp();
-    };
-    auto zeros = [&]() {  // the rows of requests without a context (a whole step stores their tokens all the same)
+    auto zeros = [&]() {  // the rows of requests without a context
         for (int s = blockIdx.x; s < p.requests; s += gridDim.x) {
             if (PORTIONS || tokens_of(s) == 0 || context_of(s) > 0) continue;
             const int row = p.q_start != nullptr ? p.q_start[s] : s;
             for (int i = tid; i < p.nh * HD; i += blockDim.x) ((bf16*)p.out)[(size_t)row * p.nh * HD + i] = __float2bfloat16_rn(0.f);
-            if (!STEP || p.slots[row] < 0) continue;
-            turn(s);
-#pragma unroll 1
-            for (int kvh = warp; kvh < p.nkv; kvh += WARPS) row_of_step<HD>(p, turn_s[STEP ? warp : 0], row, kvh, true, nullptr, nullptr, lane);
         }
     };
     if ((long long)blockIdx.x * block_units >= total) {
@@ -480,9 +331,7 @@ __global__ void __launch_bounds__(WARPS * 32, Stream<HD, NT>::PER_SM) decode_e4m
             for (int h = 0; h < HALVES; ++h) {
                 const int pos = ahead_pos + 32 * h, page = ahead_page[h];
                 uint32_t row = ~0u, power_at = 0;
-                if (STEP && pos == ahead.ctx - 1) {
-                    // (the new token: its row is made below)
-                } else if (page >= 0 && page < p.num_pages) {
+                if (page >= 0 && page < p.num_pages) {
                     const int off = p.page_shift >= 0 ? pos & (p.page_size - 1) : pos % p.page_size;
                     row = ((uint32_t)(page * p.page_size + off) * p.nkv + kvh) * CH;
                     power_at = ((uint32_t)page * p.nkv + kvh) * p.page_size + off;
@@ -543,7 +392,6 @@ __global__ void __launch_bounds__(WARPS * 32, Stream<HD, NT>::PER_SM) decode_e4m
     while (at.left > 0) {
         const int row = query_row(at), head = kv_head(at) * each, x0 = first_of(at), rows = rows_of(at);
         const int n_tiles = min(at.tiles - at.tile, at.left);
-        turn(at.s);
         // ---- the group's queries, as B fragments over the entries that a lane's pieces of K hold: half precision, a power of two out ----
         uint32_t qb[NT][PIECES][STEPS][2];
         float qf[NT][2], m[NT][2], l[NT][2], o[NT][HD / 16][4];
@@ -560,15 +408,6 @@ __global__ void __launch_bounds__(WARPS * 32, Stream<HD, NT>::PER_SM) decode_e4m
                         uint32_t w = 0;
                         if (8 * n + g < rows) w = *reinterpret_cast<const uint32_t*>(q + b * 4 * PIECE + t * PIECE + 4 * i + 2 * e);
                         qb[n][b][i][e] = w;
-                    }
-            if (STEP) queries_of_step<HD, PIECES, STEPS>(qb[n], p, turn_s[STEP ? warp : 0], t);
-#pragma unroll
-            for (int b = 0; b < PIECES; ++b)
-#pragma unroll
-                for (int i = 0; i < STEPS; ++i)
-#pragma unroll
-                    for (int e = 0; e < 2; ++e) {
-                        const uint32_t w = qb[n][b][i][e];
                         big = fmaxf(big, fmaxf(fabsf(__uint_as_float(w << 16)), fabsf(__uint_as_float(w & 0xFFFF0000u))));
                     }
             big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 1));
@@ -606,19 +445,6 @@ __global__ void __launch_bounds__(WARPS * 32, Stream<HD, NT>::PER_SM) decode_e4m
             cp_async_wait<ST - 1>();
             __syncwarp();
             const int next = stage + 1 == ST ? 0 : stage + 1;
-            if (STEP && at.tile + i == at.tiles - 1) {  // the new token's row, into this tile and the cache
-                const int r = at.ctx - 1 - pos0;
-                uint8_t* k_at = my_ring + stage * 2 * C::TILE_BYTES + C::at(r, lane * (HD / 32) / 16) + lane * (HD / 32) % 16;
-                const uint32_t made = row_of_step<HD>(p, turn_s[STEP ? warp : 0], row, kv_head(at), x0 == 0, k_at, k_at + C::TILE_BYTES, lane);
-#pragma unroll
-                for (int h = 0; h < HALVES; ++h)
-                    if (32 * h + 8 * (TOKENS >= 32 ? t : t & 1) + g == r) {
-                        counts[h] = 0;
-                        k_power[h] = made & 255;
-                        v_power[h] = made >> 8;
-                    }
-                __syncwarp();
-            }
             uint32_t powers[HALVES];
 #pragma unroll
             for (int h = 0; h < HALVES; ++h) powers[h] = counts[h] == ~0u ? 0u : k_power[h] | v_power[h] << 8 | 1u << 16;
@@ -1072,23 +898,23 @@ __global__ void __launch_bounds__(ANY_TOKENS) decode_e4m3_any_kernel(const Decod
         if (tid + e * ANY_TOKENS < p.hd) out[tid + e * ANY_TOKENS] = from_f<T>(l > 0.f ? acc[e] / l : (l == l ? 0.f : l));
 }
 
-template <int HD, int NT, int MODE>
+template <int HD, int NT, bool PORTIONS>
 static int stream_launch(const DecodeE4m3Params& p, int sms, cudaStream_t stream) {
     using C = Stream<HD, NT>;
     static bool configured[64] = {};  // (per device)
     int device = 0;
     cudaGetDevice(&device);
     if (device < 0 || device >= 64 || !configured[device]) {
-        const cudaError_t e = cudaFuncSetAttribute(decode_e4m3_kernel<HD, NT, MODE>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::RING);
+        const cudaError_t e = cudaFuncSetAttribute(decode_e4m3_kernel<HD, NT, PORTIONS>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::RING);
         if (e != cudaSuccess) return (int)e;
         if (device >= 0 && device < 64) configured[device] = true;
     }
-    return cw_launch(decode_e4m3_kernel<HD, NT, MODE>, dim3(sms * C::PER_SM), dim3(WARPS * 32), C::RING, stream, 1u, p);
+    return cw_launch(decode_e4m3_kernel<HD, NT, PORTIONS>, dim3(sms * C::PER_SM), dim3(WARPS * 32), C::RING, stream, 1u, p);
 }
-template <int HD, int MODE>
+template <int HD>
 static int stream_launch_heads(const DecodeE4m3Params& p, int sms, cudaStream_t stream) {
-    if (p.heads_each <= 8) return stream_launch<HD, 1, MODE>(p, sms, stream);
-    return stream_launch<(HD <= 128 ? HD : 64), 2, MODE>(p, sms, stream);  // (head sizes beyond 128 come in groups of 8)
+    if (p.heads_each <= 8) return stream_launch<HD, 1, false>(p, sms, stream);
+    return stream_launch<(HD <= 128 ? HD : 32), 2, false>(p, sms, stream);  // (head sizes beyond 128 come in groups of 8)
 }
 
 // How a KV head's query heads are shared out: groups of 16 at most, of 8 where heads are so large that the sums of 16 would not
@@ -1149,57 +975,19 @@ extern "C" int cw_attention_decode_e4m3(const char* block) {
         p.heads_each = (nh / nkv + groups - 1) / groups;
         p.teams = hd == 32 && nkv % 4 == 0 ? 4 : hd < 128 && nkv % 2 == 0 ? 2 : 1;
         switch (hd) {
-            case 32: return stream_launch_heads<32, TOKENS_READY>(p, sms, stream);
-            case 64: return stream_launch_heads<64, TOKENS_READY>(p, sms, stream);
-            case 96: return stream_launch_heads<96, TOKENS_READY>(p, sms, stream);
-            case 128: return stream_launch_heads<128, TOKENS_READY>(p, sms, stream);
-            case 160: return stream_launch_heads<160, TOKENS_READY>(p, sms, stream);
-            case 192: return stream_launch_heads<192, TOKENS_READY>(p, sms, stream);
-            case 224: return stream_launch_heads<224, TOKENS_READY>(p, sms, stream);
-            case 256: return stream_launch_heads<256, TOKENS_READY>(p, sms, stream);
+            case 32: return stream_launch_heads<32>(p, sms, stream);
+            case 64: return stream_launch_heads<64>(p, sms, stream);
+            case 96: return stream_launch_heads<96>(p, sms, stream);
+            case 128: return stream_launch_heads<128>(p, sms, stream);
+            case 160: return stream_launch_heads<160>(p, sms, stream);
+            case 192: return stream_launch_heads<192>(p, sms, stream);
+            case 224: return stream_launch_heads<224>(p, sms, stream);
+            case 256: return stream_launch_heads<256>(p, sms, stream);
         }
     }
     if (dtype == 0) return cw_launch(decode_e4m3_any_kernel<float>, dim3(nh, requests), dim3(ANY_TOKENS), 0, stream, 1u, p);
     if (dtype == 1) return cw_launch(decode_e4m3_any_kernel<bf16>, dim3(nh, requests), dim3(ANY_TOKENS), 0, stream, 1u, p);
     return CW_ERR_BAD_DTYPE;
-}
-
-// norm_rotate_store of one new token per request and attention of it in one kernel: qkv [requests, (nh + 2 nkv) hd] as the product left
-// it, request s's new token at positions[s] and slots[s] (< 0: not stored) and the last of its ctx_lens[s] tokens.  bfloat16, heads
-// of 64, 128 and 256 entries that turn whole (inv_freq [hd / 2]) or not at all (null); CW_ERR_UNSUPPORTED otherwise.
-extern "C" int cw_decode_step_e4m3(const char* block) {
-    ArgumentWords w(block);
-    const void* qkv = w.pointer(); void* out = w.pointer();
-    const int *positions = (const int*)w.pointer(), *slots = (const int*)w.pointer();
-    const float *inv_freq = (const float*)w.pointer(), *q_weight = (const float*)w.pointer(), *k_weight = (const float*)w.pointer();
-    const uint8_t *k = (const uint8_t*)w.pointer(), *v = (const uint8_t*)w.pointer(), *k_exp = (const uint8_t*)w.pointer(), *v_exp = (const uint8_t*)w.pointer();
-    const int *block_tables = (const int*)w.pointer(), *ctx_lens = (const int*)w.pointer();
-    float* floats = (float*)w.pointer();
-    int *words = (int*)w.pointer(), *status = (int*)w.pointer();
-    const cudaStream_t stream = (cudaStream_t)w.pointer();
-    const int requests = w.number(), nh = w.number(), nkv = w.number(), hd = w.number(), page_size = w.number(), max_blocks = w.number(),
-              num_pages = w.number(), window = w.number(), sms = w.number();
-    const float scale = (float)w.real(), eps = (float)w.real();
-    if (requests == 0) return CW_OK;
-    if (requests < 0 || nh <= 0 || nkv <= 0 || nh % nkv || page_size <= 0 || max_blocks <= 0 || num_pages <= 0 || window < 0 ||
-        ((uintptr_t)k | (uintptr_t)v) % 16 || sms <= 0 || (long long)num_pages * page_size > 0x7FFFFFFF ||
-        (long long)max_blocks * page_size > 0x7FFFFFFF || (long long)(nh + 2 * nkv) * hd > 0x7FFFFFFF)
-        return CW_ERR_BAD_SIZE;
-    if (((uintptr_t)q_weight | (uintptr_t)k_weight) % 8) return CW_ERR_UNSUPPORTED;
-    DecodeE4m3Params p = {qkv, (nh + 2 * nkv) * hd, out, k, v, k_exp, v_exp, block_tables, ctx_lens, nullptr, requests, nh, nkv, hd, page_size,
-                          max_blocks, num_pages, window, scale, status};
-    const int groups = groups_of(nh, nkv, hd, 1);
-    if (!groups || !streams(p, (long long)requests * groups, sms, floats, words)) return CW_ERR_UNSUPPORTED;
-    p.groups = groups;
-    p.heads_each = (nh / nkv + groups - 1) / groups;
-    p.teams = hd < 128 && nkv % 2 == 0 ? 2 : 1;
-    p.positions = positions; p.slots = slots; p.inv_freq = inv_freq; p.q_weight = q_weight; p.k_weight = k_weight; p.eps = eps;
-    switch (hd) {
-        case 64: return stream_launch_heads<64, WHOLE_STEP>(p, sms, stream);
-        case 128: return stream_launch_heads<128, WHOLE_STEP>(p, sms, stream);
-        case 256: return stream_launch_heads<256, WHOLE_STEP>(p, sms, stream);
-    }
-    return CW_ERR_UNSUPPORTED;
 }
 
 // Causal attention of the portions of requests that bring `least_rows` to `most_rows` rows, q_start[s] .. q_start[s + 1] of q and out
@@ -1229,10 +1017,10 @@ extern "C" int cw_attention_portions_e4m3(const char* block) {
     p.most_rows = most_rows;
     if (!streams(p, (long long)rows * (nh / nkv) / 16 + requests, sms, floats, words)) return CW_ERR_UNSUPPORTED;
     switch (hd) {
-        case 32: return stream_launch<32, 2, PORTION_ROWS>(p, sms, stream);
-        case 64: return stream_launch<64, 2, PORTION_ROWS>(p, sms, stream);
-        case 96: return stream_launch<96, 2, PORTION_ROWS>(p, sms, stream);
-        case 128: return stream_launch<128, 2, PORTION_ROWS>(p, sms, stream);
+        case 32: return stream_launch<32, 2, true>(p, sms, stream);
+        case 64: return stream_launch<64, 2, true>(p, sms, stream);
+        case 96: return stream_launch<96, 2, true>(p, sms, stream);
+        case 128: return stream_launch<128, 2, true>(p, sms, stream);
     }
     return CW_ERR_UNSUPPORTED;
 }

@@ -23,6 +23,20 @@ struct StoreParams {
     int* status;
 };
 
+// sin and cos of position * freq (a product that float64 holds exactly), rounded once: the angle less the nearest multiple k of pi/2,
+// which leaves |x| <= pi/4, then the Taylor sums to x^11 and x^10 (the next terms are below 2^-33), turned by k quarters.
+__device__ __forceinline__ void turn_of(int position, float freq, float& sn, float& cs) {
+    const double angle = (double)position * (double)freq, k = rint(angle * 0.63661977236758134308);
+    // pi/2 as a float64 and what that leaves of it
+    const double x = fma(-k, 6.123233995736766e-17, fma(-k, 1.5707963267948966, angle)), y = x * x;
+    const double s = x * fma(y, fma(y, fma(y, fma(y, fma(y, -1.0 / 39916800, 1.0 / 362880), -1.0 / 5040), 1.0 / 120), -1.0 / 6), 1.0);
+    const double c = fma(y, fma(y, fma(y, fma(y, fma(y, -1.0 / 3628800, 1.0 / 40320), -1.0 / 720), 1.0 / 24), -0.5), 1.0);
+    const int quarter = (int)((long long)k & 3);
+    const float a = (float)(quarter & 1 ? c : s), b = (float)(quarter & 1 ? s : c);
+    sn = quarter & 2 ? -a : a;
+    cs = (quarter == 1 || quarter == 2) ? -b : b;
+}
+
 // Two float32 products, or products and sums, at a time.
 __device__ __forceinline__ float2 mul2(float2 a, float2 b) {
     unsigned long long d;

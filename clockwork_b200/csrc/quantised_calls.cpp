@@ -18,7 +18,7 @@ namespace {
 
 using at::Tensor;
 typedef int (*Entry)(const char*);
-Entry store_entry, read_entry, decode_entry, step_entry;
+Entry store_entry, read_entry, decode_entry;
 PyTypeObject *e4m3_type, *plain_type;
 
 struct Refused : std::exception {};
@@ -169,11 +169,7 @@ struct Scratch {
     }
 };
 
-// qkv, positions, slots, inv_freq, cache, heads, KV heads, entries, status, q_weight, k_weight, eps, early
-PyObject* store(PyObject* const* a) {
-    const Rows r(a[0], a[1], a[2], a[3], a[4], a[5], a[6], a[7], a[8], a[9], a[10]);
-    const double eps = real(a[11]);
-    const int early = truth(a[12]);
+Tensor stored(const Rows& r, double eps, int early) {
     Tensor q = at::empty({r.n, r.nh * r.hd}, r.qkv.options());
     Words()
         .pointer(r.qkv.const_data_ptr()).pointer(q.const_data_ptr()).pointer(r.positions).pointer(r.slots).pointer(r.inv_freq)
@@ -181,51 +177,58 @@ PyObject* store(PyObject* const* a) {
         .whole(r.n).whole(r.nh).whole(r.nkv).whole(r.hd).whole(r.rot).whole(r.cache.page_size).whole(r.cache.pages)
         .whole(type_code(r.qkv)).whole(early).number(eps)
         .call(store_entry);
-    return THPVariable_Wrap(std::move(q));
+    return q;
 }
-
-// the same but early, then block tables, ctx_lens, scale, window, workspace, SMs
-PyObject* step(PyObject* const* a) {
+// qkv, positions, slots, inv_freq, cache, heads, KV heads, entries, status, q_weight, k_weight, eps, early
+PyObject* store(PyObject* const* a) {
     const Rows r(a[0], a[1], a[2], a[3], a[4], a[5], a[6], a[7], a[8], a[9], a[10]);
-    const double eps = real(a[11]), scale = real(a[14]);
-    const Tensor &tables = of_type(a[12], at::kInt, 2, r.device), &ctx = of_type(a[13], at::kInt, 1, r.device);
-    need(r.cache.k_exp != nullptr && type_code(r.qkv) == 1 && r.nh % r.nkv == 0 && r.hd % 32 == 0 && (r.rot == 0 ? a[3] == Py_None : r.rot == r.hd));
-    need(tables.size(0) == r.n && ctx.size(0) == r.n);
-    const long long window = window_of(a[15]), sms = number(a[17]);
-    const Scratch scratch(a[16], r.hd, r.device);
-    Tensor out = at::empty({r.n, r.nh * r.hd}, r.qkv.options());
-    Words()
-        .pointer(r.qkv.const_data_ptr()).pointer(out.const_data_ptr()).pointer(r.positions).pointer(r.slots).pointer(r.inv_freq)
-        .pointer(r.q_weight).pointer(r.k_weight).pages(r.cache).pointer(tables.const_data_ptr()).pointer(ctx.const_data_ptr())
-        .pointer(scratch.floats).pointer(scratch.words).pointer(r.status).stream()
-        .whole(r.n).whole(r.nh).whole(r.nkv).whole(r.hd).whole(r.cache.page_size).whole(tables.size(1)).whole(r.cache.pages)
-        .whole(window).whole(sms).number(scale).number(eps)
-        .call(step_entry);
-    return THPVariable_Wrap(std::move(out));
+    return THPVariable_Wrap(stored(r, real(a[11]), truth(a[12])));
 }
 
+// What attention of single tokens reads besides its queries and the cache.
+struct Tokens {
+    const Tensor &tables, &ctx;
+    int64_t s, nh;
+    double scale;
+    const void* status;
+    long long window, sms;
+    Scratch scratch;
+    Tokens(PyObject* table, PyObject* lens, PyObject* heads, PyObject* factor, PyObject* words, PyObject* seen, PyObject* room, PyObject* count,
+           const Pages& cache, int device)
+        : tables(of_type(table, at::kInt, 2, device)), ctx(of_type(lens, at::kInt, 1, device)), s(tables.size(0)), nh(number(heads)),
+          scale(real(factor)), status(status_of(words, device)), window(window_of(seen)), sms(number(count)), scratch(room, cache.hd, device) {
+        need(nh > 0 && nh < (1 << 20) && cache.nkv > 0 && nh % cache.nkv == 0 && cache.hd % 32 == 0 && cache.hd <= 256 && ctx.size(0) == s);
+    }
+    Tensor attended(const Tensor& q, const Pages& cache, int early) const {
+        Tensor out = at::empty({s, nh * cache.hd}, q.options());
+        Words()
+            .pointer(q.const_data_ptr()).pointer(out.const_data_ptr()).pages(cache).pointer(tables.const_data_ptr()).pointer(ctx.const_data_ptr())
+            .pointer(nullptr).pointer(scratch.floats).pointer(scratch.words).pointer(status).stream()
+            .whole(s > 1 ? q.stride(0) : nh * cache.hd).whole(s).whole(nh).whole(cache.nkv).whole(cache.hd).whole(cache.page_size)
+            .whole(tables.size(1)).whole(cache.pages).whole(window).whole(1).whole(sms).whole(early).number(scale)
+            .call(decode_entry);
+        return out;
+    }
+};
 // q, cache, block tables, ctx_lens, heads, scale, status, window, workspace, SMs, early
 PyObject* decode(PyObject* const* a) {
     const Tensor& q = tensor(a[0]);
     const int device = cuda_device(q);
     const Pages cache = quantised_pages(a[1], device);
-    const Tensor &tables = of_type(a[2], at::kInt, 2, device), &ctx = of_type(a[3], at::kInt, 1, device);
-    const int64_t nh = number(a[4]), s = tables.size(0);
-    need(type_code(q) == 1 && nh > 0 && nh < (1 << 20) && cache.nkv > 0 && nh % cache.nkv == 0 && cache.hd % 32 == 0 && cache.hd <= 256);
-    need(q.dim() == 2 && q.size(0) == s && q.size(1) >= nh * cache.hd && q.stride(1) == 1 && ctx.size(0) == s);
-    const double scale = real(a[5]);
-    const void* status = status_of(a[6], device);
-    const long long window = window_of(a[7]), sms = number(a[9]);
-    const Scratch scratch(a[8], cache.hd, device);
-    const int early = truth(a[10]);
-    Tensor out = at::empty({s, nh * cache.hd}, q.options());
-    Words()
-        .pointer(q.const_data_ptr()).pointer(out.const_data_ptr()).pages(cache).pointer(tables.const_data_ptr()).pointer(ctx.const_data_ptr())
-        .pointer(nullptr).pointer(scratch.floats).pointer(scratch.words).pointer(status).stream()
-        .whole(s > 1 ? q.stride(0) : nh * cache.hd).whole(s).whole(nh).whole(cache.nkv).whole(cache.hd).whole(cache.page_size)
-        .whole(tables.size(1)).whole(cache.pages).whole(window).whole(1).whole(sms).whole(early).number(scale)
-        .call(decode_entry);
-    return THPVariable_Wrap(std::move(out));
+    const Tokens t(a[2], a[3], a[4], a[5], a[6], a[7], a[8], a[9], cache, device);
+    need(type_code(q) == 1 && q.dim() == 2 && q.size(0) == t.s && q.size(1) >= t.nh * cache.hd && q.stride(1) == 1);
+    return THPVariable_Wrap(t.attended(q, cache, truth(a[10])));
+}
+// store's arguments, then block tables, ctx_lens, scale, window, workspace, SMs
+PyObject* step(PyObject* const* a) {
+    const Rows r(a[0], a[1], a[2], a[3], a[4], a[5], a[6], a[7], a[8], a[9], a[10]);
+    const double eps = real(a[11]);
+    const int early = truth(a[12]);
+    need(r.cache.k_exp != nullptr && type_code(r.qkv) == 1);
+    const Tokens t(a[13], a[14], a[5], a[15], a[8], a[16], a[17], a[18], r.cache, r.device);
+    need(t.s == r.n);
+    // (what the attention could still refuse, sizes beyond its counters, is refused again by the caller's way, behind the same store)
+    return THPVariable_Wrap(t.attended(stored(r, eps, early), r.cache, 1));
 }
 
 // cache, block tables, ctx_lens, out_k, out_v, status, window, blocks
@@ -257,17 +260,16 @@ PyObject* guarded(PyObject*, PyObject* const* args, Py_ssize_t n) {
     Py_RETURN_NONE;
 }
 
-// addresses of the entry points (store, read, decode, step), E4M3Pages, PlainPages
+// addresses of the entry points (store, read, decode), E4M3Pages, PlainPages
 PyObject* bind(PyObject*, PyObject* args) {
-    unsigned long long s, r, d, w;
+    unsigned long long s, r, d;
     PyObject *e, *p;
-    if (!PyArg_ParseTuple(args, "KKKKO!O!", &s, &r, &d, &w, &PyType_Type, &e, &PyType_Type, &p)) return nullptr;
+    if (!PyArg_ParseTuple(args, "KKKO!O!", &s, &r, &d, &PyType_Type, &e, &PyType_Type, &p)) return nullptr;
     Py_INCREF(e);
     Py_INCREF(p);
     store_entry = (Entry)s;
     read_entry = (Entry)r;
     decode_entry = (Entry)d;
-    step_entry = (Entry)w;
     e4m3_type = (PyTypeObject*)e;
     plain_type = (PyTypeObject*)p;
     Py_RETURN_NONE;
@@ -275,7 +277,7 @@ PyObject* bind(PyObject*, PyObject* args) {
 
 PyMethodDef methods[] = {{"bind", bind, METH_VARARGS, nullptr},
                          {"store", (PyCFunction)(void*)guarded<store, 13>, METH_FASTCALL, nullptr},
-                         {"step", (PyCFunction)(void*)guarded<step, 18>, METH_FASTCALL, nullptr},
+                         {"step", (PyCFunction)(void*)guarded<step, 19>, METH_FASTCALL, nullptr},
                          {"decode", (PyCFunction)(void*)guarded<decode, 11>, METH_FASTCALL, nullptr},
                          {"read", (PyCFunction)(void*)guarded<read, 8>, METH_FASTCALL, nullptr},
                          {nullptr, nullptr, 0, nullptr}};

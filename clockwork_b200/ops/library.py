@@ -79,8 +79,7 @@ _SIGNATURES: dict[str, list] = {
     "cw_latent_attention_on_tensor_cores": [I, I],
     # a cache in 8 bits (csrc/kv_e4m3.cu, csrc/attention_decode_e4m3.cu)
     "cw_norm_rotate_store": [c_char_p], "cw_read_pages": [c_char_p], "cw_attention_decode_e4m3": [c_char_p],
-    "cw_attention_portions_e4m3": [c_char_p], "cw_decode_step_e4m3": [c_char_p],
-    "cw_attention_e4m3_scratch": [I, I, P, P],
+    "cw_attention_portions_e4m3": [c_char_p], "cw_attention_e4m3_scratch": [I, I, P, P],
 }
 _OPTIONAL: dict[str, list] = {}
 

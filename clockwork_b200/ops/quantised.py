@@ -28,8 +28,6 @@ _STORE_ARGS = struct.Struct("22qd").pack
 _READ_ARGS = struct.Struct("21q").pack
 _DECODE_ARGS = struct.Struct("25qd").pack
 _PORTION_ARGS = struct.Struct("26qd").pack
-_STEP_ARGS = struct.Struct("26qdd").pack
-_UNSUPPORTED = -3
 
 CODES = torch.float8_e4m3fn
 MAX_HEAD_DIM = 256
@@ -71,8 +69,7 @@ def _calls():
             loader.exec_module(module)
         except Exception as exc:  # noqa: BLE001
             raise KernelLibraryError(f"the module of the 8-bit cache's calls is unavailable ({exc})") from exc
-        entries = [ctypes.cast(f, ctypes.c_void_p).value for f in (lib.cw_norm_rotate_store, lib.cw_read_pages, lib.cw_attention_decode_e4m3,
-                                                                   lib.cw_decode_step_e4m3)]
+        entries = [ctypes.cast(f, ctypes.c_void_p).value for f in (lib.cw_norm_rotate_store, lib.cw_read_pages, lib.cw_attention_decode_e4m3)]
         module.bind(*entries, E4M3Pages, PlainPages)
         _calls_module = module
     return _calls_module
@@ -380,24 +377,22 @@ def attention_decode(q: torch.Tensor, cache: E4M3Pages, block_tables: torch.Tens
     return out
 
 
-STEP_HEAD_DIMS = (64, 128, 256)
-
-
 def decode_step(qkv: torch.Tensor, positions: torch.Tensor, slots: torch.Tensor, inv_freq: torch.Tensor | None, cache: E4M3Pages,
                 block_tables: torch.Tensor, ctx_lens: torch.Tensor, num_heads: int, num_kv_heads: int, head_dim: int, scale: float,
                 status: torch.Tensor, *, q_weight: torch.Tensor | None = None, k_weight: torch.Tensor | None = None,
                 eps: float = 0.0, window: int | None = None, workspace: DecodeWorkspace | None = None, early: bool = False) -> torch.Tensor:
-    """``norm_rotate_store`` of one new token per request and ``attention_decode`` of it: what an attention layer does between its two
-    products while every request decodes.  ``slots`` name the places of the new tokens, the last of their requests' ``ctx_lens``, in the
-    block tables (< 0: not stored, and whether it is attended is left open).  ``early``: the promises of both; two kernels run then, each of
-    which begins while the one in front finishes.  Without it one does it all in bfloat16, for heads of 64, 128 and 256 entries that
-    turn whole or not at all."""
-    if not early and qkv.is_cuda and head_dim in STEP_HEAD_DIMS:
+    """``norm_rotate_store`` of one new token per request, then ``attention_decode`` of it: what an attention layer does between
+    its two products while every request decodes.  ``ctx_lens`` count the new tokens; ``slots`` name their places (the last of their
+    requests) in the block tables, < 0: not stored.  ``early``: the promise of ``norm_rotate_store``."""
+    # (Attention begins while the store finishes whether or not this call does while the kernel in front of it finishes: a store that
+    # makes no such promise lets its successor come only when everything in front of it is complete, and itself writes only the newest rows.)
+    if qkv.is_cuda:
         scratch = _scratch_of(workspace, cache)
         if scratch is not None:
-            out = _calls().step(qkv, positions, slots, inv_freq, cache, num_heads, num_kv_heads, head_dim, status, q_weight, k_weight, eps,
+            out = _calls().step(qkv, positions, slots, inv_freq, cache, num_heads, num_kv_heads, head_dim, status, q_weight, k_weight, eps, early,
                                 block_tables, ctx_lens, scale, window, scratch, _sm_count(qkv.get_device()))
             if out is not None:
+                counted()
                 counted()
                 return out
     code, n = dtype_code(qkv.dtype), _check_rows(qkv, num_heads, num_kv_heads, head_dim)
@@ -413,23 +408,11 @@ def decode_step(qkv: torch.Tensor, positions: torch.Tensor, slots: torch.Tensor,
     index = qkv.get_device()
     _elsewhere(index, block_tables, ctx_lens)
     _check_device(index)
-    if not early and code == 1 and head_dim in STEP_HEAD_DIMS and (inv_freq is None or 2 * inv_freq.shape[0] == head_dim):
-        out, stream = _new_rows(qkv, n, num_heads * head_dim), _stream()
-        scratch = _workspace(workspace, head_dim, index, stream)
-        result = library().cw_decode_step_e4m3(_STEP_ARGS(
-            qkv.data_ptr(), out.data_ptr(), positions.data_ptr(), slots.data_ptr(), 0 if inv_freq is None else inv_freq.data_ptr(),
-            0 if q_weight is None else q_weight.data_ptr(), 0 if k_weight is None else k_weight.data_ptr(), cache.k.data_ptr(), cache.v.data_ptr(),
-            cache.k_exp.data_ptr(), cache.v_exp.data_ptr(), block_tables.data_ptr(), ctx_lens.data_ptr(), scratch.floats.data_ptr(),
-            scratch.words.data_ptr(), status.data_ptr(), stream, n, num_heads, num_kv_heads, head_dim, shape[1], block_tables.shape[1], shape[0],
-            window or 0, _sm_count(index), scale, eps))
-        if result != _UNSUPPORTED:  # (sizes and addresses that only the two kernels take)
-            check(result, "decode_step_e4m3")
-            return out
     q, words = _store_words(qkv, n, positions, slots, inv_freq, cache, num_heads, num_kv_heads, head_dim, shape, status, code, q_weight, k_weight,
                             eps, early)
     check(library().cw_norm_rotate_store(words), "norm_rotate_store")
     out = torch.empty_like(q)
-    _decode_call(q, out, cache, block_tables, ctx_lens, None, num_heads, shape, scale, window, code, status, index, workspace, early)
+    _decode_call(q, out, cache, block_tables, ctx_lens, None, num_heads, shape, scale, window, code, status, index, workspace, True)
     return out
 
 

@@ -159,7 +159,7 @@ def _turned(x, w, eps, at, freq):
 @pytest.mark.parametrize("heads, ctx, page, window, rot, norm, dtype", STEPS)
 def test_whole_step(heads, ctx, page, window, rot, norm, dtype, early):
     """One call of norms, rotation, store and attention: the rows that it stores (contexts of 0 too, whose output is 0), against the
-    formulas; its output over the cache that it leaves; nothing else in the cache changes; without slots nothing does."""
+    formulas; its output over the cache that it leaves; nothing else in the cache changes."""
     nh, nkv, hd = heads
     n, g = len(ctx), torch.Generator().manual_seed(sum(ctx) + nh * hd + rot)
     before, tables = filled_pages(ctx, page, nkv, hd, g)
@@ -210,14 +210,10 @@ def test_whole_step(heads, ctx, page, window, rot, norm, dtype, early):
         bound = attention_bound(want, size, score, hd, dtype, WEIGHT_BITS) + 2.5 * open_by * size
         got = out[s].double().cpu().view(1, nh, hd)
         assert got.isfinite().all() and float(((got - want).abs() / bound).max()) <= 1.0, f"request {s}"
-    if not early and dtype == torch.bfloat16 and hd in quantised.STEP_HEAD_DIMS and rot in (0, hd):
-        cache = quantised.E4M3Pages(*_on(*before))
-        assert torch.equal(run(torch.full_like(slots, -1), cache), out)
-        assert all(torch.equal(a.cpu().view(torch.uint8), b.view(torch.uint8)) for a, b in zip(cache, before))
 
 
 def test_whole_step_reports_slots_outside_the_pool():
-    """Such tokens are attended and not stored."""
+    """Such tokens are not stored."""
     g = torch.Generator().manual_seed(16)
     cache, tables = filled_pages([33, 5], 16, 1, 64, g)
     status, held = ops.new_status(DEV), quantised.E4M3Pages(*_on(*cache))

@@ -58,7 +58,6 @@ struct DecodeE4m3Params {
 #define MERGE_AT_ONCE 8
 #define MOST_TEAMS 4
 #define TEAMS_FROM_BYTES 170000000LL
-#define LEAST_UNITS 2  // a warp's run: 8 requests of 1,024 tokens 16.4 us with 1 (nine pieces a segment to add up), 14.4 with 2
 
 __device__ __forceinline__ void mma_half(float* d, const uint32_t* a, uint32_t b0, uint32_t b1) {
     asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
@@ -198,9 +197,13 @@ __global__ void __launch_bounds__(WARPS * 32, Stream<HD, NT>::PER_SM) decode_e4m
     // 90; 2 of 96, 200 MB 53.6 and 59.4, 400 MB 137 and 92; 4 of 32 (four teams), 100 MB 50.9 and 65.0, 200 MB 106 and 93.
     const int teams = !PORTIONS && (long long)total * p.nkv * 2 * C::TILE_BYTES >= TEAMS_FROM_BYTES ? p.teams : 1;
     const int of_team = WARPS / teams, team = warp / of_team, member = warp - team * of_team, warps = gridDim.x * of_team;
+    // A run's least: a unit, which takes 1.5 us, where segments then have no more blocks' pieces than are added up at once; two where they
+    // are longer.  Measured, us, runs of one and of two: 2 requests of 411 and 96 tokens, 12 heads over 2, store in front, 11.3 and 12.5; 8 of 300,
+    // 28 over 4 11.7 and 13.5; 8 of 1,000, 12 over 2, store in front, 13.3 and 12.7 (beginning under the kernel in front 12.9 and 11.5).
+    const int least = PORTIONS || total > p.requests * p.groups * MERGE_AT_ONCE * WARPS ? 2 : 1;
     const int kv_units = p.nkv / teams;
     total *= kv_units;
-    const int quota = max(LEAST_UNITS, (total + warps - 1) / warps), block_units = quota * of_team;
+    const int quota = max(least, (total + warps - 1) / warps), block_units = quota * of_team;
     const int first = (int)min((long long)(blockIdx.x * of_team + member) * quota, (long long)total);
     auto zeros = [&]() {  // the rows of requests without a context
         for (int s = blockIdx.x; s < p.requests; s += gridDim.x) {

@@ -3,7 +3,7 @@
 // call through Python's checks, 60 look-ups of tensors' fields, 10 to 14.
 //
 // Whatever is not as it should be (a type, a shape, a device, an entry point that refuses) makes the function here return None
-// without having launched anything; the caller then takes Python's way through the same checks, which says what is wrong or has a kernel
+// without having launched anything (a step's store at most, which is then made once more); the caller then takes Python's way through the same checks, which says what is wrong or has a kernel
 // for it.  So every condition there is here too, and none of its words.
 #include <ATen/ATen.h>
 #include <c10/cuda/CUDAFunctions.h>

@@ -3,7 +3,7 @@
 // call through Python's checks, 60 look-ups of tensors' fields, 10 to 14.
 //
 // Whatever is not as it should be (a type, a shape, a device, an entry point that refuses) makes the function here return None
-// without having launched anything (a step's store at most, which is then made once more); the caller then takes Python's way through the same checks, which says what is wrong or has a kernel
+// without having launched anything (of a step or of portions at most what comes first, which is then made once more); the caller then takes Python's way through the same checks, which says what is wrong or has a kernel
 // for it.  So every condition there is here too, and none of its words.
 #include <ATen/ATen.h>
 #include <c10/cuda/CUDAFunctions.h>
@@ -18,7 +18,10 @@ namespace {
 
 using at::Tensor;
 typedef int (*Entry)(const char*);
-Entry store_entry, read_entry, decode_entry;
+Entry store_entry, read_entry, decode_entry, portions_entry;
+typedef int (*PrefillEntry)(const void*, int, int, int, void*, const void*, const void*, const int*, const int*, const int*, const int*, const int*,
+                            const int*, float*, float*, int*, int, int, int, int, int, int, int, float, int, int, int*, cudaStream_t);
+PrefillEntry prefill_entry;  // (the packed form, which takes one query head to a tile as well)
 PyTypeObject *e4m3_type, *plain_type;
 
 struct Refused : std::exception {};
@@ -250,6 +253,80 @@ PyObject* read(PyObject* const* a) {
     Py_RETURN_TRUE;
 }
 
+// q, cache, block tables, q_start, ctx_lens, plan, heads, scale, status, window, workspace, SMs, blocks, then for portions that are read
+// back (or None): k pages, v pages, (part_o, part_ml, counters: addresses; or None)
+// The plan's fields go by their places in ops/quantised.py's PortionPlan.
+enum { Q_LENS, CTX_LENS, SHAPE, SHORT, LEAST_ROWS, MOST_ROWS, ITEMS, EACH, ITEM_SEQ, ITEM_Q0, ITEM_SPLIT, TOK_SEQ, POSITIONS, FIELDS };
+PyObject* portions(PyObject* const* a) {
+    const Tensor& q = tensor(a[0]);
+    const int device = cuda_device(q);
+    const Pages cache = quantised_pages(a[1], device);
+    const Tensor &tables = of_type(a[2], at::kInt, 2, device), &starts = of_type(a[3], at::kInt, 1, device), &ctx = of_type(a[4], at::kInt, 1, device);
+    PyObject* plan = a[5];
+    need(PyTuple_Check(plan) && PyTuple_GET_SIZE(plan) == FIELDS);
+    auto field = [&](int i) { return PyTuple_GET_ITEM(plan, i); };
+    const int64_t nh = number(a[6]), s = tables.size(0), rows = q.size(0);
+    const Tensor& tok_seq = of_type(field(TOK_SEQ), at::kInt, 1, device);
+    need(PyTuple_Check(field(Q_LENS)) && PyTuple_GET_SIZE(field(Q_LENS)) == s && tok_seq.size(0) <= rows);
+    PyObject* shape = field(SHAPE);
+    need(PyTuple_Check(shape) && PyTuple_GET_SIZE(shape) == 4 && number(PyTuple_GET_ITEM(shape, 0)) == nh && number(PyTuple_GET_ITEM(shape, 1)) == cache.nkv &&
+         number(PyTuple_GET_ITEM(shape, 2)) == cache.hd && number(PyTuple_GET_ITEM(shape, 3)) == cache.page_size);
+    const long long items = number(field(ITEMS)), least = number(field(LEAST_ROWS)), most = number(field(MOST_ROWS)), few = number(field(SHORT)),
+                    each = number(field(EACH));
+    need(type_code(q) == 1 && nh > 0 && nh < (1 << 20) && cache.nkv > 0 && nh % cache.nkv == 0 && (cache.hd == 64 || cache.hd == 128));
+    need(q.dim() == 2 && q.size(1) >= nh * cache.hd && q.stride(1) == 1 && ctx.size(0) == s && starts.size(0) == s + 1);
+    need(cache.page_size >= 8 && cache.page_size <= 128 && (cache.page_size & (cache.page_size - 1)) == 0);
+    const double scale = real(a[7]);
+    const void* status = status_of(a[8], device);
+    const long long window = window_of(a[9]), sms = number(a[11]), blocks = number(a[12]);
+    const int64_t q_stride = rows > 1 ? q.stride(0) : nh * cache.hd;
+    need(q.stride(0) < (1LL << 31) && rows < (1LL << 31) && window < (1LL << 31) && tables.size(1) < (1LL << 31));
+    const void *floats = nullptr, *words = nullptr;
+    if (few > 0) {
+        const Scratch scratch(a[10], cache.hd, device);
+        floats = scratch.floats;
+        words = scratch.words;
+    }
+    Tensor out = at::empty({rows, nh * cache.hd}, q.options());
+    if (items > 0) {
+        const Tensor &k = of_type(a[13], at::kBFloat16, 4, device), &v = of_type(a[14], at::kBFloat16, 4, device);
+        const Tensor &seq = of_type(field(ITEM_SEQ), at::kInt, 1, device), &q0 = of_type(field(ITEM_Q0), at::kInt, 1, device);
+        need(k.sizes() == v.sizes() && k.size(0) == cache.pages && k.size(1) == cache.page_size && k.size(2) == cache.nkv && k.size(3) == cache.hd);
+        need(seq.size(0) == items && q0.size(0) == items);
+        const int* split = nullptr;
+        const void* scratch[3] = {nullptr, nullptr, nullptr};
+        if (field(ITEM_SPLIT) != Py_None) {
+            const Tensor& cut = of_type(field(ITEM_SPLIT), at::kInt, 1, device);
+            need(cut.size(0) == items && PyTuple_Check(a[15]) && PyTuple_GET_SIZE(a[15]) == 3);
+            split = (const int*)cut.const_data_ptr();
+            for (int i = 0; i < 3; ++i) scratch[i] = (const void*)number(PyTuple_GET_ITEM(a[15], i));
+        }
+        Words()
+            .pages(cache).pointer(k.const_data_ptr()).pointer(v.const_data_ptr()).pointer(tables.const_data_ptr()).pointer(ctx.const_data_ptr())
+            .pointer(starts.const_data_ptr()).pointer(status).stream().whole(s).whole(cache.nkv).whole(cache.hd).whole(cache.page_size)
+            .whole(tables.size(1)).whole(cache.pages).whole(window).whole(most + 1 > least ? most + 1 : least).whole(blocks).whole(1)
+            .call(read_entry);
+        int result;
+        Py_BEGIN_ALLOW_THREADS;
+        result = prefill_entry(q.const_data_ptr(), (int)q.stride(0), (int)q.size(1), (int)rows, out.mutable_data_ptr(), k.const_data_ptr(), v.const_data_ptr(),
+                               (const int*)tables.const_data_ptr(), (const int*)starts.const_data_ptr(), (const int*)ctx.const_data_ptr(),
+                               (const int*)seq.const_data_ptr(), (const int*)q0.const_data_ptr(), split, (float*)scratch[0], (float*)scratch[1],
+                               (int*)scratch[2], (int)items, (int)nh, (int)cache.nkv, (int)cache.hd, (int)cache.page_size, (int)tables.size(1),
+                               (int)cache.pages, (float)scale, (int)window, (int)each, (int*)status, c10::cuda::getCurrentCUDAStream().stream());
+        Py_END_ALLOW_THREADS;
+        need(result == 0);
+    }
+    if (few > 0) {
+        Words()
+            .pointer(q.const_data_ptr()).pointer(out.const_data_ptr()).pages(cache).pointer(tables.const_data_ptr()).pointer(ctx.const_data_ptr())
+            .pointer(starts.const_data_ptr()).pointer(floats).pointer(words).pointer(status).stream().whole(q_stride).whole(s)
+            .whole(nh).whole(cache.nkv).whole(cache.hd).whole(cache.page_size).whole(tables.size(1)).whole(cache.pages).whole(window).whole(sms)
+            .whole(few).whole(least).whole(most).number(scale)
+            .call(portions_entry);
+    }
+    return THPVariable_Wrap(std::move(out));
+}
+
 template <PyObject* (*CALL)(PyObject* const*), int ARGUMENTS>
 PyObject* guarded(PyObject*, PyObject* const* args, Py_ssize_t n) {
     try {
@@ -260,16 +337,18 @@ PyObject* guarded(PyObject*, PyObject* const* args, Py_ssize_t n) {
     Py_RETURN_NONE;
 }
 
-// addresses of the entry points (store, read, decode), E4M3Pages, PlainPages
+// addresses of the entry points (store, read, decode, portions of few rows, packed prefill), E4M3Pages, PlainPages
 PyObject* bind(PyObject*, PyObject* args) {
-    unsigned long long s, r, d;
+    unsigned long long s, r, d, w, t;
     PyObject *e, *p;
-    if (!PyArg_ParseTuple(args, "KKKO!O!", &s, &r, &d, &PyType_Type, &e, &PyType_Type, &p)) return nullptr;
+    if (!PyArg_ParseTuple(args, "KKKKKO!O!", &s, &r, &d, &w, &t, &PyType_Type, &e, &PyType_Type, &p)) return nullptr;
     Py_INCREF(e);
     Py_INCREF(p);
     store_entry = (Entry)s;
     read_entry = (Entry)r;
     decode_entry = (Entry)d;
+    portions_entry = (Entry)w;
+    prefill_entry = (PrefillEntry)t;
     e4m3_type = (PyTypeObject*)e;
     plain_type = (PyTypeObject*)p;
     Py_RETURN_NONE;
@@ -279,6 +358,7 @@ PyMethodDef methods[] = {{"bind", bind, METH_VARARGS, nullptr},
                          {"store", (PyCFunction)(void*)guarded<store, 13>, METH_FASTCALL, nullptr},
                          {"step", (PyCFunction)(void*)guarded<step, 19>, METH_FASTCALL, nullptr},
                          {"decode", (PyCFunction)(void*)guarded<decode, 11>, METH_FASTCALL, nullptr},
+                         {"portions", (PyCFunction)(void*)guarded<portions, 16>, METH_FASTCALL, nullptr},
                          {"read", (PyCFunction)(void*)guarded<read, 8>, METH_FASTCALL, nullptr},
                          {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "quantised_calls", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};

@@ -69,7 +69,8 @@ def _calls():
             loader.exec_module(module)
         except Exception as exc:  # noqa: BLE001
             raise KernelLibraryError(f"the module of the 8-bit cache's calls is unavailable ({exc})") from exc
-        entries = [ctypes.cast(f, ctypes.c_void_p).value for f in (lib.cw_norm_rotate_store, lib.cw_read_pages, lib.cw_attention_decode_e4m3)]
+        entries = [ctypes.cast(f, ctypes.c_void_p).value for f in (lib.cw_norm_rotate_store, lib.cw_read_pages, lib.cw_attention_decode_e4m3,
+                                                                   lib.cw_attention_portions_e4m3, lib.cw_attention_prefill_tc_packed)]
         module.bind(*entries, E4M3Pages, PlainPages)
         _calls_module = module
     return _calls_module
@@ -430,6 +431,7 @@ def short_rows(num_heads: int, num_kv_heads: int, head_dim: int) -> int:
 
 
 SHORT_PAIRS = 96
+TOGETHER_ENTRIES = 1 << 23
 
 
 class PortionPlan(NamedTuple):
@@ -454,7 +456,7 @@ class PortionPlan(NamedTuple):
 def plan_portions(q_lens, ctx_lens, num_heads: int, num_kv_heads: int, head_dim: int, page_size: int, device,
                   most_rows: int | None = None, least_rows: int = 1, packed: bool | None = None) -> PortionPlan:
     """``q_lens``: the rows that each request brings; ``ctx_lens``: its tokens in the cache with them (both on the host).
-    ``most_rows``: see ``short_rows``, which decides by default.  bfloat16 requests that bring fewer than ``least_rows`` rows are
+    ``most_rows``: see ``short_rows``, which decides by default (0 where the others' contexts make it little to read these back too).  bfloat16 requests that bring fewer than ``least_rows`` rows are
     left alone.  ``packed``: whether the query heads of a KV head share the longer portions' tiles (default: where that leaves fewer of them)."""
     from . import attention_fast as fast
 
@@ -464,7 +466,14 @@ def plan_portions(q_lens, ctx_lens, num_heads: int, num_kv_heads: int, head_dim:
     if len(q_lens) != len(ctx_lens) or any(n < 0 or c < n for n, c in zip(q_lens, ctx_lens)):
         raise ValueError("every request has a length and a context that holds its rows")
     if most_rows is None:
+        # A kernel more for the requests of few rows costs 10 to 15 us beside others that are read back: those with little context are read back
+        # with them (us, apart and together: 117 rows behind 780, 10 and 7 behind 17 and 168, 12 heads over 2 of 128 39.1 and 20.6; 200, and 4
+        # behind 12,000, 28 over 4, 6.1 million entries, 41.3 and 38.8, 16 over 16 of 64, 12.3 million, 34.7 and 41.0; 200, and 2 each behind
+        # eight of 2,000, 28 over 4, 8.2 million, 32.9 and 30.8, 16 over 16 of 64, 16.4 million, 32.8 and 43.6).
         most_rows = short_rows(num_heads, num_kv_heads, head_dim)
+        behind = sum(c for n, c in zip(q_lens, ctx_lens) if least_rows <= n <= most_rows)
+        if any(n > most_rows for n in q_lens) and behind * num_kv_heads * head_dim <= TOGETHER_ENTRIES:
+            most_rows = 0
     short = sum(n for n in q_lens if least_rows <= n <= most_rows)
     long = [n if n > max(most_rows, least_rows - 1) else 0 for n in q_lens]
     each = num_heads // num_kv_heads
@@ -534,6 +543,21 @@ def attention_portions(q: torch.Tensor, cache: E4M3Pages, block_tables: torch.Te
     from . import attention_ref
     from . import attention_fast as fast
 
+    common = q.is_cuda and q.dtype is torch.bfloat16 and type(cache) is E4M3Pages and cache.k.dim() == 4
+    scratch = _scratch_of(workspace, cache) if common else None
+    if common and (scratch is not None or plan.short == 0):
+        k = v = parts = None
+        if plan.items:
+            k, v = portion_scratch(cache, q.dtype)
+            if plan.item_split is not None:
+                held = fast._prefill_scratch(q.device, plan.items, num_heads // plan.each, cache.k.shape[-1])
+                parts = held["part_o"].data_ptr(), held["part_ml"].data_ptr(), held["counters"].data_ptr()
+        out = _calls().portions(q, cache, block_tables, q_start, ctx_lens, plan, num_heads, scale, status, window, scratch, _sm_count(q.get_device()),
+                                READ_BLOCKS, k, v, parts)
+        if out is not None:
+            for _ in range(2 * (plan.items > 0) + (plan.short > 0)):
+                counted()
+            return out
     code, shape = dtype_code(q.dtype), check_pages(cache)
     _, page_size, nkv, hd = shape
     if q.dim() != 2 or q.shape[1] < num_heads * hd or q.stride(1) != 1:

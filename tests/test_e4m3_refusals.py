@@ -116,6 +116,17 @@ def test_plans_of_impossible_portions_are_refused():
         quantised.plan_portions([3], [5], 5, 2, 32, 8, "cpu")
 
 
+def test_requests_of_few_rows_go_with_the_others_where_they_have_little_behind_them():
+    most = quantised.short_rows(12, 2, 128)
+    assert most == 16 and quantised.plan_portions([7, 10], [7, 200], 12, 2, 128, 5, "cpu").short == 17  # there are no others
+    assert quantised.plan_portions([7, 10, 200], [7, 200, 200], 12, 2, 128, 5, "cpu").short == 0
+    edge = quantised.TOGETHER_ENTRIES // 256
+    assert quantised.plan_portions([7, 200], [edge, 200], 12, 2, 128, 5, "cpu").short == 0
+    assert quantised.plan_portions([7, 200], [edge + 1, 200], 12, 2, 128, 5, "cpu").short == 7
+    assert quantised.plan_portions([7, 1, 200], [edge + 1, 9, 200], 12, 2, 128, 5, "cpu", least_rows=2).short == 7
+    assert quantised.plan_portions([1, 7, 200], [10 * edge, 9, 200], 12, 2, 128, 5, "cpu", least_rows=2).short == 0  # (the one is served apart)
+
+
 def test_the_oracle_rounds_as_the_type_does():
     x = torch.cat([torch.linspace(-448, 448, 4097).double(), torch.ldexp(torch.linspace(1, 2, 65).double(), torch.tensor(-9))])
     assert torch.equal(nearest_codes(x), x.float().to(CODES).double())

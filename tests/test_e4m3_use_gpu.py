@@ -109,7 +109,7 @@ def test_portions_in_a_graph():
     q = torch.randn(sum(new), NH * HD, generator=g).bfloat16().to(DEV)
     starts = torch.tensor([0, 7, 157, 158], dtype=torch.int32, device=DEV)
     lens = torch.tensor(ctx, dtype=torch.int32, device=DEV)
-    plan = quantised.plan_portions(new, ctx, NH, NKV, HD, PAGE, torch.device(DEV))
+    plan = quantised.plan_portions(new, ctx, NH, NKV, HD, PAGE, torch.device(DEV), most_rows=quantised.short_rows(NH, NKV, HD))
     assert plan.short == 8 and plan.items > 0  # both kernels
 
     def run():
@@ -264,7 +264,7 @@ def entry_points():
     module, reached = quantised._calls(), []
     entry = ctypes.CFUNCTYPE(ctypes.c_int, ctypes.c_void_p)(lambda words: reached.append(words) or 0)
     address = ctypes.cast(entry, ctypes.c_void_p).value
-    module.bind(address, address, address, quantised.E4M3Pages, quantised.PlainPages)
+    module.bind(*[address] * 5, quantised.E4M3Pages, quantised.PlainPages)
     yield module, reached
     quantised._calls_module = None  # (bound anew by the next call)
 
@@ -282,14 +282,25 @@ def test_common_calls_refuse_what_the_others_name(entry_points):
                   scale=1.0, status=base["status"], window=None, scratch=scratch, sms=148, early=False)
     plain = torch.zeros(4, 8, 2, 32, device=DEV)
     read = dict(cache=base["cache"], block_tables=ints(3, 2), ctx_lens=ints(3), out_k=plain, out_v=plain.clone(), status=base["status"], window=None, blocks=4)
-    forms = [(module.store, store, (*names, "early"), refusals.STORE),
+    few = refusals._args(hd=64)
+    pages = torch.zeros(4, 8, 2, 64, dtype=torch.bfloat16, device=DEV)
+    portions = dict(q=torch.zeros(5, 256, dtype=torch.bfloat16, device=DEV), cache=_moved(few["cache"]), block_tables=ints(3, 2),
+                    q_start=torch.tensor([0, 2, 2, 5], dtype=torch.int32, device=DEV), ctx_lens=ints(3),
+                    plan=quantised.plan_portions([2, 0, 3], [2, 0, 9], 4, 2, 64, 8, DEV, most_rows=2), num_heads=4, scale=1.0, status=base["status"],
+                    window=None, scratch=scratch, sms=148, blocks=4, k=pages, v=pages.clone(), parts=(16, 32, 48))
+    assert portions["plan"].items > 0 and portions["plan"].short == 2
+    other_plans = [quantised.plan_portions([2, 0, 3], [2, 0, 9], *shape, DEV, most_rows=2) for shape in ((8, 2, 64, 8), (4, 4, 64, 8), (4, 2, 128, 8), (4, 2, 64, 16))]
+    other_plans += [quantised.plan_portions([2, 3], [2, 9], 4, 2, 64, 8, DEV, most_rows=2), quantised.plan_portions([2, 1, 3], [2, 1, 9], 4, 2, 64, 8, DEV, most_rows=2)]
+    plans = [({"plan": plan}, "") for plan in (*other_plans, tuple(portions["plan"])[:-1], "x", None)]
+    forms = [(module.portions, portions, tuple(portions), [c for c in refusals.PORTIONS if not {"plan", "cache", "q", "q_start", "block_tables"} & set(c[0])] + plans),
+             (module.store, store, (*names, "early"), refusals.STORE),
              (module.step, step, (*names, "early", "block_tables", "ctx_lens", "scale", "window", "scratch", "sms"), refusals.STEP),
              (module.decode, decode, tuple(decode), [c for c in refusals.DECODE if not {"q_start", "out"} & set(c[0])]),
              (module.read, read, tuple(read), [c for c in refusals.READ if "q_start" not in c[0]])]
     for call, good, order, refused in forms:
-        assert call(*(good[name] for name in order)) is not None and len(reached) == (2 if call is module.step else 1)
+        assert call(*(good[name] for name in order)) is not None and len(reached) == {module.step: 2, module.portions: 3}.get(call, 1)
         reached.clear()
-        cases = [{k: _moved(v) for k, v in change.items()} for change, _ in refused if change]
+        cases = [{k: v if k == "plan" else _moved(v) for k, v in change.items()} for change, _ in refused if change]
         for name, value in good.items():  # a tensor elsewhere, of another type, of other sizes; what is no tensor at all
             if isinstance(value, torch.Tensor):
                 cases += [{name: value.cpu()}, {name: value.to(torch.float16)}, {name: value[1:]}, {name: value[None]}, {name: "x"}, {name: None}]

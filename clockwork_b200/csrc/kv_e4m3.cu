@@ -9,7 +9,7 @@
 // last bits, which decide between two codes, are not the sine's.  (An angle serves all heads: 64 of them beside 4,608 entries.)
 //
 // read_pages: code * 2^(E - 127) in bfloat16 (exact) or float32 for the positions of every request's context, at the same page
-// and slot of a plain cache; the rest of a request's last page becomes zero.  Both are streams over memory.
+// and slot of a plain cache; what no request holds of a last page becomes zero.  Both are streams over memory.
 #include "kv_e4m3.cuh"
 
 struct StoreParams {
@@ -452,8 +452,39 @@ struct ReadParams {
     void* k_out; void* v_out;
     const int* block_tables; const int* ctx_lens; const int* q_start;
     int requests, nkv, hd, page_size, max_blocks, num_pages, window, least_rows;
+    int behind_zeros;  // zero_rests_kernel is the kernel in front
     int* status;
 };
+
+// The blocks of request s that are read: how many, and the first.
+__device__ __forceinline__ int read_span(const ReadParams& p, int s, int& from) {
+    int ctx = p.ctx_lens[s], first = ctx;
+    if (p.q_start != nullptr) {
+        const int rows = p.q_start[s + 1] - p.q_start[s];
+        if (rows < p.least_rows) return 0;
+        first = ctx - rows + 1;  // (a portion's first row sees `window` keys, its own among them: the window reaches back from there)
+    }
+    from = p.window > 0 ? max(0, first - p.window) / p.page_size : 0;
+    return max(0, min((ctx + p.page_size - 1) / p.page_size, p.max_blocks) - from);
+}
+
+// Zeros behind the last token of every request that is read, to the end of its last page.  Requests may share a page of which one
+// holds more than the other (a table may also name a page twice), so these come before any value is written, in a kernel of their own: the
+// rows that a request holds are then written by read_pages_kernel whoever's zeros lay there, with the same numbers by all who hold them.
+// (That kernel's set-up runs beside this one: 5,778 tokens of two KV heads 5.8 us for both, 6.8 with the zeros in its own pages' units.)
+template <typename T>
+__global__ void __launch_bounds__(256) zero_rests_kernel(const ReadParams p) {
+    pdl_enter();
+    const int s = blockIdx.x;
+    int from = 0;
+    const int n = read_span(p, s, from);
+    if (n == 0) return;
+    const int block = from + n - 1, page = p.block_tables[(size_t)s * p.max_blocks + block], live = p.ctx_lens[s] - block * p.page_size;
+    if (page < 0 || page >= p.num_pages || live >= p.page_size) return;  // (reported by read_pages_kernel)
+    const int row_words = p.nkv * (p.hd * (int)sizeof(T) / 16);
+    uint4* to = reinterpret_cast<uint4*>(blockIdx.y ? p.v_out : p.k_out) + (size_t)page * p.page_size * row_words;
+    for (int i = live * row_words + threadIdx.x; i < p.page_size * row_words; i += blockDim.x) to[i] = make_uint4(0, 0, 0, 0);
+}
 
 __device__ __forceinline__ void store8(float* at, float a, float b, float c, float d, float e, float f, float g, float h) {
     *reinterpret_cast<float4*>(at) = make_float4(a, b, c, d);
@@ -479,21 +510,14 @@ struct Quotient {
 template <typename T>
 __global__ void __launch_bounds__(256) read_pages_kernel(const ReadParams p, const Quotient by_chunks, const Quotient by_heads) {
     __shared__ int sh[36];
-    pdl_enter();
-    auto span = [&](int s, int& from) {  // a request's blocks that are read: how many, and the first
-        int ctx = p.ctx_lens[s], first = ctx;
-        if (p.q_start != nullptr) {
-            const int rows = p.q_start[s + 1] - p.q_start[s];
-            if (rows < p.least_rows) return 0;
-            first = ctx - rows + 1;  // (a portion's first row sees `window` keys, its own among them: the window reaches back from there)
-        }
-        from = p.window > 0 ? max(0, first - p.window) / p.page_size : 0;
-        return max(0, min((ctx + p.page_size - 1) / p.page_size, p.max_blocks) - from);
-    };
+    // (the kernel of zeros lets this one come when all in front of it is complete: the lengths can be looked at beside it)
+    if (!p.behind_zeros) pdl_enter();
+    auto span = [&](int s, int& from) { return read_span(p, s, from); };
     const int warps = blockDim.x >> 5, lane = threadIdx.x & 31;
     const int chunks = p.page_size * p.nkv * (p.hd >> 3), at_once = 32 * READ_AT_ONCE;
     const UnitRange r = units_of_block([&](int s) { int from; return 2 * span(s, from); }, p.requests, warps, (chunks + at_once - 1) / at_once,
                                        gridDim.x, blockIdx.x, sh);
+    if (p.behind_zeros) pdl_enter();
     int s = r.request, at = r.offset + (threadIdx.x >> 5);  // units of a block go to its warps in turn
     for (int u = r.first + (threadIdx.x >> 5); u < r.last; u += warps, at += warps) {
         int from = 0, n = 2 * r.parts * span(s, from);
@@ -528,7 +552,7 @@ __global__ void __launch_bounds__(256) read_pages_kernel(const ReadParams p, con
 #pragma unroll
             for (int k = 0; k < READ_AT_ONCE; ++k) {
                 const int i = i0 + 32 * k;
-                if (i >= chunks) break;
+                if (i >= chunks || (int)by_chunks.of(i) >= live) break;
                 const float up = kv_up(power[k]);
                 const float2 x0 = kv_float2(codes[k].x), x1 = kv_float2(codes[k].x >> 16), x2 = kv_float2(codes[k].y), x3 = kv_float2(codes[k].y >> 16);
                 store8(dst + (size_t)i * 8, x0.x * up, x0.y * up, x1.x * up, x1.y * up, x2.x * up, x2.y * up, x3.x * up, x3.y * up);
@@ -554,11 +578,16 @@ extern "C" int cw_read_pages(const char* block) {
         (long long)page_size * nkv * (hd >> 3) * max(hd >> 3, nkv) > 0x7FFFFFFF)  // (Quotient's range)
         return CW_ERR_BAD_SIZE;
     const ReadParams p = {k, v, k_exp, v_exp, k_out, v_out, block_tables, ctx_lens, q_start, requests, nkv, hd, page_size,
-                          max_blocks, num_pages, window, least_rows, status};
+                          max_blocks, num_pages, window, least_rows, page_size > 1, status};
+    if (dtype != 0 && dtype != 1) return CW_ERR_BAD_DTYPE;
+    if (p.behind_zeros) {
+        const int result = dtype == 0 ? cw_launch(zero_rests_kernel<float>, dim3(requests, 2), dim3(256), 0, stream, 1u, p)
+                                      : cw_launch(zero_rests_kernel<bf16>, dim3(requests, 2), dim3(256), 0, stream, 1u, p);
+        if (result != CW_OK) return result;
+    }
     const Quotient by_chunks = Quotient::by(hd >> 3), by_heads = Quotient::by(nkv);
     if (dtype == 0) return cw_launch(read_pages_kernel<float>, dim3(blocks), dim3(256), 0, stream, 1u, p, by_chunks, by_heads);
-    if (dtype == 1) return cw_launch(read_pages_kernel<bf16>, dim3(blocks), dim3(256), 0, stream, 1u, p, by_chunks, by_heads);
-    return CW_ERR_BAD_DTYPE;
+    return cw_launch(read_pages_kernel<bf16>, dim3(blocks), dim3(256), 0, stream, 1u, p, by_chunks, by_heads);
 }
 
 CW_TRACE_TU(kv_e4m3)

@@ -222,18 +222,21 @@ def _read_call(cache, shape, block_tables, ctx_lens, q_start, out_k, out_v, wind
         cache.k.data_ptr(), cache.v.data_ptr(), cache.k_exp.data_ptr(), cache.v_exp.data_ptr(), out_k.data_ptr(), out_v.data_ptr(),
         block_tables.data_ptr(), ctx_lens.data_ptr(), 0 if q_start is None else q_start.data_ptr(), status.data_ptr(), _stream(), block_tables.shape[0], nkv, hd,
         page_size, block_tables.shape[1], pages, window or 0, least_rows, READ_BLOCKS, code)), "read_pages")
+    if page_size > 1:
+        counted()  # (the zeros behind the contexts are a kernel of their own)
 
 
 def read_pages(cache: E4M3Pages, block_tables: torch.Tensor, ctx_lens: torch.Tensor, out_k: torch.Tensor, out_v: torch.Tensor,
                status: torch.Tensor, *, window: int | None = None, q_start: torch.Tensor | None = None, least_rows: int = 1) -> None:
     """The keys and values of positions [0, ctx_lens[s]) of every request, through ``block_tables`` [S, max_blocks], into plain
     pages ``out_k``, ``out_v`` [pages, page_size, nkv, hd] (float32 or bfloat16) at the same pages and slots.  What is left of a
-    request's last page becomes zero; no other page is touched.  ``window``: from the page on that a query at the request's last
+    request's last page becomes zero where no other request that is read holds it; no other page is touched.  ``window``: from the page on that a query at the request's last
     position sees with that window.  ``q_start`` [S + 1] (the rows that the requests bring to a step): only requests that bring
     at least ``least_rows`` rows are read, and the window is that of their first row."""
     if q_start is None and least_rows == 1 and out_k.is_cuda and _calls().read(cache, block_tables, ctx_lens, out_k, out_v, status, window,
                                                                                READ_BLOCKS):
-        counted()
+        for _ in range(1 + (cache.k.shape[1] > 1)):
+            counted()
         return
     pages, page_size, nkv, hd = check_pages(cache)
     for name, t in (("out_k", out_k), ("out_v", out_v)):
@@ -556,7 +559,7 @@ def attention_portions(q: torch.Tensor, cache: E4M3Pages, block_tables: torch.Te
         out = _calls().portions(q, cache, block_tables, q_start, ctx_lens, plan, num_heads, scale, status, window, scratch, _sm_count(q.get_device()),
                                 READ_BLOCKS, k, v, parts)
         if out is not None:
-            for _ in range(2 * (plan.items > 0) + (plan.short > 0)):
+            for _ in range((2 + (plan.shape[3] > 1)) * (plan.items > 0) + (plan.short > 0)):
                 counted()
             return out
     code, shape = dtype_code(q.dtype), check_pages(cache)

@@ -285,3 +285,23 @@ def test_a_request_from_its_prompt_on(norm):
             out = quantised.decode_step(qkv, at.to(DEV), slots.to(DEV), freq, cache, tables.to(DEV), ctx, nh, nkv, hd, 0.09, status, **args)
         ops.raise_on_status(status)
         _check(out, q.cpu(), tuple(t.cpu() for t in cache), tables, [done], [(0, 0, n, done - n)], page, None, 0.09, dtype, 8 if n > 1 else WEIGHT_BITS)
+
+
+@pytest.mark.parametrize("dtype, most", [(torch.bfloat16, 0), (torch.bfloat16, None), (torch.float32, None)])
+@pytest.mark.parametrize("ctx, new, page", [([1000, 1010], [100, 60], 16), ([70, 95, 66], [30, 3, 40], 32)])
+def test_portions_of_requests_over_one_table(ctx, new, page, dtype, most):
+    """Portions whose contexts end in the same page, one before the other: what the shorter does not hold the longer one sees."""
+    nh, nkv, hd = 12, 2, 128
+    g = torch.Generator().manual_seed(sum(ctx))
+    cache, tables = filled_pages([max(ctx)], page, nkv, hd, g)
+    tables = tables.repeat(len(ctx), 1)
+    starts = [sum(new[:i]) for i in range(len(new) + 1)]
+    q = torch.randn(starts[-1], nh * hd, generator=g).to(dtype)
+    status, on = ops.new_status(DEV), quantised.E4M3Pages(*_on(*cache))
+    plan = quantised.plan_portions(new, ctx, nh, nkv, hd, page, torch.device(DEV), most_rows=most)
+    lens = _on(tables, torch.tensor(starts, dtype=torch.int32), torch.tensor(ctx, dtype=torch.int32))
+    outs = [quantised.attention_portions(q.to(DEV), on, *lens, plan, nh, hd**-0.5, status) for _ in range(10)]
+    ops.raise_on_status(status)
+    assert all(torch.equal(out, outs[0]) for out in outs)
+    _check(outs[0], q, cache, tables, ctx, [(s, starts[s], n, ctx[s] - n) for s, n in enumerate(new)], page, None, hd**-0.5, dtype,
+           24 if dtype == torch.float32 else 8)

@@ -243,3 +243,39 @@ def test_pages_outside_the_pool_are_reported_on_reading():
     with pytest.raises(RuntimeError, match="page id"):
         ops.raise_on_status(status)
     assert (out[0][tables[0, 0].item()] != 3.0).any() and (out[0][tables[0, 2].item()] != 3.0).any()
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("ctx, page", [([1000, 1010, 1003], 16), ([30, 33, 1, 38], 8), ([70, 95, 66], 32)])
+def test_requests_that_share_a_partly_filled_page(ctx, page, dtype):
+    """Requests over one table, each with a context of its own, and one whose last page, filled in part, stands in its table a second time
+    and there in full: every held row arrives, whichever request comes first; zeros are left where none holds anything."""
+    g = torch.Generator().manual_seed(sum(ctx))
+    longest = max(range(len(ctx)), key=lambda s: ctx[s])
+    cache, tables = filled_pages([ctx[longest]], page, 2, 64, g)
+    blocks = tables.shape[1]
+    tables = tables.repeat(len(ctx) + 1, 1)
+    last = (ctx[0] - 1) // page  # request 0's last page; the further request holds all of it as its first
+    tables[-1, 0], ctx = tables[0, last], [*ctx, min(page + 1, ctx[longest])]
+    full = min(page, ctx[longest] - last * page) == page
+    if not full:
+        ctx[-1] = ctx[longest] - last * page
+    want = torch.zeros(cache[0].shape, dtype=torch.float64)
+    touched = torch.zeros(cache[0].shape[:2], dtype=torch.bool)
+    values = [held(cache[i], cache[2 + i]) for i in range(2)]
+    rows = torch.zeros(cache[0].shape[:2], dtype=torch.bool)
+    for s, c in enumerate(ctx):
+        for b in range(-(-c // page)):
+            touched[tables[s, b]] = True
+            rows[tables[s, b], : min(page, c - b * page)] = True
+    assert blocks > 1 and (touched & ~rows).any()
+    on, lens, status = quantised.E4M3Pages(*_on(*cache)), torch.tensor(ctx, dtype=torch.int32, device=DEV), ops.new_status(DEV)
+    tables = tables.to(DEV)
+    for order in (list(range(len(ctx))), list(range(len(ctx)))[::-1]):
+        for _ in range(20):
+            out = [torch.full(cache[0].shape, 3.0, dtype=dtype, device=DEV) for _ in range(2)]
+            quantised.read_pages(on, tables[order].contiguous(), lens[order].contiguous(), *out, status)
+            for got, value in zip(out, values):
+                want = torch.where(rows[..., None, None], value, torch.where(touched, 0.0, 3.0).double()[..., None, None])
+                assert torch.equal(got.double().cpu(), want)
+    ops.raise_on_status(status)

@@ -212,7 +212,8 @@ attn_prefill_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
         }
         const int* table = p.block_tables + (size_t)s * p.max_blocks;
         const int pages_per_tile = AK >> p.page_shift;  // at most 16
-        const int own = table[min((kv_hi - 1) >> p.page_shift, p.max_blocks - 1)];
+        // (a context shorter than the rows that are said to end it: tiles of no key, which look nothing up)
+        const int own = kv_hi > 0 ? table[min((kv_hi - 1) >> p.page_shift, p.max_blocks - 1)] : 0;
         auto page_of = [&](int j) -> int {
             // pages without a visible key: any finite data of the request's own will do, their probabilities are zero
             const int pos = tile_lo + j * AK + lane * p.page_size;

@@ -42,7 +42,7 @@ struct DecodeE4m3Params {
     int requests, nh, nkv, hd, page_size, max_blocks, num_pages, window;
     float scale;
     int* status;
-    int early;               // lengths, tables and all of the cache but the newest tokens' rows are older than the kernel in front
+    int early;               // 1: lengths, tables and all rows but a request's own newest are older than the kernel in front; 2: lengths and tables are
     // the streaming kernel
     int page_shift;          // log2 of the page size, or -1
     int teams;               // KV heads that long walks take side by side
@@ -381,6 +381,7 @@ __global__ void __launch_bounds__(WARPS * 32, Stream<HD, NT>::PER_SM) decode_e4m
         }
     };
     look_up();
+    if (p.early == 2) wait();
     if (at.left > 0 && waited) call_queries(at);
 #pragma unroll 1
     for (int i = 0; i < ST - 1; ++i) fetch();

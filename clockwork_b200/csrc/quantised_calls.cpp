@@ -208,7 +208,7 @@ struct Tokens {
             .pointer(q.const_data_ptr()).pointer(out.const_data_ptr()).pages(cache).pointer(tables.const_data_ptr()).pointer(ctx.const_data_ptr())
             .pointer(nullptr).pointer(scratch.floats).pointer(scratch.words).pointer(status).stream()
             .whole(s > 1 ? q.stride(0) : nh * cache.hd).whole(s).whole(nh).whole(cache.nkv).whole(cache.hd).whole(cache.page_size)
-            .whole(tables.size(1)).whole(cache.pages).whole(window).whole(1).whole(sms).whole(early).number(scale)
+            .whole(tables.size(1)).whole(cache.pages).whole(window).whole(1).whole(sms).whole(early).number(scale)  // (early: 0, 1 or 2)
             .call(decode_entry);
         return out;
     }
@@ -231,7 +231,7 @@ PyObject* step(PyObject* const* a) {
     const Tokens t(a[13], a[14], a[5], a[15], a[8], a[16], a[17], a[18], r.cache, r.device);
     need(t.s == r.n);
     // (what the attention could still refuse, sizes beyond its counters, is refused again by the caller's way, behind the same store)
-    return THPVariable_Wrap(t.attended(stored(r, eps, early), r.cache, 1));
+    return THPVariable_Wrap(t.attended(stored(r, eps, early), r.cache, early ? 1 : 2));
 }
 
 // cache, block tables, ctx_lens, out_k, out_v, status, window, blocks

@@ -197,7 +197,7 @@ def norm_rotate_store(qkv: torch.Tensor, positions: torch.Tensor, slots: torch.T
     j + len(inv_freq)), and the write of k and v at ``slots`` (< 0: not stored) of ``cache`` (``E4M3Pages``, or ``PlainPages``
     of qkv's type).  Returns q [N, nh * hd].  Everything up to the one rounding of each output is float32.
 
-    ``early``: a promise that ``positions``, ``slots`` and ``inv_freq`` were complete before the kernel in front of this call was
+    ``early``: a promise that ``positions``, ``slots``, ``inv_freq`` and the weights were complete before the kernel in front of this call was
     launched, as a step's inputs are; the call then begins while that kernel finishes."""
     if qkv.is_cuda:
         q = _calls().store(qkv, positions, slots, inv_freq, cache, num_heads, num_kv_heads, head_dim, status, q_weight, k_weight, eps, early)
@@ -316,7 +316,7 @@ def _scratch_of(workspace: DecodeWorkspace | None, cache) -> tuple | None:
 
 
 def _decode_call(q, out, cache, block_tables, ctx_lens, q_start, num_heads, shape, scale, window, code, status, index, workspace,
-                 early=False) -> None:
+                 early=0) -> None:
     pages, page_size, nkv, hd = shape
     s = block_tables.shape[0]
     stream, sms, floats, words = _stream(), _sm_count(index), 0, 0
@@ -340,8 +340,8 @@ def attention_decode(q: torch.Tensor, cache: E4M3Pages, block_tables: torch.Tens
 
     ``q_start`` (int32 [S + 1]) with ``out`` ([N, nh * hd]): the requests are those of a flat batch of N rows that also holds
     prompt portions; only requests with exactly one row are served, the others' rows are left alone.  ``workspace``: the call's scratch (default:
-    one per stream).  ``early``: a promise that ``ctx_lens``, ``block_tables``, ``q_start`` and all of the cache but the requests' newest rows
-    were complete before the kernel in front of this call was launched, as they are in a step whose inputs were uploaded before
+    one per stream).  ``early``: a promise that ``ctx_lens``, ``block_tables``, ``q_start`` and all rows that a request sees but its own
+    last one were complete before the kernel in front of this call was launched, as they are in a step whose inputs were uploaded before
     it; the call then begins to read while that kernel finishes."""
     if q_start is None and out is None and q.is_cuda:
         scratch = _scratch_of(workspace, cache)
@@ -388,9 +388,11 @@ def decode_step(qkv: torch.Tensor, positions: torch.Tensor, slots: torch.Tensor,
                 eps: float = 0.0, window: int | None = None, workspace: DecodeWorkspace | None = None, early: bool = False) -> torch.Tensor:
     """``norm_rotate_store`` of one new token per request, then ``attention_decode`` of it: what an attention layer does between
     its two products while every request decodes.  ``ctx_lens`` count the new tokens; ``slots`` name their places (the last of their
-    requests) in the block tables, < 0: not stored.  ``early``: the promise of ``norm_rotate_store``."""
-    # (Attention begins while the store finishes whether or not this call does while the kernel in front of it finishes: a store that
-    # makes no such promise lets its successor come only when everything in front of it is complete, and itself writes only the newest rows.)
+    requests) in the block tables, < 0: not stored.  ``early``: a promise that all the call reads but ``qkv`` (``positions``, ``slots``,
+    ``inv_freq``, the weights, ``ctx_lens``, ``block_tables``, the cache) was complete before the kernel in front of it was launched, and that
+    no request sees a row that this call stores for another; the call then begins while that kernel finishes."""
+    # (Without the promise attention still comes while the store finishes: that lets its successor come only when everything in front of it
+    # is complete, and leaves lengths and tables alone.  Rows are then read behind the store: one request's newest may be another's last but one.)
     if qkv.is_cuda:
         scratch = _scratch_of(workspace, cache)
         if scratch is not None:
@@ -417,7 +419,8 @@ def decode_step(qkv: torch.Tensor, positions: torch.Tensor, slots: torch.Tensor,
                             eps, early)
     check(library().cw_norm_rotate_store(words), "norm_rotate_store")
     out = torch.empty_like(q)
-    _decode_call(q, out, cache, block_tables, ctx_lens, None, num_heads, shape, scale, window, code, status, index, workspace, True)
+    _decode_call(q, out, cache, block_tables, ctx_lens, None, num_heads, shape, scale, window, code, status, index, workspace,
+                 1 if early else 2)
     return out
 
 

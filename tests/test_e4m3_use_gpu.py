@@ -321,3 +321,50 @@ def test_common_calls_refuse_what_the_others_name(entry_points):
                 continue  # (four words of any shape)
             result = call(*({**good, **case}[name] for name in order))
             assert result is None and not reached, (call, case.keys(), [getattr(v, "shape", v) for v in case.values()])
+
+
+@pytest.mark.parametrize("tile, nh, nkv, hd", [(64, 8, 2, 64), (32, NH, NKV, HD), (16, 4, 1, 256)])
+def test_tokens_of_one_sequence_as_requests_of_a_step(tile, nh, nkv, hd):
+    """Draft tokens: the rows of one call are neighbours in one sequence, so that each sees the rows that the call stores for those before
+    it, in its last tile of keys or the one before that.  The same bits as a store that is complete before attention begins."""
+    status, rows = ops.new_status(DEV), 5
+    g = torch.Generator().manual_seed(31)
+    for base in (tile - 2, 3 * tile - 3, 40 * tile - 4):
+        cache, tables = filled_pages([base + rows], PAGE, nkv, hd, g)
+        at = torch.arange(base, base + rows, dtype=torch.int32)
+        slots = tables[0, at.long() // PAGE] * PAGE + at % PAGE
+        tables, at, slots, ctx = tables.repeat(rows, 1).to(DEV), at.to(DEV), slots.to(torch.int32).to(DEV), (at + 1).to(DEV)
+        for _ in range(10):
+            qkv = torch.randn(rows, (nh + 2 * nkv) * hd, generator=g).bfloat16().to(DEV)
+            one, two = (quantised.E4M3Pages(*(t.to(DEV) for t in cache)) for _ in range(2))
+            q = quantised.norm_rotate_store(qkv, at, slots, None, one, nh, nkv, hd, status)
+            torch.cuda.synchronize()
+            want = quantised.attention_decode(q, one, tables, ctx, nh, 0.09, status)
+            torch.cuda.synchronize()
+            got = quantised.decode_step(qkv, at, slots, None, two, tables, ctx, nh, nkv, hd, 0.09, status)
+            assert torch.equal(got, want) and all(torch.equal(a.view(torch.uint8), b.view(torch.uint8)) for a, b in zip(one, two))
+    ops.raise_on_status(status)
+
+
+@pytest.mark.parametrize("early", [False, True])
+def test_rows_that_the_kernel_in_front_writes(early):
+    """``qkv`` comes from a kernel that lets this call begin before it has finished, and is written anew each time."""
+    status, steps = ops.new_status(DEV), 30
+    fresh, tables, qkv, slots, ctx = _steps(25, [300, 31, 2000], steps)
+    heads, cache, plain, want = NH + 2 * NKV, fresh(), fresh(), []
+    for i in range(steps):
+        want.append(quantised.decode_step(qkv[i], ctx[i] - 1, slots[i], None, plain, tables, ctx[i], NH, NKV, HD, 0.09, status))
+        torch.cuda.synchronize()
+    spare = quantised.allocate_pages(1, PAGE, 1, HD, DEV)
+    wide = torch.zeros(steps, 3, (heads + 2) * HD, dtype=torch.bfloat16, device=DEV)
+    wide[:, :, : heads * HD] = qkv
+    nowhere = torch.full((3,), -1, dtype=torch.int32, device=DEV)
+    at = ctx - 1
+    torch.cuda.synchronize()
+    got = []
+    for i in range(steps):  # (rows that neither norm nor turn: the store hands them on as they are)
+        torch.cuda.synchronize()  # (the rows of the steps before are complete)
+        made = quantised.norm_rotate_store(wide[i], at[i], nowhere, None, spare, heads, 1, HD, status, early=True)
+        got.append(quantised.decode_step(made, at[i], slots[i], None, cache, tables, ctx[i], NH, NKV, HD, 0.09, status, early=early))
+    ops.raise_on_status(status)
+    assert all(torch.equal(a, b) for a, b in zip(got, want))

@@ -24,9 +24,12 @@
 //
 // Query heads are scaled by a power of two each into half precision's upper range (bfloat16's 8 bits are kept; what falls below
 // 2^-39 of the head's largest entry is dropped).  The powers of K multiply scores in float32.  Those of V are taken into
-// the exponent: weights are p_j = 2^(s_j log2 e + Ev_j - 127 - M + 14), M the running maximum of s_j log2 e + Ev_j - 127, in half precision
-// (11 bits, off by at most 2^-12 of themselves, or by 2^-39 of the largest contribution), and the denominator, float32, sums
-// p_j 2^(127 - Ev_j).  (It overflows, and the result is 0, where a context's values are all below 2^-88.)
+// the exponent: weights are p_j = 2^(s_j log2 e + Ev_j - 127 - M + 14), M the running maximum of s_j log2 e + max(Ev_j, 37) - 127, in half
+// precision (11 bits: off by at most 2^-11 of themselves, or by 2^-25, which is 2^-38 of the largest contribution).  A row of zeros
+// contributes nothing, whatever its power of 127 says, and has Ev_j = 37 here: it would otherwise push the others down to where half
+// precision has few bits.  (With a power below 37, values below 2^-81, an error is at most 2^-120.)  The denominator, float32, sums
+// 2^(s_j log2 e - M + 14) by itself, below 2^105 a token, and is taken from one maximum to the next in two halves: 2^(difference) by
+// itself may be no number any more where the sum times it still counts.
 //
 // A segment (request, KV head and group) that lies in one warp's run is finished by it.  At the end of its run a block adds up
 // its warps' pieces of shared segments in order; the pieces of one that several blocks share go to scratch of two per block, and
@@ -55,6 +58,7 @@ struct DecodeE4m3Params {
 };
 
 #define WARPS 4
+#define LEAST_POWER 37
 #define MERGE_AT_ONCE 8
 #define MOST_TEAMS 4
 #define TEAMS_FROM_BYTES 170000000LL
@@ -456,6 +460,28 @@ __global__ void __launch_bounds__(WARPS * 32, Stream<HD, NT>::PER_SM) decode_e4m
             const uint8_t* kt = my_ring + stage * 2 * C::TILE_BYTES;
             const uint8_t* vt = kt + C::TILE_BYTES;
             stage = next;
+            bool rare = false;  // rows of zeros, or of values below 2^-81
+#pragma unroll
+            for (int h = 0; h < HALVES; ++h) {
+                const uint32_t ev = (powers[h] >> 8) & 255;
+                rare |= (powers[h] >> 16) != 0 && (ev == 127 || ev < LEAST_POWER);
+            }
+            rare = __any_sync(0xffffffffu, rare);
+            if (__builtin_expect(rare, 0)) {
+#pragma unroll 1
+                for (int h = 0; h < HALVES; ++h) {
+                    const int token = 32 * h + 8 * (TOKENS >= 32 ? t : t & 1) + g;
+                    uint32_t codes = 0;
+#pragma unroll 1
+                    for (int c = 0; c < CH; ++c) {
+                        const uint4 x = *reinterpret_cast<const uint4*>(vt + C::at(token, c));
+                        codes |= x.x | x.y | x.z | x.w;
+                    }
+#pragma unroll
+                    for (int i = 0; i < HALVES; ++i)  // (registers, not an array in memory)
+                        if (i == h && ((powers[i] >> 8) & 255) == 127 && (codes & 0x7F7F7F7Fu) == 0) powers[i] = (powers[i] & ~0xFF00u) | LEAST_POWER << 8;
+                }
+            }
             if (PORTIONS && (pos0 > seen_by_any || (p.window > 0 && pos0 + TOKENS - 1 <= seen_by_all - p.window))) {
                 __syncwarp();  // no row sees any of the tile
                 continue;
@@ -492,16 +518,16 @@ __global__ void __launch_bounds__(WARPS * 32, Stream<HD, NT>::PER_SM) decode_e4m
                 }
             }
             // scores of tokens 8 x + g (x = 2 u, 2 u + 1) for heads 2 t, 2 t + 1
-            float vs[2 * U];  // 2^(127 - Ev)
+            float ev[2 * U];  // max(Ev, 37) - 127
 #pragma unroll
             for (int x = 0; x < 2 * U; ++x) {
                 const uint32_t w = __shfl_sync(0xffffffffu, powers[x >> 2], (lane & ~3) | (x & 3));
-                const float kf = kv_up(w & 255), ev = (w >> 16) != 0 ? (float)((int)((w >> 8) & 255) - 127) : -INFINITY;
-                vs[x] = kv_down((w >> 8) & 255);
+                const float kf = kv_up(w & 255), counted = (w >> 16) != 0 ? 0.f : -INFINITY;
+                ev[x] = (float)(max((int)((w >> 8) & 255), LEAST_POWER) - 127);
 #pragma unroll
                 for (int n = 0; n < NT; ++n)
 #pragma unroll
-                    for (int e = 0; e < 2; ++e) sc[n][x >> 1][2 * (x & 1) + e] = fmaf(sc[n][x >> 1][2 * (x & 1) + e] * qf[n][e], kf, ev);
+                    for (int e = 0; e < 2; ++e) sc[n][x >> 1][2 * (x & 1) + e] = fmaf(sc[n][x >> 1][2 * (x & 1) + e] * qf[n][e], kf, counted);
             }
             if (PORTIONS && (pos0 + TOKENS - 1 > seen_by_all || p.window > 0)) {
 #pragma unroll
@@ -525,22 +551,31 @@ __global__ void __launch_bounds__(WARPS * 32, Stream<HD, NT>::PER_SM) decode_e4m
                 for (int e = 0; e < 2; ++e) {
                     float top = -INFINITY;
 #pragma unroll
-                    for (int u = 0; u < U; ++u) top = fmaxf(top, fmaxf(sc[n][u][e], sc[n][u][2 + e]));
+                    for (int u = 0; u < U; ++u) top = fmaxf(top, fmaxf(sc[n][u][e] + ev[2 * u], sc[n][u][2 + e] + ev[2 * u + 1]));
 #pragma unroll
                     for (int d = 4; d < 32; d <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
                     const float m_new = fmaxf(m[n][e], top), ref = m_new == -INFINITY ? 0.f : m_new - 14.f;
-                    keep[e] = fast_exp2(m[n][e] - 14.f - ref);
+                    const float half = fast_exp2(0.5f * (m[n][e] - 14.f - ref));
+                    keep[e] = half * half;
                     m[n][e] = m_new;
                     float sum = 0.f;
 #pragma unroll
                     for (int u = 0; u < U; ++u)
 #pragma unroll
                         for (int r = 0; r < 2; ++r) {
-                            const float w = fast_exp2(sc[n][u][2 * r + e] - ref);
-                            sc[n][u][2 * r + e] = w;
-                            sum = fmaf(w, vs[2 * u + r], sum);
+                            sum += fast_exp2(sc[n][u][2 * r + e] - ref);
+                            sc[n][u][2 * r + e] = fast_exp2(sc[n][u][2 * r + e] + (ev[2 * u + r] - ref));
                         }
-                    l[n][e] = fmaf(l[n][e], keep[e], sum);
+                    l[n][e] = fmaf(l[n][e] * half, half, sum);
+                }
+                if (__builtin_expect(rare, 0)) {
+#pragma unroll
+                    for (int x = 0; x < 2 * U; ++x) {
+                        const uint32_t w = __shfl_sync(0xffffffffu, powers[x >> 2], (lane & ~3) | (x & 3));
+                        const float less = kv_up(127 + min((int)((w >> 8) & 255) - LEAST_POWER, 0));
+                        sc[n][x >> 1][2 * (x & 1)] *= less;
+                        sc[n][x >> 1][2 * (x & 1) + 1] *= less;
+                    }
                 }
                 if (__any_sync(0xffffffffu, keep[0] != 1.f || keep[1] != 1.f)) {
 #pragma unroll
@@ -659,7 +694,10 @@ __global__ void __launch_bounds__(WARPS * 32, Stream<HD, NT>::PER_SM) decode_e4m
         }
 #pragma unroll
         for (int y = 0; y < 2 * WARPS; ++y)
-            if (m[y] != -INFINITY) sum = fmaf(fast_exp2(m[y] - top), l_s[y][r], sum);
+            if (m[y] != -INFINITY) {
+                const float half = fast_exp2(0.5f * (m[y] - top));
+                sum = fmaf(half * l_s[y][r], half, sum);
+            }
         const float own = m_s[x][r];
         f_s[x][r] = own == -INFINITY ? 0.f : fast_exp2(own - top);
         top_s[x][r] = top;
@@ -782,13 +820,14 @@ __global__ void __launch_bounds__(WARPS * 32, Stream<HD, NT>::PER_SM) decode_e4m
                         float next = top[e];
 #pragma unroll
                         for (int k = 0; k < MERGE_AT_ONCE; ++k) next = fmaxf(next, ml[e][k].x);
-                        const float keep = top[e] == -INFINITY ? 0.f : fast_exp2(top[e] - next);
-                        total[e] *= keep; sum[e].x *= keep; sum[e].y *= keep; sum[e].z *= keep; sum[e].w *= keep;
+                        const float half = top[e] == -INFINITY ? 0.f : fast_exp2(0.5f * (top[e] - next)), keep = half * half;
+                        total[e] = total[e] * half * half;
+                        sum[e].x *= keep; sum[e].y *= keep; sum[e].z *= keep; sum[e].w *= keep;
                         top[e] = next;
 #pragma unroll
                         for (int k = 0; k < MERGE_AT_ONCE; ++k) {
-                            const float f = ml[e][k].x == -INFINITY ? 0.f : fast_exp2(ml[e][k].x - next);
-                            total[e] = fmaf(f, ml[e][k].y, total[e]);
+                            const float h = ml[e][k].x == -INFINITY ? 0.f : fast_exp2(0.5f * (ml[e][k].x - next)), f = h * h;
+                            total[e] = fmaf(h * ml[e][k].y, h, total[e]);
                             sum[e].x = fmaf(f, v[e][k].x, sum[e].x); sum[e].y = fmaf(f, v[e][k].y, sum[e].y);
                             sum[e].z = fmaf(f, v[e][k].z, sum[e].z); sum[e].w = fmaf(f, v[e][k].w, sum[e].w);
                         }

@@ -5,7 +5,7 @@ import torch
 
 from clockwork_b200 import ops
 from clockwork_b200.ops import quantised
-from tests.e4m3_tools import CODES, attention, attention_bound, context, filled_pages
+from tests.e4m3_tools import CODES, attention, attention_bound, context, filled_pages, quantise
 from tests.gpu_tools import DEV
 
 pytestmark = pytest.mark.gpu
@@ -305,3 +305,72 @@ def test_portions_of_requests_over_one_table(ctx, new, page, dtype, most):
     assert all(torch.equal(out, outs[0]) for out in outs)
     _check(outs[0], q, cache, tables, ctx, [(s, starts[s], n, ctx[s] - n) for s, n in enumerate(new)], page, None, hd**-0.5, dtype,
            24 if dtype == torch.float32 else 8)
+
+
+def _stated_bound(q, k, v, first, scale, hd):
+    """What the operator states, summed over the tokens: 2^-11 of each contribution, 2^-38 of a row's largest, 2^-120; scores in float32 from
+    queries that count down to 2^-39 of their head's largest entry, which move every weight by as much relatively; sums in float32 (2^-18);
+    half a step of the output."""
+    rows, nh, _ = q.shape
+    group = nh // k.shape[1]
+    k, v = k.repeat_interleave(group, 1), v.repeat_interleave(group, 1)
+    s = torch.einsum("rhd,thd->rht", q, k) * scale
+    n = k.shape[0]
+    s = s.masked_fill((torch.arange(n) > first + torch.arange(rows)[:, None])[:, None], float("-inf"))
+    w = torch.softmax(s, -1)
+    want, size = torch.einsum("rht,thd->rhd", w, v), torch.einsum("rht,thd->rhd", w, v.abs())
+    largest = (w[..., None] * v.abs().transpose(0, 1)).flatten(2).amax(-1)[..., None]
+    score = scale * (2 * (hd + 4) * 2.0**-24 * torch.einsum("rhd,thd->rht", q.abs(), k.abs()).amax(-1) +
+                     hd * 2.0**-39 * q.abs().amax(-1) * k.abs().amax((0, 2)))[..., None]
+    off = (2.0**-11 + 2.0**-18 + 2 * score) * size + n * (2.0**-38 * largest + 2.0**-120)
+    return want, off + 2.0**-8 * (want.abs() + off)
+
+
+SMALL = [("one zero row of weight 2^20", 20, 0), ("2^25", 25, 0), ("2^30", 30, 0), ("2^35", 35, 0), ("2^60", 60, 0), ("2^100", 100, 0),
+         ("tiny values beside it", 0, -30), ("smaller ones", 3, -70), ("values at the format's end", 0, -118), ("no zero row", None, -80),
+         ("a huge value of little weight", -150, 118)]
+
+
+@pytest.mark.parametrize("rows", [1, 3])
+@pytest.mark.parametrize("heads, ctx", [((4, 1, 64), 200), ((12, 2, 128), 3000), ((4, 1, 256), 70), ((6, 3, 32), 5000)])
+@pytest.mark.parametrize("what, lead, power", SMALL)
+def test_small_contributions(what, lead, power, heads, ctx, rows):
+    """A token that has most of the weight and a value of zeros (its power says 2^0), or all values tiny, or one huge: the others'
+    contributions keep their bits.  ``lead``: log2 of that token's weight over the others'; ``power``: of the others' values (of the one
+    huge value, where there is such).  Portions of few rows go the same way."""
+    nh, nkv, hd = heads
+    page, scale = 16, hd**-0.5
+    g = torch.Generator().manual_seed(ctx + hd + (lead or 0))
+    (k, v, ke, ve), tables = filled_pages([ctx], page, nkv, hd, g, spread=0.1)
+    ids, at = tables[0].long(), ctx // 3
+    huge = power > 0
+    if not huge:
+        ve[ids] = torch.where(ve[ids] == 254, ve[ids].int(), (ve[ids].int() + power).clamp(min=3)).to(torch.uint8)
+    q = torch.randn(rows, nh, hd, generator=g).bfloat16()
+    if lead is not None:
+        q[:, :, 0] = 8.0  # (the token's key: as much in this entry as the lead takes, nothing elsewhere)
+        k.view(torch.uint8)[ids[at // page], at % page] = 0
+        size = lead / 1.4426950408889634 / (8.0 * scale)
+        codes, e = quantise(torch.cat([torch.full((nkv, 1), size), torch.zeros(nkv, hd - 1)], 1))
+        k.view(torch.uint8)[ids[at // page], at % page] = codes.view(torch.uint8)
+        ke[ids[at // page], :, at % page] = e
+        value = torch.zeros(nkv, hd) if not huge else 2.0**power * (1.0 + torch.rand(nkv, hd, generator=g))
+        codes, e = quantise(value)
+        v.view(torch.uint8)[ids[at // page], at % page] = codes.view(torch.uint8)
+        ve[ids[at // page], :, at % page] = e
+        assert huge or (e == 127).all()
+    cache, status = (k, v, ke, ve), ops.new_status(DEV)
+    on, lens = quantised.E4M3Pages(*_on(*cache)), torch.tensor([ctx], dtype=torch.int32)
+    if rows == 1:
+        out = quantised.attention_decode(q.flatten(1).to(DEV), on, *_on(tables, lens), nh, scale, status)
+    elif hd in quantised.SHORT_HEAD_DIMS:
+        plan = quantised.plan_portions([rows], [ctx], nh, nkv, hd, page, torch.device(DEV), most_rows=rows)
+        assert plan.short == rows
+        out = quantised.attention_portions(q.flatten(1).to(DEV), on, *_on(tables, torch.tensor([0, rows], dtype=torch.int32), lens), plan, nh, scale, status)
+    else:
+        pytest.skip("this head size is read back")
+    ops.raise_on_status(status)
+    keys, values = (context(cache[i], cache[2 + i], tables[0], ctx, page) for i in (0, 1))
+    want, bound = _stated_bound(q.double(), keys, values, ctx - rows, scale, hd)
+    got = out.double().cpu().view(rows, nh, hd)
+    assert got.isfinite().all() and float(((got - want).abs() / bound).max()) <= 1.0

@@ -15,7 +15,8 @@ row per ``every`` positions instead of one per position (``PagedKVNeed.every``: 
 blocks of positions); its tables are that much shorter and its pool that much smaller.  Mixers that
 keep a state of fixed size (``SlotStateNeed``) get a row per request in a slot tensor instead of
 pages.  A mixer may name several needs (a tuple): pages of one or two kinds and a state slot.  With ``kv_dtype`` "e4m3" pages
-hold 8-bit codes and a power of two per token and KV head (``ops.quantised``): about half of what bfloat16 takes.
+hold 8-bit codes and a power of two per token and KV head (``ops.quantised``): about half of what bfloat16 takes, and one layer's pages in
+the run's type beside them (``PageGroup.back``), allocated with the pool.
 """
 
 from __future__ import annotations
@@ -33,8 +34,9 @@ KV_DTYPES = ("auto", "e4m3")  # keys and values in the run's type, or in 8 bits
 
 class PageGroup:
     """Layers with identical needs: one allocator, one device tensor
-    ``[layers, planes (K, V; or one row per token), pages, page_size, kv_heads, head_dim]``.  ``e4m3``: that holds codes, and
-    ``exps`` the powers of their rows, ``[layers, 2, pages, kv_heads, page_size]``."""
+    ``[layers, planes (K, V; or one row per token), pages, page_size, kv_heads, head_dim]``.  ``e4m3``: that holds codes,
+    ``exps`` the powers of their rows, ``[layers, 2, pages, kv_heads, page_size]``, and ``back`` is one layer's pages in the run's type, where
+    the layers, one after the other, read back what their prompt portions see."""
 
     def __init__(self, need: PagedKVNeed, cache_layers: list[int], num_pages: int, page_size: int,
                  dtype: torch.dtype | None, device, e4m3: bool = False) -> None:
@@ -46,6 +48,7 @@ class PageGroup:
         self.allocator = PageAllocator(num_pages, page_size)
         self.kv: torch.Tensor | None = None
         self.exps: torch.Tensor | None = None
+        self.back: tuple[torch.Tensor, torch.Tensor] | None = None
         if device is not None and dtype is not None:
             self.kv = torch.zeros(
                 (len(cache_layers), need.planes, num_pages, page_size, need.num_kv_heads, need.head_dim),
@@ -54,6 +57,7 @@ class PageGroup:
             if e4m3:
                 self.kv = self.kv.view(torch.float8_e4m3fn)
                 self.exps = torch.zeros((len(cache_layers), 2, num_pages, need.num_kv_heads, page_size), dtype=torch.uint8, device=device)
+                self.back = tuple(torch.zeros((num_pages, page_size, need.num_kv_heads, need.head_dim), dtype=dtype, device=device) for _ in range(2))
         self._index = {layer: i for i, layer in enumerate(self.cache_layers)}
 
     def layer_kv(self, cache_layer: int) -> tuple[torch.Tensor, torch.Tensor]:
@@ -65,6 +69,10 @@ class PageGroup:
             return None, None
         plane = self.exps[self._index[cache_layer]]
         return plane[0], plane[1]
+
+    def shared_bytes(self) -> int:
+        """What the group holds on the device beside its tokens."""
+        return 0 if self.back is None else sum(t.numel() * t.element_size() for t in self.back)
 
     def bytes_per_token(self) -> int:
         elem = self.kv.element_size() if self.kv is not None else 1 if self.e4m3 else 2
@@ -391,7 +399,7 @@ class CacheManager:
 
         def paged(g: int, layer: int) -> PagedView:
             k, v = self.groups[g].layer_kv(layer)
-            return PagedView(k, v, block_tables[g], slots[g], True, *self.groups[g].layer_exps(layer))
+            return PagedView(k, v, block_tables[g], slots[g], True, *self.groups[g].layer_exps(layer), self.groups[g].back)
 
         def state(layer: int) -> StateView:
             return StateView(self.state.tensors[layer], state_slots, list(state_slots_host))
@@ -414,6 +422,10 @@ class CacheManager:
 
     def bytes_per_token(self) -> int:
         return sum(g.bytes_per_token() for g in self.groups)
+
+    def shared_bytes(self) -> int:
+        """What the pools hold on the device beside their tokens (all of it allocated with them)."""
+        return sum(g.shared_bytes() for g in self.groups)
 
     def check_invariants(self, extra_refs: dict[int, int] | None = None) -> None:
         """No page lost, held twice without a reference for each holder, or freed twice.

@@ -596,14 +596,15 @@ def attention_prefill(q, k_cache, v_cache, block_tables, q_start, ctx_lens, item
 
 
 def launch_prefill(q, k_cache, v_cache, block_tables, q_start, ctx_lens, item_seq, item_q0, items, num_heads, num_kv_heads, head_dim, scale,
-                   window, status, use_tc, item_split, out, each: int = 1) -> None:
+                   window, status, use_tc, item_split, out, each: int = 1, parts: dict | None = None) -> None:
     """The launch of ``attention_prefill``, its arguments as that has checked them.  ``each``: the query heads of a KV head, packed
-    into the tiles' rows (tcgen05 kernel; the items are then those of tiles of 128 // each tokens)."""
+    into the tiles' rows (tcgen05 kernel; the items are then those of tiles of 128 // each tokens).  ``parts``: the cut items' scratch
+    (default: the device's)."""
     _configure()
     if use_tc:
         st = {"part_o": None, "part_ml": None, "counters": None}
         if item_split is not None:
-            st = _prefill_scratch(q.device, items, num_heads // each, head_dim)
+            st = parts or _prefill_scratch(q.device, items, num_heads // each, head_dim)
         if each > 1:
             check(library().cw_attention_prefill_tc_packed(
                 _ptr(q), q.stride(0), q.shape[1], q.shape[0], _ptr(out), _ptr(k_cache), _ptr(v_cache), _ptr(block_tables),

@@ -262,8 +262,8 @@ def read_pages(cache: E4M3Pages, block_tables: torch.Tensor, ctx_lens: torch.Ten
 
 class DecodeWorkspace:
     """Scratch of ``attention_decode`` and ``attention_portions`` for heads of ``head_dim`` entries: partial results and counters that
-    are zero between calls, of a size that goes by the GPU and the head size alone.  Calls that may overlap on the GPU must not
-    share one."""
+    are zero between calls, of a size that goes by the GPU and the head size alone; for portions whose rows of keys are cut into parts, more of
+    both, from the first such call on.  Calls that may overlap on the GPU must not share one."""
 
     def __init__(self, head_dim: int, device) -> None:
         device = torch.device(device)
@@ -272,6 +272,26 @@ class DecodeWorkspace:
         self.floats = torch.empty(floats, dtype=torch.float32, device=device)
         self.words = torch.zeros(words, dtype=torch.int32, device=device)
         self.pointers = (self.floats.data_ptr(), self.words.data_ptr(), head_dim, self.floats.get_device())
+        self._parts: dict | None = None
+        self._outgrown: list = []  # (captured graphs may point at them)
+        self._of_a_graph = torch.cuda.is_current_stream_capturing()
+
+    def parts(self, slots: int, head_dim: int) -> dict:
+        """Room for the parts of ``slots`` (work item, head) pairs of the kernel of whole tiles."""
+        from .attention_fast import QUERY_TILE
+
+        held = self._parts
+        if held is None or held["part_o"].numel() < slots * QUERY_TILE * head_dim or held["counters"].numel() < slots:
+            if torch.cuda.is_current_stream_capturing() and not self._of_a_graph:
+                raise RuntimeError("the workspace of a captured call must have room for its portions: run the call once before it is captured")
+            if held is not None:
+                self._outgrown.append(held)
+            device = self.floats.device
+            held = self._parts = {"part_o": torch.empty(slots * QUERY_TILE * head_dim, dtype=torch.float32, device=device),
+                                  "part_ml": torch.empty(slots * QUERY_TILE * 2, dtype=torch.float32, device=device),
+                                  "counters": torch.zeros(slots, dtype=torch.int32, device=device)}
+            held["pointers"] = tuple(held[name].data_ptr() for name in ("part_o", "part_ml", "counters"))
+        return held
 
 
 @functools.lru_cache(maxsize=None)
@@ -306,12 +326,17 @@ def _workspace(workspace: DecodeWorkspace | None, head_dim: int, index: int, str
     return held
 
 
-def _scratch_of(workspace: DecodeWorkspace | None, cache) -> tuple | None:
-    """The pointers of a call's workspace, if it is there already."""
+def _made_workspace(workspace: DecodeWorkspace | None, cache) -> DecodeWorkspace | None:
+    """A call's workspace, if it is there already."""
     if workspace is None:
         if type(cache) is not E4M3Pages or torch.cuda.is_current_stream_capturing():
             return None
         workspace = _workspaces.get((cache.k.get_device(), _stream(), cache.k.shape[-1]))
+    return workspace
+
+
+def _scratch_of(workspace: DecodeWorkspace | None, cache) -> tuple | None:
+    workspace = _made_workspace(workspace, cache)
     return None if workspace is None else workspace.pointers
 
 
@@ -521,47 +546,39 @@ def _short_call(q, out, cache, block_tables, ctx_lens, q_start, num_heads, shape
         block_tables.shape[1], pages, window or 0, _sm_count(index), rows, least_rows, most_rows, scale)), "attention_portions_e4m3")
 
 
-_read_scratch: dict = {}
-_retired_scratch: list = []  # outgrown sets stay: captured graphs may point at them
-
-
-def portion_scratch(cache: E4M3Pages, dtype: torch.dtype) -> PlainPages:
-    """One layer's pages in the run's type, where portions' contexts are read back to; one set per device, type and shape of a
-    row, zero at first, replaced by a larger one when a cache has more pages."""
-    pages, page_size, nkv, hd = cache.k.shape
-    key = (cache.k.get_device(), dtype, page_size, nkv, hd)
-    held = _read_scratch.get(key)
-    if held is None or held.shape[1] < pages:
-        if torch.cuda.is_current_stream_capturing():
-            raise RuntimeError("the scratch pages of attention_portions must exist before a graph is captured: run the step once first")
-        if held is not None:
-            _retired_scratch.append(held)
-        held = _read_scratch[key] = torch.zeros(2, pages, page_size, nkv, hd, dtype=dtype, device=cache.k.device)
-    return PlainPages(held[0, :pages], held[1, :pages])
+def _check_back(pages: PlainPages | None, cache: E4M3Pages, like: torch.Tensor) -> PlainPages:
+    """Where contexts are read back to: the caller's pages, or some for this call."""
+    shape = cache.k.shape
+    if pages is None:
+        return PlainPages(like.new_empty(shape), like.new_empty(shape))
+    if not isinstance(pages, PlainPages) or any(t.shape != shape or t.dtype is not like.dtype or not t.is_contiguous() or t.data_ptr() % 16 for t in pages):
+        raise ValueError("back must be PlainPages like the codes in shape, of q's type, contiguous and 16-byte aligned")
+    _elsewhere(like.get_device(), *pages)
+    return pages
 
 
 def attention_portions(q: torch.Tensor, cache: E4M3Pages, block_tables: torch.Tensor, q_start: torch.Tensor, ctx_lens: torch.Tensor,
                        plan: PortionPlan, num_heads: int, scale: float, status: torch.Tensor, *, window: int | None = None,
-                       workspace: DecodeWorkspace | None = None) -> torch.Tensor:
+                       workspace: DecodeWorkspace | None = None, back: PlainPages | None = None) -> torch.Tensor:
     """Causal attention of prompt portions over an 8-bit cache: ``q`` [N, >= nh * hd]; request s owns rows
     q_start[s]:q_start[s + 1] and has ctx_lens[s] tokens in the cache, its rows' among them, at the end (``plan`` holds the same
     numbers).  Returns [N, nh * hd] (rows behind the last request's: undefined).  bfloat16 requests of few rows are attended
-    straight from the codes; the contexts of the others are read back into scratch pages that calls on a device share: calls that
-    may overlap on the GPU (different streams) must be serialised."""
+    straight from the codes; the contexts of the others are read back first, into ``back`` (pages like the cache's of q's type, which
+    calls that may overlap on the GPU must not share; default: pages of the call's own, in bfloat16 twice the codes' bytes).
+    ``workspace``: as in ``attention_decode``."""
     from . import attention_ref
     from . import attention_fast as fast
 
     common = q.is_cuda and q.dtype is torch.bfloat16 and type(cache) is E4M3Pages and cache.k.dim() == 4
-    scratch = _scratch_of(workspace, cache) if common else None
-    if common and (scratch is not None or plan.short == 0):
+    made = _made_workspace(workspace, cache) if common else None
+    if common and (made is not None or plan.short == 0 and plan.item_split is None):
         k = v = parts = None
         if plan.items:
-            k, v = portion_scratch(cache, q.dtype)
+            k, v = _check_back(back, cache, q)
             if plan.item_split is not None:
-                held = fast._prefill_scratch(q.device, plan.items, num_heads // plan.each, cache.k.shape[-1])
-                parts = held["part_o"].data_ptr(), held["part_ml"].data_ptr(), held["counters"].data_ptr()
-        out = _calls().portions(q, cache, block_tables, q_start, ctx_lens, plan, num_heads, scale, status, window, scratch, _sm_count(q.get_device()),
-                                READ_BLOCKS, k, v, parts)
+                parts = made.parts(plan.items * (num_heads // plan.each), cache.k.shape[-1])["pointers"]
+        out = _calls().portions(q, cache, block_tables, q_start, ctx_lens, plan, num_heads, scale, status, window, made and made.pointers,
+                                _sm_count(q.get_device()), READ_BLOCKS, k, v, parts)
         if out is not None:
             for _ in range((2 + (plan.shape[3] > 1)) * (plan.items > 0) + (plan.short > 0)):
                 counted()
@@ -589,16 +606,18 @@ def attention_portions(q: torch.Tensor, cache: E4M3Pages, block_tables: torch.Te
     if code == 1 and hd in fast.PREFILL_HEAD_DIMS:
         out = _new_rows(q, q.shape[0], num_heads * hd)
         if plan.items:
-            held = portion_scratch(cache, q.dtype)
+            held, parts = _check_back(back, cache, q), None
+            if plan.item_split is not None:
+                parts = _workspace(workspace, hd, index, _stream()).parts(plan.items * (num_heads // plan.each), hd)
             _read_call(cache, shape, block_tables, ctx_lens, q_start, held.k, held.v, window, max(plan.most_rows + 1, plan.least_rows), code, status)
             fast.launch_prefill(q, held.k, held.v, block_tables, q_start, ctx_lens, plan.item_seq, plan.item_q0, plan.items, num_heads, nkv, hd,
-                                scale, window, status, fast.prefill_tc_takes(hd, page_size), plan.item_split, out, plan.each)
+                                scale, window, status, fast.prefill_tc_takes(hd, page_size), plan.item_split, out, plan.each, parts)
         if plan.short:
             _short_call(q, out, cache, block_tables, ctx_lens, q_start, num_heads, shape, scale, window, plan.short, plan.least_rows, plan.most_rows, status,
                         index, workspace)
         return out
     rows = sum(plan.q_lens)
-    held = portion_scratch(cache, q.dtype)
+    held = _check_back(back, cache, q)
     read_pages(cache, block_tables, ctx_lens, held.k, held.v, status, window=window, q_start=q_start)
     out = attention_ref(q[:rows], held.k, held.v, block_tables, plan.tok_seq, plan.positions, num_heads, nkv, hd, scale, window, status, q_start,
                         list(zip(plan.q_lens, plan.ctx_lens)))
@@ -610,7 +629,8 @@ _step_workspaces: dict = {}
 
 
 def step_workspace(head_dim: int, index: int) -> DecodeWorkspace:
-    """The workspace that the layers of a device's engine steps share (steps run one after the other, captured ones too)."""
+    """The workspace that the layers of a device's engine steps share (steps run one after the other, captured ones and those of several
+    engines too: the other attention kernels' scratch is one set per device as well)."""
     held = _step_workspaces.get((index, head_dim))
     if held is None:
         if torch.cuda.is_current_stream_capturing():
@@ -620,10 +640,10 @@ def step_workspace(head_dim: int, index: int) -> DecodeWorkspace:
 
 
 def paged_attention(ctx, q: torch.Tensor, cache: E4M3Pages, block_tables: torch.Tensor, num_heads: int, scale: float,
-                    window: int | None) -> torch.Tensor:
+                    window: int | None, back: PlainPages) -> torch.Tensor:
     """Attention of a step of the engine that brings prompt portions, over an 8-bit cache that already holds the step's keys and
-    values: single tokens and short portions straight from the codes; longer ones from their requests' pages read back into scratch pages, by the kernels of the
-    run's type."""
+    values: single tokens and short portions straight from the codes; longer ones from their requests' pages read back into ``back``, by the
+    kernels of the run's type."""
     from . import attention_ref
     from .attention_fast import _Prefill
 
@@ -646,7 +666,7 @@ def paged_attention(ctx, q: torch.Tensor, cache: E4M3Pages, block_tables: torch.
             if plan is None:
                 plan = ctx.extras[key] = plan_portions(ctx.q_lens_host, ctx.ctx_lens_host, num_heads, nkv, hd, shape[1], ctx.device, least_rows=least)
             out = attention_portions(q, cache, block_tables, ctx.q_start, ctx.ctx_lens, plan, num_heads, scale, ctx.status, window=window,
-                                     workspace=scratch)
+                                     workspace=scratch, back=back)
             return singles(out) if apart else out
         # a captured step: how its rows are divided among its requests is not known here, but that none brings more than there are
         most = short_rows(num_heads, nkv, hd) if streams else 0
@@ -655,11 +675,9 @@ def paged_attention(ctx, q: torch.Tensor, cache: E4M3Pages, block_tables: torch.
             _short_call(q, out, cache, block_tables, ctx.ctx_lens, ctx.q_start, num_heads, shape, scale, window, ctx.num_tokens, least, most,
                         ctx.status, index, scratch)
             return singles(out) if apart else out
-        held = portion_scratch(cache, q.dtype)
-        read_pages(cache, block_tables, ctx.ctx_lens, held.k, held.v, ctx.status, window=window, q_start=ctx.q_start, least_rows=least)
-        out = _Prefill.portions(ctx, q, held.k, held.v, block_tables, num_heads, nkv, hd, scale, window, apart)
+        read_pages(cache, block_tables, ctx.ctx_lens, back.k, back.v, ctx.status, window=window, q_start=ctx.q_start, least_rows=least)
+        out = _Prefill.portions(ctx, q, back.k, back.v, block_tables, num_heads, nkv, hd, scale, window, apart)
         return singles(out) if apart else out
-    held = portion_scratch(cache, q.dtype)
-    read_pages(cache, block_tables, ctx.ctx_lens, held.k, held.v, ctx.status, window=window, q_start=ctx.q_start)
-    return attention_ref(q, held.k, held.v, block_tables, ctx.tok_seq, ctx.positions, num_heads, nkv, hd, scale, window, ctx.status,
+    read_pages(cache, block_tables, ctx.ctx_lens, back.k, back.v, ctx.status, window=window, q_start=ctx.q_start)
+    return attention_ref(q, back.k, back.v, block_tables, ctx.tok_seq, ctx.positions, num_heads, nkv, hd, scale, window, ctx.status,
                          ctx.q_start, list(zip(ctx.q_lens_host, ctx.ctx_lens_host)))

@@ -141,7 +141,7 @@ class Attention(Mixer):
         q = quantised.norm_rotate_store(qkv, ctx.positions, view.slots, constants[0], cache, nh, nkv, hd, ctx.status, early=True, **norms)
         if view.k_exp is None:
             return attention_ops.paged_attention(ctx, q, view, nh, nkv, hd, self.scale, self.window)
-        return quantised.paged_attention(ctx, q, cache, view.block_tables, nh, self.scale, self.window)
+        return quantised.paged_attention(ctx, q, cache, view.block_tables, nh, self.scale, self.window, quantised.PlainPages(*view.back))
 
 
 register_mixer("attention", Attention, replace=True)

@@ -75,6 +75,7 @@ class PagedView:
     write: bool = True
     k_exp: torch.Tensor | None = None  # 8-bit caches: powers, uint8 [pages, kv_heads, page_size]; k_cache and v_cache then hold
     v_exp: torch.Tensor | None = None  # the codes, float8_e4m3fn
+    back: tuple[torch.Tensor, torch.Tensor] | None = None  # 8-bit caches: pages like k_cache in the run's type, shared by the layers
 
     @property
     def page_size(self) -> int:

@@ -141,3 +141,11 @@ def test_the_oracle_holds_rows_within_half_a_step():
     assert (codes.double().abs().amax(1) > 216).all()  # no power is larger than it has to be (224, rounded)
     cache, tables = filled_pages([9, 0, 3], 4, 2, 16, g)
     assert tables.shape == (3, 3) and (tables[1] == -1).all() and cache[0].dtype == CODES
+
+
+@pytest.mark.parametrize("back", [torch.zeros(2, 4, 8, 2, 32, dtype=torch.bfloat16), quantised.PlainPages(torch.zeros(4, 8, 2, 32), torch.zeros(4, 8, 2, 32)),
+                                  quantised.PlainPages(torch.zeros(4, 8, 2, 32, dtype=torch.bfloat16), torch.zeros(3, 8, 2, 32, dtype=torch.bfloat16)),
+                                  quantised.PlainPages(*(torch.zeros(4, 2, 8, 32, dtype=torch.bfloat16).transpose(1, 2) for _ in range(2)))])
+def test_pages_to_read_back_to_that_do_not_fit_are_refused(back):
+    with pytest.raises(ValueError, match="back must be"):
+        quantised._check_back(back, _args()["cache"], torch.zeros(5, 128, dtype=torch.bfloat16))

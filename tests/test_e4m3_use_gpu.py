@@ -368,3 +368,63 @@ def test_rows_that_the_kernel_in_front_writes(early):
         got.append(quantised.decode_step(made, at[i], slots[i], None, cache, tables, ctx[i], NH, NKV, HD, 0.09, status, early=early))
     ops.raise_on_status(status)
     assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+def _portion_problem(new, behind, seed):
+    ctx = [a + b for a, b in zip(new, behind)]
+    g = torch.Generator().manual_seed(seed)
+    cache, tables = filled_pages(ctx, PAGE, NKV, HD, g)
+    q = torch.randn(sum(new), NH * HD, generator=g).bfloat16().to(DEV)
+    starts = torch.tensor([sum(new[:i]) for i in range(len(new) + 1)], dtype=torch.int32, device=DEV)
+    plan = quantised.plan_portions(new, ctx, NH, NKV, HD, PAGE, torch.device(DEV), most_rows=8)
+    assert plan.items > 0 and plan.item_split is not None  # (parts, which meet through counters)
+    return q, quantised.E4M3Pages(*(t.to(DEV) for t in cache)), tables.to(DEV), starts, torch.tensor(ctx, dtype=torch.int32, device=DEV), plan
+
+
+def test_portions_on_two_streams_and_in_graphs_at_once():
+    """Calls that bring nothing share nothing: two streams whose caches have the same shape, two graphs of them, and a graph beside plain
+    calls, over and over."""
+    status = [ops.new_status(DEV), ops.new_status(DEV)]
+    problems = [_portion_problem([130, 5], [6000, 900], 41), _portion_problem([130, 7], [6000, 900], 42)]
+    assert problems[0][1].k.shape == problems[1][1].k.shape
+
+    def run(i, **kwargs):
+        q, cache, tables, starts, ctx, plan = problems[i]
+        return quantised.attention_portions(q, cache, tables, starts, ctx, plan, NH, 0.09, status[i], **kwargs)
+
+    want = [run(0), run(1)]
+    back = quantised.PlainPages(*(torch.full(problems[0][1].k.shape, float("nan"), dtype=torch.bfloat16, device=DEV) for _ in range(2)))
+    workspace = quantised.DecodeWorkspace(HD, DEV)
+    assert all(torch.equal(run(i, back=back, workspace=workspace), want[i]) for i in range(2))
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    torch.cuda.synchronize()
+    got = [[], []]
+    for _ in range(30):
+        for i in range(2):
+            with torch.cuda.stream(streams[i]):
+                got[i].append(run(i))
+    torch.cuda.synchronize()
+    graphs, outs = [], []
+    for i in range(2):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            outs.append(run(i))
+        graphs.append(graph)
+    for k in range(30):
+        for i in range(2):
+            with torch.cuda.stream(streams[i]):
+                graphs[i].replay() if k % 2 == 0 or i == 0 else got[i].append(run(i))
+    torch.cuda.synchronize()
+    for i in range(2):
+        ops.raise_on_status(status[i])
+        assert torch.equal(outs[i], want[i]) and all(torch.equal(x, want[i]) for x in got[i])
+    empty = quantised.DecodeWorkspace(HD, DEV)
+    graph = torch.cuda.CUDAGraph()
+    with pytest.raises(RuntimeError, match="before it is captured"):
+        with torch.cuda.graph(graph):
+            run(0, workspace=empty)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):  # (and with one that has room)
+        out = run(0, workspace=workspace, back=back)
+    graph.replay()
+    assert torch.equal(out, want[0])

@@ -10,6 +10,7 @@ from clockwork_b200.config import PartSpec
 from clockwork_b200.engine import LLMEngine
 from clockwork_b200.engine.step import StepBuilder, StepEntry
 from clockwork_b200.engine.trace import TraceSession
+from clockwork_b200.ops import quantised
 from clockwork_b200.parts import build_part
 from clockwork_b200.sampling import SamplingParams
 from clockwork_b200.weights import write_random_model
@@ -239,3 +240,32 @@ def test_models_whose_rows_cannot_be_held_in_8_bits_are_refused():
             CacheManager(needs, num_pages=4, page_size=8, kv_dtype="e4m3")
     with pytest.raises(ValueError, match="kv_dtype"):
         CacheManager({0: PagedKVNeed(1, 64, e4m3=True)}, num_pages=4, page_size=8, kv_dtype="e5m2")
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_what_prompts_are_read_back_to_is_allocated_with_the_pool(dtype):
+    """A pool that fits when it is made still does when the first prompt comes: a step allocates nothing of the pool's size."""
+    part = build_part("mixer", PartSpec("attention", dict(hidden_size=80, num_heads=4, num_kv_heads=2, head_dim=64, qkv_bias=True, o_bias=False,
+                                                          scale=0.125, window=None, position=PartSpec("rope_neox", {"theta": 5000.0, "rotary_dim": 64}))), "a", dtype, DEV)
+    load(part, weights(part.tensor_decls(), dtype, seed=4))
+    part.o = Untouched()
+    before = torch.cuda.memory_allocated()
+    cache = CacheManager({0: part.cache_need()}, num_pages=8000, page_size=16, dtype=dtype, device=DEV, num_state_slots=4, kv_dtype="e4m3")
+    tokens = 8000 * 16
+    assert cache.shared_bytes() == tokens * 2 * 2 * 64 * torch.finfo(dtype).bits // 8
+    assert torch.cuda.memory_allocated() - before >= cache.shared_bytes() + tokens * cache.bytes_per_token()
+    builder = StepBuilder(cache, dtype, DEV, cache.status)
+    for rid, n in (("a", 300), ("b", 40), ("a", 200)):
+        if rid not in cache.requests:
+            cache.open(rid)
+        prepared = builder.prepare([StepEntry(rid, [0] * n, [])])
+        x = torch.randn(n, 80, device=DEV).to(dtype)
+        part.qkv(x)
+        quantised.step_workspace(64, 0)
+        torch.cuda.synchronize()
+        torch.cuda.reset_peak_memory_stats()
+        held = torch.cuda.memory_allocated()
+        part.forward(prepared.ctx, x, prepared.ctx.views[0], None)
+        ops.raise_on_status(cache.status)
+        assert torch.cuda.max_memory_allocated() - held < cache.shared_bytes() // 2
+        builder.commit(prepared)

@@ -279,7 +279,8 @@ PyObject* portions(PyObject* const* a) {
     const double scale = real(a[7]);
     const void* status = status_of(a[8], device);
     const long long window = window_of(a[9]), sms = number(a[11]), blocks = number(a[12]);
-    const int64_t q_stride = rows > 1 ? q.stride(0) : nh * cache.hd;
+    const int64_t q_stride = rows > 1 ? q.stride(0) : nh * cache.hd, unit = items > 0 ? 16 : few > 0 ? 4 : 1;
+    need((uintptr_t)q.const_data_ptr() % unit == 0 && 2 * q.stride(0) % unit == 0);
     need(q.stride(0) < (1LL << 31) && rows < (1LL << 31) && window < (1LL << 31) && tables.size(1) < (1LL << 31));
     const void *floats = nullptr, *words = nullptr;
     if (few > 0) {

@@ -562,7 +562,8 @@ def attention_portions(q: torch.Tensor, cache: E4M3Pages, block_tables: torch.Te
                        workspace: DecodeWorkspace | None = None, back: PlainPages | None = None) -> torch.Tensor:
     """Causal attention of prompt portions over an 8-bit cache: ``q`` [N, >= nh * hd]; request s owns rows
     q_start[s]:q_start[s + 1] and has ctx_lens[s] tokens in the cache, its rows' among them, at the end (``plan`` holds the same
-    numbers).  Returns [N, nh * hd] (rows behind the last request's: undefined).  bfloat16 requests of few rows are attended
+    numbers).  bfloat16 rows must begin at multiples of 16 bytes, of 4 where the plan has requests of few rows only.
+    Returns [N, nh * hd] (rows behind the last request's: undefined).  bfloat16 requests of few rows are attended
     straight from the codes; the contexts of the others are read back first, into ``back`` (pages like the cache's of q's type, which
     calls that may overlap on the GPU must not share; default: pages of the call's own, in bfloat16 twice the codes' bytes).
     ``workspace``: as in ``attention_decode``."""
@@ -601,6 +602,9 @@ def attention_portions(q: torch.Tensor, cache: E4M3Pages, block_tables: torch.Te
         raise ValueError("window must be positive or None")
     _check_status(status)
     index = q.get_device()
+    unit = 0 if code != 1 or hd not in fast.PREFILL_HEAD_DIMS else 16 if plan.items else 4 if plan.short else 0
+    if unit and (q.data_ptr() % unit or 2 * q.stride(0) % unit):
+        raise ValueError(f"q's rows must begin at multiples of {unit} bytes")
     _elsewhere(index, cache.k, block_tables, ctx_lens, q_start, plan.tok_seq, status)
     _check_device(index)
     if code == 1 and hd in fast.PREFILL_HEAD_DIMS:

@@ -149,3 +149,14 @@ def test_the_oracle_holds_rows_within_half_a_step():
 def test_pages_to_read_back_to_that_do_not_fit_are_refused(back):
     with pytest.raises(ValueError, match="back must be"):
         quantised._check_back(back, _args()["cache"], torch.zeros(5, 128, dtype=torch.bfloat16))
+
+
+@pytest.mark.parametrize("new, most, start, width, refused", [([2, 0, 3], 0, 1, 160, "16 bytes"), ([2, 0, 3], 0, 0, 161, "16 bytes"), ([2, 0, 3], 5, 1, 160, "4 bytes"),
+                                                              ([2, 0, 3], 5, 0, 161, "4 bytes"), ([2, 0, 3], 5, 2, 162, "CUDA"), ([2, 0, 3], 0, 8, 168, "CUDA")])
+def test_portions_whose_rows_begin_where_no_kernel_reads_them_are_refused(new, most, start, width, refused):
+    """Before anything is launched; rows that can be read get as far as the device's check."""
+    args = dict(q=torch.zeros(5, width, dtype=torch.bfloat16)[:, start : start + 128], cache=_args()["cache"], block_tables=torch.zeros(3, 2, dtype=torch.int32),
+                q_start=torch.tensor([0, 2, 2, 5], dtype=torch.int32), ctx_lens=torch.tensor([2, 0, 9], dtype=torch.int32),
+                plan=quantised.plan_portions(new, [2, 0, 9], 4, 2, 32, 8, "cpu", most_rows=most), num_heads=4, scale=1.0, status=torch.zeros(4, dtype=torch.int32))
+    with pytest.raises(ValueError, match=refused):
+        quantised.attention_portions(**args)

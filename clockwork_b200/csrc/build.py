@@ -22,6 +22,7 @@ import subprocess
 import sys
 import sysconfig
 import tempfile
+import threading
 import time
 from concurrent.futures import ThreadPoolExecutor, as_completed
 from pathlib import Path
@@ -148,7 +149,7 @@ def ensure_calls_built() -> Path:
     if compiler is None:
         raise RuntimeError("no C++ compiler found")
     _log(f"compiling {src.name} into {out_dir} (first use)")
-    t0, tmp = time.time(), out_dir / f".{CALLS_NAME}.{os.getpid()}"
+    t0, tmp = time.time(), out_dir / f".{CALLS_NAME}.{os.getpid()}.{threading.get_ident()}"
     root = Path(torch.__file__).parent
     cuda = Path(find_nvcc()).resolve().parent.parent
     includes = [root / "include", root / "include/torch/csrc/api/include", cuda / "include", sysconfig.get_path("include")]

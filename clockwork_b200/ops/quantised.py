@@ -14,13 +14,14 @@ from __future__ import annotations
 import ctypes
 import functools
 import struct
+import warnings
 from typing import NamedTuple
 
 import numpy as np
 import torch
 
 from . import _stream, dtype_code
-from .library import KernelLibraryError, check, counted, library
+from .library import check, counted, library
 
 # The entry points of this module take one block of words (pointers and whole numbers, then the floats), which costs a third of what
 # as many ctypes arguments do: 2 of 5 us of a call whose kernel may take 4.
@@ -52,6 +53,17 @@ class E4M3Pages(NamedTuple):
 _calls_module = None
 
 
+class _NoCalls:
+    """In the module's place where it cannot be built (it needs a host compiler and the headers of Python and torch, which the library
+    itself does not): every call goes Python's way to the same kernels."""
+
+    @staticmethod
+    def store(*args) -> None:
+        return None
+
+    step = decode = read = portions = store
+
+
 def _calls():
     """``csrc/quantised_calls.cpp``: the common calls without the interpreter's share (the store of 8 tokens 12 us of host time in
     Python, 5 there).  Its functions do nothing and return None where they find anything amiss; the code below then says what."""
@@ -68,7 +80,9 @@ def _calls():
             module = module_from_spec(spec_from_loader(CALLS_NAME, loader))
             loader.exec_module(module)
         except Exception as exc:  # noqa: BLE001
-            raise KernelLibraryError(f"the module of the 8-bit cache's calls is unavailable ({exc})") from exc
+            warnings.warn(f"the module of the 8-bit cache's calls is unavailable ({exc}); they take 5 to 10 us of host time more", RuntimeWarning, stacklevel=3)
+            _calls_module = _NoCalls
+            return _calls_module
         entries = [ctypes.cast(f, ctypes.c_void_p).value for f in (lib.cw_norm_rotate_store, lib.cw_read_pages, lib.cw_attention_decode_e4m3,
                                                                    lib.cw_attention_portions_e4m3, lib.cw_attention_prefill_tc_packed)]
         module.bind(*entries, E4M3Pages, PlainPages)

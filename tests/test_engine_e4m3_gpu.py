@@ -269,3 +269,65 @@ def test_what_prompts_are_read_back_to_is_allocated_with_the_pool(dtype):
         ops.raise_on_status(cache.status)
         assert torch.cuda.max_memory_allocated() - held < cache.shared_bytes() // 2
         builder.commit(prepared)
+
+
+@pytest.mark.parametrize("kv_dtype", ["auto", "e4m3"])
+@pytest.mark.parametrize("heads", [(6, 2, 48), (4, 1, 128)])
+def test_normed_heads_from_the_layer_s_input_on(heads, kv_dtype):
+    """float32, from x to the output in float64 by the tensors' names: the query heads' norm is ``q_norm.weight``'s, the key heads' ``k_norm.weight``'s,
+    before the rotation.  (The other tests take q and k from the kernel.)"""
+    nh, nkv, hd = heads
+    eps, theta, n, dtype, scale = 1e-5, 5000.0, 30, torch.float32, heads[2] ** -0.5
+    part = build_part("mixer", PartSpec("attention", dict(hidden_size=80, num_heads=nh, num_kv_heads=nkv, head_dim=hd, qkv_bias=True, o_bias=False,
+                                                          scale=scale, window=None, qk_norm=eps,
+                                                          position=PartSpec("rope_neox", {"theta": theta, "rotary_dim": hd}))), "a", dtype, DEV)
+    w = weights(part.tensor_decls(), dtype, seed=hd)
+    w["a.q_norm.weight"] = 1.0 + 0.5 * torch.rand(hd, generator=torch.Generator().manual_seed(1))
+    w["a.k_norm.weight"] = 1.0 - 0.5 * torch.rand(hd, generator=torch.Generator().manual_seed(2))
+    load(part, w)
+    part.o = Untouched()
+    cache = CacheManager({0: part.cache_need()}, num_pages=8, page_size=8, dtype=dtype, device=DEV, num_state_slots=4, kv_dtype=kv_dtype)
+    builder = StepBuilder(cache, dtype, DEV, cache.status)
+    cache.open("a")
+    x = torch.randn(n, 80, generator=torch.Generator().manual_seed(3))
+    angle = torch.arange(n).double()[:, None] * (theta ** -(torch.arange(0, hd, 2).double() / hd)).float().double()
+
+    def exact(name, count, norm):
+        """A projection's heads, normed and turned, and how far float32 may be off: a sum of 81 terms, its error divided by the heads' size as
+        it is; 24 roundings of each result (as in the store's own tests)."""
+        m, b = w[f"a.{name}.weight"].double(), w[f"a.{name}.bias"].double()
+        y = (x.double() @ m.T + b).view(n, count, hd)
+        off = (82 * 2.0**-24 * (x.double().abs() @ m.abs().T + b.abs())).view(n, count, hd)
+        if norm is None:
+            return y, off
+        root = (y.square().mean(-1, keepdim=True) + eps).sqrt()
+        weight = w[f"a.{norm}.weight"].double()
+        off = (off + y.abs() * off.square().mean(-1, keepdim=True).sqrt() / root) / root * weight
+        y = y / root * weight
+        c, s, h = angle.cos()[:, None], angle.sin()[:, None], hd // 2
+        turn = lambda t, c, s: torch.cat([t[..., :h] * c - t[..., h:] * s, t[..., h:] * c + t[..., :h] * s], -1)  # noqa: E731
+        off = turn(off, c.abs(), -s.abs()).abs() + torch.cat([off[..., :h], off[..., :h]], -1) * s.abs().repeat(1, 1, 2)
+        return turn(y, c, s), off + 24 * 2.0**-24 * (y.abs() + torch.cat([y[..., h:], y[..., :h]], -1).abs())
+
+    q, q_off = exact("q_proj", nh, "q_norm")
+    k, k_off = exact("k_proj", nkv, "k_norm")
+    v, v_off = exact("v_proj", nkv, None)
+    if kv_dtype == "e4m3":  # half a step of the codes, and the whole of one where float32's error decides between two
+        k_off, v_off = (off + 2.0**-4 * t.abs() + 2.0**-10 * t.abs().amax(-1, keepdim=True) / 223.0 * 2 for t, off in ((k, k_off), (v, v_off)))
+    outs, done = [], 0
+    for m in (17, 12, 1):
+        prepared = builder.prepare([StepEntry("a", [0] * m, [])])
+        outs.append(part.forward(prepared.ctx, x[done : done + m].to(DEV), prepared.ctx.views[0], None).double().cpu())
+        ops.raise_on_status(cache.status)
+        builder.commit(prepared)
+        done += m
+    want, size, _ = attention(q, k, v, 0, None, scale)
+    group = nh // nkv
+    k, k_off, v_off = (t.repeat_interleave(group, 1) for t in (k, k_off, v_off))
+    score_off = scale * (torch.einsum("rhd,thd->rht", q_off, k.abs() + k_off) + torch.einsum("rhd,thd->rht", q.abs(), k_off)).amax(-1)[..., None]
+    bound = 1.05 * torch.expm1(2 * score_off) * (size + v_off.amax((0, 2))[:, None]) + v_off.amax(0) + 2.0**-18 * size
+    got = torch.cat(outs).view(n, nh, hd)
+    worst = float(((got - want).abs() / bound).max())
+    assert worst <= 1.0
+    other, _, _ = attention(q / w["a.q_norm.weight"].double() * w["a.k_norm.weight"].double(), k[:, ::group] , v, 0, None, scale)
+    assert kv_dtype == "e4m3" or float(((got - other).abs() / bound).max()) > 100  # (a mistaken norm would be far outside)

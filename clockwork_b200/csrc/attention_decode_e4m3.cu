@@ -93,7 +93,6 @@ struct Stream {
     static constexpr int FIT = 196608 / PER_SM / (WARPS * 2 * TILE_BYTES);
     static constexpr int ST = FIT > 8 ? 8 : FIT;       // tiles in a warp's ring
     static constexpr int RING = WARPS * ST * 2 * TILE_BYTES;
-    static constexpr bool SWIZZLED = HD % 128 == 0 || HD == 64;
     // Where chunk c of row r lies.  Rows of 128 bytes and multiples are swizzled so that the reads below (K: two rows' four chunks
     // at a time; V: a chunk of four rows two apart) meet no bank twice; of 64 bytes: the same over lines of two rows.
     static __device__ __forceinline__ int at(int r, int c) {

@@ -564,12 +564,11 @@ class _Prefill:
 
 def attention_prefill(q, k_cache, v_cache, block_tables, q_start, ctx_lens, item_seq, item_q0, items, num_heads,
                       num_kv_heads, head_dim, scale, window, status, use_tc: bool | None = None,
-                      item_split: torch.Tensor | None = None, out: torch.Tensor | None = None) -> torch.Tensor:
+                      item_split: torch.Tensor | None = None) -> torch.Tensor:
     """Any mixture of portions: ``q`` [N, >= nh*hd]; request s owns rows q_start[s]:q_start[s+1] and has
     ctx_lens[s] tokens in the cache, its portion at the end.  Returns [N, nh*hd].  ``use_tc``: the
     tcgen05 kernel (default: whenever it takes the head size and the page size) or the mma.sync one.
-    ``item_split`` (tcgen05 kernel only): the split words of ``prefill_work_items`` when items are parts.  ``out``: where the rows
-    go instead of a new tensor."""
+    ``item_split`` (tcgen05 kernel only): the split words of ``prefill_work_items`` when items are parts."""
     _configure()
     if q.dtype != torch.bfloat16 or q.dim() != 2 or q.stride(1) != 1:
         raise ValueError("q must be a 2-d bfloat16 tensor with unit column stride")
@@ -580,10 +579,7 @@ def attention_prefill(q, k_cache, v_cache, block_tables, q_start, ctx_lens, item
         _need(t, torch.int32, name, 1)
     if head_dim not in PREFILL_HEAD_DIMS:
         raise ValueError(f"head_dim {head_dim} is not one of {PREFILL_HEAD_DIMS}")
-    if out is None:
-        out = torch.empty((q.shape[0], num_heads * head_dim), dtype=torch.bfloat16, device=q.device)
-    elif out.dtype != torch.bfloat16 or tuple(out.shape) != (q.shape[0], num_heads * head_dim) or not out.is_contiguous():
-        raise ValueError("out must be a contiguous bfloat16 [N, nh*hd] tensor")
+    out = torch.empty((q.shape[0], num_heads * head_dim), dtype=torch.bfloat16, device=q.device)
     if use_tc is None:
         use_tc = prefill_tc_takes(head_dim, k_cache.shape[1])
     if item_split is not None:

@@ -208,8 +208,8 @@ def norm_rotate_store(qkv: torch.Tensor, positions: torch.Tensor, slots: torch.T
     """What lies between the [q | k | v] product and attention, in one pass: ``qkv`` [N, (nh + 2 nkv) hd] (float32 or bfloat16;
     left as it is), RMS norms of every query and key head with float32 ``q_weight``, ``k_weight`` [hd] (None: not normed), the
     rotation of each head's leading ``2 * len(inv_freq)`` entries by ``positions`` (None: none turn; entry j pairs with
-    j + len(inv_freq)), and the write of k and v at ``slots`` (< 0: not stored) of ``cache`` (``E4M3Pages``, or ``PlainPages``
-    of qkv's type).  Returns q [N, nh * hd].  Everything up to the one rounding of each output is float32.
+    j + len(inv_freq)), and the write of k and v at ``slots`` (< 0: not stored; the others all different) of ``cache``
+    (``E4M3Pages``, or ``PlainPages`` of qkv's type).  Returns q [N, nh * hd].  Everything up to the one rounding of each output is float32.
 
     ``early``: a promise that ``positions``, ``slots``, ``inv_freq`` and the weights were complete before the kernel in front of this call was
     launched, as a step's inputs are; the call then begins while that kernel finishes."""
@@ -374,7 +374,7 @@ def attention_decode(q: torch.Tensor, cache: E4M3Pages, block_tables: torch.Tens
                      out: torch.Tensor | None = None, workspace: DecodeWorkspace | None = None, early: bool = False) -> torch.Tensor:
     """One query token per request over an 8-bit cache: ``q`` [S, >= nh * hd] (float32 or bfloat16, unit column stride; row s
     belongs to request s), ``ctx_lens`` [S] the tokens of each request in the cache, its own included.  ``window``: a request sees
-    its last ``window`` tokens only.  Returns [S, nh * hd]; a request of no tokens gets zeros.  In bfloat16 (head sizes in 32s) a token's
+    its last ``window`` tokens only.  Up to 65,535 requests.  Returns [S, nh * hd]; a request of no tokens gets zeros.  In bfloat16 (head sizes in 32s) a token's
     contribution is off by at most 2^-11 of itself, or by 2^-38 of the largest one of its row where that is more (2^-120 where no value of
     weight reaches 2^-81), and entries of a query count down to 2^-39 of the largest of its head; sums are float32.
 
@@ -580,7 +580,9 @@ def attention_portions(q: torch.Tensor, cache: E4M3Pages, block_tables: torch.Te
     Returns [N, nh * hd] (rows behind the last request's: undefined).  bfloat16 requests of few rows are attended
     straight from the codes; the contexts of the others are read back first, into ``back`` (pages like the cache's of q's type, which
     calls that may overlap on the GPU must not share; default: pages of the call's own, in bfloat16 twice the codes' bytes).
-    ``workspace``: as in ``attention_decode``."""
+    ``workspace``: as in ``attention_decode``.  Weights are held in bfloat16 over contexts read back, as by the kernels of a bfloat16 cache (off by
+    at most 2^-8 of themselves), and as in ``attention_decode`` straight from the codes.  Cached values must be finite: a NaN shows in rows
+    before it too."""
     from . import attention_ref
     from . import attention_fast as fast
 

@@ -24,12 +24,13 @@
 //
 // Query heads are scaled by a power of two each into half precision's upper range (bfloat16's 8 bits are kept; what falls below
 // 2^-39 of the head's largest entry is dropped).  The powers of K multiply scores in float32.  Those of V are taken into
-// the exponent: weights are p_j = 2^(s_j log2 e + Ev_j - 127 - M + 14), M the running maximum of s_j log2 e + max(Ev_j, 37) - 127, in half
+// the exponent: weights are p_j = 2^(s_j log2 e + Ev_j - 127 - M + 14), M the running maximum of s_j log2 e + max(Ev_j, 67) - 127, in half
 // precision (11 bits: off by at most 2^-11 of themselves, or by 2^-25, which is 2^-38 of the largest contribution).  A row of zeros
-// contributes nothing, whatever its power of 127 says, and has Ev_j = 37 here: it would otherwise push the others down to where half
-// precision has few bits.  (With a power below 37, values below 2^-81, an error is at most 2^-120.)  The denominator, float32, sums
-// 2^(s_j log2 e - M + 14) by itself, below 2^105 a token, and is taken from one maximum to the next in two halves: 2^(difference) by
-// itself may be no number any more where the sum times it still counts.
+// contributes nothing, whatever its power of 127 says, and has Ev_j = 67 here: it would otherwise push the others down to where half
+// precision has few bits.  (With a power below 67, values below 2^-51, an error is at most 2^-90.)  The denominator, float32, sums
+// 2^(s_j log2 e - M + 14) 2^24, which p_j is made from by its power: below 2^99 a token, and no number any more only where p_j is below 2^-31.
+// Sums go from one maximum to the next by a factor that is 2^-126 at least, which suffices where powers, those below 67 counting as
+// that, are no more than 100 apart.
 //
 // A segment (request, KV head and group) that lies in one warp's run is finished by it.  At the end of its run a block adds up
 // its warps' pieces of shared segments in order; the pieces of one that several blocks share go to scratch of two per block, and
@@ -58,7 +59,8 @@ struct DecodeE4m3Params {
 };
 
 #define WARPS 4
-#define LEAST_POWER 37
+#define LEAST_POWER 67
+#define SUMS_UP 24  // sums of weights are held times 2^24
 #define MERGE_AT_ONCE 8
 #define MOST_TEAMS 4
 #define TEAMS_FROM_BYTES 170000000LL
@@ -459,28 +461,6 @@ __global__ void __launch_bounds__(WARPS * 32, Stream<HD, NT>::PER_SM) decode_e4m
             const uint8_t* kt = my_ring + stage * 2 * C::TILE_BYTES;
             const uint8_t* vt = kt + C::TILE_BYTES;
             stage = next;
-            bool rare = false;  // rows of zeros, or of values below 2^-81
-#pragma unroll
-            for (int h = 0; h < HALVES; ++h) {
-                const uint32_t ev = (powers[h] >> 8) & 255;
-                rare |= (powers[h] >> 16) != 0 && (ev == 127 || ev < LEAST_POWER);
-            }
-            rare = __any_sync(0xffffffffu, rare);
-            if (__builtin_expect(rare, 0)) {
-#pragma unroll 1
-                for (int h = 0; h < HALVES; ++h) {
-                    const int token = 32 * h + 8 * (TOKENS >= 32 ? t : t & 1) + g;
-                    uint32_t codes = 0;
-#pragma unroll 1
-                    for (int c = 0; c < CH; ++c) {
-                        const uint4 x = *reinterpret_cast<const uint4*>(vt + C::at(token, c));
-                        codes |= x.x | x.y | x.z | x.w;
-                    }
-#pragma unroll
-                    for (int i = 0; i < HALVES; ++i)  // (registers, not an array in memory)
-                        if (i == h && ((powers[i] >> 8) & 255) == 127 && (codes & 0x7F7F7F7Fu) == 0) powers[i] = (powers[i] & ~0xFF00u) | LEAST_POWER << 8;
-                }
-            }
             if (PORTIONS && (pos0 > seen_by_any || (p.window > 0 && pos0 + TOKENS - 1 <= seen_by_all - p.window))) {
                 __syncwarp();  // no row sees any of the tile
                 continue;
@@ -516,13 +496,37 @@ __global__ void __launch_bounds__(WARPS * 32, Stream<HD, NT>::PER_SM) decode_e4m
                     }
                 }
             }
+            bool rare = false;  // rows of zeros, or of values below 2^-51
+#pragma unroll
+            for (int h = 0; h < HALVES; ++h) {
+                const uint32_t ev = (powers[h] >> 8) & 255;
+                rare |= (powers[h] >> 16) != 0 && (ev == 127 || ev < LEAST_POWER);
+            }
+            rare = __any_sync(0xffffffffu, rare);
+            if (__builtin_expect(rare, 0)) {
+#pragma unroll 1
+                for (int h = 0; h < HALVES; ++h) {
+                    const int token = 32 * h + 8 * (TOKENS >= 32 ? t : t & 1) + g;
+                    uint32_t codes = 0;
+#pragma unroll 1
+                    for (int c = 0; c < CH; ++c) {
+                        const uint4 x = *reinterpret_cast<const uint4*>(vt + C::at(token, c));
+                        codes |= x.x | x.y | x.z | x.w;
+                    }
+#pragma unroll
+                    for (int i = 0; i < HALVES; ++i)  // (registers, not an array in memory)
+                        if (i == h && ((powers[i] >> 8) & 255) == 127 && (codes & 0x7F7F7F7Fu) == 0) powers[i] = (powers[i] & ~0xFF00u) | LEAST_POWER << 8;
+                }
+            }
             // scores of tokens 8 x + g (x = 2 u, 2 u + 1) for heads 2 t, 2 t + 1
-            float ev[2 * U];  // max(Ev, 37) - 127
+            float ev[2 * U], up[2 * U];  // max(Ev, 67) - 127; 2^(that - 24)
 #pragma unroll
             for (int x = 0; x < 2 * U; ++x) {
                 const uint32_t w = __shfl_sync(0xffffffffu, powers[x >> 2], (lane & ~3) | (x & 3));
                 const float kf = kv_up(w & 255), counted = (w >> 16) != 0 ? 0.f : -INFINITY;
-                ev[x] = (float)(max((int)((w >> 8) & 255), LEAST_POWER) - 127);
+                const int at_least = max((int)((w >> 8) & 255), LEAST_POWER);
+                ev[x] = (float)(at_least - 127);
+                up[x] = kv_up(at_least - SUMS_UP);
 #pragma unroll
                 for (int n = 0; n < NT; ++n)
 #pragma unroll
@@ -554,18 +558,18 @@ __global__ void __launch_bounds__(WARPS * 32, Stream<HD, NT>::PER_SM) decode_e4m
 #pragma unroll
                     for (int d = 4; d < 32; d <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
                     const float m_new = fmaxf(m[n][e], top), ref = m_new == -INFINITY ? 0.f : m_new - 14.f;
-                    const float half = fast_exp2(0.5f * (m[n][e] - 14.f - ref));
-                    keep[e] = half * half;
+                    keep[e] = fast_exp2(m[n][e] - 14.f - ref);
                     m[n][e] = m_new;
                     float sum = 0.f;
 #pragma unroll
                     for (int u = 0; u < U; ++u)
 #pragma unroll
                         for (int r = 0; r < 2; ++r) {
-                            sum += fast_exp2(sc[n][u][2 * r + e] - ref);
-                            sc[n][u][2 * r + e] = fast_exp2(sc[n][u][2 * r + e] + (ev[2 * u + r] - ref));
+                            const float w = fast_exp2(sc[n][u][2 * r + e] - (ref - SUMS_UP));
+                            sum += w;
+                            sc[n][u][2 * r + e] = w * up[2 * u + r];
                         }
-                    l[n][e] = fmaf(l[n][e] * half, half, sum);
+                    l[n][e] = fmaf(l[n][e], keep[e], sum);
                 }
                 if (__builtin_expect(rare, 0)) {
 #pragma unroll
@@ -665,7 +669,7 @@ __global__ void __launch_bounds__(WARPS * 32, Stream<HD, NT>::PER_SM) decode_e4m
                     const int r = 8 * n + 2 * t + e;
                     const float4 x = make_float4(o[n][2 * j][e], o[n][2 * j][2 + e], o[n][2 * j + 1][e], o[n][2 * j + 1][2 + e]);
                     if (begins && ends) {
-                        const float inv = l[n][e] == 0.f ? 0.f : 1.f / l[n][e];
+                        const float inv = l[n][e] == 0.f ? 0.f : (float)(1 << SUMS_UP) / l[n][e];
                         if (r < rows)
                             Vec4<bf16>::store((bf16*)p.out + row_at(row, head, x0 + r, p.nh * HD) + d, make_float4(x.x * inv, x.y * inv, x.z * inv, x.w * inv));
                     } else {
@@ -693,10 +697,7 @@ __global__ void __launch_bounds__(WARPS * 32, Stream<HD, NT>::PER_SM) decode_e4m
         }
 #pragma unroll
         for (int y = 0; y < 2 * WARPS; ++y)
-            if (m[y] != -INFINITY) {
-                const float half = fast_exp2(0.5f * (m[y] - top));
-                sum = fmaf(half * l_s[y][r], half, sum);
-            }
+            if (m[y] != -INFINITY) sum = fmaf(fast_exp2(m[y] - top), l_s[y][r], sum);
         const float own = m_s[x][r];
         f_s[x][r] = own == -INFINITY ? 0.f : fast_exp2(own - top);
         top_s[x][r] = top;
@@ -742,7 +743,7 @@ __global__ void __launch_bounds__(WARPS * 32, Stream<HD, NT>::PER_SM) decode_e4m
                 }
                 const float total = total_s[x][r];
                 if (whole) {
-                    const float inv = total == 0.f ? 0.f : 1.f / total;
+                    const float inv = total == 0.f ? 0.f : (float)(1 << SUMS_UP) / total;
                     Vec4<bf16>::store((bf16*)p.out + row_at(s.row, s.head, s.first + r, p.nh * HD) + i % (HD / 4) * 4, make_float4(sum.x * inv, sum.y * inv, sum.z * inv, sum.w * inv));
                 } else {
                     *reinterpret_cast<float4*>(part + i * 4) = sum;
@@ -819,14 +820,13 @@ __global__ void __launch_bounds__(WARPS * 32, Stream<HD, NT>::PER_SM) decode_e4m
                         float next = top[e];
 #pragma unroll
                         for (int k = 0; k < MERGE_AT_ONCE; ++k) next = fmaxf(next, ml[e][k].x);
-                        const float half = top[e] == -INFINITY ? 0.f : fast_exp2(0.5f * (top[e] - next)), keep = half * half;
-                        total[e] = total[e] * half * half;
-                        sum[e].x *= keep; sum[e].y *= keep; sum[e].z *= keep; sum[e].w *= keep;
+                        const float keep = top[e] == -INFINITY ? 0.f : fast_exp2(top[e] - next);
+                        total[e] *= keep; sum[e].x *= keep; sum[e].y *= keep; sum[e].z *= keep; sum[e].w *= keep;
                         top[e] = next;
 #pragma unroll
                         for (int k = 0; k < MERGE_AT_ONCE; ++k) {
-                            const float h = ml[e][k].x == -INFINITY ? 0.f : fast_exp2(0.5f * (ml[e][k].x - next)), f = h * h;
-                            total[e] = fmaf(h * ml[e][k].y, h, total[e]);
+                            const float f = ml[e][k].x == -INFINITY ? 0.f : fast_exp2(ml[e][k].x - next);
+                            total[e] = fmaf(f, ml[e][k].y, total[e]);
                             sum[e].x = fmaf(f, v[e][k].x, sum[e].x); sum[e].y = fmaf(f, v[e][k].y, sum[e].y);
                             sum[e].z = fmaf(f, v[e][k].z, sum[e].z); sum[e].w = fmaf(f, v[e][k].w, sum[e].w);
                         }
@@ -837,7 +837,7 @@ __global__ void __launch_bounds__(WARPS * 32, Stream<HD, NT>::PER_SM) decode_e4m
                     const int i = i0 + e * WARPS * 32;
                     if (i >= items) break;
                     if (final) {
-                        const float inv = total[e] == 0.f ? 0.f : 1.f / total[e];
+                        const float inv = total[e] == 0.f ? 0.f : (float)(1 << SUMS_UP) / total[e];
                         Vec4<bf16>::store((bf16*)p.out + row_at(s.row, s.head, s.first + i / (HD / 4), p.nh * HD) + i % (HD / 4) * 4,
                                           make_float4(sum[e].x * inv, sum[e].y * inv, sum[e].z * inv, sum[e].w * inv));
                     } else {  // over the first of the eight, whose four sums this thread alone reads and writes

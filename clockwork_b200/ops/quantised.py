@@ -375,8 +375,9 @@ def attention_decode(q: torch.Tensor, cache: E4M3Pages, block_tables: torch.Tens
     """One query token per request over an 8-bit cache: ``q`` [S, >= nh * hd] (float32 or bfloat16, unit column stride; row s
     belongs to request s), ``ctx_lens`` [S] the tokens of each request in the cache, its own included.  ``window``: a request sees
     its last ``window`` tokens only.  Up to 65,535 requests.  Returns [S, nh * hd]; a request of no tokens gets zeros.  In bfloat16 (head sizes in 32s) a token's
-    contribution is off by at most 2^-11 of itself, or by 2^-38 of the largest one of its row where that is more (2^-120 where no value of
-    weight reaches 2^-81), and entries of a query count down to 2^-39 of the largest of its head; sums are float32.
+    contribution is off by at most 2^-11 of itself, or by 2^-38 of the largest one of its row where that is more (2^-90 where no value of
+    weight reaches 2^-51), and entries of a query count down to 2^-39 of the largest of its head; sums are float32.  The powers of a context's
+    values, those of 2^-60 or less counting as that, must be within 2^100 of one another.
 
     ``q_start`` (int32 [S + 1]) with ``out`` ([N, nh * hd]): the requests are those of a flat batch of N rows that also holds
     prompt portions; only requests with exactly one row are served, the others' rows are left alone.  ``workspace``: the call's scratch (default:

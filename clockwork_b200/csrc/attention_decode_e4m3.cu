@@ -12,9 +12,9 @@
 // way) and on into the next request, so that warps never wait for one another while they stream.
 //
 // Bound by memory while it streams, and by latency before and after that.  Measured, us, and what the bytes take at the rate of a copy: 64
-// requests of 1 to 7,650 tokens, 28 heads over 4 of 128, 251 MB 55.5 and 38.9 (the stream itself 36; the first tiles come after 6,
+// requests of 1 to 7,650 tokens, 28 heads over 4 of 128, 251 MB 55 and 38.9 (the stream itself 36; the first tiles come after 6,
 // the last pieces are added up 8 after the last tile); four of 65,536 to 131,072, 40 heads over 8, 861 MB 160 and 133; 8 of 1,024, 12 over
-// 2, 4.3 MB 11 and 0.7: lengths, block table and rows are three trips to memory one after the other, and joining the pieces is four.
+// 2, 4.3 MB 13 and 0.7: lengths, block table and rows are three trips to memory one after the other, and joining the pieces is four.
 //
 // Codes become half-precision numbers exactly (cvt) on their way into mma.sync.m16n8k16, which costs less here than it could
 // save elsewhere: at the rate of memory the tensor cores are a fifth busy.  Tokens are the M side of S^T = K Q^T and the codes'

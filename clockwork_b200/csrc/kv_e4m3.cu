@@ -100,9 +100,9 @@ struct Four<bf16> {
 // LG neighbouring lanes hold a head, a lane two octets of it (octet i, i < rot / 8: four entries and the four that turn with them;
 // behind those, eight neighbours), so that pairs never leave a thread, the mean of squares and the largest magnitude are shuffles
 // among LG lanes, and accesses are of 8 or 16 bytes.  A thread keeps its head and its entries for a block's tokens, whose rows are
-// loaded one ahead: weights, offsets and the kind of head are found out once.  Bound by its instructions (304 a warp and token,
-// half of the issue slots taken at 78 registers a thread), which is why products go two at a time and the root is an estimate and
-// a step: 2,048 tokens of 36 normed heads of 128 13.7 -> 10.9 us (in the L2), 8,192 64 -> 38; what the bytes take: 5.5 and 22.
+// loaded one ahead: weights, offsets and the kind of head are found out once.  Neither memory nor issue slots are full (304 instructions a warp and
+// token take half of them, 18 warps an SM at 78 registers a thread, a row under way in each); fewer instructions a row were what helped, products two at a time
+// and the root by an estimate and a step: 2,048 tokens of 36 normed heads of 128 13.7 -> 10.9 us (in the L2), 8,192 64 -> 38; what the bytes take: 5.5 and 22.
 #define STORE_TOKENS 8
 template <typename T, int LG>
 __global__ void __launch_bounds__(512) norm_rotate_store_kernel(const StoreParams p, int most_tokens, int block_heads) {
@@ -503,7 +503,7 @@ struct Quotient {
 };
 
 // Units are pages of a request, keys and values apart, a warp to each, so that thousands are on their way at once; where there are few,
-// parts of a page that a warp reads in one go (5,778 tokens of two KV heads of 128 8.3 -> 6.7 us, 16,000 of eight 26.9 -> 18.4).  A page's codes
+// parts of a page that a warp reads in one go (5,778 tokens of two KV heads of 128 8.3 -> 6.7 us, now 5.8, 16,000 of eight 26.9 -> 18.4).  A page's codes
 // are one run of memory, and so is where they go; a lane takes 8 codes at a time (they share a row and its power), so that a
 // warp writes whole lines.
 #define READ_AT_ONCE 8
